@@ -37,6 +37,7 @@ extern "C" {
 /* KV cache element types */
 #define QE_KV_F32 0
 #define QE_KV_BF16 1
+#define QE_KV_FP8 2 /* e4m3 with a power-of-two scale per row: pages only (qe_pages) */
 
 /* Subset of config.json the forward pass reads. Replaces `Config`, cpu_inference.rs:20-33. */
 typedef struct qe_config {
@@ -256,6 +257,91 @@ int qe_op_read_sum(const float* src, uint64_t n, float* partial, uint32_t grid, 
  * faster than the strided one, so the read ceiling is the better of the two. It replaces nothing
  * in the reference, whose read_bandwidth.rs kernel has one form (tests/read_bandwidth.rs:16-54). */
 int qe_op_read_sum_nt(const float* src, uint64_t n, float* partial, uint32_t grid, void* stream);
+
+/* ---- paged K/V cache for several sequences, and the attention that reads it: operators on
+ *      caller-owned device memory, for one layer. No reference counterpart: its cache is one
+ *      buffer per layer and sequence (metal_inference.rs:115-138). ----
+ * Pages hold K and V of page_size positions each (a power of two, 16..65536), head_dim 128, as bf16
+ * or e4m3 (QE_KV_BF16, QE_KV_FP8):
+ *   k [n_pages][n_kv_heads][page_size][128]
+ *   v [n_pages][n_kv_heads][page_size / 16][128][16]: each 16 positions transposed, the form in
+ *     which the matrix cores take V
+ * and, with QE_KV_FP8, one exponent byte e per position and KV head in k_exp and v_exp
+ * [n_pages][n_kv_heads][page_size]: the row's values are the stored ones times 2^(e - 127).
+ * The plan of a call is device memory too, read when the call runs: row s of `table` names the
+ * pages of sequence s in order, lens[s] is its length with the call's new tokens, and the packed
+ * rows starts[s] .. starts[s + 1] are its new tokens, the last of them at position lens[s] - 1
+ * (starts has n_seqs + 1 entries and does not decrease). A table entry outside 0 .. n_pages - 1, or
+ * a position past the table, means that the page is not there. Packed rows that belong to no
+ * sequence are left as they were. Pages may be shared by sequences that only read them. */
+typedef struct qe_pages {
+  void* k;               /* 16-byte aligned, as v and the exponents */
+  void* v;
+  uint8_t* k_exp;        /* QE_KV_FP8 only */
+  uint8_t* v_exp;
+  const int32_t* table;  /* [n_seqs][table_stride] */
+  const int32_t* lens;   /* [n_seqs] */
+  const int32_t* starts; /* [n_seqs + 1] */
+  uint64_t n_pages;      /* below 2^31 */
+  uint64_t page_size;
+  uint64_t n_kv_heads;   /* 1..1024 */
+  uint64_t n_seqs;       /* 1..65536 */
+  uint64_t table_stride; /* table_stride * page_size below 2^31 */
+  int kv_dtype;
+} qe_pages;
+/* Bytes of k, and of v (0 for another kv_dtype). */
+uint64_t qe_page_bytes(uint64_t n_pages, uint64_t page_size, uint64_t n_kv_heads, int kv_dtype);
+/* Writes the new tokens' K and V rows into their pages: k, v [n_rows][n_kv_heads][128] of dtype
+ * QE_KV_F32 or QE_KV_BF16, rows row_stride elements apart, 16-byte aligned. bf16 pages take the
+ * nearest value. e4m3 pages: the exponent is the smallest for which the row's largest finite
+ * magnitude is at most 448 of its scale, the values are the nearest (ties to even), and infinities
+ * and NaN become NaN. A position whose page is not there is not written. Two rows for one position
+ * of one page: either may win. n_rows = 0 does nothing. */
+int qe_op_page_append(const qe_pages* pages, const void* k, const void* v, uint64_t n_rows, uint64_t row_stride,
+                      int dtype, void* stream);
+/* The same rows out of the pages (arguments as qe_op_page_append; k and v are written): zeros where
+ * a page is not there. */
+int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, uint64_t row_stride, int dtype,
+                    void* stream);
+/* Causal GQA attention of the new tokens over the pages (their own K and V appended before):
+ * out[t][h] = softmax over j <= position of t of (q[t][h] . k[j] / sqrt(128)), times v[j], over the
+ * positions whose page is there; zeros for a row that has none. q and out are [n_rows][n_heads][128]
+ * of `dtype` (QE_KV_F32 or QE_KV_BF16), rows q_stride and out_stride elements apart, 16-byte
+ * aligned; out must not overlap q or the pages. n_heads is a multiple of n_kv_heads. Softmax and
+ * sums are f32; f32 rows keep f32's precision, bf16 rows take the softmax weights rounded to bf16.
+ * max_new: the most new tokens any sequence has (0: not known). It chooses how the work is cut up;
+ * the results are right for any value. `work` is scratch memory of the call, overwritten by every
+ * call: work_bytes at least what qe_op_page_attention_work_bytes gives for the same values. Calls
+ * that may overlap need one each. n_rows = 0 does nothing. */
+uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new);
+int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
+                         uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work,
+                         uint64_t work_bytes, void* stream);
+
+/* ---- drafted tokens against the target's probabilities, from given random numbers: the sampled
+ *      form of qe_verify_greedy's rule, on device memory. No reference counterpart. ----
+ * Rows starts[s] .. starts[s + 1] of the logits [n_rows][vocab] (f32, rows row_stride apart) are
+ * sequence s's: one per draft and one for the token after the last. Row r's target is
+ * p = softmax(logits / temperature[s]); drafts[r] is its drafted token (the last row of a sequence
+ * has none) and draft_probs[r] (rows probs_stride apart) what it was drawn from. The drafts are
+ * accepted in order while accept[r] * draft_probs[r][d] < p[d]. The first row that does not accept
+ * draws its token from max(p - draft_probs[r], 0); the last row draws from p. A draw takes the
+ * smallest token whose running sum of weights is above sample[s] times their sum. accept [n_rows]
+ * and sample [n_seqs] are numbers in [0, 1). With draft_probs NULL each draft was certain
+ * (probability 1), as a lookup's are. temperature NULL is 1; one that is not above 0 is greedy: all
+ * of p on the first largest logit. NaN logits count as -inf, infinite ones share p; a row with
+ * nothing above -inf gives token 0. Draft probabilities that are not above 0 count as 0, and where
+ * nothing is left of p - q the draw is from p. A draft that is not below vocab is not accepted.
+ * tokens_out [n_rows]: each sequence's accepted drafts, then the drawn token, then 0xFFFFFFFF;
+ * count_out [n_seqs]: how many tokens that is (0 for a sequence without rows); logprobs_out
+ * [n_rows] (nullable): log p of each, 0 behind them. Rows that belong to no sequence are left as
+ * they were. Sums are f64. `work` as qe_op_page_attention's. */
+uint64_t qe_op_verify_drafts_work_bytes(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab);
+int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, uint64_t row_stride,
+                        const int32_t* starts, uint64_t n_seqs, const uint32_t* drafts, const float* draft_probs,
+                        uint64_t probs_stride, const float* accept, const float* sample, const float* temperature,
+                        uint32_t* tokens_out, uint32_t* count_out, float* logprobs_out, void* work,
+                        uint64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

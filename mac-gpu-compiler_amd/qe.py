@@ -37,6 +37,7 @@ QE_DRAFT_ERROR = 0xFFFFFFFF  # a draft callback's failure return (qe_draft_fn)
 
 QE_KV_F32 = 0
 QE_KV_BF16 = 1
+QE_KV_FP8 = 2  # pages only
 
 ERROR_NAMES = {
     QE_ERR_IO: "io", QE_ERR_FORMAT: "format", QE_ERR_TENSOR: "tensor", QE_ERR_POS: "pos",
@@ -110,6 +111,13 @@ def lookup_draft(history, ngram: int = 3, k_max: int = 4) -> list:
 class _LookupStats(ctypes.Structure):
     _fields_ = [("passes", ctypes.c_uint64), ("drafted", ctypes.c_uint64), ("accepted", ctypes.c_uint64),
                 ("single_steps", ctypes.c_uint64), ("plain_steps", ctypes.c_uint64)]
+
+
+class _CPages(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("k", "v", "k_exp", "v_exp", "table", "lens", "starts")]
+                + [(f, ctypes.c_uint64) for f in ("n_pages", "page_size", "n_kv_heads", "n_seqs", "table_stride")]
+                + [("kv_dtype", ctypes.c_int)])
+
 
 _lib = None
 
@@ -214,6 +222,13 @@ def lib() -> ctypes.CDLL:
         "qe_op_read_sum": (i32, [vp, u64, vp, u32, vp]),
         "qe_op_read_sum_nt": (i32, [vp, u64, vp, u32, vp]),
         "qe_op_argmax": (i32, [vp, u64, u64, vp, vp]),
+        "qe_page_bytes": (u64, [u64, u64, u64, i32]),
+        "qe_op_page_append": (i32, [ctypes.POINTER(_CPages), vp, vp, u64, u64, i32, vp]),
+        "qe_op_page_read": (i32, [ctypes.POINTER(_CPages), vp, vp, u64, u64, i32, vp]),
+        "qe_op_page_attention_work_bytes": (u64, [u64, u64, u64]),
+        "qe_op_page_attention": (i32, [ctypes.POINTER(_CPages), vp, vp, u64, u64, u64, u64, u64, i32, vp, u64, vp]),
+        "qe_op_verify_drafts_work_bytes": (u64, [u64, u64, u64]),
+        "qe_op_verify_drafts": (i32, [vp, u64, u64, u64, vp, u64, vp, vp, u64, vp, vp, vp, vp, vp, vp, vp, u64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -487,3 +502,198 @@ def op_read_sum(src, partial, grid: int = 0, stream=None) -> None:
 
 def op_read_sum_nt(src, partial, grid: int = 0, stream=None) -> None:
     _check(lib().qe_op_read_sum_nt(_ptr(src), src.numel(), _ptr(partial), grid, _stream_ptr(stream)))
+
+
+# ---- paged K/V cache and the check of drafts, on torch tensors. These check what a wrong tensor
+#      would turn into a stray read or write: types, shapes, strides and the device. `stream` None is
+#      torch's current stream. ----
+
+def _refuse(message: str) -> None:
+    raise QeError(QE_ERR_ARG, message)
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _on_stream(stream) -> Optional[int]:
+    return _stream_ptr(_torch().cuda.current_stream() if stream is None else stream)
+
+
+def _same_device(first, *tensors) -> None:
+    torch = _torch()
+    if first.device.type != "cuda":
+        _refuse(f"tensors are on {first.device}: device memory is needed")
+    if first.device.index != torch.cuda.current_device():
+        _refuse(f"tensors are on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            _refuse(f"tensors are on {first.device} and {t.device}")
+
+
+def _dense(name: str, t, dtypes, shape) -> None:
+    """t has one of the types, is contiguous and has this shape"""
+    if t.dtype not in dtypes or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse(f"{name}: need a contiguous {' or '.join(str(d) for d in dtypes)} tensor of shape {tuple(shape)}, "
+                f"got {t.dtype} {tuple(t.shape)}" + ("" if t.is_contiguous() else ", not contiguous"))
+
+
+def _row_dtype(name: str, t) -> int:
+    torch = _torch()
+    if t.dtype == torch.float32:
+        return QE_KV_F32
+    if t.dtype == torch.bfloat16:
+        return QE_KV_BF16
+    _refuse(f"{name}: rows are float32 or bfloat16, got {t.dtype}")
+
+
+def _row_stride(name: str, t, heads: int) -> int:
+    """distance of the rows of t [rows, heads, 128], whose heads lie one after the other"""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != 128:
+        _refuse(f"{name}: need [rows, {heads}, 128], got {tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128)):
+        _refuse(f"{name}: the heads of a row must lie one after the other")
+    return int(t.stride(0)) if t.shape[0] > 1 else heads * 128
+
+
+class Pages:
+    """A paged K/V cache of one layer and the plan of a call (qe_pages in include/qe.h).
+
+    k [n_pages, n_kv, page_size, 128] and v [n_pages, n_kv, page_size / 16, 128, 16] are bfloat16, or
+    float8_e4m3fn (or its uint8 bytes) with the exponent bytes k_exp, v_exp [n_pages, n_kv, page_size]
+    uint8. table [n_seqs, pages of a sequence], lens [n_seqs] and starts [n_seqs + 1] are int32. All
+    are device tensors that the object keeps; their contents are read when a call runs, so a program
+    changes them in place from step to step."""
+
+    def __init__(self, k, v, table, lens, starts, k_exp=None, v_exp=None):
+        torch = _torch()
+        fp8 = k.dtype in (torch.float8_e4m3fn, torch.uint8)
+        if k.dim() != 4 or k.shape[3] != 128 or not (fp8 or k.dtype == torch.bfloat16):
+            _refuse(f"k: need bfloat16 or float8_e4m3fn pages [n_pages, n_kv, page_size, 128], got {k.dtype} {tuple(k.shape)}")
+        n_pages, n_kv, size, _ = (int(n) for n in k.shape)
+        if n_pages == 0 or size < 16 or size > 65536 or size & (size - 1):
+            _refuse("page_size must be a power of two from 16 to 65536, and there must be pages")
+        _dense("k", k, (k.dtype,), k.shape)
+        _dense("v", v, (k.dtype,), (n_pages, n_kv, size // 16, 128, 16))
+        if fp8:
+            if k_exp is None or v_exp is None:
+                _refuse("float8 pages need k_exp and v_exp")
+            _dense("k_exp", k_exp, (torch.uint8,), k.shape[:3])
+            _dense("v_exp", v_exp, (torch.uint8,), k.shape[:3])
+        elif k_exp is not None or v_exp is not None:
+            _refuse("bfloat16 pages have no exponents")
+        if table.dim() != 2 or lens.dim() != 1:
+            _refuse("table must be [n_seqs, pages of a sequence] and lens [n_seqs]")
+        n_seqs = int(lens.shape[0])
+        _dense("table", table, (torch.int32,), (n_seqs, table.shape[1]))
+        _dense("lens", lens, (torch.int32,), (n_seqs,))
+        _dense("starts", starts, (torch.int32,), (n_seqs + 1,))
+        for t in (v, table, lens, starts, k_exp, v_exp):
+            if t is not None and t.device != k.device:
+                _refuse(f"tensors are on {k.device} and {t.device}")
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self.table, self.lens, self.starts = table, lens, starts
+        self.n_kv_heads = n_kv
+        self._c = _CPages(*[None if t is None else t.data_ptr() for t in (k, v, k_exp, v_exp, table, lens, starts)],
+                          n_pages, size, n_kv, n_seqs, int(table.shape[1]), QE_KV_FP8 if fp8 else QE_KV_BF16)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, table, lens, starts, kv_dtype: int = QE_KV_BF16):
+        """Pages of their own memory (not cleared) on the plan's device."""
+        torch = _torch()
+        if kv_dtype not in (QE_KV_BF16, QE_KV_FP8):
+            raise QeError(QE_ERR_UNSUPPORTED, "pages hold QE_KV_BF16 or QE_KV_FP8")
+        if page_size < 16 or page_size % 16:
+            _refuse("page_size must be a power of two from 16 to 65536, and there must be pages")
+        fp8 = kv_dtype == QE_KV_FP8
+        new = dict(dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16, device=table.device)
+        exps = [torch.empty(n_pages, n_kv_heads, page_size, dtype=torch.uint8, device=table.device) if fp8 else None
+                for _ in range(2)]
+        return cls(torch.empty(n_pages, n_kv_heads, page_size, 128, **new),
+                   torch.empty(n_pages, n_kv_heads, page_size // 16, 128, 16, **new), table, lens, starts, *exps)
+
+
+def _page_rows(call, pages: Pages, k, v, stream) -> None:
+    dtype = _row_dtype("k", k)
+    if v.dtype != k.dtype or v.shape != k.shape:
+        _refuse("k and v must have the same type and shape")
+    stride = _row_stride("k", k, pages.n_kv_heads)
+    if stride != _row_stride("v", v, pages.n_kv_heads):
+        _refuse("the rows of k and v must be equally far apart")
+    _same_device(k, v, pages.k)
+    _check(call(ctypes.byref(pages._c), _ptr(k), _ptr(v), k.shape[0], stride, dtype, _on_stream(stream)))
+
+
+def op_page_append(pages: Pages, k, v, stream=None) -> None:
+    """The new tokens' rows k, v [rows, n_kv, 128] (float32 or bfloat16) into their pages."""
+    _page_rows(lib().qe_op_page_append, pages, k, v, stream)
+
+
+def op_page_read(pages: Pages, k, v, stream=None) -> None:
+    """The same rows out of the pages into k, v (zeros where a page is not there)."""
+    _page_rows(lib().qe_op_page_read, pages, k, v, stream)
+
+
+def op_page_attention_work_bytes(n_heads: int, n_kv_heads: int, max_new: int = 0) -> int:
+    return int(lib().qe_op_page_attention_work_bytes(n_heads, n_kv_heads, max_new))
+
+
+def op_page_attention(pages: Pages, q, out, work, max_new: int = 0, stream=None) -> None:
+    """Causal GQA attention of the new tokens q [rows, n_heads, 128] over the pages, into out. work:
+    op_page_attention_work_bytes() device bytes; max_new: the most new tokens of a sequence (0: not
+    known)."""
+    dtype = _row_dtype("q", q)
+    heads = int(q.shape[1]) if q.dim() == 3 else 0
+    if out.dtype != q.dtype or out.shape != q.shape:
+        _refuse("q and out must have the same type and shape")
+    if not work.is_contiguous():
+        _refuse("work must be contiguous")
+    if max_new < 0:
+        _refuse("max_new must not be negative")
+    _same_device(q, out, work, pages.k)
+    _check(lib().qe_op_page_attention(ctypes.byref(pages._c), _ptr(q), _ptr(out), q.shape[0], heads,
+                                      _row_stride("q", q, heads), _row_stride("out", out, heads), max_new, dtype,
+                                      _ptr(work), work.numel() * work.element_size(), _on_stream(stream)))
+
+
+def op_verify_drafts_work_bytes(n_rows: int, n_seqs: int, vocab: int) -> int:
+    return int(lib().qe_op_verify_drafts_work_bytes(n_rows, n_seqs, vocab))
+
+
+def op_verify_drafts(logits, starts, drafts, accept, sample, tokens, count, work, draft_probs=None, temperature=None,
+                     logprobs=None, stream=None) -> None:
+    """Checks drafts [rows] against softmax(logits [rows, vocab] / temperature) by the numbers accept
+    [rows] and sample [n_seqs], and draws the token after the accepted ones (qe_op_verify_drafts):
+    tokens [rows], count [n_seqs] and logprobs [rows] are written. work:
+    op_verify_drafts_work_bytes() device bytes."""
+    torch = _torch()
+    f32, whole = (torch.float32,), (torch.int32, torch.uint32)
+    if logits.dim() != 2 or starts.dim() != 1 or starts.shape[0] < 2:
+        _refuse("need logits [rows, vocab] and starts [n_seqs + 1]")
+    (rows, vocab), n_seqs = logits.shape, starts.shape[0] - 1
+    strides = []
+    for name, t in (("logits", logits), ("draft_probs", draft_probs)):
+        if t is None:
+            strides.append(0)
+            continue
+        if t.dtype != torch.float32 or t.shape != logits.shape or (vocab > 1 and rows and t.stride(1) != 1):
+            _refuse(f"{name}: need float32 [{rows}, {vocab}] with each row's values one after the other")
+        strides.append(int(t.stride(0)) if rows > 1 else vocab)
+    _dense("starts", starts, (torch.int32,), (n_seqs + 1,))
+    _dense("drafts", drafts, whole, (rows,))
+    _dense("accept", accept, f32, (rows,))
+    _dense("sample", sample, f32, (n_seqs,))
+    _dense("tokens", tokens, whole, (rows,))
+    _dense("count", count, whole, (n_seqs,))
+    if temperature is not None:
+        _dense("temperature", temperature, f32, (n_seqs,))
+    if logprobs is not None:
+        _dense("logprobs", logprobs, f32, (rows,))
+    if not work.is_contiguous():
+        _refuse("work must be contiguous")
+    _same_device(logits, starts, drafts, accept, sample, tokens, count, work, draft_probs, temperature, logprobs)
+    opt = [None if t is None else _ptr(t) for t in (draft_probs, temperature, logprobs)]
+    _check(lib().qe_op_verify_drafts(_ptr(logits), rows, vocab, strides[0], _ptr(starts), n_seqs, _ptr(drafts), opt[0],
+                                     strides[1], _ptr(accept), _ptr(sample), opt[1], _ptr(tokens), _ptr(count), opt[2],
+                                     _ptr(work), work.numel() * work.element_size(), _on_stream(stream)))

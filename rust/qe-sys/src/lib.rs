@@ -24,6 +24,7 @@ pub const QE_ERR_KERNEL: c_int = 9;
 
 pub const QE_KV_F32: c_int = 0;
 pub const QE_KV_BF16: c_int = 1;
+pub const QE_KV_FP8: c_int = 2;
 
 /// A draft source's failure return (qe_draft_fn).
 pub const QE_DRAFT_ERROR: u32 = 0xFFFF_FFFF;
@@ -65,6 +66,25 @@ pub struct qe_model {
 #[repr(C)]
 pub struct qe_kv {
     _private: [u8; 0],
+}
+
+/// A paged K/V cache and the plan of a call (include/qe.h: layout and meaning).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct qe_pages {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_exp: *mut u8,
+    pub v_exp: *mut u8,
+    pub table: *const i32,
+    pub lens: *const i32,
+    pub starts: *const i32,
+    pub n_pages: u64,
+    pub page_size: u64,
+    pub n_kv_heads: u64,
+    pub n_seqs: u64,
+    pub table_stride: u64,
+    pub kv_dtype: c_int,
 }
 
 /// Called once per finished decode step with that step's greedy token, in order.
@@ -145,4 +165,21 @@ extern "C" {
     pub fn qe_op_argmax(logits: *const f32, rows: u64, n: u64, tokens_out: *mut u32, stream: *mut c_void) -> c_int;
     pub fn qe_op_read_sum(src: *const f32, n: u64, partial: *mut f32, grid: u32, stream: *mut c_void) -> c_int;
     pub fn qe_op_read_sum_nt(src: *const f32, n: u64, partial: *mut f32, grid: u32, stream: *mut c_void) -> c_int;
+
+    // paged K/V cache and the check of drafts, on caller-owned device memory (no reference counterpart)
+    pub fn qe_page_bytes(n_pages: u64, page_size: u64, n_kv_heads: u64, kv_dtype: c_int) -> u64;
+    pub fn qe_op_page_append(pages: *const qe_pages, k: *const c_void, v: *const c_void, n_rows: u64,
+                             row_stride: u64, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn qe_op_page_read(pages: *const qe_pages, k: *mut c_void, v: *mut c_void, n_rows: u64, row_stride: u64,
+                           dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn qe_op_page_attention_work_bytes(n_heads: u64, n_kv_heads: u64, max_new: u64) -> u64;
+    pub fn qe_op_page_attention(pages: *const qe_pages, q: *const c_void, out: *mut c_void, n_rows: u64,
+                                n_heads: u64, q_stride: u64, out_stride: u64, max_new: u64, dtype: c_int,
+                                work: *mut c_void, work_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn qe_op_verify_drafts_work_bytes(n_rows: u64, n_seqs: u64, vocab: u64) -> u64;
+    pub fn qe_op_verify_drafts(logits: *const f32, n_rows: u64, vocab: u64, row_stride: u64, starts: *const i32,
+                               n_seqs: u64, drafts: *const u32, draft_probs: *const f32, probs_stride: u64,
+                               accept: *const f32, sample: *const f32, temperature: *const f32,
+                               tokens_out: *mut u32, count_out: *mut u32, logprobs_out: *mut f32,
+                               work: *mut c_void, work_bytes: u64, stream: *mut c_void) -> c_int;
 }
