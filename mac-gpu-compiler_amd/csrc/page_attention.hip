@@ -5,6 +5,16 @@
 //   out[t][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(q[t][h] . k_j / sqrt(128)),  j = 0 .. pos(t),
 //
 // over the positions j whose page is there; a row that has none gives zeros.
+//
+// How the work is cut. The rows of a sequence and KV head are (token, q head) pairs, token first; an
+// item is one tile of them (16 to 128 rows) with its positions in blocks of 64, up to the last
+// position that any of its rows attends. The blocks of all items, in order (sequence, head, tile),
+// are dealt to a fixed number of workgroups in equal contiguous parts, whatever the lengths: the
+// lengths are device data, so the host cannot choose a split by them, and a batch of ragged lengths
+// keeps every CU busy to the end. A workgroup that holds all blocks of an item writes its rows out;
+// one that holds a part leaves the part's unnormalised sums, maxima and weight sums in `work`, and
+// k_page_join adds the parts of an item in order. The cut depends on the plan alone, so results are
+// the same every time.
 #include "pages.h"
 
 #include "device_common.h"
@@ -13,71 +23,651 @@
 namespace qe {
 namespace {
 
-// A wave per (row, q head): lane l holds dims 2 l and 2 l + 1. One position at a time with the
-// running maximum and sum of the softmax in f32.
-template <bool FP8, bool BF16_ROWS>
-__global__ __launch_bounds__(256) void k_page_attention(PagePlan p, PageStore st, const uint8_t* q, uint8_t* out,
-                                                        uint32_t n_rows, uint32_t n_heads, uint64_t q_stride,
-                                                        uint64_t out_stride, float scale) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t unit = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const uint32_t t = uint32_t(unit / n_heads), h = uint32_t(unit % n_heads), head = h / (n_heads / p.n_kv);
-  if (t >= n_rows) return;
-  const int32_t s = sequence_of(p, int32_t(t));
-  if (s < 0) return;
-  const int64_t last = position_of(p, s, int32_t(t)), cap = capacity_of(p);
-  const int64_t end = last + 1 < cap ? last + 1 : cap;
-  float q0, q1;
-  if constexpr (BF16_ROWS) {
-    const uint32_t u = reinterpret_cast<const uint32_t*>(q + (t * q_stride + h * kPageDim) * 2)[lane];
-    q0 = __uint_as_float(u << 16);
-    q1 = __uint_as_float(u & 0xFFFF0000u);
-  } else {
-    const float2 u = reinterpret_cast<const float2*>(q + (t * q_stride + h * kPageDim) * 4)[lane];
-    q0 = u.x;
-    q1 = u.y;
-  }
-  float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int64_t j = 0; j < end; j++) {
-    const int32_t page = page_of(p, s, j);
-    if (page < 0) continue;
-    const uint32_t off = uint32_t(j) & ((1u << p.page_shift) - 1);
-    const size_t row = page_row(p, page, head, off), ve = v_element(p, page, head, off);
-    float k0, k1, v0, v1;
-    if constexpr (FP8) {
-      const float ks = exp_scale(st.k_exp[row]), vs = exp_scale(st.v_exp[row]);
-      const uint32_t u = reinterpret_cast<const uint16_t*>(st.k + row * kPageDim)[lane];
-      const uint32_t w = st.v[ve + 32 * lane] | uint32_t(st.v[ve + 32 * lane + 16]) << 8;
-      k0 = __builtin_amdgcn_cvt_f32_fp8(int(u), 0) * ks;
-      k1 = __builtin_amdgcn_cvt_f32_fp8(int(u), 1) * ks;
-      v0 = __builtin_amdgcn_cvt_f32_fp8(int(w), 0) * vs;
-      v1 = __builtin_amdgcn_cvt_f32_fp8(int(w), 1) * vs;
-    } else {
-      const uint32_t u = reinterpret_cast<const uint32_t*>(st.k + row * kPageDim * 2)[lane];
-      const uint16_t* o = reinterpret_cast<const uint16_t*>(st.v) + ve + 32 * lane;
-      k0 = __uint_as_float(u << 16);
-      k1 = __uint_as_float(u & 0xFFFF0000u);
-      v0 = bf16f(o[0]);
-      v1 = bf16f(o[16]);
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kBlock = 64;    // positions
+constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
+
+struct AttnArgs {
+  PagePlan p;
+  PageStore st;
+  const uint8_t* q;
+  uint8_t* out;
+  uint64_t q_stride, out_stride;  // elements
+  float* parts;                   // [workgroup][2][rows of a tile][kPartRow]
+  struct Joint* joints;           // [workgroup]
+  uint32_t n_rows, n_heads, group;
+  uint32_t min_blocks;            // a workgroup takes at least so many
+  float c;                        // log2(e) / sqrt(128)
+};
+
+// An item whose first part is the last one of a workgroup: parts of `n` workgroups from there.
+struct Joint {
+  uint32_t n, seq, head, tile;
+};
+
+// ---- the plan of a sequence: its rows and how far each tile's positions go ----
+struct Seq {
+  int64_t first;   // position of its first row (may be negative)
+  int32_t row0;    // first packed row
+  uint32_t rows;   // new tokens * group
+  __device__ uint32_t tiles(uint32_t R) const { return (rows + R - 1) / R; }
+};
+
+__device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
+  const int64_t b = a.p.starts[s], e = a.p.starts[s + 1];
+  const int64_t lo = b < 0 ? 0 : b, hi = e < int64_t(a.n_rows) ? e : int64_t(a.n_rows);
+  Seq q;
+  q.row0 = int32_t(lo);
+  q.rows = hi > lo ? uint32_t(hi - lo) * a.group : 0;
+  q.first = int64_t(a.p.lens[s]) - (e - lo);
+  return q;
+}
+
+// Positions that some row of the tile attends: 0 .. limit - 1 (within the table).
+__device__ __forceinline__ uint32_t tile_limit(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
+  const uint32_t last = min((tile + 1) * R, q.rows) - 1;
+  const int64_t end = q.first + last / a.group + 1, cap = capacity_of(a.p);
+  return end < 0 ? 0 : uint32_t(end < cap ? end : cap);
+}
+// A tile that attends nothing still counts one block: its rows are zeros that someone writes.
+__device__ __forceinline__ uint32_t tile_blocks(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
+  return max((tile_limit(a, q, tile, R) + kBlock - 1) / kBlock, 1u);
+}
+__device__ uint64_t seq_blocks(const AttnArgs& a, const Seq& q, uint32_t R) {
+  uint64_t n = 0;
+  for (uint32_t i = 0, t = q.tiles(R); i < t; i++) n += tile_blocks(a, q, i, R);
+  return n;
+}
+
+// Where a workgroup is in the list of all blocks.
+struct Cursor {
+  Seq q;
+  uint32_t seq, head, tile, block, blocks;  // block of the tile's `blocks`
+};
+
+struct PlanShared {
+  uint64_t sum[256];
+  uint64_t per, total;
+  Cursor at;
+  uint32_t found;
+};
+
+// The next tile with rows after `cu`'s (false: there is none).
+__device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_t R) {
+  cu.block = 0;
+  if (++cu.tile >= cu.q.tiles(R)) {
+    cu.tile = 0;
+    if (++cu.head >= a.p.n_kv) {
+      cu.head = 0;
+      do {
+        if (++cu.seq >= a.p.n_seqs) return false;
+        cu.q = read_seq(a, cu.seq);
+      } while (cu.q.rows == 0);
     }
-    const float x = wave_sum(fmaf(q0, k0, q1 * k1)) * scale;
-    const float mn = fmaxf(m, x);
-    const float c = m == -INFINITY ? 0.f : expf(m - mn), w = x == -INFINITY ? 0.f : expf(x - mn);
-    l = fmaf(l, c, w);
-    a0 = fmaf(a0, c, w * v0);
-    a1 = fmaf(a1, c, w * v1);
-    m = mn;
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  a0 *= inv;
-  a1 *= inv;
-  if constexpr (BF16_ROWS) {
-    reinterpret_cast<uint32_t*>(out + (t * out_stride + h * kPageDim) * 2)[lane] =
-        f32_to_bf16(a0) | uint32_t(f32_to_bf16(a1)) << 16;
+  cu.blocks = tile_blocks(a, cu.q, cu.tile, R);
+  return true;
+}
+
+// Block `at` = w * per of the list (per: the blocks of one of W workgroups): fills sh.at and sh.found.
+// Each thread sums a contiguous range of sequences; the one whose range holds the block walks it.
+__device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh) {
+  const uint32_t t = threadIdx.x, each = (a.p.n_seqs + 255) / 256;
+  const uint32_t s0 = min(t * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
+  uint64_t mine = 0;
+  for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
+  mine *= a.p.n_kv;
+  if (t == 0) sh.found = 0;
+  sh.sum[t] = mine;
+  __syncthreads();
+  for (uint32_t d = 1; d < 256; d *= 2) {
+    const uint64_t v = t >= d ? sh.sum[t - d] : 0;
+    __syncthreads();
+    sh.sum[t] += v;
+    __syncthreads();
+  }
+  const uint64_t total = sh.sum[255];
+  const uint64_t even = (total + W - 1) / W, per = even > a.min_blocks ? even : a.min_blocks;
+  if (t == 0) {
+    sh.per = per;
+    sh.total = total;
+  }
+  const uint64_t at = w * per;
+  uint64_t before = sh.sum[t] - mine;
+  if (at >= before && at < sh.sum[t]) {
+    Cursor cu;
+    for (uint32_t s = s0; s < s1; s++) {
+      cu.q = read_seq(a, s);
+      const uint64_t one = seq_blocks(a, cu.q, R);
+      if (at < before + one * a.p.n_kv) {
+        cu.seq = s;
+        cu.head = uint32_t((at - before) / one);
+        uint64_t rest = (at - before) % one;
+        cu.tile = 0;
+        while (rest >= (cu.blocks = tile_blocks(a, cu.q, cu.tile, R))) {
+          rest -= cu.blocks;
+          cu.tile++;
+        }
+        cu.block = uint32_t(rest);
+        break;
+      }
+      before += one * a.p.n_kv;
+    }
+    sh.at = cu;
+    sh.found = 1;
+  }
+  __syncthreads();
+}
+
+// a workgroup's place in the list: consecutive parts on one XCD (workgroups go to the 8 XCDs in turn)
+__device__ __forceinline__ uint32_t part_index() {
+  const uint32_t n = gridDim.x;
+  return n % 8 ? blockIdx.x : (blockIdx.x % 8) * (n / 8) + blockIdx.x / 8;
+}
+
+// ---- arithmetic ----
+// maximum over the four groups of 16 lanes, to all of them
+__device__ __forceinline__ float max_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 2^x by the hardware (1 ulp; results below 2^-126 are 0, which a weight relative to the largest may be)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the factor from sums relative to maximum `from` to sums relative to `to` >= from
+__device__ __forceinline__ float rebase(float from, float to) { return from == to ? 1.f : exp2_fast(from - to); }
+
+// 8 floats as NS bf16 parts that add up to them: 1 rounded to nearest, or 3 cut (8 + 8 + 8 of f32's 24
+// bits: nothing is lost), so that NS matrix products against bf16 values keep f32's precision.
+template <int NS>
+__device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&o)[NS]) {
+  if constexpr (NS == 1) {
+    u32x4 u;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), bf16x2));
+    o[0] = __builtin_bit_cast(bf16x8, u);
   } else {
-    reinterpret_cast<float2*>(out + (t * out_stride + h * kPageDim) * 4)[lane] = make_float2(a0, a1);
+    static_assert(NS == 3, "1 or 3");
+    u32x4 h, m, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t a[3], b[3];
+      auto cut = [](float v, uint32_t (&w)[3]) {
+        w[0] = __float_as_uint(v);
+        const float r = v - __uint_as_float(w[0] & 0xFFFF0000u);
+        w[1] = __float_as_uint(r);
+        w[2] = __float_as_uint(r - __uint_as_float(w[1] & 0xFFFF0000u));
+      };
+      cut(x[2 * i], a);
+      cut(x[2 * i + 1], b);
+      // the upper halves of b and a
+      h[i] = __builtin_amdgcn_perm(b[0], a[0], 0x07060302u);
+      m[i] = __builtin_amdgcn_perm(b[1], a[1], 0x07060302u);
+      l[i] = __builtin_amdgcn_perm(b[2], a[2], 0x07060302u);
+    }
+    o[0] = __builtin_bit_cast(bf16x8, l);
+    o[1] = __builtin_bit_cast(bf16x8, m);
+    o[2] = __builtin_bit_cast(bf16x8, h);
   }
 }
+
+// 8 e4m3 values (two words) as bf16 times a power of two
+__device__ __forceinline__ bf16x8 fp8_bf16(uint32_t a, uint32_t b, float scale) {
+  u32x4 u;
+  u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false));
+  u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true));
+  u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false));
+  u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true));
+  return __builtin_bit_cast(bf16x8, u);
+}
+__device__ __forceinline__ float byte_scale(uint32_t w, int i) {  // 2^(e - 127) of byte i of w
+  return __uint_as_float((i == 3 ? w >> 1 : w << (23 - 8 * i)) & 0x7F800000u);
+}
+
+// 8 values of a row of q as floats
+template <bool BF16_ROWS>
+__device__ __forceinline__ void load_q8(const uint8_t* q, uint64_t element, float (&x)[8]) {
+  if constexpr (BF16_ROWS) {
+    const u32x4 u = *reinterpret_cast<const u32x4*>(q + element * 2);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  } else {
+    const f32x4 u = *reinterpret_cast<const f32x4*>(q + element * 4);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(q + element * 4 + 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[i] = u[i];
+      x[i + 4] = v[i];
+    }
+  }
+}
+template <bool BF16_ROWS>
+__device__ __forceinline__ void store_out8(uint8_t* out, uint64_t element, const float (&x)[8]) {
+  if constexpr (BF16_ROWS) {
+    bf16x8 o[1];
+    split_bf16<1>(x, o);
+    *reinterpret_cast<bf16x8*>(out + element * 2) = o[0];
+  } else {
+    *reinterpret_cast<f32x4*>(out + element * 4) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4*>(out + element * 4 + 16) = f32x4{x[4], x[5], x[6], x[7]};
+  }
+}
+// element of row r of a tile's item in rows of `stride` elements
+__device__ __forceinline__ uint64_t row_element(const AttnArgs& a, const Seq& q, uint32_t head, uint32_t r,
+                                                uint64_t stride) {
+  return (uint64_t(q.row0) + r / a.group) * stride + (head * a.group + r % a.group) * kPageDim;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: tiles of 16 NQ rows, the positions of a part dealt to the workgroup's four waves in steps
+// of 32 (bf16) or 64 (e4m3) positions, 16 KB of K and V a step.
+//
+// Bound by the K/V bytes, so the layout serves the loads. Scores are computed transposed, S^T = K Q^T
+// with v_mfma_f32_16x16x32_bf16: operand A's lane l holds row l % 16 of K, which may be any position,
+// and result lane l holds column (row of q) l % 16 and, of group g = l / 16, rows 4 g .. 4 g + 3.
+// Out^T = V^T P^T wants in lane l of operand B the weights of q row l % 16 at 8 positions, in A the
+// same positions of dim l % 16. With K's rows taken in the order below, a lane's results of two (e4m3:
+// four) score tiles are the weights of consecutive positions from 8 g (16 g), that is B as it stands,
+// and A is 16 bytes of one line of the transposed V page. So K and V go from memory to registers to
+// the matrix cores, with no LDS, no exchange between lanes but the maximum, and no barrier until a
+// part's end. The loads of a step are issued a step ahead (the page numbers two).
+// ---------------------------------------------------------------------------------------------
+template <bool FP8>
+struct StepData {
+  u32x4 k[8], v[8];
+  u32x4 ke, ve;     // e4m3: exponents of the 16 positions of the lane's K rows, and of its V
+  bool there;       // the page of the lane's V (and scores) is
+};
+
+template <bool FP8, bool BF16_ROWS, int NQ>
+__global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn_rows(AttnArgs a) {
+  constexpr int NS = BF16_ROWS ? 1 : 3, R = 16 * NQ, KEYS = FP8 ? 64 : 32, NT = KEYS / 16, EL = FP8 ? 1 : 2;
+  constexpr int LDO = 132;  // floats of a row's sums in LDS
+  __shared__ PlanShared sh;
+  __shared__ __align__(16) float sums[4][R][LDO];
+  __shared__ float top[4][R], mass[4][R];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t w = part_index();
+  find_start(a, w, gridDim.x, R, sh);
+  if (tid == 0) a.joints[w].n = 0;
+  if (!sh.found) return;
+  const uint64_t per = sh.per;
+  const uint64_t part_end = min((w + 1) * per, sh.total);
+  uint64_t at = w * per;
+  Cursor cu = sh.at;
+  const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
+  float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
+
+  while (true) {
+    const uint32_t take = uint32_t(min(uint64_t(cu.blocks - cu.block), part_end - at));
+    const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
+    const uint32_t rows = min(cu.q.rows - cu.tile * R, uint32_t(R));
+    // the positions of this part, in steps
+    const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
+    const uint32_t head = cu.head;
+    // the least position any row attends up to: below it no score is masked
+    const int64_t free64 = cu.q.first + (cu.tile * R) / a.group;
+    const int32_t free_to = int32_t(max(min(free64, int64_t(0x7FFFFFFF)), int64_t(-1)));
+    const bool one_token = (cu.tile * R) / a.group == (cu.tile * R + rows - 1) / a.group;
+    int32_t row_pos[NQ];
+    bf16x8 qf[NQ][4][NS];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      const uint32_t r = cu.tile * R + 16 * n + col;
+      const bool real = r < cu.q.rows;
+      const int64_t pos = cu.q.first + r / a.group;
+      row_pos[n] = real ? int32_t(max(min(pos, int64_t(0x7FFFFFFF)), int64_t(-1))) : -1;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t d = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
+        float x[8] = {};
+        if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + d, x);
+        split_bf16<NS>(x, qf[n][j]);
+      }
+    }
+    f32x4 acc[NQ][8];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // the 16 positions a lane's K rows and its V lie in, counted from the step's start
+    const uint32_t k16 = FP8 ? (col >> 2) * 16 : (col >> 3) * 16, v16 = FP8 ? g * 16 : (g >> 1) * 16;
+    const uint32_t k_in = (FP8 ? (col & 3) : 8 * ((col >> 2) & 1) + (col & 3)) * kPageDim * EL + 16 * g;
+    const uint32_t v_in = col * 16 * EL + (FP8 ? 0 : 16 * (g & 1));
+    const int32_t* const table = a.p.table + size_t(cu.seq) * a.p.table_stride;
+    auto look_up = [&](uint32_t x, int32_t& kp, int32_t& vp) __attribute__((always_inline)) {
+      kp = table[min((x + k16) >> a.p.page_shift, a.p.table_stride - 1)];
+      vp = table[min((x + v16) >> a.p.page_shift, a.p.table_stride - 1)];
+    };
+    auto load = [&](StepData<FP8>& d, uint32_t x, int32_t kp, int32_t vp) __attribute__((always_inline)) {
+      // a page that is not there is read as page 0, and what comes of it is masked
+      d.there = uint32_t(vp) < a.p.n_pages;
+      const size_t kr = page_row(a.p, uint32_t(kp) < a.p.n_pages ? kp : 0, head, (x + k16) & ps_mask);
+      const size_t vr = page_row(a.p, d.there ? vp : 0, head, (x + v16) & ps_mask);
+      const uint8_t* ka = a.st.k + kr * kPageDim * EL + k_in;
+      const uint8_t* va = a.st.v + vr * kPageDim * EL + v_in;
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int j = 0; j < 8 / NT; j++)
+          d.k[t * (8 / NT) + j] = *reinterpret_cast<const u32x4*>(ka + t * 4 * kPageDim * EL + 64 * j);
+#pragma unroll
+      for (int i = 0; i < 8; i++) d.v[i] = *reinterpret_cast<const u32x4*>(va + i * 256 * EL);
+      if constexpr (FP8) {
+        d.ke = *reinterpret_cast<const u32x4*>(a.st.k_exp + kr);
+        d.ve = *reinterpret_cast<const u32x4*>(a.st.v_exp + vr);
+      }
+    };
+    // one step of positions x .. x + KEYS - 1
+    auto step = [&](StepData<FP8>& d, uint32_t x) __attribute__((always_inline)) {
+      f32x4 s[NQ][NT];
+#pragma unroll
+      for (int n = 0; n < NQ; n++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float ks = 1.f;
+        if constexpr (FP8) ks = __uint_as_float(((d.ke[t] >> (8 * (col & 3))) & 0xFFu) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          bf16x8 kf;
+          if constexpr (FP8) kf = fp8_bf16(d.k[2 * t + j / 2][2 * (j & 1)], d.k[2 * t + j / 2][2 * (j & 1) + 1], ks);
+          else kf = __builtin_bit_cast(bf16x8, d.k[4 * t + j]);
+#pragma unroll
+          for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+              s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][j][i], s[n][t], 0, 0, 0);
+        }
+      }
+      // positions of this lane's scores and V: base .. base + 4 NT - 1
+      const uint32_t base = x + g * (KEYS / 4);
+      const bool masked = int32_t(x + KEYS - 1) > free_to || !__all(d.there);
+      bool foul = false;  // V is not finite at a position that only some rows of the tile attend
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (int32_t(base + 4 * t + i) > row_pos[n] || !d.there) s[n][t][i] = -INFINITY;
+        // V at positions no row attends may hold anything: 0 x NaN is NaN
+        const uint32_t ok = d.there && limit > base ? min(limit - base, uint32_t(KEYS / 4)) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          constexpr uint32_t PER = 4 / EL;
+          const uint32_t have = ok > i * PER ? min(ok - i * PER, PER) : 0;
+          const uint32_t bits = have == PER ? ~0u : (1u << (8 * EL * have)) - 1;
+#pragma unroll
+          for (int t = 0; t < 8; t++) d.v[t][i] &= bits;
+          if constexpr (FP8) d.ve[i] &= bits;
+        }
+        if (!one_token) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int t = 0; t < 8; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t u = d.v[t][i];
+              if constexpr (FP8) {
+                const uint32_t z = ~u & 0x7F7F7F7Fu;  // a byte of zeros: NaN
+                any |= (z - 0x01010101u) & ~z & 0x80808080u;
+              } else {
+                any |= uint32_t((u & 0x7F80u) == 0x7F80u) | uint32_t((u & 0x7F800000u) == 0x7F800000u);
+              }
+            }
+          foul = __any(any != 0);
+        }
+      }
+      bf16x8 pf[NQ][NT / 2][NS];
+#pragma unroll
+      for (int n = 0; n < NQ; n++) {
+        float mx = s[n][0][0];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[n][t][i]);
+        mx = fmaxf(m[n], max_groups(mx) * a.c);
+        if (__any(mx > m[n])) {
+          const float f = rebase(m[n], mx);
+          l[n] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) acc[n][i] *= f;
+          m[n] = mx;
+        }
+        const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int u = 0; u < NT / 2; u++) {
+          float e[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float y = exp2_fast(fmaf(s[n][2 * u + i / 4][i & 3], a.c, -ref));
+            l[n] += y;
+            e[i] = y;
+            if constexpr (FP8) e[i] = y == 0.f ? 0.f : y * byte_scale(d.ve[2 * u + i / 4], i & 3);
+          }
+          split_bf16<NS>(e, pf[n][u]);
+        }
+      }
+      if (foul) [[unlikely]] {
+        // token by token, with V cut at the token's position, and only its rows' sums kept
+        for (uint32_t r0 = cu.tile * R; r0 < cu.tile * R + rows; r0 = (r0 / a.group + 1) * a.group) {
+          const int64_t pos = cu.q.first + r0 / a.group;
+          const uint32_t ok = pos >= int64_t(base) ? uint32_t(min(pos + 1 - int64_t(base), int64_t(KEYS / 4))) : 0;
+          u32x4 bits;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            constexpr uint32_t PER = 4 / EL;
+            const uint32_t have = ok > i * PER ? min(ok - i * PER, PER) : 0;
+            bits[i] = have == PER ? ~0u : (1u << (8 * EL * have)) - 1;
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; n++) {
+            const bool mine = (cu.tile * R + 16 * n + col) / a.group == r0 / a.group;
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+              f32x4 z{0.f, 0.f, 0.f, 0.f};
+              const u32x4 v = d.v[t] & bits;
+#pragma unroll
+              for (int u = 0; u < NT / 2; u++) {
+                bf16x8 vf;
+                if constexpr (FP8) vf = fp8_bf16(v[2 * u], v[2 * u + 1], 1.f);
+                else vf = __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+                for (int i = 0; i < NS; i++) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u][i], z, 0, 0, 0);
+              }
+              if (mine) acc[n][t] += z;
+            }
+          }
+        }
+        return;
+      }
+#pragma unroll
+      for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < NT / 2; u++) {
+          bf16x8 vf;
+          if constexpr (FP8) vf = fp8_bf16(d.v[t][2 * u], d.v[t][2 * u + 1], 1.f);
+          else vf = __builtin_bit_cast(bf16x8, d.v[t]);
+#pragma unroll
+          for (int n = 0; n < NQ; n++)
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+              acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u][i], acc[n][t], 0, 0, 0);
+        }
+    };
+
+    uint32_t x = first + wave * KEYS;
+    if (x < last) {
+      StepData<FP8> d0, d1;
+      int32_t kp, vp;
+      look_up(x, kp, vp);
+      load(d0, x, kp, vp);
+      look_up(x + 4 * KEYS, kp, vp);
+      while (true) {
+        // (past the end the loads of a step are of pages that are there, and unused)
+        load(d1, x + 4 * KEYS, kp, vp);
+        look_up(x + 8 * KEYS, kp, vp);
+        step(d0, x);
+        x += 4 * KEYS;
+        if (x >= last) break;
+        load(d0, x + 4 * KEYS, kp, vp);
+        look_up(x + 8 * KEYS, kp, vp);
+        step(d1, x);
+        x += 4 * KEYS;
+        if (x >= last) break;
+      }
+    }
+
+    // the four waves' sums meet in LDS, in wave order
+    __syncthreads();  // the part before has been read
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      const float s = add_groups(l[n]);
+      if (g == 0) {
+        top[wave][16 * n + col] = m[n];
+        mass[wave][16 * n + col] = s;
+      }
+#pragma unroll
+      for (int t = 0; t < 8; t++) *reinterpret_cast<f32x4*>(&sums[wave][16 * n + col][16 * t + 4 * g]) = acc[n][t];
+    }
+    __syncthreads();
+    const bool whole = cu.block == 0 && take == cu.blocks;
+    float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);  // slot 1 begins an item, 0 goes on with one
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+      const uint32_t r = 16 * n + tid / 16, d = (tid % 16) * 8;
+      if (r < rows) {
+        float mx = top[0][r];
+        for (int i = 1; i < 4; i++) mx = fmaxf(mx, top[i][r]);
+        float o[8] = {}, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float f = rebase(top[i][r], mx);
+          sum = fmaf(mass[i][r], f, sum);
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[e] = fmaf(sums[i][r][d + e], f, o[e]);
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[e] *= inv;
+          store_out8<BF16_ROWS>(a.out, row_element(a, cu.q, head, cu.tile * R + r, a.out_stride) + d, o);
+        } else {
+          *reinterpret_cast<f32x4*>(part + r * kPageDim + d) = f32x4{o[0], o[1], o[2], o[3]};
+          *reinterpret_cast<f32x4*>(part + r * kPageDim + d + 4) = f32x4{o[4], o[5], o[6], o[7]};
+          if (d == 0) {
+            part[R * kPageDim + r] = mx;
+            part[R * kPageDim + R + r] = sum;
+          }
+        }
+      }
+    }
+    if (!whole && cu.block == 0 && tid == 0) {
+      const uint64_t end = at + cu.blocks;  // the item's blocks are at .. end - 1
+      a.joints[w] = Joint{uint32_t((end - 1) / per) - w + 1, cu.seq, cu.head, cu.tile};
+    }
+    at += take;
+    if (at >= part_end || !next_tile(a, cu, R)) break;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Joins the parts of the items that more than one workgroup attended: workgroup (w, y) the item whose
+// first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
+// slots 0 of the workgroups after w. With fewer rows than 16 the threads also share the parts.
+// ---------------------------------------------------------------------------------------------
+template <bool BF16_ROWS>
+__global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
+  const uint32_t w = blockIdx.x, tid = threadIdx.x;
+  const Joint j = a.joints[w];
+  if (j.n == 0) return;
+  const Seq q = read_seq(a, j.seq);
+  const uint32_t rows = min(q.rows - j.tile * R, R), r0 = blockIdx.y * 16;
+  if (r0 >= rows) return;
+  const uint32_t here = min(rows - r0, 16u);
+  uint32_t slots = 1;
+  while (slots < here) slots *= 2;  // rows side by side; 16 / slots threads share a row's parts
+  const uint32_t share = 16 / slots, me = tid / 16 / slots, r = r0 + (tid / 16) % slots, d = (tid % 16) * 8;
+  const size_t slot = size_t(R) * kPartRow;
+  const bool real = r < rows;
+  float mx = -INFINITY, sum = 0.f, o[8] = {};
+  if (real) {
+    for (uint32_t i = me; i < j.n; i += share)
+      mx = fmaxf(mx, a.parts[(2 * size_t(w + i) + (i == 0)) * slot + R * kPageDim + r]);
+#pragma unroll 4
+    for (uint32_t i = me; i < j.n; i += share) {
+      const float* part = a.parts + (2 * size_t(w + i) + (i == 0)) * slot;
+      const float f = rebase(part[R * kPageDim + r], mx);
+      const f32x4 u = *reinterpret_cast<const f32x4*>(part + r * kPageDim + d);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(part + r * kPageDim + d + 4);
+      sum = fmaf(part[R * kPageDim + R + r], f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        o[e] = fmaf(u[e], f, o[e]);
+        o[e + 4] = fmaf(v[e], f, o[e + 4]);
+      }
+    }
+  }
+  __shared__ __align__(16) float sums[16][kPageDim];
+  __shared__ float top[16], mass[16];
+  if (share > 1) {  // in order of the shares
+#pragma unroll
+    for (int e = 0; e < 8; e++) sums[tid / 16][d + e] = o[e];
+    if (d == 0) {
+      top[tid / 16] = mx;
+      mass[tid / 16] = sum;
+    }
+    __syncthreads();
+    if (me != 0) return;
+    float all = mx;
+    for (uint32_t i = 1; i < share; i++) all = fmaxf(all, top[tid / 16 + i * slots]);
+    float f = rebase(mx, all);
+    sum *= f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] *= f;
+    for (uint32_t i = 1; i < share; i++) {
+      const uint32_t k = tid / 16 + i * slots;
+      f = rebase(top[k], all);
+      sum = fmaf(mass[k], f, sum);
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = fmaf(sums[k][d + e], f, o[e]);
+    }
+  }
+  if (!real) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 8; e++) o[e] *= inv;
+  store_out8<BF16_ROWS>(a.out, row_element(a, q, j.head, j.tile * R + r, a.out_stride) + d, o);
+}
+
+constexpr uint32_t kWorkgroups = 512;  // two for each CU
 
 }  // namespace
 }  // namespace qe
@@ -87,17 +677,16 @@ extern "C" {
 uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
   (void)max_new;
   if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
-  return 256;
+  return uint64_t(qe::kWorkgroups) * (2 * 32 * qe::kPartRow * 4 + sizeof(qe::Joint));
 }
 
 int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
                          uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work,
                          uint64_t work_bytes, void* stream) {
-  qe::PagePlan p;
-  qe::PageStore st;
-  if (int rc = qe::check_pages(pages, &p, &st)) return rc;
+  qe::AttnArgs a{};
+  if (int rc = qe::check_pages(pages, &a.p, &a.st)) return rc;
   if (dtype != QE_KV_F32 && dtype != QE_KV_BF16) return qe::set_error(QE_ERR_ARG, "rows are QE_KV_F32 or QE_KV_BF16");
-  if (n_heads == 0 || n_heads % p.n_kv || n_heads > 65536)
+  if (n_heads == 0 || n_heads % a.p.n_kv || n_heads > 65536)
     return qe::set_error(QE_ERR_ARG, "n_heads must be a multiple of n_kv_heads, at most 65536");
   if (n_rows == 0) return QE_OK;
   if (!q || !out || !work) return qe::set_error(QE_ERR_ARG, "null argument");
@@ -108,17 +697,35 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
       return qe::set_error(QE_ERR_ARG, "row strides must be at least n_heads * 128 elements and multiples of 16 bytes");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) % 16)
     return qe::set_error(QE_ERR_ARG, "q, out and work must be 16-byte aligned");
-  if (work_bytes < qe_op_page_attention_work_bytes(n_heads, p.n_kv, max_new))
+  if (work_bytes < qe_op_page_attention_work_bytes(n_heads, a.p.n_kv, max_new))
     return qe::set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_page_attention_work_bytes gives",
                          (unsigned long long)work_bytes);
-  const uint32_t grid = qe::ceil_div(uint32_t(n_rows) * uint32_t(n_heads), 4u);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
-  auto* kern = fp8 ? (bf16 ? qe::k_page_attention<true, true> : qe::k_page_attention<true, false>)
-                   : (bf16 ? qe::k_page_attention<false, true> : qe::k_page_attention<false, false>);
-  kern<<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(p, st, static_cast<const uint8_t*>(q),
-                                                           static_cast<uint8_t*>(out), uint32_t(n_rows),
-                                                           uint32_t(n_heads), q_stride, out_stride,
-                                                           1.0f / sqrtf(float(qe::kPageDim)));
+  a.q = static_cast<const uint8_t*>(q);
+  a.out = static_cast<uint8_t*>(out);
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.n_rows = uint32_t(n_rows);
+  a.n_heads = uint32_t(n_heads);
+  a.group = uint32_t(n_heads / a.p.n_kv);
+  a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
+  a.min_blocks = 4;
+  a.joints = static_cast<qe::Joint*>(work);
+  a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
+  const bool two = max_new * a.group > 16;
+  const uint32_t R = two ? 32 : 16, grid = qe::kWorkgroups;
+  auto go = [&](auto* kern) { kern<<<grid, 256, 0, st>>>(a); };
+  if (two) {
+    if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 2> : qe::k_page_attn_rows<true, false, 2>);
+    else go(bf16 ? qe::k_page_attn_rows<false, true, 2> : qe::k_page_attn_rows<false, false, 2>);
+  } else {
+    if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 1> : qe::k_page_attn_rows<true, false, 1>);
+    else go(bf16 ? qe::k_page_attn_rows<false, true, 1> : qe::k_page_attn_rows<false, false, 1>);
+  }
+  const dim3 join(grid, R / 16);
+  if (bf16) qe::k_page_join<true><<<join, 256, 0, st>>>(a, R);
+  else qe::k_page_join<false><<<join, 256, 0, st>>>(a, R);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page attention launch failed: %s", hipGetErrorString(e));
   return QE_OK;
