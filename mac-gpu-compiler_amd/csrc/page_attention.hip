@@ -18,6 +18,7 @@
 #include "pages.h"
 
 #include "device_common.h"
+#include "dma.h"
 #include "status.h"
 
 namespace qe {
@@ -27,6 +28,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kBlock = 64;    // positions
@@ -599,6 +601,338 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 }
 
 // ---------------------------------------------------------------------------------------------
+// Many rows: tiles of 128, 32 for each of the workgroup's four waves, which share blocks of 64
+// positions of K and V through LDS, two blocks deep: while one is multiplied the next is on its way.
+//
+// Bound by the matrix cores: v_mfma_f32_32x32x16_bf16, transposed as above (a lane's 16 results of a
+// score tile are the weights of 8 consecutive positions in two groups of 16, operand B of
+// Out^T = V^T P^T as they stand), against the exponentials and their arithmetic on the vector unit, some
+// 900 cycles a block beside 1024 of products; two workgroups on a CU run one beside the other. f32 rows
+// take three products for one and are alone on a CU.
+// LDS: K [64][128] with the 16-byte piece c of row r at place c ^ (r & 15), V as it lies in memory
+// ([4][128][16]): what the lanes of a product read at once lies in different banks. bf16 pages are
+// loaded straight into it; e4m3 pages go through registers and are widened once for all rows (K with
+// its scale, V's scale is put on the weights). Wave i loads positions 16 i .. 16 i + 15 of a block,
+// which lie in one page.
+// ---------------------------------------------------------------------------------------------
+template <bool FP8, bool BF16_ROWS>
+__global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(AttnArgs a) {
+  constexpr int NS = BF16_ROWS ? 1 : 3, R = 128;
+  constexpr uint32_t TILE = kBlock * kPageDim * 2;  // bytes of K, and of V
+  __shared__ __align__(16) uint8_t buf[2][2 * TILE];
+  __shared__ __align__(16) float vscale[2][FP8 ? kBlock : 4];
+  __shared__ PlanShared sh;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t w = part_index();
+  find_start(a, w, gridDim.x, R, sh);
+  if (tid == 0) a.joints[w].n = 0;
+  if (!sh.found) return;
+  const uint64_t per = sh.per;
+  const uint64_t part_end = min((w + 1) * per, sh.total);
+  uint64_t at = w * per;
+  Cursor cu = sh.at;
+  const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
+  float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
+
+  while (true) {
+    const uint32_t take = uint32_t(min(uint64_t(cu.blocks - cu.block), part_end - at));
+    const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
+    const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
+    const uint32_t head = cu.head;
+    // this wave's rows, and the positions that all of them (free_to) and some of them (end) attend
+    const uint32_t wr0 = cu.tile * R + 32 * wave;
+    const uint32_t wrows = cu.q.rows > wr0 ? min(cu.q.rows - wr0, 32u) : 0;
+    const int64_t free64 = cu.q.first + wr0 / a.group;
+    const int32_t free_to = int32_t(max(min(free64, int64_t(0x7FFFFFFF)), int64_t(-1)));
+    uint32_t end = 0;
+    if (wrows) {
+      const int64_t e = cu.q.first + (wr0 + wrows - 1) / a.group + 1;
+      end = e < 0 ? 0 : uint32_t(min(e, int64_t(limit)));
+    }
+    const bool one_token = wrows == 0 || wr0 / a.group == (wr0 + wrows - 1) / a.group;
+    const uint32_t r = wr0 + col;
+    const bool real = col < wrows;
+    const int64_t pos = cu.q.first + r / a.group;
+    const int32_t row_pos = real ? int32_t(max(min(pos, int64_t(0x7FFFFFFF)), int64_t(-1))) : -1;
+    bf16x8 qf[8][NS];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float x[8] = {};
+      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * half, x);
+      split_bf16<NS>(x, qf[j]);
+    }
+    f32x16 acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[t][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    const int32_t* const table = a.p.table + size_t(cu.seq) * a.p.table_stride;
+    // page of the 16 positions from x on (uniform)
+    auto page_at = [&](uint32_t x) __attribute__((always_inline)) {
+      return table[min(x >> a.p.page_shift, a.p.table_stride - 1)];
+    };
+    auto is_page = [&](int32_t page) __attribute__((always_inline)) { return uint32_t(page) < a.p.n_pages; };
+    u32x4 raw[4];   // e4m3: 32 bytes of a K row, 2 dims of V
+    uint32_t ke = 0, ve = 0;
+    // starts the loads of this wave's 16 positions of the block at x (a page that is not there is read
+    // as page 0, and what comes of it is masked)
+    auto fetch = [&](uint32_t x, uint32_t b, int32_t page) __attribute__((always_inline)) {
+      const uint32_t p0 = x + 16 * wave;
+      const size_t row = page_row(a.p, is_page(page) ? page : 0, head, p0 & ps_mask);
+      if constexpr (FP8) {
+        const u32x4* k = reinterpret_cast<const u32x4*>(a.st.k + row * kPageDim + 32 * lane);
+        const u32x4* v = reinterpret_cast<const u32x4*>(a.st.v + row * kPageDim + 32 * lane);
+        raw[0] = k[0];
+        raw[1] = k[1];
+        raw[2] = v[0];
+        raw[3] = v[1];
+        ke = a.st.k_exp[row + (lane >> 2)];
+        ve = a.st.v_exp[row + (lane & 15)];
+      } else {
+        const uint32_t dst = lds_address(buf[b]) + wave * 4096;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t kr = 4 * i + (lane >> 4), c = (lane & 15) ^ kr;  // row of the 16, piece of the row
+          dma16(dst + i * 1024, a.st.k + (row + kr) * kPageDim * 2 + c * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) dma16(dst + TILE + i * 1024, a.st.v + row * kPageDim * 2 + i * 1024 + lane * 16);
+      }
+    };
+    // e4m3: what fetch loaded, widened, into LDS
+    auto widen = [&](uint32_t b) __attribute__((always_inline)) {
+      if constexpr (FP8) {
+        uint8_t* k = buf[b] + wave * 4096 + (lane >> 2) * 256;
+        uint8_t* v = buf[b] + TILE + wave * 4096 + lane * 64;
+        const float ks = __uint_as_float(ke << 23);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t c = 4 * (lane & 3) + i;
+          *reinterpret_cast<bf16x8*>(k + ((c ^ (lane >> 2)) * 16)) =
+              fp8_bf16(raw[i / 2][2 * (i & 1)], raw[i / 2][2 * (i & 1) + 1], ks);
+          *reinterpret_cast<bf16x8*>(v + 16 * i) =
+              fp8_bf16(raw[2 + i / 2][2 * (i & 1)], raw[2 + i / 2][2 * (i & 1) + 1], 1.f);
+        }
+        if (lane < 16) vscale[b][16 * wave + lane] = __uint_as_float(ve << 23);
+      }
+    };
+    auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {  // dims 32 t + col, positions 16 u + 8 half ..
+      return *reinterpret_cast<const u32x4*>(buf[b] + TILE + u * 4096 + (32 * t + col) * 32 + half * 16);
+    };
+    // words of the 8 positions from base on of which the first `ok` count
+    auto keep = [&](uint32_t ok) __attribute__((always_inline)) {
+      u32x4 bits;
+#pragma unroll
+      for (int i = 0; i < 4; i++) bits[i] = ok >= 2u * i + 2 ? ~0u : ok > 2u * i ? 0xFFFFu : 0u;
+      return bits;
+    };
+    // this wave's rows against the block at x in buffer b; there: which of its four pages are
+    auto multiply = [&](uint32_t x, uint32_t b, uint32_t there) __attribute__((always_inline)) {
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[u][i] = 0.f;
+        // operand A's row `col` is position 32 u + kr of the block
+        const uint32_t kr = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+        const uint8_t* k = buf[b] + (32 * u + kr) * 256;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(k + (((2 * j + half) ^ (kr & 15)) * 16));
+#pragma unroll
+          for (int i = 0; i < NS; i++) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j][i], s[u], 0, 0, 0);
+        }
+      }
+      const bool masked = int32_t(x + kBlock - 1) > free_to || there != 15;
+      bool foul = false;
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int in = 32 * u + 16 * (i >> 3) + 4 * ((i >> 2) & 1) + (i & 3);  // + 8 half
+            if (int32_t(x + in + 8 * half) > row_pos || !(there >> (in / 16) & 1)) s[u][i] = -INFINITY;
+          }
+        if (!one_token) {  // V that is not finite at a position that only some rows attend
+          uint32_t any = 0;
+          for (int u = 0; u < 4; u++) {
+            const uint32_t base = x + 16 * u + 8 * half;
+            const u32x4 bits = keep((there >> u & 1) && limit > base ? limit - base : 0);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+              const u32x4 z = v_part(b, t, u) & bits;
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                any |= uint32_t((z[i] & 0x7F80u) == 0x7F80u) | uint32_t((z[i] & 0x7F800000u) == 0x7F800000u);
+            }
+          }
+          foul = __any(any != 0);
+        }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
+      {
+        const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
+      }
+      mx = fmaxf(m, mx * a.c);
+      if (__any(mx > m)) {
+        const float f = rebase(m, mx);
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[t] *= f;
+        m = mx;
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      bf16x8 pf[4][NS];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        float e[8];
+        f32x4 vs[2];
+        if constexpr (FP8) {
+          vs[0] = *reinterpret_cast<const f32x4*>(&vscale[b][16 * u + 8 * half]);
+          vs[1] = *reinterpret_cast<const f32x4*>(&vscale[b][16 * u + 8 * half + 4]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float y = exp2_fast(fmaf(s[u / 2][8 * (u & 1) + i], a.c, -ref));
+          l += y;
+          e[i] = y;
+          if constexpr (FP8) e[i] *= vs[i / 4][i & 3];
+        }
+        if constexpr (FP8) {
+          if (masked)  // a scale behind the last position may be anything
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              if (s[u / 2][8 * (u & 1) + i] == -INFINITY) e[i] = 0.f;
+        }
+        split_bf16<NS>(e, pf[u]);
+      }
+      if (foul) [[unlikely]] {
+        // token by token, with V cut at the token's position, and only its rows' sums kept
+        for (uint32_t r0 = wr0; r0 < wr0 + wrows; r0 = (r0 / a.group + 1) * a.group) {
+          const int64_t to = min(cu.q.first + r0 / a.group + 1, int64_t(limit));
+          const bool mine = r / a.group == r0 / a.group;
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            f32x16 z;
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[i] = 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+              const int64_t base = int64_t(x) + 16 * u + 8 * half;
+              const u32x4 bits = keep((there >> u & 1) && to > base ? uint32_t(min(to - base, int64_t(8))) : 0);
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u) & bits);
+#pragma unroll
+              for (int i = 0; i < NS; i++) z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], z, 0, 0, 0);
+            }
+            if (mine) acc[t] += z;
+          }
+        }
+        return;
+      }
+      if (masked) {
+        // V at positions no row attends may hold anything: 0 x NaN is NaN
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const uint32_t base = x + 16 * u + 8 * half;
+          const u32x4 bits = keep((there >> u & 1) && limit > base ? limit - base : 0);
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u) & bits);
+#pragma unroll
+            for (int i = 0; i < NS; i++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], acc[t], 0, 0, 0);
+          }
+        }
+        return;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u));
+#pragma unroll
+          for (int i = 0; i < NS; i++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], acc[t], 0, 0, 0);
+        }
+    };
+    auto pages_there = [&](uint32_t x) __attribute__((always_inline)) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) bits |= uint32_t(is_page(page_at(x + 16 * i))) << i;
+      return bits;
+    };
+
+    __syncthreads();  // the buffers' last readers are done
+    if (first < last) {
+      fetch(first, 0, page_at(first + 16 * wave));
+      widen(0);
+      uint32_t b = 0;
+      for (uint32_t x = first; x < last; x += kBlock, b ^= 1) {
+        const uint32_t there = pages_there(x);
+        if constexpr (!FP8) wait_dma<0>();
+        __syncthreads();  // block x is in LDS; the other buffer's readers are done
+        const bool more = x + kBlock < last;
+        if (more) fetch(x + kBlock, b ^ 1, page_at(x + kBlock + 16 * wave));
+        if (x < end) multiply(x, b, there);
+        if (more) widen(b ^ 1);
+      }
+    }
+
+    {
+      const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+      l = __uint_as_float(z[0]) + __uint_as_float(z[1]);
+    }
+    const bool whole = cu.block == 0 && take == cu.blocks;
+    if (whole) {
+      if (real) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint64_t o = row_element(a, cu.q, head, r, a.out_stride) + 4 * half;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const f32x4 v = f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * inv;
+            const uint64_t e = o + 32 * t + 8 * i;
+            if constexpr (BF16_ROWS) {
+              uint2 u;
+              u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2));
+              u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2));
+              *reinterpret_cast<uint2*>(a.out + e * 2) = u;
+            } else {
+              *reinterpret_cast<f32x4*>(a.out + e * 4) = v;
+            }
+          }
+      }
+    } else {
+      float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);
+      if (real) {
+        const uint32_t in = 32 * wave + col;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            *reinterpret_cast<f32x4*>(part + in * kPageDim + 32 * t + 8 * i + 4 * half) =
+                f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+        if (half == 0) {
+          part[R * kPageDim + in] = m;
+          part[R * kPageDim + R + in] = l;
+        }
+      }
+      if (cu.block == 0 && tid == 0)
+        a.joints[w] = Joint{uint32_t((at + cu.blocks - 1) / per) - w + 1, cu.seq, cu.head, cu.tile};
+    }
+    at += take;
+    if (at >= part_end || !next_tile(a, cu, R)) break;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Joins the parts of the items that more than one workgroup attended: workgroup (w, y) the item whose
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
 // slots 0 of the workgroups after w. With fewer rows than 16 the threads also share the parts.
@@ -669,15 +1003,19 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
 
 constexpr uint32_t kWorkgroups = 512;  // two for each CU
 
+// Rows of a tile by the most rows a sequence can have: 16 or 32 with K and V straight from memory, or 128
+// with them shared through LDS.
+uint32_t tile_rows(uint64_t max_rows) { return max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 128; }
+
 }  // namespace
 }  // namespace qe
 
 extern "C" {
 
 uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
-  (void)max_new;
   if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
-  return uint64_t(qe::kWorkgroups) * (2 * 32 * qe::kPartRow * 4 + sizeof(qe::Joint));
+  const uint64_t most = max_new && max_new < 128 ? max_new * (n_heads / n_kv_heads) : 128;
+  return uint64_t(qe::kWorkgroups) * (2 * qe::tile_rows(most) * qe::kPartRow * 4 + sizeof(qe::Joint));
 }
 
 int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
@@ -713,10 +1051,14 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   a.min_blocks = 4;
   a.joints = static_cast<qe::Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
-  const bool two = max_new * a.group > 16;
-  const uint32_t R = two ? 32 : 16, grid = qe::kWorkgroups;
+  const uint64_t most = max_new && max_new < 128 ? max_new * a.group : 128;
+  const uint32_t R = qe::tile_rows(most);
+  const uint32_t grid = R == 128 && !bf16 ? qe::kWorkgroups / 2 : qe::kWorkgroups;
   auto go = [&](auto* kern) { kern<<<grid, 256, 0, st>>>(a); };
-  if (two) {
+  if (R == 128) {
+    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true> : qe::k_page_attn_tiles<true, false>);
+    else go(bf16 ? qe::k_page_attn_tiles<false, true> : qe::k_page_attn_tiles<false, false>);
+  } else if (R == 32) {
     if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 2> : qe::k_page_attn_rows<true, false, 2>);
     else go(bf16 ? qe::k_page_attn_rows<false, true, 2> : qe::k_page_attn_rows<false, false, 2>);
   } else {
