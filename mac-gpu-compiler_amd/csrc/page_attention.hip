@@ -32,6 +32,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kBlock = 64;    // positions
+constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
 struct AttnArgs {
@@ -54,7 +55,7 @@ struct Joint {
 
 // ---- the plan of a sequence: its rows and how far each tile's positions go ----
 struct Seq {
-  int64_t first;   // position of its first row (may be negative)
+  int32_t first;   // position of its first row (may be negative: such rows attend nothing)
   int32_t row0;    // first packed row
   uint32_t rows;   // new tokens * group
   __device__ uint32_t tiles(uint32_t R) const { return (rows + R - 1) / R; }
@@ -66,15 +67,23 @@ __device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
   Seq q;
   q.row0 = int32_t(lo);
   q.rows = hi > lo ? uint32_t(hi - lo) * a.group : 0;
-  q.first = int64_t(a.p.lens[s]) - (e - lo);
+  // its last row is at lens[s] - 1 < 2^31; below -2^31 every row is at a negative position
+  const int64_t first = int64_t(a.p.lens[s]) - (e - lo);
+  q.first = int32_t(first > -0x80000000ll ? first : -0x80000000ll);
   return q;
 }
 
-// Positions that some row of the tile attends: 0 .. limit - 1 (within the table).
+// Position of row r of a sequence's rows.
+__device__ __forceinline__ int32_t row_position(const AttnArgs& a, const Seq& q, uint32_t r) {
+  return q.first + int32_t(r / a.group);
+}
+// Positions that rows up to r attend: 0 .. limit - 1 (within the table).
+__device__ __forceinline__ uint32_t row_limit(const AttnArgs& a, const Seq& q, uint32_t r) {
+  const int32_t pos = row_position(a, q, r);
+  return pos < 0 ? 0 : min(uint32_t(pos) + 1, a.p.table_stride << a.p.page_shift);
+}
 __device__ __forceinline__ uint32_t tile_limit(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
-  const uint32_t last = min((tile + 1) * R, q.rows) - 1;
-  const int64_t end = q.first + last / a.group + 1, cap = capacity_of(a.p);
-  return end < 0 ? 0 : uint32_t(end < cap ? end : cap);
+  return row_limit(a, q, min((tile + 1) * R, q.rows) - 1);
 }
 // A tile that attends nothing still counts one block: its rows are zeros that someone writes.
 __device__ __forceinline__ uint32_t tile_blocks(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
@@ -94,9 +103,9 @@ struct Cursor {
 
 struct PlanShared {
   uint64_t sum[256];
-  uint64_t per, total;
-  Cursor at;
-  uint32_t found;
+  uint32_t per;   // blocks of a workgroup
+  uint32_t mine;  // of this one: fewer for the last, 0 behind it
+  Cursor at;      // where they start
 };
 
 // The next tile with rows after `cu`'s (false: there is none).
@@ -116,7 +125,8 @@ __device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_
   return true;
 }
 
-// Block `at` = w * per of the list (per: the blocks of one of W workgroups): fills sh.at and sh.found.
+// Workgroup w's part of the list, of W parts of `per` blocks, into sh. (A part is far below 2^32 blocks:
+// that many are 70 TB of K and V.)
 // Each thread sums a contiguous range of sequences; the one whose range holds the block walks it.
 __device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh) {
   const uint32_t t = threadIdx.x, each = (a.p.n_seqs + 255) / 256;
@@ -124,7 +134,6 @@ __device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R
   uint64_t mine = 0;
   for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
   mine *= a.p.n_kv;
-  if (t == 0) sh.found = 0;
   sh.sum[t] = mine;
   __syncthreads();
   for (uint32_t d = 1; d < 256; d *= 2) {
@@ -135,11 +144,11 @@ __device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R
   }
   const uint64_t total = sh.sum[255];
   const uint64_t even = (total + W - 1) / W, per = even > a.min_blocks ? even : a.min_blocks;
-  if (t == 0) {
-    sh.per = per;
-    sh.total = total;
-  }
   const uint64_t at = w * per;
+  if (t == 0) {
+    sh.per = uint32_t(per);
+    sh.mine = at < total ? uint32_t(min(per, total - at)) : 0;
+  }
   uint64_t before = sh.sum[t] - mine;
   if (at >= before && at < sh.sum[t]) {
     Cursor cu;
@@ -161,9 +170,24 @@ __device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R
       before += one * a.p.n_kv;
     }
     sh.at = cu;
-    sh.found = 1;
   }
   __syncthreads();
+}
+
+// A value that all lanes hold, in a scalar register: what comes out of LDS would stay in vector
+// registers, and everything worked out from it with it.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Cursor uniform(const Cursor& c) {
+  Cursor u;
+  u.q.first = int32_t(uniform(uint32_t(c.q.first)));
+  u.q.row0 = int32_t(uniform(uint32_t(c.q.row0)));
+  u.q.rows = uniform(c.q.rows);
+  u.seq = uniform(c.seq);
+  u.head = uniform(c.head);
+  u.tile = uniform(c.tile);
+  u.block = uniform(c.block);
+  u.blocks = uniform(c.blocks);
+  return u;
 }
 
 // a workgroup's place in the list: consecutive parts on one XCD (workgroups go to the 8 XCDs in turn)
@@ -241,6 +265,26 @@ __device__ __forceinline__ float byte_scale(uint32_t w, int i) {  // 2^(e - 127)
   return __uint_as_float((i == 3 ? w >> 1 : w << (23 - 8 * i)) & 0x7F800000u);
 }
 
+// Clears the values of two bf16 (e4m3: four) that are not finite and says whether there were any.
+template <bool FP8>
+__device__ __forceinline__ uint32_t clear_foul(uint32_t& u) {
+  uint32_t bad;
+  if constexpr (FP8) {
+    bad = (((u & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;  // bytes 0x7F and 0xFF, as 1 each
+    u &= ~(bad * 0xFFu);
+  } else {
+    bad = ((u & 0x7F80u) == 0x7F80u ? 1u : 0u) | ((u & 0x7F800000u) == 0x7F800000u ? 0x10000u : 0u);
+    u &= ~(bad * 0xFFFFu);
+  }
+  return bad;
+}
+// Element i of V as a float (without its scale).
+template <bool FP8>
+__device__ __forceinline__ float v_value(const uint8_t* v, size_t i) {
+  if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(v[i], 0);
+  else return bf16f(reinterpret_cast<const uint16_t*>(v)[i]);
+}
+
 // 8 values of a row of q as floats
 template <bool BF16_ROWS>
 __device__ __forceinline__ void load_q8(const uint8_t* q, uint64_t element, float (&x)[8]) {
@@ -311,24 +355,22 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
   const uint32_t w = part_index();
   find_start(a, w, gridDim.x, R, sh);
   if (tid == 0) a.joints[w].n = 0;
-  if (!sh.found) return;
-  const uint64_t per = sh.per;
-  const uint64_t part_end = min((w + 1) * per, sh.total);
-  uint64_t at = w * per;
-  Cursor cu = sh.at;
+  uint32_t left = uniform(sh.mine);
+  if (left == 0) return;
+  const uint32_t per = uniform(sh.per), whole_part = left;
+  Cursor cu = uniform(sh.at);
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
   float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
 
   while (true) {
-    const uint32_t take = uint32_t(min(uint64_t(cu.blocks - cu.block), part_end - at));
+    const uint32_t take = min(cu.blocks - cu.block, left);
     const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
     const uint32_t rows = min(cu.q.rows - cu.tile * R, uint32_t(R));
     // the positions of this part, in steps
     const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // the least position any row attends up to: below it no score is masked
-    const int64_t free64 = cu.q.first + (cu.tile * R) / a.group;
-    const int32_t free_to = int32_t(max(min(free64, int64_t(0x7FFFFFFF)), int64_t(-1)));
+    const int32_t free_to = row_position(a, cu.q, cu.tile * R);
     const bool one_token = (cu.tile * R) / a.group == (cu.tile * R + rows - 1) / a.group;
     int32_t row_pos[NQ];
     bf16x8 qf[NQ][4][NS];
@@ -336,8 +378,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     for (int n = 0; n < NQ; n++) {
       const uint32_t r = cu.tile * R + 16 * n + col;
       const bool real = r < cu.q.rows;
-      const int64_t pos = cu.q.first + r / a.group;
-      row_pos[n] = real ? int32_t(max(min(pos, int64_t(0x7FFFFFFF)), int64_t(-1))) : -1;
+      row_pos[n] = real ? row_position(a, cu.q, r) : -1;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const uint32_t d = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
@@ -384,6 +425,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
         d.ve = *reinterpret_cast<const u32x4*>(a.st.v_exp + vr);
       }
     };
+    uint32_t foul_from = kNowhere;  // the first step that cleared something
     // one step of positions x .. x + KEYS - 1
     auto step = [&](StepData<FP8>& d, uint32_t x) __attribute__((always_inline)) {
       f32x4 s[NQ][NT];
@@ -410,7 +452,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
       // positions of this lane's scores and V: base .. base + 4 NT - 1
       const uint32_t base = x + g * (KEYS / 4);
       const bool masked = int32_t(x + KEYS - 1) > free_to || !__all(d.there);
-      bool foul = false;  // V is not finite at a position that only some rows of the tile attend
+      uint32_t foul = 0;  // V is not finite at a position that only some rows of the tile attend
       if (masked) {
 #pragma unroll
         for (int n = 0; n < NQ; n++)
@@ -431,20 +473,14 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
           if constexpr (FP8) d.ve[i] &= bits;
         }
         if (!one_token) {
-          uint32_t any = 0;
 #pragma unroll
           for (int t = 0; t < 8; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const uint32_t u = d.v[t][i];
-              if constexpr (FP8) {
-                const uint32_t z = ~u & 0x7F7F7F7Fu;  // a byte of zeros: NaN
-                any |= (z - 0x01010101u) & ~z & 0x80808080u;
-              } else {
-                any |= uint32_t((u & 0x7F80u) == 0x7F80u) | uint32_t((u & 0x7F800000u) == 0x7F800000u);
-              }
+              uint32_t u = d.v[t][i];
+              foul |= clear_foul<FP8>(u);
+              d.v[t][i] = u;
             }
-          foul = __any(any != 0);
         }
       }
       bf16x8 pf[NQ][NT / 2][NS];
@@ -477,39 +513,6 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
           split_bf16<NS>(e, pf[n][u]);
         }
       }
-      if (foul) [[unlikely]] {
-        // token by token, with V cut at the token's position, and only its rows' sums kept
-        for (uint32_t r0 = cu.tile * R; r0 < cu.tile * R + rows; r0 = (r0 / a.group + 1) * a.group) {
-          const int64_t pos = cu.q.first + r0 / a.group;
-          const uint32_t ok = pos >= int64_t(base) ? uint32_t(min(pos + 1 - int64_t(base), int64_t(KEYS / 4))) : 0;
-          u32x4 bits;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            constexpr uint32_t PER = 4 / EL;
-            const uint32_t have = ok > i * PER ? min(ok - i * PER, PER) : 0;
-            bits[i] = have == PER ? ~0u : (1u << (8 * EL * have)) - 1;
-          }
-#pragma unroll
-          for (int n = 0; n < NQ; n++) {
-            const bool mine = (cu.tile * R + 16 * n + col) / a.group == r0 / a.group;
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-              f32x4 z{0.f, 0.f, 0.f, 0.f};
-              const u32x4 v = d.v[t] & bits;
-#pragma unroll
-              for (int u = 0; u < NT / 2; u++) {
-                bf16x8 vf;
-                if constexpr (FP8) vf = fp8_bf16(v[2 * u], v[2 * u + 1], 1.f);
-                else vf = __builtin_bit_cast(bf16x8, v);
-#pragma unroll
-                for (int i = 0; i < NS; i++) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u][i], z, 0, 0, 0);
-              }
-              if (mine) acc[n][t] += z;
-            }
-          }
-        }
-        return;
-      }
 #pragma unroll
       for (int t = 0; t < 8; t++)
 #pragma unroll
@@ -523,6 +526,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
             for (int i = 0; i < NS; i++)
               acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u][i], acc[n][t], 0, 0, 0);
         }
+      if (foul_from == kNowhere && __any(foul != 0)) foul_from = x;
     };
 
     uint32_t x = first + wave * KEYS;
@@ -544,6 +548,25 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
         step(d1, x);
         x += 4 * KEYS;
         if (x >= last) break;
+      }
+    }
+
+    // what was cleared, to the rows that attend it: infinity and NaN stay what they are under a weight
+    for (uint32_t y = foul_from; y < last; y += 4 * KEYS) {
+      for (uint32_t j = y; j < min(y + KEYS, limit); j++) {
+        const int32_t page = table[j >> a.p.page_shift];
+        if (uint32_t(page) >= a.p.n_pages) continue;
+        const size_t e = v_element(a.p, page, head, j & ps_mask);
+#pragma unroll
+        for (int t = 0; t < 8; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float v = v_value<FP8>(a.st.v, e + 16 * (16 * t + 4 * g + i));
+            if (!(fabsf(v) < INFINITY))
+#pragma unroll
+              for (int n = 0; n < NQ; n++)
+                if (int32_t(j) <= row_pos[n]) acc[n][t][i] += v;
+          }
       }
     }
 
@@ -591,12 +614,10 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
         }
       }
     }
-    if (!whole && cu.block == 0 && tid == 0) {
-      const uint64_t end = at + cu.blocks;  // the item's blocks are at .. end - 1
-      a.joints[w] = Joint{uint32_t((end - 1) / per) - w + 1, cu.seq, cu.head, cu.tile};
-    }
-    at += take;
-    if (at >= part_end || !next_tile(a, cu, R)) break;
+    if (!whole && cu.block == 0 && tid == 0)  // the item's last block is in the part (...) / per after this one
+      a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
+    left -= take;
+    if (left == 0 || !next_tile(a, cu, R)) break;
   }
 }
 
@@ -621,40 +642,34 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
   constexpr uint32_t TILE = kBlock * kPageDim * 2;  // bytes of K, and of V
   __shared__ __align__(16) uint8_t buf[2][2 * TILE];
   __shared__ __align__(16) float vscale[2][FP8 ? kBlock : 4];
+  __shared__ uint32_t foul[2];
   __shared__ PlanShared sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t w = part_index();
   find_start(a, w, gridDim.x, R, sh);
   if (tid == 0) a.joints[w].n = 0;
-  if (!sh.found) return;
-  const uint64_t per = sh.per;
-  const uint64_t part_end = min((w + 1) * per, sh.total);
-  uint64_t at = w * per;
-  Cursor cu = sh.at;
+  uint32_t left = uniform(sh.mine);
+  if (left == 0) return;
+  const uint32_t per = uniform(sh.per), whole_part = left;
+  Cursor cu = uniform(sh.at);
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
   float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
 
   while (true) {
-    const uint32_t take = uint32_t(min(uint64_t(cu.blocks - cu.block), part_end - at));
+    const uint32_t take = min(cu.blocks - cu.block, left);
     const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
     const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // this wave's rows, and the positions that all of them (free_to) and some of them (end) attend
     const uint32_t wr0 = cu.tile * R + 32 * wave;
     const uint32_t wrows = cu.q.rows > wr0 ? min(cu.q.rows - wr0, 32u) : 0;
-    const int64_t free64 = cu.q.first + wr0 / a.group;
-    const int32_t free_to = int32_t(max(min(free64, int64_t(0x7FFFFFFF)), int64_t(-1)));
-    uint32_t end = 0;
-    if (wrows) {
-      const int64_t e = cu.q.first + (wr0 + wrows - 1) / a.group + 1;
-      end = e < 0 ? 0 : uint32_t(min(e, int64_t(limit)));
-    }
-    const bool one_token = wrows == 0 || wr0 / a.group == (wr0 + wrows - 1) / a.group;
+    const int32_t free_to = row_position(a, cu.q, wr0);
+    const uint32_t end = wrows ? row_limit(a, cu.q, wr0 + wrows - 1) : 0;
+    const int32_t tile_free = row_position(a, cu.q, cu.tile * R);  // all rows of the tile attend up to it
     const uint32_t r = wr0 + col;
     const bool real = col < wrows;
-    const int64_t pos = cu.q.first + r / a.group;
-    const int32_t row_pos = real ? int32_t(max(min(pos, int64_t(0x7FFFFFFF)), int64_t(-1))) : -1;
+    const int32_t row_pos = real ? row_position(a, cu.q, r) : -1;
     bf16x8 qf[8][NS];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -722,32 +737,64 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
     auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {  // dims 32 t + col, positions 16 u + 8 half ..
       return *reinterpret_cast<const u32x4*>(buf[b] + TILE + u * 4096 + (32 * t + col) * 32 + half * 16);
     };
-    // words of the 8 positions from base on of which the first `ok` count
-    auto keep = [&](uint32_t ok) __attribute__((always_inline)) {
-      u32x4 bits;
+    // V of the block in buffer b as every row may multiply it: zeros at positions that no row of the tile
+    // attends, which may hold anything (0 x NaN is NaN), and where it is not finite at one that only some
+    // attend (`foul`: those get it in multiply). Each wave clears its 16 positions.
+    auto clear = [&](uint32_t x, uint32_t b, bool page) __attribute__((always_inline)) {
+      // lane: positions 8 (lane & 1) .. + 7 of the 16 at dims lane / 2, lane / 2 + 32, ...
+      const uint32_t base = x + 16 * wave + 8 * (lane & 1), ok = page && limit > base ? limit - base : 0;
+      uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) bits[i] = ok >= 2u * i + 2 ? ~0u : ok > 2u * i ? 0xFFFFu : 0u;
-      return bits;
+      for (int i = 0; i < 4; i++) {
+        u32x4* v = reinterpret_cast<u32x4*>(buf[b] + TILE + wave * 4096 + i * 1024 + lane * 16);
+        u32x4 u = *v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          uint32_t z = u[k] & (ok >= 2u * k + 2 ? ~0u : ok > 2u * k ? 0xFFFFu : 0u);
+          any |= clear_foul<false>(z);
+          u[k] = z;
+        }
+        *v = u;
+      }
+      if (any) foul[b] = 1;
+      // (scales behind the last position may be anything too)
+      if constexpr (FP8)
+        if (lane < 16 && !(page && x + 16 * wave + lane < limit)) vscale[b][16 * wave + lane] = 0.f;
     };
+    uint32_t foul_from = kNowhere;  // the first block that `clear` cleared something of
     // this wave's rows against the block at x in buffer b; there: which of its four pages are
     auto multiply = [&](uint32_t x, uint32_t b, uint32_t there) __attribute__((always_inline)) {
+      // Fragments come from LDS four at a time, a group ahead of the products that use them; the scheduling
+      // barriers keep it so (left alone the compiler waits for every read right behind it).
       f32x16 s[2];
+      bf16x8 kf[2][4];
+      // operand A's row `col` is position 32 u + kr of the block
+      const uint32_t kr = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+      auto k_part = [&](int n) __attribute__((always_inline)) {  // fragment n: rows 32 (n / 8) .., dims 16 (n % 8) ..
+        return *reinterpret_cast<const bf16x8*>(buf[b] + (32 * (n / 8) + kr) * 256 +
+                                                (((2 * (n % 8) + half) ^ (kr & 15)) * 16));
+      };
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int n = 0; n < 4; n++) kf[0][n] = k_part(n);
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[u][i] = 0.f;
-        // operand A's row `col` is position 32 u + kr of the block
-        const uint32_t kr = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
-        const uint8_t* k = buf[b] + (32 * u + kr) * 256;
+      for (int o = 0; o < 4; o++) {
+        if (o < 3)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(k + (((2 * j + half) ^ (kr & 15)) * 16));
+          for (int n = 0; n < 4; n++) kf[(o + 1) & 1][n] = k_part(4 * o + 4 + n);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < NS; i++) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j][i], s[u], 0, 0, 0);
+        for (int n = 0; n < 4; n++) {
+          const int u = o / 2, j = 4 * (o & 1) + n;
+          if (j == 0)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[u][i] = 0.f;
+#pragma unroll
+          for (int i = 0; i < NS; i++)
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[o & 1][n], qf[j][i], s[u], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       const bool masked = int32_t(x + kBlock - 1) > free_to || there != 15;
-      bool foul = false;
       if (masked) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -756,21 +803,6 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
             const int in = 32 * u + 16 * (i >> 3) + 4 * ((i >> 2) & 1) + (i & 3);  // + 8 half
             if (int32_t(x + in + 8 * half) > row_pos || !(there >> (in / 16) & 1)) s[u][i] = -INFINITY;
           }
-        if (!one_token) {  // V that is not finite at a position that only some rows attend
-          uint32_t any = 0;
-          for (int u = 0; u < 4; u++) {
-            const uint32_t base = x + 16 * u + 8 * half;
-            const u32x4 bits = keep((there >> u & 1) && limit > base ? limit - base : 0);
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-              const u32x4 z = v_part(b, t, u) & bits;
-#pragma unroll
-              for (int i = 0; i < 4; i++)
-                any |= uint32_t((z[i] & 0x7F80u) == 0x7F80u) | uint32_t((z[i] & 0x7F800000u) == 0x7F800000u);
-            }
-          }
-          foul = __any(any != 0);
-        }
       }
       float mx = s[0][0];
 #pragma unroll
@@ -790,9 +822,10 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
         m = mx;
       }
       const float ref = mx == -INFINITY ? 0.f : mx;
-      bf16x8 pf[4][NS];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
+      bf16x8 pf[2][NS];
+      bf16x8 vf[2][4];
+      // weights of positions 16 u + 8 half ..
+      auto weights = [&](int u, bf16x8 (&o)[NS]) __attribute__((always_inline)) {
         float e[8];
         f32x4 vs[2];
         if constexpr (FP8) {
@@ -806,60 +839,26 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
           e[i] = y;
           if constexpr (FP8) e[i] *= vs[i / 4][i & 3];
         }
-        if constexpr (FP8) {
-          if (masked)  // a scale behind the last position may be anything
+        split_bf16<NS>(e, o);
+      };
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-              if (s[u / 2][8 * (u & 1) + i] == -INFINITY) e[i] = 0.f;
-        }
-        split_bf16<NS>(e, pf[u]);
+      for (int t = 0; t < 4; t++) vf[0][t] = __builtin_bit_cast(bf16x8, v_part(b, t, 0));
+      weights(0, pf[0]);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        if (u < 3)
+#pragma unroll
+          for (int t = 0; t < 4; t++) vf[(u + 1) & 1][t] = __builtin_bit_cast(bf16x8, v_part(b, t, u + 1));
+        __builtin_amdgcn_sched_barrier(0);
+        // products of these positions beside the next ones' weights
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+          for (int i = 0; i < NS; i++)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u & 1][t], pf[u & 1][i], acc[t], 0, 0, 0);
+        if (u < 3) weights(u + 1, pf[(u + 1) & 1]);
       }
-      if (foul) [[unlikely]] {
-        // token by token, with V cut at the token's position, and only its rows' sums kept
-        for (uint32_t r0 = wr0; r0 < wr0 + wrows; r0 = (r0 / a.group + 1) * a.group) {
-          const int64_t to = min(cu.q.first + r0 / a.group + 1, int64_t(limit));
-          const bool mine = r / a.group == r0 / a.group;
-#pragma unroll
-          for (int t = 0; t < 4; t++) {
-            f32x16 z;
-#pragma unroll
-            for (int i = 0; i < 16; i++) z[i] = 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-              const int64_t base = int64_t(x) + 16 * u + 8 * half;
-              const u32x4 bits = keep((there >> u & 1) && to > base ? uint32_t(min(to - base, int64_t(8))) : 0);
-              const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u) & bits);
-#pragma unroll
-              for (int i = 0; i < NS; i++) z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], z, 0, 0, 0);
-            }
-            if (mine) acc[t] += z;
-          }
-        }
-        return;
-      }
-      if (masked) {
-        // V at positions no row attends may hold anything: 0 x NaN is NaN
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const uint32_t base = x + 16 * u + 8 * half;
-          const u32x4 bits = keep((there >> u & 1) && limit > base ? limit - base : 0);
-#pragma unroll
-          for (int t = 0; t < 4; t++) {
-            const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u) & bits);
-#pragma unroll
-            for (int i = 0; i < NS; i++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], acc[t], 0, 0, 0);
-          }
-        }
-        return;
-      }
-#pragma unroll
-      for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, v_part(b, t, u));
-#pragma unroll
-          for (int i = 0; i < NS; i++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][i], acc[t], 0, 0, 0);
-        }
+      if (masked && foul_from == kNowhere && uniform(foul[b]) != 0) foul_from = x;
     };
     auto pages_there = [&](uint32_t x) __attribute__((always_inline)) {
       uint32_t bits = 0;
@@ -872,18 +871,37 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
     if (first < last) {
       fetch(first, 0, page_at(first + 16 * wave));
       widen(0);
+      if (tid == 0) foul[0] = 0;
       uint32_t b = 0;
       for (uint32_t x = first; x < last; x += kBlock, b ^= 1) {
         const uint32_t there = pages_there(x);
         if constexpr (!FP8) wait_dma<0>();
         __syncthreads();  // block x is in LDS; the other buffer's readers are done
+        if (int32_t(x + kBlock - 1) > tile_free || there != 15) {
+          clear(x, b, there >> wave & 1);
+          __syncthreads();
+        }
         const bool more = x + kBlock < last;
         if (more) fetch(x + kBlock, b ^ 1, page_at(x + kBlock + 16 * wave));
         if (x < end) multiply(x, b, there);
         if (more) widen(b ^ 1);
+        if (tid == 0) foul[b ^ 1] = 0;  // (its last readers are done; its next writers come after a barrier)
       }
     }
 
+    // what was cleared, to the rows that attend it: infinity and NaN stay what they are under a weight
+    for (uint32_t j = foul_from; j < min(last, end); j++) {
+      const int32_t page = page_at(j);
+      if (!is_page(page)) continue;
+      const size_t e = v_element(a.p, page, head, j & ps_mask);
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float v = v_value<FP8>(a.st.v, e + 16 * (32 * t + 8 * (i / 4) + 4 * half + (i & 3)));
+          if (!(fabsf(v) < INFINITY) && int32_t(j) <= row_pos) acc[t][i] += v;
+        }
+    }
     {
       const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
       l = __uint_as_float(z[0]) + __uint_as_float(z[1]);
@@ -925,10 +943,10 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
         }
       }
       if (cu.block == 0 && tid == 0)
-        a.joints[w] = Joint{uint32_t((at + cu.blocks - 1) / per) - w + 1, cu.seq, cu.head, cu.tile};
+        a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
     }
-    at += take;
-    if (at >= part_end || !next_tile(a, cu, R)) break;
+    left -= take;
+    if (left == 0 || !next_tile(a, cu, R)) break;
   }
 }
 
