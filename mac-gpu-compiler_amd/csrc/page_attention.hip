@@ -685,9 +685,10 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
     float m = -INFINITY, l = 0.f;
 
     const int32_t* const table = a.p.table + size_t(cu.seq) * a.p.table_stride;
-    // page of the 16 positions from x on (uniform)
+    // page of the 16 positions from x on, by a scalar load (the plan does not change while a call runs)
     auto page_at = [&](uint32_t x) __attribute__((always_inline)) {
-      return table[min(x >> a.p.page_shift, a.p.table_stride - 1)];
+      const uint32_t i = min(x >> a.p.page_shift, a.p.table_stride - 1);
+      return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(table))[i];
     };
     auto is_page = [&](int32_t page) __attribute__((always_inline)) { return uint32_t(page) < a.p.n_pages; };
     u32x4 raw[4];   // e4m3: 32 bytes of a K row, 2 dims of V
@@ -860,6 +861,7 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       }
       if (masked && foul_from == kNowhere && uniform(foul[b]) != 0) foul_from = x;
     };
+    // which of a block's four runs of 16 positions have a page
     auto pages_there = [&](uint32_t x) __attribute__((always_inline)) {
       uint32_t bits = 0;
 #pragma unroll
@@ -872,9 +874,9 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       fetch(first, 0, page_at(first + 16 * wave));
       widen(0);
       if (tid == 0) foul[0] = 0;
-      uint32_t b = 0;
+      uint32_t b = 0, there = pages_there(first);
+      int32_t page = page_at(first + kBlock + 16 * wave);  // of this wave's part of the next block
       for (uint32_t x = first; x < last; x += kBlock, b ^= 1) {
-        const uint32_t there = pages_there(x);
         if constexpr (!FP8) wait_dma<0>();
         __syncthreads();  // block x is in LDS; the other buffer's readers are done
         if (int32_t(x + kBlock - 1) > tile_free || there != 15) {
@@ -882,10 +884,13 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
           __syncthreads();
         }
         const bool more = x + kBlock < last;
-        if (more) fetch(x + kBlock, b ^ 1, page_at(x + kBlock + 16 * wave));
+        if (more) fetch(x + kBlock, b ^ 1, page);
+        const uint32_t there_next = pages_there(x + kBlock);
+        page = page_at(x + 2 * kBlock + 16 * wave);
         if (x < end) multiply(x, b, there);
         if (more) widen(b ^ 1);
         if (tid == 0) foul[b ^ 1] = 0;  // (its last readers are done; its next writers come after a barrier)
+        there = there_next;
       }
     }
 
