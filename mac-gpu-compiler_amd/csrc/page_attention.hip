@@ -32,6 +32,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kBlock = 64;    // positions
+// Weights are 2^(score - m) with m the largest score so far, or up to kSlack below it: sums are only put
+// on a new m when a score exceeds it by that much (in some row of 32 one is a little larger in most blocks).
+constexpr float kSlack = 8.f;
 constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
@@ -492,14 +495,14 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 #pragma unroll
           for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[n][t][i]);
         mx = fmaxf(m[n], max_groups(mx) * a.c);
-        if (__any(mx > m[n])) {
+        if (__any(mx > m[n] + kSlack)) {
           const float f = rebase(m[n], mx);
           l[n] *= f;
 #pragma unroll
           for (int i = 0; i < 8; i++) acc[n][i] *= f;
           m[n] = mx;
         }
-        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
         for (int u = 0; u < NT / 2; u++) {
           float e[8];
@@ -631,7 +634,8 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 // 900 cycles a block beside 1024 of products; two workgroups on a CU run one beside the other. f32 rows
 // take three products for one and are alone on a CU.
 // LDS: K [64][128] with the 16-byte piece c of row r at place c ^ (r & 15), V as it lies in memory
-// ([4][128][16]): what the lanes of a product read at once lies in different banks. bf16 pages are
+// ([4][128][16]) with the two pieces of every second 8 dims exchanged: what 16 lanes read at once lies in
+// different banks. bf16 pages are
 // loaded straight into it; e4m3 pages go through registers and are widened once for all rows (K with
 // its scale, V's scale is put on the weights). Wave i loads positions 16 i .. 16 i + 15 of a block,
 // which lie in one page.
@@ -691,7 +695,7 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(table))[i];
     };
     auto is_page = [&](int32_t page) __attribute__((always_inline)) { return uint32_t(page) < a.p.n_pages; };
-    u32x4 raw[4];   // e4m3: 32 bytes of a K row, 2 dims of V
+    u32x4 raw[4];   // e4m3: 32 bytes of a K row; dims `lane` and lane + 64 of V
     uint32_t ke = 0, ve = 0;
     // starts the loads of this wave's 16 positions of the block at x (a page that is not there is read
     // as page 0, and what comes of it is masked)
@@ -700,11 +704,11 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       const size_t row = page_row(a.p, is_page(page) ? page : 0, head, p0 & ps_mask);
       if constexpr (FP8) {
         const u32x4* k = reinterpret_cast<const u32x4*>(a.st.k + row * kPageDim + 32 * lane);
-        const u32x4* v = reinterpret_cast<const u32x4*>(a.st.v + row * kPageDim + 32 * lane);
+        const u32x4* v = reinterpret_cast<const u32x4*>(a.st.v + row * kPageDim + 16 * lane);
         raw[0] = k[0];
         raw[1] = k[1];
         raw[2] = v[0];
-        raw[3] = v[1];
+        raw[3] = v[64];
         ke = a.st.k_exp[row + (lane >> 2)];
         ve = a.st.v_exp[row + (lane & 15)];
       } else {
@@ -715,35 +719,36 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
           dma16(dst + i * 1024, a.st.k + (row + kr) * kPageDim * 2 + c * 16);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) dma16(dst + TILE + i * 1024, a.st.v + row * kPageDim * 2 + i * 1024 + lane * 16);
+        for (int i = 0; i < 4; i++)
+          dma16(dst + TILE + i * 1024, a.st.v + row * kPageDim * 2 + i * 1024 + (lane ^ (lane >> 4 & 1)) * 16);
       }
     };
     // e4m3: what fetch loaded, widened, into LDS
     auto widen = [&](uint32_t b) __attribute__((always_inline)) {
       if constexpr (FP8) {
         uint8_t* k = buf[b] + wave * 4096 + (lane >> 2) * 256;
-        uint8_t* v = buf[b] + TILE + wave * 4096 + lane * 64;
+        uint8_t* v = buf[b] + TILE + wave * 4096 + lane * 32;
         const float ks = __uint_as_float(ke << 23);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const uint32_t c = 4 * (lane & 3) + i;
           *reinterpret_cast<bf16x8*>(k + ((c ^ (lane >> 2)) * 16)) =
               fp8_bf16(raw[i / 2][2 * (i & 1)], raw[i / 2][2 * (i & 1) + 1], ks);
-          *reinterpret_cast<bf16x8*>(v + 16 * i) =
+          *reinterpret_cast<bf16x8*>(v + (i / 2) * 2048 + (((i & 1) ^ (lane >> 3 & 1)) * 16)) =
               fp8_bf16(raw[2 + i / 2][2 * (i & 1)], raw[2 + i / 2][2 * (i & 1) + 1], 1.f);
         }
         if (lane < 16) vscale[b][16 * wave + lane] = __uint_as_float(ve << 23);
       }
     };
     auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {  // dims 32 t + col, positions 16 u + 8 half ..
-      return *reinterpret_cast<const u32x4*>(buf[b] + TILE + u * 4096 + (32 * t + col) * 32 + half * 16);
+      return *reinterpret_cast<const u32x4*>(buf[b] + TILE + u * 4096 + (32 * t + col) * 32 + (half ^ (col >> 3 & 1)) * 16);
     };
     // V of the block in buffer b as every row may multiply it: zeros at positions that no row of the tile
     // attends, which may hold anything (0 x NaN is NaN), and where it is not finite at one that only some
     // attend (`foul`: those get it in multiply). Each wave clears its 16 positions.
     auto clear = [&](uint32_t x, uint32_t b, bool page) __attribute__((always_inline)) {
-      // lane: positions 8 (lane & 1) .. + 7 of the 16 at dims lane / 2, lane / 2 + 32, ...
-      const uint32_t base = x + 16 * wave + 8 * (lane & 1), ok = page && limit > base ? limit - base : 0;
+      // lane: 8 of the 16 positions at dims lane / 2, lane / 2 + 32, ...
+      const uint32_t base = x + 16 * wave + 8 * ((lane ^ (lane >> 4)) & 1), ok = page && limit > base ? limit - base : 0;
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -815,14 +820,14 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
         mx = fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
       }
       mx = fmaxf(m, mx * a.c);
-      if (__any(mx > m)) {
+      if (__any(mx > m + kSlack)) {
         const float f = rebase(m, mx);
         l *= f;
 #pragma unroll
         for (int t = 0; t < 4; t++) acc[t] *= f;
         m = mx;
       }
-      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float ref = m == -INFINITY ? 0.f : m;
       bf16x8 pf[2][NS];
       bf16x8 vf[2][4];
       // weights of positions 16 u + 8 half ..
