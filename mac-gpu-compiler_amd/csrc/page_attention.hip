@@ -105,7 +105,7 @@ struct Cursor {
 };
 
 struct PlanShared {
-  uint64_t sum[256];
+  uint64_t sum[512];
   uint32_t per;   // blocks of a workgroup
   uint32_t mine;  // of this one: fewer for the last, 0 behind it
   Cursor at;      // where they start
@@ -132,20 +132,20 @@ __device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_
 // that many are 70 TB of K and V.)
 // Each thread sums a contiguous range of sequences; the one whose range holds the block walks it.
 __device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh) {
-  const uint32_t t = threadIdx.x, each = (a.p.n_seqs + 255) / 256;
+  const uint32_t t = threadIdx.x, T = blockDim.x, each = (a.p.n_seqs + T - 1) / T;
   const uint32_t s0 = min(t * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
   uint64_t mine = 0;
   for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
   mine *= a.p.n_kv;
   sh.sum[t] = mine;
   __syncthreads();
-  for (uint32_t d = 1; d < 256; d *= 2) {
+  for (uint32_t d = 1; d < T; d *= 2) {
     const uint64_t v = t >= d ? sh.sum[t - d] : 0;
     __syncthreads();
     sh.sum[t] += v;
     __syncthreads();
   }
-  const uint64_t total = sh.sum[255];
+  const uint64_t total = sh.sum[T - 1];
   const uint64_t even = (total + W - 1) / W, per = even > a.min_blocks ? even : a.min_blocks;
   const uint64_t at = w * per;
   if (t == 0) {
@@ -625,28 +625,31 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 128, 32 for each of the workgroup's four waves, which share blocks of 64
-// positions of K and V through LDS, two blocks deep: while one is multiplied the next is on its way.
+// Many rows: tiles of 32 for each of the workgroup's 4 or 8 waves, which share blocks of 64 positions of K
+// and V through LDS: while one is multiplied the next (two, where LDS has room) are on their way.
 //
 // Bound by the matrix cores: v_mfma_f32_32x32x16_bf16, transposed as above (a lane's 16 results of a
 // score tile are the weights of 8 consecutive positions in two groups of 16, operand B of
 // Out^T = V^T P^T as they stand), against the exponentials and their arithmetic on the vector unit, some
-// 900 cycles a block beside 1024 of products; two workgroups on a CU run one beside the other. f32 rows
-// take three products for one and are alone on a CU.
+// 1400 cycles a block beside 1024 of products, so two waves on each SIMD run one beside the other. bf16
+// rows go in tiles of 256 where there are so many: with 128 every CU pulls 32 KB from L2 for 2 MFLOP, and
+// with all of them loading L2 gives some 50 B/ns each, less than the products take. f32 rows take three
+// products for one, and their registers leave room for one wave on a SIMD: tiles of 128.
 // LDS: K [64][128] with the 16-byte piece c of row r at place c ^ (r & 15), V as it lies in memory
 // ([4][128][16]) with the two pieces of every second 8 dims exchanged: what 16 lanes read at once lies in
-// different banks. bf16 pages are
-// loaded straight into it; e4m3 pages go through registers and are widened once for all rows (K with
-// its scale, V's scale is put on the weights). Wave i loads positions 16 i .. 16 i + 15 of a block,
-// which lie in one page.
+// different banks. bf16 pages are loaded straight into it; e4m3 pages go through registers and are widened
+// once for all rows (K with its scale, V's scale is put on the weights). A wave loads positions of one run
+// of 16, which lie in one page.
 // ---------------------------------------------------------------------------------------------
-template <bool FP8, bool BF16_ROWS>
-__global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(AttnArgs a) {
-  constexpr int NS = BF16_ROWS ? 1 : 3, R = 128;
+template <bool FP8, bool BF16_ROWS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(AttnArgs a) {
+  constexpr int NS = BF16_ROWS ? 1 : 3, R = 32 * WAVES;
+  constexpr int PARTS = WAVES / 4, LOADS = 4 / PARTS;  // waves that share a run; 1 KB loads of K (and V) of each
+  constexpr int STAGES = !FP8 && (WAVES == 8 || !BF16_ROWS) ? 3 : 2;  // LDS of one workgroup on a CU holds 3
   constexpr uint32_t TILE = kBlock * kPageDim * 2;  // bytes of K, and of V
-  __shared__ __align__(16) uint8_t buf[2][2 * TILE];
+  __shared__ __align__(16) uint8_t buf[STAGES][2 * TILE];
   __shared__ __align__(16) float vscale[2][FP8 ? kBlock : 4];
-  __shared__ uint32_t foul[2];
+  __shared__ uint32_t foul[STAGES];
   __shared__ PlanShared sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -695,49 +698,51 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(table))[i];
     };
     auto is_page = [&](int32_t page) __attribute__((always_inline)) { return uint32_t(page) < a.p.n_pages; };
-    u32x4 raw[4];   // e4m3: 32 bytes of a K row; dims `lane` and lane + 64 of V
-    uint32_t ke = 0, ve = 0;
-    // starts the loads of this wave's 16 positions of the block at x (a page that is not there is read
-    // as page 0, and what comes of it is masked)
+    const uint32_t run = wave / PARTS, part_of = wave % PARTS;
+    u32x4 rk[FP8 ? 2 / PARTS : 1], rv[FP8 ? 2 / PARTS : 1];  // e4m3: 16 bytes of K rows, the 16 positions of V's dims
+    uint32_t ke[FP8 ? 2 / PARTS : 1] = {}, ve = 0;
+    // starts the loads of this wave's part of the block at x (a page that is not there is read as page 0,
+    // and what comes of it is masked)
     auto fetch = [&](uint32_t x, uint32_t b, int32_t page) __attribute__((always_inline)) {
-      const uint32_t p0 = x + 16 * wave;
-      const size_t row = page_row(a.p, is_page(page) ? page : 0, head, p0 & ps_mask);
+      const size_t row = page_row(a.p, is_page(page) ? page : 0, head, (x + 16 * run) & ps_mask);
       if constexpr (FP8) {
-        const u32x4* k = reinterpret_cast<const u32x4*>(a.st.k + row * kPageDim + 32 * lane);
-        const u32x4* v = reinterpret_cast<const u32x4*>(a.st.v + row * kPageDim + 16 * lane);
-        raw[0] = k[0];
-        raw[1] = k[1];
-        raw[2] = v[0];
-        raw[3] = v[64];
-        ke = a.st.k_exp[row + (lane >> 2)];
+#pragma unroll
+        for (int i = 0; i < 2 / PARTS; i++) {
+          const uint32_t kr = 8 * (2 / PARTS * part_of + i) + (lane >> 3), d = 64 * (2 / PARTS * part_of + i) + lane;
+          rk[i] = *reinterpret_cast<const u32x4*>(a.st.k + (row + kr) * kPageDim + 16 * (lane & 7));
+          rv[i] = *reinterpret_cast<const u32x4*>(a.st.v + row * kPageDim + 16 * d);
+          ke[i] = a.st.k_exp[row + kr];
+        }
         ve = a.st.v_exp[row + (lane & 15)];
       } else {
-        const uint32_t dst = lds_address(buf[b]) + wave * 4096;
+        const uint32_t dst = lds_address(buf[b]) + run * 4096 + part_of * LOADS * 1024;
+        const uint8_t *k = a.st.k + row * kPageDim * 2, *v = a.st.v + row * kPageDim * 2 + part_of * LOADS * 1024;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t kr = 4 * i + (lane >> 4), c = (lane & 15) ^ kr;  // row of the 16, piece of the row
-          dma16(dst + i * 1024, a.st.k + (row + kr) * kPageDim * 2 + c * 16);
+        for (int i = 0; i < LOADS; i++) {
+          const uint32_t kr = 4 * (part_of * LOADS + i) + (lane >> 4), c = (lane & 15) ^ kr;  // row, piece of the row
+          dma16(dst + i * 1024, k + kr * kPageDim * 2 + c * 16);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          dma16(dst + TILE + i * 1024, a.st.v + row * kPageDim * 2 + i * 1024 + (lane ^ (lane >> 4 & 1)) * 16);
+        for (int i = 0; i < LOADS; i++)
+          dma16(dst + TILE + i * 1024, v + i * 1024 + (lane ^ (lane >> 4 & 1)) * 16);
       }
     };
     // e4m3: what fetch loaded, widened, into LDS
     auto widen = [&](uint32_t b) __attribute__((always_inline)) {
       if constexpr (FP8) {
-        uint8_t* k = buf[b] + wave * 4096 + (lane >> 2) * 256;
-        uint8_t* v = buf[b] + TILE + wave * 4096 + lane * 32;
-        const float ks = __uint_as_float(ke << 23);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint32_t c = 4 * (lane & 3) + i;
-          *reinterpret_cast<bf16x8*>(k + ((c ^ (lane >> 2)) * 16)) =
-              fp8_bf16(raw[i / 2][2 * (i & 1)], raw[i / 2][2 * (i & 1) + 1], ks);
-          *reinterpret_cast<bf16x8*>(v + (i / 2) * 2048 + (((i & 1) ^ (lane >> 3 & 1)) * 16)) =
-              fp8_bf16(raw[2 + i / 2][2 * (i & 1)], raw[2 + i / 2][2 * (i & 1) + 1], 1.f);
+        for (int i = 0; i < 2 / PARTS; i++) {
+          const uint32_t kr = 8 * (2 / PARTS * part_of + i) + (lane >> 3), d = 64 * (2 / PARTS * part_of + i) + lane;
+          uint8_t* k = buf[b] + run * 4096 + kr * 256;
+          uint8_t* v = buf[b] + TILE + run * 4096 + d * 32;
+          const float ks = __uint_as_float(ke[i] << 23);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            *reinterpret_cast<bf16x8*>(k + (((2 * (lane & 7) + e) ^ (kr & 15)) * 16)) = fp8_bf16(rk[i][2 * e], rk[i][2 * e + 1], ks);
+            *reinterpret_cast<bf16x8*>(v + ((e ^ (d >> 3 & 1)) * 16)) = fp8_bf16(rv[i][2 * e], rv[i][2 * e + 1], 1.f);
+          }
         }
-        if (lane < 16) vscale[b][16 * wave + lane] = __uint_as_float(ve << 23);
+        if (part_of == 0 && lane < 16) vscale[b][16 * run + lane] = __uint_as_float(ve << 23);
       }
     };
     auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {  // dims 32 t + col, positions 16 u + 8 half ..
@@ -745,14 +750,14 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
     };
     // V of the block in buffer b as every row may multiply it: zeros at positions that no row of the tile
     // attends, which may hold anything (0 x NaN is NaN), and where it is not finite at one that only some
-    // attend (`foul`: those get it in multiply). Each wave clears its 16 positions.
+    // attend (`foul`: those rows get it at the end). Each wave clears what it loaded.
     auto clear = [&](uint32_t x, uint32_t b, bool page) __attribute__((always_inline)) {
-      // lane: 8 of the 16 positions at dims lane / 2, lane / 2 + 32, ...
-      const uint32_t base = x + 16 * wave + 8 * ((lane ^ (lane >> 4)) & 1), ok = page && limit > base ? limit - base : 0;
+      // lane: 8 of the 16 positions at dims lane / 2, lane / 2 + 32, ... of its part
+      const uint32_t base = x + 16 * run + 8 * ((lane ^ (lane >> 4)) & 1), ok = page && limit > base ? limit - base : 0;
       uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        u32x4* v = reinterpret_cast<u32x4*>(buf[b] + TILE + wave * 4096 + i * 1024 + lane * 16);
+      for (int i = 0; i < LOADS; i++) {
+        u32x4* v = reinterpret_cast<u32x4*>(buf[b] + TILE + run * 4096 + (part_of * LOADS + i) * 1024 + lane * 16);
         u32x4 u = *v;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -765,7 +770,7 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
       if (any) foul[b] = 1;
       // (scales behind the last position may be anything too)
       if constexpr (FP8)
-        if (lane < 16 && !(page && x + 16 * wave + lane < limit)) vscale[b][16 * wave + lane] = 0.f;
+        if (part_of == 0 && lane < 16 && !(page && x + 16 * run + lane < limit)) vscale[b][16 * run + lane] = 0.f;
     };
     uint32_t foul_from = kNowhere;  // the first block that `clear` cleared something of
     // this wave's rows against the block at x in buffer b; there: which of its four pages are
@@ -876,26 +881,33 @@ __global__ __launch_bounds__(256, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(Attn
 
     __syncthreads();  // the buffers' last readers are done
     if (first < last) {
-      fetch(first, 0, page_at(first + 16 * wave));
+      // e4m3: block x is in LDS and x + 1 in registers when x is multiplied; bf16: STAGES - 1 are on their way
+      fetch(first, 0, page_at(first + 16 * run));
       widen(0);
+      if ((FP8 || STAGES == 3) && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
       if (tid == 0) foul[0] = 0;
+      constexpr uint32_t AHEAD = FP8 || STAGES == 3 ? 2 : 1;
       uint32_t b = 0, there = pages_there(first);
-      int32_t page = page_at(first + kBlock + 16 * wave);  // of this wave's part of the next block
-      for (uint32_t x = first; x < last; x += kBlock, b ^= 1) {
-        if constexpr (!FP8) wait_dma<0>();
-        __syncthreads();  // block x is in LDS; the other buffer's readers are done
+      int32_t page = page_at(first + AHEAD * kBlock + 16 * run);  // of this wave's part of the block fetched next
+      for (uint32_t x = first; x < last; x += kBlock) {
+        if constexpr (!FP8) {
+          if (STAGES == 3 && x + kBlock < last) wait_dma<2 * LOADS>();
+          else wait_dma<0>();
+        }
+        __syncthreads();  // block x is in LDS; the readers of the block before are done
         if (int32_t(x + kBlock - 1) > tile_free || there != 15) {
-          clear(x, b, there >> wave & 1);
+          clear(x, b, there >> run & 1);
           __syncthreads();
         }
-        const bool more = x + kBlock < last;
-        if (more) fetch(x + kBlock, b ^ 1, page);
+        const uint32_t b1 = b + 1 == STAGES ? 0 : b + 1, b2 = b1 + 1 == STAGES ? 0 : b1 + 1;
+        if (FP8 && x + kBlock < last) widen(b1);
+        if (x + AHEAD * kBlock < last) fetch(x + AHEAD * kBlock, STAGES == 3 ? b2 : b1, page);
         const uint32_t there_next = pages_there(x + kBlock);
-        page = page_at(x + 2 * kBlock + 16 * wave);
+        page = page_at(x + (AHEAD + 1) * kBlock + 16 * run);
         if (x < end) multiply(x, b, there);
-        if (more) widen(b ^ 1);
-        if (tid == 0) foul[b ^ 1] = 0;  // (its last readers are done; its next writers come after a barrier)
+        if (tid == 0) foul[b1] = 0;  // (its last readers are done; its next writers come after a barrier)
         there = there_next;
+        b = b1;
       }
     }
 
@@ -1031,9 +1043,18 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
 
 constexpr uint32_t kWorkgroups = 512;  // two for each CU
 
-// Rows of a tile by the most rows a sequence can have: 16 or 32 with K and V straight from memory, or 128
-// with them shared through LDS.
-uint32_t tile_rows(uint64_t max_rows) { return max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 128; }
+// How calls are cut, by the most rows (new tokens x q heads of a KV head) a sequence can have: tiles of 16
+// or 32 rows with K and V straight from memory, or tiles of 128 or (bf16 rows) 256 with them shared
+// through LDS. One workgroup on a CU at 256 rows, and of f32 rows through LDS, else two.
+struct Cut {
+  uint32_t rows, workgroups;
+};
+Cut cut_of(uint64_t max_new, uint64_t group, bool bf16) {
+  const uint64_t most = max_new && max_new < 256 ? max_new * group : 256;
+  if (most <= 32) return {most <= 16 ? 16u : 32u, kWorkgroups};
+  if (!bf16) return {128, kWorkgroups / 2};
+  return most <= 128 ? Cut{128, kWorkgroups} : Cut{256, kWorkgroups / 2};
+}
 
 }  // namespace
 }  // namespace qe
@@ -1042,8 +1063,12 @@ extern "C" {
 
 uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
   if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
-  const uint64_t most = max_new && max_new < 128 ? max_new * (n_heads / n_kv_heads) : 128;
-  return uint64_t(qe::kWorkgroups) * (2 * qe::tile_rows(most) * qe::kPartRow * 4 + sizeof(qe::Joint));
+  uint64_t rows = 0;  // of all workgroups
+  for (bool bf16 : {false, true}) {
+    const qe::Cut c = qe::cut_of(max_new, n_heads / n_kv_heads, bf16);
+    rows = rows > uint64_t(c.rows) * c.workgroups ? rows : uint64_t(c.rows) * c.workgroups;
+  }
+  return rows * 2 * qe::kPartRow * 4 + qe::kWorkgroups * sizeof(qe::Joint);
 }
 
 int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
@@ -1079,13 +1104,14 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   a.min_blocks = 4;
   a.joints = static_cast<qe::Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
-  const uint64_t most = max_new && max_new < 128 ? max_new * a.group : 128;
-  const uint32_t R = qe::tile_rows(most);
-  const uint32_t grid = R == 128 && !bf16 ? qe::kWorkgroups / 2 : qe::kWorkgroups;
-  auto go = [&](auto* kern) { kern<<<grid, 256, 0, st>>>(a); };
-  if (R == 128) {
-    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true> : qe::k_page_attn_tiles<true, false>);
-    else go(bf16 ? qe::k_page_attn_tiles<false, true> : qe::k_page_attn_tiles<false, false>);
+  const qe::Cut c = qe::cut_of(max_new, a.group, bf16);
+  const uint32_t R = c.rows, grid = c.workgroups;
+  auto go = [&](auto* kern) { kern<<<grid, R == 256 ? 512 : 256, 0, st>>>(a); };
+  if (R == 256) {
+    go(fp8 ? qe::k_page_attn_tiles<true, true, 8> : qe::k_page_attn_tiles<false, true, 8>);
+  } else if (R == 128) {
+    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true, 4> : qe::k_page_attn_tiles<true, false, 4>);
+    else go(bf16 ? qe::k_page_attn_tiles<false, true, 4> : qe::k_page_attn_tiles<false, false, 4>);
   } else if (R == 32) {
     if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 2> : qe::k_page_attn_rows<true, false, 2>);
     else go(bf16 ? qe::k_page_attn_rows<false, true, 2> : qe::k_page_attn_rows<false, false, 2>);
