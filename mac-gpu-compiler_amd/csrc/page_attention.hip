@@ -47,6 +47,7 @@ struct AttnArgs {
   float* parts;                   // [workgroup][2][rows of a tile][kPartRow]
   struct Joint* joints;           // [workgroup]
   uint32_t n_rows, n_heads, group;
+  uint32_t group_magic, group_shift;  // r / group = (2 r * magic >> 32) >> shift for r < 2^31
   uint32_t min_blocks;            // a workgroup takes at least so many
   float c;                        // log2(e) / sqrt(128)
 };
@@ -55,6 +56,10 @@ struct AttnArgs {
 struct Joint {
   uint32_t n, seq, head, tile;
 };
+
+__device__ __forceinline__ uint32_t token_of(const AttnArgs& a, uint32_t r) {  // r / group
+  return __umulhi(2 * r, a.group_magic) >> a.group_shift;
+}
 
 // ---- the plan of a sequence: its rows and how far each tile's positions go ----
 struct Seq {
@@ -78,7 +83,7 @@ __device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
 
 // Position of row r of a sequence's rows.
 __device__ __forceinline__ int32_t row_position(const AttnArgs& a, const Seq& q, uint32_t r) {
-  return q.first + int32_t(r / a.group);
+  return q.first + int32_t(token_of(a, r));
 }
 // Positions that rows up to r attend: 0 .. limit - 1 (within the table).
 __device__ __forceinline__ uint32_t row_limit(const AttnArgs& a, const Seq& q, uint32_t r) {
@@ -197,6 +202,13 @@ __device__ __forceinline__ Cursor uniform(const Cursor& c) {
 __device__ __forceinline__ uint32_t part_index() {
   const uint32_t n = gridDim.x;
   return n % 8 ? blockIdx.x : (blockIdx.x % 8) * (n / 8) + blockIdx.x / 8;
+}
+
+// v, of which the compiler does not know that it is the same in every round of a loop: what is worked out
+// from it once an item then does not stay in registers over the loop on blocks.
+__device__ __forceinline__ uint32_t afresh(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // ---- arithmetic ----
@@ -322,7 +334,8 @@ __device__ __forceinline__ void store_out8(uint8_t* out, uint64_t element, const
 // element of row r of a tile's item in rows of `stride` elements
 __device__ __forceinline__ uint64_t row_element(const AttnArgs& a, const Seq& q, uint32_t head, uint32_t r,
                                                 uint64_t stride) {
-  return (uint64_t(q.row0) + r / a.group) * stride + (head * a.group + r % a.group) * kPageDim;
+  const uint32_t t = token_of(a, r);
+  return (uint64_t(q.row0) + t) * stride + (head * a.group + (r - t * a.group)) * kPageDim;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -374,7 +387,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     const uint32_t head = cu.head;
     // the least position any row attends up to: below it no score is masked
     const int32_t free_to = row_position(a, cu.q, cu.tile * R);
-    const bool one_token = (cu.tile * R) / a.group == (cu.tile * R + rows - 1) / a.group;
+    const bool one_token = token_of(a, cu.tile * R) == token_of(a, cu.tile * R + rows - 1);
     int32_t row_pos[NQ];
     bf16x8 qf[NQ][4][NS];
 #pragma unroll
@@ -929,43 +942,54 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
       l = __uint_as_float(z[0]) + __uint_as_float(z[1]);
     }
     const bool whole = cu.block == 0 && take == cu.blocks;
-    if (whole) {
-      if (real) {
+    {
+      const uint32_t lane = afresh(tid & 63), col = lane & 31, half = lane >> 5;
+      if (whole) {
+        // through LDS (each wave in its own part of the buffers), so that rows are stored in one piece
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const uint64_t o = row_element(a, cu.q, head, r, a.out_stride) + 4 * half;
-#pragma unroll
+        constexpr uint32_t ROW = kPageDim * (BF16_ROWS ? 2 : 4), PIECES = ROW / 16;
+        uint8_t* const rows_at = buf[0] + wave * 32 * ROW;
+        __syncthreads();  // the buffers' last readers are done
+  #pragma unroll
         for (int t = 0; t < 4; t++)
-#pragma unroll
+  #pragma unroll
           for (int i = 0; i < 4; i++) {
             const f32x4 v = f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * inv;
-            const uint64_t e = o + 32 * t + 8 * i;
             if constexpr (BF16_ROWS) {
               uint2 u;
               u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2));
               u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2));
-              *reinterpret_cast<uint2*>(a.out + e * 2) = u;
+              *reinterpret_cast<uint2*>(rows_at + col * ROW + (((4 * t + i) ^ (col & 15)) * 16) + 8 * half) = u;
             } else {
-              *reinterpret_cast<f32x4*>(a.out + e * 4) = v;
+              *reinterpret_cast<f32x4*>(rows_at + col * ROW + (((8 * t + 2 * i + half) ^ col) * 16)) = v;
             }
           }
-      }
-    } else {
-      float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);
-      if (real) {
-        const uint32_t in = 32 * wave + col;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            *reinterpret_cast<f32x4*>(part + in * kPageDim + 32 * t + 8 * i + 4 * half) =
-                f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-        if (half == 0) {
-          part[R * kPageDim + in] = m;
-          part[R * kPageDim + R + in] = l;
+  #pragma unroll
+        for (uint32_t i = 0; i < 32 * PIECES / 64; i++) {
+          const uint32_t in = i * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
+          if (in < wrows) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(rows_at + in * ROW + ((piece ^ (in & (PIECES - 1))) * 16));
+            *reinterpret_cast<u32x4*>(a.out + row_element(a, cu.q, head, wr0 + in, a.out_stride) * (BF16_ROWS ? 2 : 4) + piece * 16) = v;
+          }
         }
+      } else {
+        // sums as the lanes hold them: [wave][8 dims][half][row of the 32][4 dims]
+        float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);
+        if (wrows) {
+  #pragma unroll
+          for (int t = 0; t < 4; t++)
+  #pragma unroll
+            for (int i = 0; i < 4; i++)
+              *reinterpret_cast<f32x4*>(part + ((wave * 16 + 4 * t + i) * 64 + lane) * 4) =
+                  f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+          if (half == 0) {
+            part[R * kPageDim + 32 * wave + col] = m;
+            part[R * kPageDim + R + 32 * wave + col] = l;
+          }
+        }
+        if (cu.block == 0 && tid == 0)
+          a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
       }
-      if (cu.block == 0 && tid == 0)
-        a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
     }
     left -= take;
     if (left == 0 || !next_tile(a, cu, R)) break;
@@ -975,9 +999,10 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
 // ---------------------------------------------------------------------------------------------
 // Joins the parts of the items that more than one workgroup attended: workgroup (w, y) the item whose
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
-// slots 0 of the workgroups after w. With fewer rows than 16 the threads also share the parts.
+// slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; with fewer than 16 of them
+// the threads also share the parts. TILES: parts as the tiles' lanes wrote them.
 // ---------------------------------------------------------------------------------------------
-template <bool BF16_ROWS>
+template <bool BF16_ROWS, bool TILES>
 __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const uint32_t w = blockIdx.x, tid = threadIdx.x;
   const Joint j = a.joints[w];
@@ -988,50 +1013,56 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const uint32_t here = min(rows - r0, 16u);
   uint32_t slots = 1;
   while (slots < here) slots *= 2;  // rows side by side; 16 / slots threads share a row's parts
-  const uint32_t share = 16 / slots, me = tid / 16 / slots, r = r0 + (tid / 16) % slots, d = (tid % 16) * 8;
+  if (TILES) slots = 16;
+  // neighbouring threads read what lies together: 8 dims after another of a row, or one row after another
+  const uint32_t u = TILES ? tid % 16 : tid / 16, d = (TILES ? tid / 16 : tid % 16) * 8;
+  const uint32_t share = 16 / slots, me = u / slots, r = r0 + u % slots;
+  const uint32_t e0 = TILES ? ((r / 32 * 16 + d / 8) * 64 + r % 32) * 4 : r * kPageDim + d, e1 = e0 + (TILES ? 128 : 4);
   const size_t slot = size_t(R) * kPartRow;
   const bool real = r < rows;
   float mx = -INFINITY, sum = 0.f, o[8] = {};
   if (real) {
+#pragma unroll 4
     for (uint32_t i = me; i < j.n; i += share)
       mx = fmaxf(mx, a.parts[(2 * size_t(w + i) + (i == 0)) * slot + R * kPageDim + r]);
 #pragma unroll 4
     for (uint32_t i = me; i < j.n; i += share) {
       const float* part = a.parts + (2 * size_t(w + i) + (i == 0)) * slot;
       const float f = rebase(part[R * kPageDim + r], mx);
-      const f32x4 u = *reinterpret_cast<const f32x4*>(part + r * kPageDim + d);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(part + r * kPageDim + d + 4);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + e0), y = *reinterpret_cast<const f32x4*>(part + e1);
       sum = fmaf(part[R * kPageDim + R + r], f, sum);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        o[e] = fmaf(u[e], f, o[e]);
-        o[e + 4] = fmaf(v[e], f, o[e + 4]);
+        o[e] = fmaf(x[e], f, o[e]);
+        o[e + 4] = fmaf(y[e], f, o[e + 4]);
       }
     }
   }
-  __shared__ __align__(16) float sums[16][kPageDim];
-  __shared__ float top[16], mass[16];
-  if (share > 1) {  // in order of the shares
+  if constexpr (!TILES) {
+    __shared__ __align__(16) float sums[16][kPageDim];
+    __shared__ float top[16], mass[16];
+    if (share > 1) {  // in order of the shares
 #pragma unroll
-    for (int e = 0; e < 8; e++) sums[tid / 16][d + e] = o[e];
-    if (d == 0) {
-      top[tid / 16] = mx;
-      mass[tid / 16] = sum;
-    }
-    __syncthreads();
-    if (me != 0) return;
-    float all = mx;
-    for (uint32_t i = 1; i < share; i++) all = fmaxf(all, top[tid / 16 + i * slots]);
-    float f = rebase(mx, all);
-    sum *= f;
+      for (int e = 0; e < 8; e++) sums[u][d + e] = o[e];
+      if (d == 0) {
+        top[u] = mx;
+        mass[u] = sum;
+      }
+      __syncthreads();
+      if (me != 0) return;
+      float all = mx;
+      for (uint32_t i = 1; i < share; i++) all = fmaxf(all, top[u + i * slots]);
+      float f = rebase(mx, all);
+      sum *= f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) o[e] *= f;
-    for (uint32_t i = 1; i < share; i++) {
-      const uint32_t k = tid / 16 + i * slots;
-      f = rebase(top[k], all);
-      sum = fmaf(mass[k], f, sum);
+      for (int e = 0; e < 8; e++) o[e] *= f;
+      for (uint32_t i = 1; i < share; i++) {
+        const uint32_t k = u + i * slots;
+        f = rebase(top[k], all);
+        sum = fmaf(mass[k], f, sum);
 #pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = fmaf(sums[k][d + e], f, o[e]);
+        for (int e = 0; e < 8; e++) o[e] = fmaf(sums[k][d + e], f, o[e]);
+      }
     }
   }
   if (!real) return;
@@ -1100,6 +1131,9 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   a.n_rows = uint32_t(n_rows);
   a.n_heads = uint32_t(n_heads);
   a.group = uint32_t(n_heads / a.p.n_kv);
+  // shift = ceil(log2 group), magic = ceil(2^(31 + shift) / group): exact below 2^31
+  while ((1ull << a.group_shift) < a.group) a.group_shift++;
+  a.group_magic = uint32_t(((1ull << (31 + a.group_shift)) + a.group - 1) / a.group);
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
   a.min_blocks = 4;
   a.joints = static_cast<qe::Joint*>(work);
@@ -1120,8 +1154,9 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
     else go(bf16 ? qe::k_page_attn_rows<false, true, 1> : qe::k_page_attn_rows<false, false, 1>);
   }
   const dim3 join(grid, R / 16);
-  if (bf16) qe::k_page_join<true><<<join, 256, 0, st>>>(a, R);
-  else qe::k_page_join<false><<<join, 256, 0, st>>>(a, R);
+  auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
+  if (R >= 128) join_by(bf16 ? qe::k_page_join<true, true> : qe::k_page_join<false, true>);
+  else join_by(bf16 ? qe::k_page_join<true, false> : qe::k_page_join<false, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page attention launch failed: %s", hipGetErrorString(e));
   return QE_OK;
