@@ -27,23 +27,6 @@ struct PageStore {
 int check_pages(const qe_pages* p, PagePlan* plan, PageStore* store);
 
 #ifdef __HIPCC__
-// The sequence that packed row t belongs to, or -1: the last s with starts[s] <= t, if t <
-// starts[s + 1]. (On starts that decrease somewhere the search still ends, at some s or -1.)
-__device__ __forceinline__ int32_t sequence_of(const PagePlan& p, int32_t t) {
-  uint32_t lo = 0, hi = p.n_seqs;  // starts[lo] <= t (or lo = 0), starts[hi] > t (or hi = n_seqs)
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (p.starts[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return p.starts[lo] <= t && t < p.starts[lo + 1] ? int32_t(lo) : -1;
-}
-
-// Position of packed row t of sequence s: its last row is at lens[s] - 1. May be negative.
-__device__ __forceinline__ int64_t position_of(const PagePlan& p, uint32_t s, int32_t t) {
-  return int64_t(p.lens[s]) - (int64_t(p.starts[s + 1]) - t);
-}
-
 // Positions the table has entries for.
 __device__ __forceinline__ int64_t capacity_of(const PagePlan& p) { return int64_t(p.table_stride) << p.page_shift; }
 

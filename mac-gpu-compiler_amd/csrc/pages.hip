@@ -15,26 +15,108 @@ namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-// 2 elements from a row of f32 or bf16
-template <bool BF16>
-__device__ __forceinline__ f32x2 load2(const void* row, uint32_t i) {
-  if constexpr (BF16) {
-    const uint32_t u = reinterpret_cast<const uint32_t*>(row)[i];
-    return f32x2{__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)};
-  } else {
-    return reinterpret_cast<const f32x2*>(row)[i];
-  }
-}
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// |x| where it is finite, else 0
-__device__ __forceinline__ float finite_magnitude(float x) {
-  const float a = fabsf(x);
-  return a <= 3.402823466e38f ? a : 0.f;
+// ---- which rows a workgroup takes ----
+// V lies transposed in runs of 16 positions, so the rows of one run are written together. Workgroup x
+// takes the runs whose first new row is one of the packed rows 16 x .. 16 x + 15: a window of a long
+// chunk is one whole run whatever the alignment of the chunk, a window of decode rows is 16 runs of one
+// row. Those rows are contiguous and at most 31.
+struct Rows {
+  uint32_t first, count;  // packed rows
+  bool whole;             // one run, all 16 positions of it
+  int64_t slot;           // of lane i < 32: where packed row 16 x + i lies (row index in the pages), -1 no page, -2 no sequence
+};
+
+constexpr uint32_t kStartsInLds = 1024;
+
+__device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, int32_t* starts) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, t0 = blockIdx.x * 16, t = t0 + (lane & 31);
+  // the search in `starts` is a chain of loads: from LDS where it fits
+  const bool in_lds = p.n_seqs < kStartsInLds;
+  if (in_lds) {
+    for (uint32_t i = tid; i <= p.n_seqs; i += blockDim.x) starts[i] = p.starts[i];
+    __syncthreads();
+  }
+  const int32_t* at = in_lds ? starts : p.starts;
+  Rows r;
+  r.slot = -2;
+  bool begins = true;  // a run (rows of no sequence are one each)
+  if (t < n_rows) {
+    uint32_t lo = 0, hi = p.n_seqs;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (at[mid] <= int32_t(t)) lo = mid;
+      else hi = mid;
+    }
+    const int32_t a = at[lo], e = at[lo + 1];
+    if (a <= int32_t(t) && int32_t(t) < e) {
+      const int64_t pos = int64_t(p.lens[lo]) - (int64_t(e) - t);
+      begins = a == int32_t(t) || (pos & (kPageRun - 1)) == 0;
+      r.slot = -1;
+      if (pos >= 0 && pos < capacity_of(p)) {
+        const int32_t page = page_of(p, lo, pos);
+        if (page >= 0) r.slot = int64_t(page_row(p, page, blockIdx.y, uint32_t(pos) & ((1u << p.page_shift) - 1)));
+      }
+    }
+  }
+  const uint32_t marks = uint32_t(__ballot(begins)) & 0xFFFFFFFFu;
+  const uint32_t here = marks & 0xFFFFu, next = marks >> 16;
+  // (of 16 consecutive rows one begins a run, so both are there; a plan whose starts decrease may lack it)
+  const uint32_t from = here ? __builtin_ctz(here) : 16, to = 16 + (next ? __builtin_ctz(next) : 16);
+  r.first = t0 + from;
+  r.count = here ? min(to, n_rows > t0 ? n_rows - t0 : 0u) - min(from, n_rows > t0 ? n_rows - t0 : 0u) : 0;
+  const int64_t s = __shfl(r.slot, from & 31);
+  r.whole = __builtin_popcount(here) == 1 && r.count == 16 && s >= 0 && (s & (kPageRun - 1)) == 0;
+  return r;
+}
+// slot of row i of r.first ..
+__device__ __forceinline__ int64_t slot_of(const Rows& r, uint32_t i) {
+  return __shfl(r.slot, int((r.first + i) & 31) - int((blockIdx.x * 16) & 31) & 31);
+}
+
+// ---- values ----
+template <bool BF16>
+__device__ __forceinline__ void load8(const uint8_t* row, uint32_t d, float (&x)[8]) {
+  if constexpr (BF16) {
+    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(row + 2 * d);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  } else {
+    const f32x4 u = *reinterpret_cast<const f32x4*>(row + 4 * d), v = *reinterpret_cast<const f32x4*>(row + 4 * d + 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[i] = u[i];
+      x[i + 4] = v[i];
+    }
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void store8(uint8_t* row, uint32_t d, const float (&x)[8]) {
+  if constexpr (BF16) {
+    u32x4_t u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<u32x4_t*>(row + 2 * d) = u;
+  } else {
+    *reinterpret_cast<f32x4*>(row + 4 * d) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4*>(row + 4 * d + 16) = f32x4{x[4], x[5], x[6], x[7]};
+  }
+}
+
+// Maximum over each 16 lanes, to all of them (quad xor 1, quad xor 2, half-row mirror, row mirror).
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  return fmaxf(v, dpp<0x140>(v));
 }
 
 // Exponent byte of a row whose largest finite magnitude is amax: 127 (scale 1) for a row of zeros.
@@ -45,95 +127,168 @@ __device__ __forceinline__ uint32_t row_exponent(float amax) {
   return uint32_t(max(e, 1));
 }
 
-// two e4m3 bytes of a and b times inv (a power of two); what is not finite becomes NaN
-__device__ __forceinline__ uint32_t pack_fp8(float a, float b, float inv) {
-  const float x = a * inv, y = b * inv;
-  uint32_t u = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false)) & 0xFFFFu;
-  if (!(fabsf(x) <= 448.f)) u = (u & 0xFF00u) | 0x7Fu;
-  if (!(fabsf(y) <= 448.f)) u = (u & 0x00FFu) | 0x7F00u;
-  return u;
+// 8 values of a row held by 16 lanes as e4m3 (o[0], o[1]), and the row's exponent byte.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&o)[4]) {
+  float a = 0.f;
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float y = fabsf(x[i]);
+    fine &= y < INFINITY;
+    a = fmaxf(a, y < INFINITY ? y : 0.f);
+  }
+  const uint32_t e = row_exponent(max16(a));
+  const float inv = exp_scale(254 - e);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    int u = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+    u = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, u, true);
+    o[i] = uint32_t(u);
+  }
+  if (!fine) {  // infinities and NaN become NaN
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (!(fabsf(x[i]) < INFINITY)) o[i / 4] |= 0x7Fu << (8 * (i & 3));
+  }
+  return e;
 }
 
-// A wave per (row, KV head): lane l holds dims 2 l and 2 l + 1 of K and of V.
+// A workgroup per (16 packed rows, KV head), see Rows: thread (tid / 16, tid % 16) has a row and 8 dims of it.
+// Bound by the rows read and written: 14,162 rows of 8 heads, f32 to e4m3 (145 MB), 48 us.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, const uint8_t* k, const uint8_t* v,
                                                      uint32_t n_rows, uint64_t stride) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t unit = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const uint32_t t = uint32_t(unit / p.n_kv), head = uint32_t(unit % p.n_kv);
-  if (t >= n_rows) return;
-  const int32_t s = sequence_of(p, int32_t(t));
-  if (s < 0) return;
-  const int64_t pos = position_of(p, s, int32_t(t));
-  if (pos < 0 || pos >= capacity_of(p)) return;
-  const int32_t page = page_of(p, s, pos);
-  if (page < 0) return;
-  const uint32_t off = uint32_t(pos) & ((1u << p.page_shift) - 1);
-  const size_t src = (t * stride + head * kPageDim) * (BF16_ROWS ? 2 : 4);
-  const f32x2 x = load2<BF16_ROWS>(k + src, lane), y = load2<BF16_ROWS>(v + src, lane);
-  const size_t row = page_row(p, page, head, off), ve = v_element(p, page, head, off);
-  if constexpr (FP8) {
-    const uint32_t kx = row_exponent(wave_max(fmaxf(finite_magnitude(x[0]), finite_magnitude(x[1]))));
-    const uint32_t vx = row_exponent(wave_max(fmaxf(finite_magnitude(y[0]), finite_magnitude(y[1]))));
-    reinterpret_cast<uint16_t*>(st.k + row * kPageDim)[lane] = uint16_t(pack_fp8(x[0], x[1], exp_scale(254 - kx)));
-    const uint32_t u = pack_fp8(y[0], y[1], exp_scale(254 - vx));
-    st.v[ve + 32 * lane] = uint8_t(u);
-    st.v[ve + 32 * lane + 16] = uint8_t(u >> 8);
-    if (lane == 0) {
-      st.k_exp[row] = uint8_t(kx);
-      st.v_exp[row] = uint8_t(vx);
+  constexpr uint32_t EL = FP8 ? 1 : 2, IN = BF16_ROWS ? 2 : 4;
+  __shared__ int32_t starts[kStartsInLds + 1];
+  __shared__ __align__(16) uint8_t run[kPageRun * kPageDim * EL];  // V of a run as it lies in the page
+  const uint32_t tid = threadIdx.x, head = blockIdx.y, d = (tid & 15) * 8;
+  const Rows r = rows_of(p, n_rows, starts);
+  for (uint32_t b = 0; b < r.count; b += 16) {
+    const uint32_t i = b + tid / 16;
+    const int64_t slot = slot_of(r, i);
+    const bool real = i < r.count && slot >= 0;
+    float x[8] = {}, y[8] = {};
+    if (real) {
+      const size_t src = (size_t(r.first + i) * stride + head * kPageDim) * IN;
+      load8<BF16_ROWS>(k + src, d, x);
+      load8<BF16_ROWS>(v + src, d, y);
     }
-  } else {
-    reinterpret_cast<uint32_t*>(st.k + row * kPageDim * 2)[lane] = pack_bf16(x[0], x[1]);
-    const uint32_t u = pack_bf16(y[0], y[1]);
-    uint16_t* o = reinterpret_cast<uint16_t*>(st.v) + ve + 32 * lane;
-    o[0] = uint16_t(u);
-    o[16] = uint16_t(u >> 16);
+    uint32_t kq[4], vq[4], ke = 0, ve = 0;
+    if constexpr (FP8) {
+      ke = quantise8(x, kq);
+      ve = quantise8(y, vq);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        kq[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+        vq[e] = pack_bf16(y[2 * e], y[2 * e + 1]);
+      }
+    }
+    auto v_byte_or_half = [&](int e) { return FP8 ? vq[e / 4] >> (8 * (e & 3)) : vq[e / 2] >> (16 * (e & 1)); };
+    if (real) {
+      uint8_t* o = st.k + (size_t(slot) * kPageDim + d) * EL;
+      if constexpr (FP8) *reinterpret_cast<uint2*>(o) = make_uint2(kq[0], kq[1]);
+      else *reinterpret_cast<uint4*>(o) = make_uint4(kq[0], kq[1], kq[2], kq[3]);
+      if (FP8 && d == 0) {
+        st.k_exp[slot] = uint8_t(ke);
+        st.v_exp[slot] = uint8_t(ve);
+      }
+    }
+    if (r.whole) {  // (then b is 0 and row i is position i of the run)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t at = (d + e) * kPageRun + i;
+        if constexpr (FP8) run[at] = uint8_t(v_byte_or_half(e));
+        else reinterpret_cast<uint16_t*>(run)[at] = uint16_t(v_byte_or_half(e));
+      }
+      __syncthreads();
+      const int64_t base = slot_of(r, 0);
+      if (tid < sizeof(run) / 16)
+        reinterpret_cast<uint4*>(st.v + size_t(base) * kPageDim * EL)[tid] = reinterpret_cast<const uint4*>(run)[tid];
+    } else if (real) {
+      const size_t at = size_t(slot & ~int64_t(kPageRun - 1)) * kPageDim + (slot & (kPageRun - 1)) + d * kPageRun;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if constexpr (FP8) st.v[at + e * kPageRun] = uint8_t(v_byte_or_half(e));
+        else reinterpret_cast<uint16_t*>(st.v)[at + e * kPageRun] = uint16_t(v_byte_or_half(e));
+      }
+    }
   }
 }
 
-template <bool BF16>
-__device__ __forceinline__ void store2(void* row, uint32_t i, float a, float b) {
-  if constexpr (BF16) reinterpret_cast<uint32_t*>(row)[i] = pack_bf16(a, b);
-  else reinterpret_cast<f32x2*>(row)[i] = f32x2{a, b};
-}
-
-// A wave per (row, KV head), the same lanes; a position without a page reads as zeros.
+// The same rows the other way; a position without a page reads as zeros.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_read(PagePlan p, PageStore st, uint8_t* k, uint8_t* v, uint32_t n_rows,
                                                    uint64_t stride) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t unit = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const uint32_t t = uint32_t(unit / p.n_kv), head = uint32_t(unit % p.n_kv);
-  if (t >= n_rows) return;
-  const int32_t s = sequence_of(p, int32_t(t));
-  if (s < 0) return;
-  const int64_t pos = position_of(p, s, int32_t(t));
-  const int32_t page = pos < 0 || pos >= capacity_of(p) ? -1 : page_of(p, s, pos);
-  const size_t dst = (t * stride + head * kPageDim) * (BF16_ROWS ? 2 : 4);
-  float a = 0.f, b = 0.f, c = 0.f, d = 0.f;
-  if (page >= 0) {
-    const uint32_t off = uint32_t(pos) & ((1u << p.page_shift) - 1);
-    const size_t row = page_row(p, page, head, off), ve = v_element(p, page, head, off);
-    if constexpr (FP8) {
-      const float ks = exp_scale(st.k_exp[row]), vs = exp_scale(st.v_exp[row]);
-      const uint32_t u = reinterpret_cast<const uint16_t*>(st.k + row * kPageDim)[lane];
-      const uint32_t w = st.v[ve + 32 * lane] | uint32_t(st.v[ve + 32 * lane + 16]) << 8;
-      a = __builtin_amdgcn_cvt_f32_fp8(int(u), 0) * ks;
-      b = __builtin_amdgcn_cvt_f32_fp8(int(u), 1) * ks;
-      c = __builtin_amdgcn_cvt_f32_fp8(int(w), 0) * vs;
-      d = __builtin_amdgcn_cvt_f32_fp8(int(w), 1) * vs;
-    } else {
-      const uint32_t u = reinterpret_cast<const uint32_t*>(st.k + row * kPageDim * 2)[lane];
-      const uint16_t* o = reinterpret_cast<const uint16_t*>(st.v) + ve + 32 * lane;
-      a = __uint_as_float(u << 16);
-      b = __uint_as_float(u & 0xFFFF0000u);
-      c = bf16f(o[0]);
-      d = bf16f(o[16]);
+  constexpr uint32_t EL = FP8 ? 1 : 2, OUT = BF16_ROWS ? 2 : 4;
+  __shared__ int32_t starts[kStartsInLds + 1];
+  __shared__ __align__(16) uint8_t run[kPageRun * kPageDim * EL];
+  const uint32_t tid = threadIdx.x, head = blockIdx.y, d = (tid & 15) * 8;
+  const Rows r = rows_of(p, n_rows, starts);
+  for (uint32_t b = 0; b < r.count; b += 16) {
+    const uint32_t i = b + tid / 16;
+    const int64_t slot = slot_of(r, i);
+    uint32_t kq[4] = {}, vq[4] = {};
+    float ks = 1.f, vs = 1.f;
+    const bool there = i < r.count && slot >= 0;
+    if (there) {
+      const uint8_t* o = st.k + (size_t(slot) * kPageDim + d) * EL;
+      if constexpr (FP8) {
+        const uint2 u = *reinterpret_cast<const uint2*>(o);
+        kq[0] = u.x;
+        kq[1] = u.y;
+        ks = exp_scale(st.k_exp[slot]);
+        vs = exp_scale(st.v_exp[slot]);
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(o);
+        kq[0] = u.x; kq[1] = u.y; kq[2] = u.z; kq[3] = u.w;
+      }
     }
+    if (r.whole) {
+      const int64_t base = slot_of(r, 0);
+      if (tid < sizeof(run) / 16)
+        reinterpret_cast<uint4*>(run)[tid] = reinterpret_cast<const uint4*>(st.v + size_t(base) * kPageDim * EL)[tid];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t at = (d + e) * kPageRun + i;
+        if constexpr (FP8) vq[e / 4] |= uint32_t(run[at]) << (8 * (e & 3));
+        else vq[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(run)[at]) << (16 * (e & 1));
+      }
+    } else if (there) {
+      const size_t at = size_t(slot & ~int64_t(kPageRun - 1)) * kPageDim + (slot & (kPageRun - 1)) + d * kPageRun;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if constexpr (FP8) vq[e / 4] |= uint32_t(st.v[at + e * kPageRun]) << (8 * (e & 3));
+        else vq[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(st.v)[at + e * kPageRun]) << (16 * (e & 1));
+      }
+    }
+    if (i >= r.count || slot == -2) continue;
+    auto widen = [&](const uint32_t (&q)[4], float scale, float (&x)[8]) {
+      if constexpr (FP8) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(int(q[e]), false), c = __builtin_amdgcn_cvt_pk_f32_fp8(int(q[e]), true);
+          x[4 * e] = a[0] * scale;
+          x[4 * e + 1] = a[1] * scale;
+          x[4 * e + 2] = c[0] * scale;
+          x[4 * e + 3] = c[1] * scale;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[2 * e] = __uint_as_float(q[e] << 16);
+          x[2 * e + 1] = __uint_as_float(q[e] & 0xFFFF0000u);
+        }
+      }
+    };
+    float x[8], y[8];
+    widen(kq, ks, x);
+    widen(vq, vs, y);
+    const size_t dst = (size_t(r.first + i) * stride + head * kPageDim) * OUT;
+    store8<BF16_ROWS>(k + dst, d, x);
+    store8<BF16_ROWS>(v + dst, d, y);
   }
-  store2<BF16_ROWS>(k + dst, lane, a, b);
-  store2<BF16_ROWS>(v + dst, lane, c, d);
 }
 
 }  // namespace
@@ -216,7 +371,7 @@ int qe_op_page_append(const qe_pages* pages, const void* k, const void* v, uint6
   qe::PageStore st;
   if (int rc = qe::check_rows(pages, k, v, n_rows, row_stride, dtype, &p, &st)) return rc;
   if (n_rows == 0) return QE_OK;
-  const uint32_t grid = qe::ceil_div(uint32_t(n_rows) * p.n_kv, 4u);
+  const dim3 grid(qe::ceil_div(uint32_t(n_rows), 16u), p.n_kv);
   const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
   auto* kern = fp8 ? (bf16 ? qe::k_page_append<true, true> : qe::k_page_append<true, false>)
                    : (bf16 ? qe::k_page_append<false, true> : qe::k_page_append<false, false>);
@@ -231,7 +386,7 @@ int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, ui
   qe::PageStore st;
   if (int rc = qe::check_rows(pages, k, v, n_rows, row_stride, dtype, &p, &st)) return rc;
   if (n_rows == 0) return QE_OK;
-  const uint32_t grid = qe::ceil_div(uint32_t(n_rows) * p.n_kv, 4u);
+  const dim3 grid(qe::ceil_div(uint32_t(n_rows), 16u), p.n_kv);
   const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
   auto* kern = fp8 ? (bf16 ? qe::k_page_read<true, true> : qe::k_page_read<true, false>)
                    : (bf16 ? qe::k_page_read<false, true> : qe::k_page_read<false, false>);
