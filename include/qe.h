@@ -335,7 +335,7 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
  * tokens_out [n_rows]: each sequence's accepted drafts, then the drawn token, then 0xFFFFFFFF;
  * count_out [n_seqs]: how many tokens that is (0 for a sequence without rows); logprobs_out
  * [n_rows] (nullable): log p of each, 0 behind them. Rows that belong to no sequence are left as
- * they were. Sums are f64. `work` as qe_op_page_attention's. */
+ * they were. Sums are f64. vocab 1..2^20, n_seqs 1..65535. `work` as qe_op_page_attention's. */
 uint64_t qe_op_verify_drafts_work_bytes(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab);
 int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, uint64_t row_stride,
                         const int32_t* starts, uint64_t n_seqs, const uint32_t* drafts, const float* draft_probs,

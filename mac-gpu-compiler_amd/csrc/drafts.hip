@@ -36,17 +36,16 @@ namespace {
 struct ChunkSum {
   double sum;
   float top;      // -inf: nothing above -inf
-  uint32_t best;  // first index of top
+  uint32_t best;  // first index of top, of greedy rows
 };
 
 // The row a sequence draws from.
 struct DrawRow {
-  double inv_total, k;  // 1 / sum of weights; log2(e) / T
-  double log_total;
-  uint32_t row;         // 0xFFFFFFFF: the sequence draws nothing here
+  double total, inv_total, k;  // sum of weights, 1 / it; log2(e) / T
+  uint32_t row;                // 0xFFFFFFFF: the sequence draws nothing here
   uint32_t best, draft;
-  float top, inv_t;
-  uint32_t greedy;
+  float top;
+  uint32_t greedy;  // all the weight on `best`
 };
 
 struct DraftArgs {
@@ -68,15 +67,15 @@ struct DraftArgs {
 
 constexpr int kThreads = 512;
 constexpr uint32_t kChunk = 2048, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMostVocab = kThreads * kChunk;  // a thread of a draw has one chunk: 2^20
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// 2^t in 64 bits for t <= 0 (6e-16; 0 below -1075): t = n + f with n the nearest whole number, and
-// 2^f = 1 + f c(f) by Chebyshev interpolation of (2^f - 1) / f at 10 points of [-1/2, 1/2]. 2^0 is
-// exactly 1. (The library's exp is some 40 instructions on the same unit, which then bounds the pass
-// instead of the memory.)
+// 2^t in 64 bits for t <= 0 (6e-16; 0 below -1000 and for NaN): t = n + f with n the nearest whole number,
+// and 2^f = 1 + f c(f) by Chebyshev interpolation of (2^f - 1) / f at 10 points of [-1/2, 1/2]; n goes
+// straight into the exponent. 2^0 is exactly 1. (The library's exp is some 40 instructions on the same
+// unit, which then bounds the pass instead of the memory.)
 __device__ __forceinline__ double exp2_64(double t) {
-  t = fmax(t, -1100.0);
   const double n = rint(t), f = t - n;
   double c = 7.070977866508138e-09;
   c = fma(c, f, 1.0205905413765595e-07);
@@ -88,14 +87,21 @@ __device__ __forceinline__ double exp2_64(double t) {
   c = fma(c, f, 0.05550410866465167);
   c = fma(c, f, 0.24022650695910075);
   c = fma(c, f, 0.6931471805599462);
-  return ldexp(fma(c, f, 1.0), int(n));
+  c = fma(c, f, 1.0);
+  const double y = __hiloint2double(__double2hiint(c) + (int(fmax(n, -1000.0)) << 20), __double2loint(c));
+  return t >= -1000.0 ? y : 0.0;
 }
 
 // weight of logit x relative to the largest one, top: NaN and -inf weigh nothing, infinite ones share
 __device__ __forceinline__ double weight(float x, float top, double k) {
-  if (x == top) return 1.0;
-  if (!(x > -INFINITY) || top == INFINITY) return 0.0;
+  if (top == INFINITY) return x == top ? 1.0 : 0.0;
   return exp2_64((double(x) - double(top)) * k);
+}
+
+// log p of a token with logit x
+__device__ __forceinline__ float log_weight(const DrawRow& d, float x, float t) {
+  if (d.greedy) return 0.f;
+  return float((x == d.top ? 0.0 : (double(x) - double(d.top)) / double(t)) - log(d.total));
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -150,171 +156,160 @@ __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
   load_chunk(a.logits + r * a.stride, c * kChunk, a.vocab, -INFINITY, x);
   const int32_t s = sequence(a, int32_t(r));
   if (s < 0) return;
+  const float t = temperature(a, s);
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 32; i++) m = fmaxf(m, x[i]);
   m = wave_max(m);
-  uint32_t at = kNone;  // the first place that holds it
-#pragma unroll
-  for (int i = 31; i >= 0; i--)
-    if (x[i] == m) at = c * kChunk + 256 * (i / 4) + 4 * lane + i % 4;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) at = min(at, uint32_t(__shfl_xor(int(at), d)));
-  const float t = temperature(a, s);
   double sum = 0.0;
+  uint32_t at = kNone;
   if (t > 0.f && m > -INFINITY) {
     const double k = rate(t);
 #pragma unroll
     for (int i = 0; i < 32; i++) sum += weight(x[i], m, k);
     sum = wave_sum64(sum);
+  } else {  // greedy: the first place that holds the largest
+#pragma unroll
+    for (int i = 31; i >= 0; i--)
+      if (x[i] == m) at = c * kChunk + 256 * (i / 4) + 4 * lane + i % 4;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) at = min(at, uint32_t(__shfl_xor(int(at), d)));
   }
   if (lane == 0) a.sums[size_t(r) * a.chunks + c] = ChunkSum{sum, m, at};
 }
 
-// ---- a workgroup's own sums ----
+// ---- a workgroup's draw ----
 struct Scratch {
   double wave[kThreads / 64];
-  double of[kThreads];
-  uint32_t pick, some;
+  uint32_t owner, last;  // the thread whose items the aim falls into; one past the last thread with any weight
+  uint32_t pick;
   double before;
-  double without;
 };
 
-// running sum of v over the threads up to and with this one, and the sum of all
-__device__ double running_sum(double v, Scratch& sc, double& all) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Items lie in order, N to a thread, w their weights. The first whose running sum is above aim(sum of
+// all), and the running sum before it; if rounding leaves none, the last with any weight; kNone if
+// nothing has any.
+template <int N, class Aim>
+__device__ __forceinline__ uint32_t find(const double (&w)[N], Aim aim, Scratch& sc, double& before) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; i++) mine += w[i];
+  double up_to = mine;  // over the wave's threads up to this one, then over all
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const double u = __shfl_up(v, d);
-    if (int(lane) >= d) v += u;
+    const double u = __shfl_up(up_to, d);
+    if (int(lane) >= d) up_to += u;
+  }
+  __syncthreads();  // the draw before has been read
+  if (lane == 63) sc.wave[wave] = up_to;
+  if (tid == 0) {
+    sc.owner = kNone;
+    sc.last = 0;
   }
   __syncthreads();
-  if (lane == 63) sc.wave[wave] = v;
-  __syncthreads();
-  double before = 0.0;
-  all = 0.0;
+  double all = 0.0, base = 0.0;
 #pragma unroll
   for (uint32_t i = 0; i < kThreads / 64; i++) {
-    if (i < wave) before += sc.wave[i];
+    if (i == wave) base = all;
     all += sc.wave[i];
   }
-  return before + v;
-}
-
-// The first of n items (item i weighs w(i), thread t asks for a contiguous range of them) whose running
-// sum is above goal(sum of all), and the running sum before it. If rounding leaves none, the last with
-// any weight; kNone if nothing has any.
-template <class W, class Goal>
-__device__ uint32_t find_item(uint32_t n, W w, Goal goal, Scratch& sc, double& before, double& all) {
-  const uint32_t per = (n + kThreads - 1) / kThreads, i0 = min(threadIdx.x * per, n), i1 = min(i0 + per, n);
-  double mine = 0.0;
-  uint32_t some = kNone;
-  for (uint32_t i = i0; i < i1; i++) {
-    const double v = w(i);
-    mine += v;
-    if (v > 0.0) some = i;
-  }
-  const double up_to = running_sum(mine, sc, all);
-  const double aim = goal(all);
-  if (threadIdx.x == 0) {
-    sc.pick = kNone;
-    sc.some = 0;
+  up_to += base;
+  const double to = aim(all);
+  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
+  if (lane == 0) {
+    if (some) atomicMax(&sc.last, wave * 64 + 64 - __builtin_clzll(some));
+    if (over) atomicMin(&sc.owner, wave * 64 + __builtin_ctzll(over));
   }
   __syncthreads();
-  if (some != kNone) atomicMax(&sc.some, some + 1);
-  if (some != kNone && up_to > aim) atomicMin(&sc.pick, threadIdx.x);
-  __syncthreads();
-  const uint32_t owner = sc.pick, last = sc.some;
-  __syncthreads();
-  if (owner == kNone) {  // not above the aim anywhere: the last item that has weight
-    if (last != 0 && last - 1 >= i0 && last - 1 < i1) sc.before = up_to - w(last - 1);
-    __syncthreads();
-    before = sc.before;
-    return last == 0 ? kNone : last - 1;
-  }
-  if (threadIdx.x == owner) {
-    double run = up_to - mine;
-    for (uint32_t i = i0; i < i1; i++) {
-      const double v = w(i);
-      if (v > 0.0 && (run + v > aim || i == some)) {
-        sc.pick = i;
-        sc.before = run;
-        break;
+  const uint32_t owner = sc.owner != kNone ? sc.owner : sc.last - 1;  // (nothing at all: kNone)
+  if (tid == owner) {
+    double run = up_to - mine, from = run;
+    uint32_t at = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (!found && w[i] > 0.0) {
+        at = i;
+        from = run;
+        found = run + w[i] > to;
       }
-      run += v;
+      run += w[i];
     }
+    sc.pick = tid * N + at;
+    sc.before = from;
   }
   __syncthreads();
   before = sc.before;
-  return sc.pick;
+  return owner == kNone ? kNone : sc.pick;
 }
 
 // sum of the chunk's weights from one logit to another: the chunk's largest to the row's
-__device__ __forceinline__ double chunk_scale(float from, const DrawRow& d) {
-  if (from == d.top) return 1.0;
-  if (!(from > -INFINITY) || d.top == INFINITY) return 0.0;
-  return exp2_64((double(from) - double(d.top)) * d.k);
+__device__ __forceinline__ double chunk_scale(float from, float top, double k) {
+  return from == top ? 1.0 : top == INFINITY ? 0.0 : exp2_64((double(from) - double(top)) * k);
 }
 
-// One token of row d.row: over the chunks by their sums, then within a chunk. REST: from max(p - q, 0).
+// One token of row d.row: over the chunks by their sums (a thread each), then within a chunk (4 tokens a
+// thread). REST: from max(p - q, 0).
 template <bool REST>
-__device__ void draw(const DraftArgs& a, uint32_t s, const DrawRow& d, bool last, Scratch& sc) {
+__device__ __forceinline__ void draw(const DraftArgs& a, uint32_t s, const DrawRow& d, bool last, Scratch& sc) {
+  constexpr int N = kChunk / kThreads;
   const float* x = a.logits + d.row * a.stride;
-  const float* q = REST ? a.probs + d.row * a.probs_stride : nullptr;
+  const uint32_t tid = threadIdx.x;
   const uint32_t skip = last || a.probs ? kNone : d.draft;  // a drafted token that has all of q
   const double v = double(a.sample[s]);
-  auto token_weight = [&](uint32_t i) -> double {
-    if (d.greedy) return i == d.best ? 1.0 : 0.0;
-    return weight(x[i], d.top, d.k);
+  const float t = temperature(a, s);
+  auto token_weight = [&](uint32_t i, float xi) -> double {
+    return d.greedy ? (i == d.best ? 1.0 : 0.0) : weight(xi, d.top, d.k);
   };
-  auto rest_weight = [&](uint32_t i) -> double {
-    if (i == skip) return 0.0;
-    const double w = token_weight(i);
-    if constexpr (REST) {
-      const float qi = q[i];
-      return qi > 0.f ? fmax(w * d.inv_total - double(qi), 0.0) : w * d.inv_total;
-    }
-    return w;
+  auto plain_chunk = [&]() -> double {
+    if (tid >= a.chunks) return 0.0;
+    if (d.greedy) return d.best / kChunk == tid ? 1.0 : 0.0;
+    const ChunkSum p = a.sums[size_t(d.row) * a.chunks + tid];
+    return p.sum * chunk_scale(p.top, d.top, d.k);
   };
-  auto plain_chunk = [&](uint32_t c) -> double {
-    if (d.greedy) return d.best / kChunk == c ? 1.0 : 0.0;
-    const ChunkSum p = a.sums[size_t(d.row) * a.chunks + c];
-    return p.sum * chunk_scale(p.top, d);
-  };
-  if (skip < a.vocab) {  // its chunk's sum without it
-    const uint32_t c0 = skip / kChunk * kChunk, n = min(kChunk, a.vocab - c0);
-    double mine = 0.0, all;
-    for (uint32_t i = threadIdx.x * (kChunk / kThreads); i < min((threadIdx.x + 1) * (kChunk / kThreads), n); i++)
-      mine += rest_weight(c0 + i);
-    running_sum(mine, sc, all);
-    if (threadIdx.x == 0) sc.without = all;
-    __syncthreads();
+  double w[1], before, aim = 0.0;
+  auto share = [&](double all) { return aim = v * all; };
+  if constexpr (REST) {
+    w[0] = tid < a.chunks ? a.rests[size_t(s) * a.chunks + tid] : 0.0;
+  } else {
+    w[0] = plain_chunk();
+    // (a draft is refused where u < 1 is at least p(d): what is left is 2^-24 of the row or more, and the
+    // difference is off by 2^-29 of that at most)
+    if (skip < a.vocab && skip / kChunk == tid) w[0] = fmax(w[0] - token_weight(skip, x[skip]), 0.0);
   }
-  const double without = sc.without;
-  double before, all, inner, unused;
-  auto chunk_weight = [&](uint32_t c) -> double {
-    if constexpr (REST) return a.rests[size_t(s) * a.chunks + c];
-    return skip < a.vocab && skip / kChunk == c ? without : plain_chunk(c);
-  };
-  double aim = 0.0;
-  auto goal = [&](double sum) { return aim = v * sum; };
-  uint32_t c = find_item(a.chunks, chunk_weight, goal, sc, before, all);
+  uint32_t c = find<1>(w, share, sc, before);
   bool plain = false;
   if (c == kNone) {  // nothing is left of p - q: from p
     plain = true;
-    c = find_item(a.chunks, plain_chunk, goal, sc, before, all);
+    w[0] = plain_chunk();
+    c = find<1>(w, share, sc, before);
   }
-  const uint32_t c0 = c == kNone ? 0 : c * kChunk, n = c == kNone ? 0 : min(kChunk, a.vocab - c0);
+  double z[N], inner;
+  const uint32_t i0 = c * kChunk + tid * N;
   const double to = aim - before;
-  const uint32_t i = find_item(
-      n, [&](uint32_t k) { return plain ? token_weight(c0 + k) : rest_weight(c0 + k); },
-      [&](double) { return to; }, sc, inner, unused);
-  if (threadIdx.x == 0) {
-    const uint32_t token = i == kNone ? d.best : c0 + i;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    z[e] = 0.0;
+    const uint32_t i = i0 + e;
+    if (c != kNone && i < a.vocab) {
+      z[e] = token_weight(i, x[i]);
+      if (!plain) {
+        if (REST) {
+          const float q = a.probs[d.row * a.probs_stride + i];
+          z[e] = z[e] * d.inv_total - (q > 0.f ? double(q) : 0.0);
+          z[e] = z[e] > 0.0 ? z[e] : 0.0;
+        } else if (i == skip) {
+          z[e] = 0.0;
+        }
+      }
+    }
+  }
+  const uint32_t in = find<N>(z, [&](double) { return to; }, sc, inner);
+  if (tid == 0) {
+    const uint32_t token = in == kNone ? d.best : c * kChunk + in;
     a.tokens[d.row] = token;
-    if (a.logprobs)
-      a.logprobs[d.row] =
-          d.greedy ? 0.f : float((x[token] == d.top ? 0.0 : (double(x[token]) - double(d.top)) / double(temperature(a, s))) - d.log_total);
+    if (a.logprobs) a.logprobs[d.row] = log_weight(d, x[token], t);
   }
 }
 
@@ -323,70 +318,72 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   constexpr uint32_t BATCH = 64, WAVES = kThreads / 64;
   __shared__ Scratch sc;
   __shared__ DrawRow rows[BATCH];
-  __shared__ float logp[BATCH];
+  __shared__ float drafted[BATCH];  // the draft's logit
   __shared__ uint32_t taken[BATCH];
   const uint32_t s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
+  const float t = temperature(a, s);
   if (r1 <= r0) {
     if (threadIdx.x == 0) {
       a.count[s] = 0;
-      a.draws[s].row = kNone;
+      if (a.probs) a.draws[s].row = kNone;
     }
     return;
   }
-  const float t = temperature(a, s);
   const double k = rate(t);
   int64_t stop = -1;
   for (int64_t b = r0; stop < 0; b += BATCH) {
     const uint32_t n = uint32_t(min(r1 - b, int64_t(BATCH)));
     for (uint32_t i = wave; i < n; i += WAVES) {
       const uint32_t r = uint32_t(b) + i;
-      const ChunkSum* p = a.sums + size_t(r) * a.chunks;
-      float top = -INFINITY;
-      for (uint32_t c = lane; c < a.chunks; c += 64) top = fmaxf(top, p[c].top);
-      top = wave_max(top);
       DrawRow d;
-      d.top = top;
       d.k = k;
-      d.greedy = !(t > 0.f) || !(top > -INFINITY);
       d.row = r;
       d.draft = a.drafts[r];
+      const bool has = r + 1 < r1 && d.draft < a.vocab;
+      const float x = has ? a.logits[r * a.stride + d.draft] : 0.f, u = a.accept[r];
+      float qd = 1.f;
+      if (has && a.probs) qd = a.probs[r * a.probs_stride + d.draft];
+      // each lane joins its chunks as they come, then the lanes
+      float top = -INFINITY;
       uint32_t best = kNone;
       double sum = 0.0;
       for (uint32_t c = lane; c < a.chunks; c += 64) {
-        const ChunkSum z = p[c];
-        if (z.top == top && top > -INFINITY) best = min(best, z.best);
-        if (!d.greedy) sum += z.sum * chunk_scale(z.top, d);
-      }
-#pragma unroll
-      for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
-      d.best = best < a.vocab ? best : 0;  // (top is -inf: the first token)
-      sum = d.greedy ? 1.0 : wave_sum64(sum);
-      d.inv_total = 1.0 / sum;
-      d.log_total = log(sum);
-      if (lane == 0) {
-        rows[i] = d;
-        bool yes = false;
-        if (r + 1 < r1 && d.draft < a.vocab) {
-          const float x = a.logits[r * a.stride + d.draft];
-          const double w = d.greedy ? (d.draft == d.best ? 1.0 : 0.0) : weight(x, top, k);
-          double qd = 1.0;
-          if (a.probs) {
-            const float y = a.probs[r * a.probs_stride + d.draft];
-            qd = y > 0.f ? double(y) : 0.0;
-          }
-          yes = double(a.accept[r]) * qd < w * d.inv_total;
-          logp[i] = d.greedy ? 0.f : float((x == top ? 0.0 : (double(x) - double(top)) / double(t)) - d.log_total);
+        const ChunkSum z = a.sums[size_t(r) * a.chunks + c];
+        if (z.top > top) {
+          sum = sum * (sum == 0.0 ? 0.0 : chunk_scale(top, z.top, k)) + z.sum;
+          top = z.top;
+          best = z.best;
+        } else if (z.top > -INFINITY) {
+          sum += z.sum * chunk_scale(z.top, top, k);
         }
-        taken[i] = yes;
+      }
+      d.top = wave_max(top);
+      d.greedy = !(t > 0.f) || !(d.top > -INFINITY);
+      if (d.greedy) {
+        if (top != d.top) best = kNone;
+#pragma unroll
+        for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
+        sum = 1.0;
+      } else {
+        sum = wave_sum64(sum == 0.0 ? 0.0 : sum * chunk_scale(top, d.top, k));
+      }
+      d.best = best < a.vocab && d.top > -INFINITY && d.greedy ? best : 0;
+      d.total = sum;
+      d.inv_total = 1.0 / sum;
+      if (lane == 0) {
+        const double w = d.greedy ? (d.draft == d.best ? 1.0 : 0.0) : weight(x, d.top, k);
+        rows[i] = d;
+        drafted[i] = x;
+        taken[i] = has && double(u) * (qd > 0.f ? double(qd) : 0.0) < w * d.inv_total;
       }
     }
     __syncthreads();
     uint32_t first = 0;
     while (first < n && taken[first]) first++;
-    for (uint32_t i = threadIdx.x; i < first; i += kThreads) {
-      a.tokens[b + i] = rows[i].draft;
-      if (a.logprobs) a.logprobs[b + i] = logp[i];
+    if (threadIdx.x < first) {
+      a.tokens[b + threadIdx.x] = rows[threadIdx.x].draft;
+      if (a.logprobs) a.logprobs[b + threadIdx.x] = log_weight(rows[threadIdx.x], drafted[threadIdx.x], t);
     }
     if (first < n) stop = b + first;
     else __syncthreads();
@@ -454,7 +451,7 @@ DraftWork draft_work(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab) {
 extern "C" {
 
 uint64_t qe_op_verify_drafts_work_bytes(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab) {
-  if (vocab == 0 || vocab > 0x7FFFFFFFull || n_rows > 0x7FFFFFFFull || n_seqs > 65535) return 0;
+  if (vocab == 0 || vocab > qe::kMostVocab || n_rows > 0x7FFFFFFFull || n_seqs > 65535) return 0;
   return qe::draft_work(n_rows, n_seqs, vocab).bytes;
 }
 
@@ -468,7 +465,7 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
   if (n_rows > 0x7FFFFFFFull) return qe::set_error(QE_ERR_ARG, "need n_rows < 2^31");
   if (!work) return qe::set_error(QE_ERR_ARG, "null argument");
   if (n_rows && (!logits || !drafts || !accept || !tokens_out)) return qe::set_error(QE_ERR_ARG, "null argument");
-  if (vocab == 0 || vocab > 0x7FFFFFFFull) return qe::set_error(QE_ERR_ARG, "need 0 < vocab < 2^31");
+  if (vocab == 0 || vocab > qe::kMostVocab) return qe::set_error(QE_ERR_ARG, "vocab must be 1..%u", qe::kMostVocab);
   if (row_stride < vocab || (draft_probs && probs_stride < vocab) || row_stride > 0xFFFFFFFFull ||
       probs_stride > 0xFFFFFFFFull)
     return qe::set_error(QE_ERR_ARG, "row strides must be at least vocab and below 2^32");

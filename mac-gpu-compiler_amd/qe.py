@@ -512,49 +512,64 @@ def _refuse(message: str) -> None:
     raise QeError(QE_ERR_ARG, message)
 
 
+_torch_module = None
+_row_types = {}  # torch dtype -> QE_KV_*, of rows
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _row_types.update({torch.float32: QE_KV_F32, torch.bfloat16: QE_KV_BF16})
+        _torch_module = torch
+    return _torch_module
 
 
-def _on_stream(stream) -> Optional[int]:
-    return _stream_ptr(_torch().cuda.current_stream() if stream is None else stream)
+def _on_stream(stream, at: int) -> Optional[int]:
+    """the stream's handle; None: torch's current stream on GPU `at`"""
+    if stream is not None:
+        return _stream_ptr(stream)
+    raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)  # a third of the time of current_stream()
+    return raw(at) if raw is not None else _torch().cuda.current_stream(at).cuda_stream
 
 
-def _same_device(first, *tensors) -> None:
-    torch = _torch()
-    if first.device.type != "cuda":
-        _refuse(f"tensors are on {first.device}: device memory is needed")
-    if first.device.index != torch.cuda.current_device():
-        _refuse(f"tensors are on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _same_device(first, *tensors) -> int:
+    """the GPU that all are on, which must be the current one (get_device(): -1 on the host)"""
+    at = first.get_device()
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != at:
             _refuse(f"tensors are on {first.device} and {t.device}")
+    if at < 0:
+        _refuse(f"tensors are on {first.device}: device memory is needed")
+    if at != _torch().cuda.current_device():
+        _refuse(f"tensors are on {first.device}, the current device is cuda:{_torch().cuda.current_device()}")
+    return at
 
 
 def _dense(name: str, t, dtypes, shape) -> None:
     """t has one of the types, is contiguous and has this shape"""
-    if t.dtype not in dtypes or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
         _refuse(f"{name}: need a contiguous {' or '.join(str(d) for d in dtypes)} tensor of shape {tuple(shape)}, "
                 f"got {t.dtype} {tuple(t.shape)}" + ("" if t.is_contiguous() else ", not contiguous"))
 
 
 def _row_dtype(name: str, t) -> int:
-    torch = _torch()
-    if t.dtype == torch.float32:
-        return QE_KV_F32
-    if t.dtype == torch.bfloat16:
-        return QE_KV_BF16
-    _refuse(f"{name}: rows are float32 or bfloat16, got {t.dtype}")
+    _torch()
+    dtype = _row_types.get(t.dtype)
+    if dtype is None:
+        _refuse(f"{name}: rows are float32 or bfloat16, got {t.dtype}")
+    return dtype
 
 
 def _row_stride(name: str, t, heads: int) -> int:
     """distance of the rows of t [rows, heads, 128], whose heads lie one after the other"""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != 128:
-        _refuse(f"{name}: need [rows, {heads}, 128], got {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128)):
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != 128:
+        _refuse(f"{name}: need [rows, {heads}, 128], got {tuple(shape)}")
+    stride = t.stride()
+    if shape[0] and heads and (stride[2] != 1 or (heads > 1 and stride[1] != 128)):
         _refuse(f"{name}: the heads of a row must lie one after the other")
-    return int(t.stride(0)) if t.shape[0] > 1 else heads * 128
+    return stride[0] if shape[0] > 1 else heads * 128
 
 
 class Pages:
@@ -597,6 +612,7 @@ class Pages:
         self.n_kv_heads = n_kv
         self._c = _CPages(*[None if t is None else t.data_ptr() for t in (k, v, k_exp, v_exp, table, lens, starts)],
                           n_pages, size, n_kv, n_seqs, int(table.shape[1]), QE_KV_FP8 if fp8 else QE_KV_BF16)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, table, lens, starts, kv_dtype: int = QE_KV_BF16):
@@ -621,8 +637,8 @@ def _page_rows(call, pages: Pages, k, v, stream) -> None:
     stride = _row_stride("k", k, pages.n_kv_heads)
     if stride != _row_stride("v", v, pages.n_kv_heads):
         _refuse("the rows of k and v must be equally far apart")
-    _same_device(k, v, pages.k)
-    _check(call(ctypes.byref(pages._c), _ptr(k), _ptr(v), k.shape[0], stride, dtype, _on_stream(stream)))
+    at = _same_device(k, v, pages.k)
+    _check(call(pages._ref, _ptr(k), _ptr(v), k.shape[0], stride, dtype, _on_stream(stream, at)))
 
 
 def op_page_append(pages: Pages, k, v, stream=None) -> None:
@@ -651,10 +667,10 @@ def op_page_attention(pages: Pages, q, out, work, max_new: int = 0, stream=None)
         _refuse("work must be contiguous")
     if max_new < 0:
         _refuse("max_new must not be negative")
-    _same_device(q, out, work, pages.k)
-    _check(lib().qe_op_page_attention(ctypes.byref(pages._c), _ptr(q), _ptr(out), q.shape[0], heads,
+    at = _same_device(q, out, work, pages.k)
+    _check(lib().qe_op_page_attention(pages._ref, _ptr(q), _ptr(out), q.shape[0], heads,
                                       _row_stride("q", q, heads), _row_stride("out", out, heads), max_new, dtype,
-                                      _ptr(work), work.numel() * work.element_size(), _on_stream(stream)))
+                                      _ptr(work), work.nbytes, _on_stream(stream, at)))
 
 
 def op_verify_drafts_work_bytes(n_rows: int, n_seqs: int, vocab: int) -> int:
@@ -692,8 +708,8 @@ def op_verify_drafts(logits, starts, drafts, accept, sample, tokens, count, work
         _dense("logprobs", logprobs, f32, (rows,))
     if not work.is_contiguous():
         _refuse("work must be contiguous")
-    _same_device(logits, starts, drafts, accept, sample, tokens, count, work, draft_probs, temperature, logprobs)
+    at = _same_device(logits, starts, drafts, accept, sample, tokens, count, work, draft_probs, temperature, logprobs)
     opt = [None if t is None else _ptr(t) for t in (draft_probs, temperature, logprobs)]
     _check(lib().qe_op_verify_drafts(_ptr(logits), rows, vocab, strides[0], _ptr(starts), n_seqs, _ptr(drafts), opt[0],
                                      strides[1], _ptr(accept), _ptr(sample), opt[1], _ptr(tokens), _ptr(count), opt[2],
-                                     _ptr(work), work.numel() * work.element_size(), _on_stream(stream)))
+                                     _ptr(work), work.nbytes, _on_stream(stream, at)))
