@@ -75,21 +75,39 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 // and 2^f = 1 + f c(f) by Chebyshev interpolation of (2^f - 1) / f at 10 points of [-1/2, 1/2]; n goes
 // straight into the exponent. 2^0 is exactly 1. (The library's exp is some 40 instructions on the same
 // unit, which then bounds the pass instead of the memory.)
+template <int N>
+__device__ __forceinline__ void exp2_64(const double (&t)[N], double (&y)[N]) {
+  constexpr double c[10] = {7.070977866508138e-09,  1.0205905413765595e-07, 1.3215451633221434e-06, 1.5252672924850737e-05,
+                            0.00015403530424776529, 0.0013333558200794592,  0.009618129107618665,   0.05550410866465167,
+                            0.24022650695910075,    0.6931471805599462};
+  double n[N], f[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    n[i] = rint(t[i]);
+    f[i] = t[i] - n[i];
+    y[i] = c[0];
+  }
+  // y f + c with c in a scalar register (the compiler would copy it into the accumulator first, two moves
+  // for each); N chains side by side, since each step waits for the one before
+#pragma unroll
+  for (int k = 1; k < 10; k++)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const double x = y[i];
+      asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y[i]) : "v"(x), "v"(f[i]), "s"(c[k]));
+    }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const double z = fma(y[i], f[i], 1.0);
+    y[i] = __hiloint2double(__double2hiint(z) + (int(fmax(n[i], -1000.0)) << 20), __double2loint(z));
+    y[i] = t[i] >= -1000.0 ? y[i] : 0.0;
+  }
+}
 __device__ __forceinline__ double exp2_64(double t) {
-  const double n = rint(t), f = t - n;
-  double c = 7.070977866508138e-09;
-  c = fma(c, f, 1.0205905413765595e-07);
-  c = fma(c, f, 1.3215451633221434e-06);
-  c = fma(c, f, 1.5252672924850737e-05);
-  c = fma(c, f, 0.00015403530424776529);
-  c = fma(c, f, 0.0013333558200794592);
-  c = fma(c, f, 0.009618129107618665);
-  c = fma(c, f, 0.05550410866465167);
-  c = fma(c, f, 0.24022650695910075);
-  c = fma(c, f, 0.6931471805599462);
-  c = fma(c, f, 1.0);
-  const double y = __hiloint2double(__double2hiint(c) + (int(fmax(n, -1000.0)) << 20), __double2loint(c));
-  return t >= -1000.0 ? y : 0.0;
+  const double x[1] = {t};
+  double y[1];
+  exp2_64<1>(x, y);
+  return y[0];
 }
 
 // weight of logit x relative to the largest one, top: NaN and -inf weigh nothing, infinite ones share
@@ -164,9 +182,20 @@ __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
   double sum = 0.0;
   uint32_t at = kNone;
   if (t > 0.f && m > -INFINITY) {
-    const double k = rate(t);
+    const double k = rate(t), top = double(m);
+    if (m < INFINITY) {
 #pragma unroll
-    for (int i = 0; i < 32; i++) sum += weight(x[i], m, k);
+      for (int i = 0; i < 32; i += 4) {
+        double t4[4], w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) t4[e] = (double(x[i + e]) - top) * k;
+        exp2_64<4>(t4, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) sum += x[i] == m ? 1.0 : 0.0;
+    }
     sum = wave_sum64(sum);
   } else {  // greedy: the first place that holds the largest
 #pragma unroll
@@ -415,11 +444,26 @@ __global__ __launch_bounds__(256) void k_draft_rest(DraftArgs a) {
   load_chunk(a.logits + d.row * a.stride, c * kChunk, a.vocab, -INFINITY, x);
   load_chunk(a.probs + d.row * a.probs_stride, c * kChunk, a.vocab, 0.f, q);
   double sum = 0.0;
+  const uint32_t greedy = __builtin_amdgcn_readfirstlane(d.greedy);
+  const bool usual = !greedy && d.top < INFINITY;
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const uint32_t token = c * kChunk + 256 * (i / 4) + 4 * lane + i % 4;
-    const double w = (d.greedy ? (token == d.best ? 1.0 : 0.0) : weight(x[i], d.top, d.k)) * d.inv_total;
-    sum += q[i] > 0.f ? fmax(w - double(q[i]), 0.0) : w;
+  for (int i = 0; i < 32; i += 4) {
+    double w[4];
+    if (usual) {
+      double t4[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) t4[e] = (double(x[i + e]) - double(d.top)) * d.k;
+      exp2_64<4>(t4, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        w[e] = (greedy ? c * kChunk + 64 * i + 4 * lane + e == d.best : x[i + e] == d.top) ? 1.0 : 0.0;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      w[e] = w[e] * d.inv_total - (q[i + e] > 0.f ? double(q[i + e]) : 0.0);
+      sum += w[e] > 0.0 ? w[e] : 0.0;
+    }
   }
   sum = wave_sum64(sum);
   if (lane == 0) a.rests[size_t(s) * a.chunks + c] = sum;
