@@ -49,12 +49,14 @@ struct AttnArgs {
   uint32_t n_rows, n_heads, group;
   uint32_t group_magic, group_shift;  // r / group = (2 r * magic >> 32) >> shift for r < 2^31
   uint32_t min_blocks;            // a workgroup takes at least so many
+  uint32_t whole_items;           // 1: an item counts as one block and is never cut
   float c;                        // log2(e) / sqrt(128)
 };
 
 // An item whose first part is the last one of a workgroup: parts of `n` workgroups from there.
 struct Joint {
-  uint32_t n, seq, head, tile;
+  uint32_t n, rows, head, first;  // rows of the tile; the first of them among its sequence's rows
+  int32_t row0;                   // first packed row of the sequence
 };
 
 __device__ __forceinline__ uint32_t token_of(const AttnArgs& a, uint32_t r) {  // r / group
@@ -95,11 +97,13 @@ __device__ __forceinline__ uint32_t tile_limit(const AttnArgs& a, const Seq& q, 
 }
 // A tile that attends nothing still counts one block: its rows are zeros that someone writes.
 __device__ __forceinline__ uint32_t tile_blocks(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
-  return max((tile_limit(a, q, tile, R) + kBlock - 1) / kBlock, 1u);
+  return a.whole_items ? 1 : max((tile_limit(a, q, tile, R) + kBlock - 1) / kBlock, 1u);
 }
 __device__ uint64_t seq_blocks(const AttnArgs& a, const Seq& q, uint32_t R) {
   uint64_t n = 0;
-  for (uint32_t i = 0, t = q.tiles(R); i < t; i++) n += tile_blocks(a, q, i, R);
+  const uint32_t t = q.tiles(R);
+  if (a.whole_items) return t;
+  for (uint32_t i = 0; i < t; i++) n += tile_blocks(a, q, i, R);
   return n;
 }
 
@@ -111,9 +115,7 @@ struct Cursor {
 
 struct PlanShared {
   uint64_t sum[512];
-  uint32_t per;   // blocks of a workgroup
-  uint32_t mine;  // of this one: fewer for the last, 0 behind it
-  Cursor at;      // where they start
+  Cursor at;
 };
 
 // The next tile with rows after `cu`'s (false: there is none).
@@ -133,53 +135,20 @@ __device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_
   return true;
 }
 
-// Workgroup w's part of the list, of W parts of `per` blocks, into sh. (A part is far below 2^32 blocks:
-// that many are 70 TB of K and V.)
-// Each thread sums a contiguous range of sequences; the one whose range holds the block walks it.
-__device__ void find_start(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh) {
-  const uint32_t t = threadIdx.x, T = blockDim.x, each = (a.p.n_seqs + T - 1) / T;
-  const uint32_t s0 = min(t * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
-  uint64_t mine = 0;
-  for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
-  mine *= a.p.n_kv;
-  sh.sum[t] = mine;
-  __syncthreads();
-  for (uint32_t d = 1; d < T; d *= 2) {
-    const uint64_t v = t >= d ? sh.sum[t - d] : 0;
-    __syncthreads();
-    sh.sum[t] += v;
-    __syncthreads();
+// The block `at` blocks into the list of sequence s's.
+__device__ __forceinline__ Cursor cursor_in(const AttnArgs& a, uint32_t s, const Seq& q, uint64_t one, uint64_t at, uint32_t R) {
+  Cursor cu;
+  cu.q = q;
+  cu.seq = s;
+  cu.head = uint32_t(at / one);
+  uint64_t rest = at % one;
+  cu.tile = 0;
+  while (rest >= (cu.blocks = tile_blocks(a, q, cu.tile, R))) {
+    rest -= cu.blocks;
+    cu.tile++;
   }
-  const uint64_t total = sh.sum[T - 1];
-  const uint64_t even = (total + W - 1) / W, per = even > a.min_blocks ? even : a.min_blocks;
-  const uint64_t at = w * per;
-  if (t == 0) {
-    sh.per = uint32_t(per);
-    sh.mine = at < total ? uint32_t(min(per, total - at)) : 0;
-  }
-  uint64_t before = sh.sum[t] - mine;
-  if (at >= before && at < sh.sum[t]) {
-    Cursor cu;
-    for (uint32_t s = s0; s < s1; s++) {
-      cu.q = read_seq(a, s);
-      const uint64_t one = seq_blocks(a, cu.q, R);
-      if (at < before + one * a.p.n_kv) {
-        cu.seq = s;
-        cu.head = uint32_t((at - before) / one);
-        uint64_t rest = (at - before) % one;
-        cu.tile = 0;
-        while (rest >= (cu.blocks = tile_blocks(a, cu.q, cu.tile, R))) {
-          rest -= cu.blocks;
-          cu.tile++;
-        }
-        cu.block = uint32_t(rest);
-        break;
-      }
-      before += one * a.p.n_kv;
-    }
-    sh.at = cu;
-  }
-  __syncthreads();
+  cu.block = uint32_t(rest);
+  return cu;
 }
 
 // A value that all lanes hold, in a scalar register: what comes out of LDS would stay in vector
@@ -196,6 +165,82 @@ __device__ __forceinline__ Cursor uniform(const Cursor& c) {
   u.block = uniform(c.block);
   u.blocks = uniform(c.blocks);
   return u;
+}
+
+// Workgroup w's part of the list, of W parts of `per` blocks: where it begins and how many blocks it has
+// (0: none). (A part is far below 2^32 blocks: that many are 70 TB of K and V.) A wave finds it alone where a
+// lane can have a sequence each; else each thread sums a contiguous range of sequences, and the one whose
+// range holds the block walks it.
+__device__ __forceinline__ uint32_t find_part(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
+                                              uint32_t& per_out, Cursor& cu) {
+  const uint32_t tid = threadIdx.x;
+  auto split = [&](uint64_t total) {
+    const uint64_t even = (total + W - 1) / W;
+    return even > a.min_blocks ? even : uint64_t(a.min_blocks);
+  };
+  if (a.p.n_seqs <= 64) {
+    const uint32_t lane = tid & 63;
+    Seq q{};
+    uint64_t one = 0;
+    if (lane < a.p.n_seqs) {
+      q = read_seq(a, lane);
+      one = seq_blocks(a, q, R);
+    }
+    uint64_t up_to = one * a.p.n_kv;
+    const uint64_t mine = up_to;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint64_t v = __shfl_up(up_to, d);
+      if (int(lane) >= d) up_to += v;
+    }
+    const uint64_t total = __shfl(up_to, 63), per = split(total), at = w * per;
+    per_out = uniform(uint32_t(per));
+    if (at >= total) return 0;
+    const bool here = at < up_to && at >= up_to - mine;
+    if (here) cu = cursor_in(a, lane, q, one, at - (up_to - mine), R);
+    const uint32_t owner = uniform(uint32_t(__builtin_ctzll(__ballot(here))));
+    auto from = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(owner))); };
+    cu.q.first = int32_t(from(uint32_t(cu.q.first)));
+    cu.q.row0 = int32_t(from(uint32_t(cu.q.row0)));
+    cu.q.rows = from(cu.q.rows);
+    cu.seq = from(cu.seq);
+    cu.head = from(cu.head);
+    cu.tile = from(cu.tile);
+    cu.block = from(cu.block);
+    cu.blocks = from(cu.blocks);
+    return uniform(uint32_t(per < total - at ? per : total - at));
+  }
+  const uint32_t T = blockDim.x, each = (a.p.n_seqs + T - 1) / T;
+  const uint32_t s0 = min(tid * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
+  uint64_t mine = 0;
+  for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
+  mine *= a.p.n_kv;
+  sh.sum[tid] = mine;
+  __syncthreads();
+  for (uint32_t d = 1; d < T; d *= 2) {
+    const uint64_t v = tid >= d ? sh.sum[tid - d] : 0;
+    __syncthreads();
+    sh.sum[tid] += v;
+    __syncthreads();
+  }
+  const uint64_t total = sh.sum[T - 1], per = split(total), at = w * per;
+  uint64_t before = sh.sum[tid] - mine;
+  if (at >= before && at < sh.sum[tid]) {
+    for (uint32_t s = s0; s < s1; s++) {
+      const Seq q = read_seq(a, s);
+      const uint64_t one = seq_blocks(a, q, R);
+      if (at < before + one * a.p.n_kv) {
+        sh.at = cursor_in(a, s, q, one, at - before, R);
+        break;
+      }
+      before += one * a.p.n_kv;
+    }
+  }
+  __syncthreads();
+  per_out = uniform(uint32_t(per));
+  if (at >= total) return 0;
+  cu = uniform(sh.at);
+  return uniform(uint32_t(per < total - at ? per : total - at));
 }
 
 // a workgroup's place in the list: consecutive parts on one XCD (workgroups go to the 8 XCDs in turn)
@@ -369,12 +414,14 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t w = part_index();
-  find_start(a, w, gridDim.x, R, sh);
-  if (tid == 0) a.joints[w].n = 0;
-  uint32_t left = uniform(sh.mine);
+  Cursor cu;
+  uint32_t per;
+  uint32_t left = uniform(find_part(a, w, gridDim.x, R, sh, per, cu));
+  cu = uniform(cu);
+  per = uniform(per);
+  if (tid == 0 && !a.whole_items) a.joints[w].n = 0;
   if (left == 0) return;
-  const uint32_t per = uniform(sh.per), whole_part = left;
-  Cursor cu = uniform(sh.at);
+  const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
   float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
 
@@ -383,7 +430,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
     const uint32_t rows = min(cu.q.rows - cu.tile * R, uint32_t(R));
     // the positions of this part, in steps
-    const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
+    const uint32_t first = cu.block * kBlock, last = a.whole_items ? limit : min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // the least position any row attends up to: below it no score is masked
     const int32_t free_to = row_position(a, cu.q, cu.tile * R);
@@ -392,6 +439,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     bf16x8 qf[NQ][4][NS];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
+      const uint32_t lane = afresh(tid & 63), col = lane & 15, g = lane >> 4;
       const uint32_t r = cu.tile * R + 16 * n + col;
       const bool real = r < cu.q.rows;
       row_pos[n] = real ? row_position(a, cu.q, r) : -1;
@@ -435,7 +483,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
         for (int j = 0; j < 8 / NT; j++)
           d.k[t * (8 / NT) + j] = *reinterpret_cast<const u32x4*>(ka + t * 4 * kPageDim * EL + 64 * j);
 #pragma unroll
-      for (int i = 0; i < 8; i++) d.v[i] = *reinterpret_cast<const u32x4*>(va + i * 256 * EL);
+      for (int i = 0; i < 8; i++) d.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(va + i * 256 * EL));
       if constexpr (FP8) {
         d.ke = *reinterpret_cast<const u32x4*>(a.st.k_exp + kr);
         d.ve = *reinterpret_cast<const u32x4*>(a.st.v_exp + vr);
@@ -586,52 +634,55 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
       }
     }
 
-    // the four waves' sums meet in LDS, in wave order
-    __syncthreads();  // the part before has been read
+    {
+      const uint32_t tid = afresh(threadIdx.x), lane = tid & 63, col = lane & 15, g = lane >> 4;
+      // the four waves' sums meet in LDS, in wave order
+      __syncthreads();  // the part before has been read
 #pragma unroll
-    for (int n = 0; n < NQ; n++) {
-      const float s = add_groups(l[n]);
-      if (g == 0) {
-        top[wave][16 * n + col] = m[n];
-        mass[wave][16 * n + col] = s;
-      }
-#pragma unroll
-      for (int t = 0; t < 8; t++) *reinterpret_cast<f32x4*>(&sums[wave][16 * n + col][16 * t + 4 * g]) = acc[n][t];
-    }
-    __syncthreads();
-    const bool whole = cu.block == 0 && take == cu.blocks;
-    float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);  // slot 1 begins an item, 0 goes on with one
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-      const uint32_t r = 16 * n + tid / 16, d = (tid % 16) * 8;
-      if (r < rows) {
-        float mx = top[0][r];
-        for (int i = 1; i < 4; i++) mx = fmaxf(mx, top[i][r]);
-        float o[8] = {}, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float f = rebase(top[i][r], mx);
-          sum = fmaf(mass[i][r], f, sum);
-#pragma unroll
-          for (int e = 0; e < 8; e++) o[e] = fmaf(sums[i][r][d + e], f, o[e]);
+      for (int n = 0; n < NQ; n++) {
+        const float s = add_groups(l[n]);
+        if (g == 0) {
+          top[wave][16 * n + col] = m[n];
+          mass[wave][16 * n + col] = s;
         }
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-          for (int e = 0; e < 8; e++) o[e] *= inv;
-          store_out8<BF16_ROWS>(a.out, row_element(a, cu.q, head, cu.tile * R + r, a.out_stride) + d, o);
-        } else {
-          *reinterpret_cast<f32x4*>(part + r * kPageDim + d) = f32x4{o[0], o[1], o[2], o[3]};
-          *reinterpret_cast<f32x4*>(part + r * kPageDim + d + 4) = f32x4{o[4], o[5], o[6], o[7]};
-          if (d == 0) {
-            part[R * kPageDim + r] = mx;
-            part[R * kPageDim + R + r] = sum;
+        for (int t = 0; t < 8; t++) *reinterpret_cast<f32x4*>(&sums[wave][16 * n + col][16 * t + 4 * g]) = acc[n][t];
+      }
+      __syncthreads();
+      const bool whole = cu.block == 0 && take == cu.blocks;
+      float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);  // slot 1 begins an item, 0 goes on with one
+#pragma unroll
+      for (int n = 0; n < NQ; n++) {
+        const uint32_t r = 16 * n + tid / 16, d = (tid % 16) * 8;
+        if (r < rows) {
+          float mx = top[0][r];
+          for (int i = 1; i < 4; i++) mx = fmaxf(mx, top[i][r]);
+          float o[8] = {}, sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float f = rebase(top[i][r], mx);
+            sum = fmaf(mass[i][r], f, sum);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = fmaf(sums[i][r][d + e], f, o[e]);
+          }
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] *= inv;
+            store_out8<BF16_ROWS>(a.out, row_element(a, cu.q, head, cu.tile * R + r, a.out_stride) + d, o);
+          } else {
+            *reinterpret_cast<f32x4*>(part + r * kPageDim + d) = f32x4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f32x4*>(part + r * kPageDim + d + 4) = f32x4{o[4], o[5], o[6], o[7]};
+            if (d == 0) {
+              part[R * kPageDim + r] = mx;
+              part[R * kPageDim + R + r] = sum;
+            }
           }
         }
       }
+      if (!whole && cu.block == 0 && tid == 0)  // the item's last block is in the part (...) / per after this one
+        a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, min(cu.q.rows - cu.tile * R, uint32_t(R)), cu.head, cu.tile * R, cu.q.row0};
     }
-    if (!whole && cu.block == 0 && tid == 0)  // the item's last block is in the part (...) / per after this one
-      a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
     left -= take;
     if (left == 0 || !next_tile(a, cu, R)) break;
   }
@@ -667,19 +718,21 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t w = part_index();
-  find_start(a, w, gridDim.x, R, sh);
-  if (tid == 0) a.joints[w].n = 0;
-  uint32_t left = uniform(sh.mine);
+  Cursor cu;
+  uint32_t per;
+  uint32_t left = uniform(find_part(a, w, gridDim.x, R, sh, per, cu));
+  cu = uniform(cu);
+  per = uniform(per);
+  if (tid == 0 && !a.whole_items) a.joints[w].n = 0;
   if (left == 0) return;
-  const uint32_t per = uniform(sh.per), whole_part = left;
-  Cursor cu = uniform(sh.at);
+  const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
   float* const my_parts = a.parts + size_t(w) * 2 * R * kPartRow;
 
   while (true) {
     const uint32_t take = min(cu.blocks - cu.block, left);
     const uint32_t limit = tile_limit(a, cu.q, cu.tile, R);
-    const uint32_t first = cu.block * kBlock, last = min((cu.block + take) * kBlock, limit);
+    const uint32_t first = cu.block * kBlock, last = a.whole_items ? limit : min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // this wave's rows, and the positions that all of them (free_to) and some of them (end) attend
     const uint32_t wr0 = cu.tile * R + 32 * wave;
@@ -687,14 +740,14 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     const int32_t free_to = row_position(a, cu.q, wr0);
     const uint32_t end = wrows ? row_limit(a, cu.q, wr0 + wrows - 1) : 0;
     const int32_t tile_free = row_position(a, cu.q, cu.tile * R);  // all rows of the tile attend up to it
-    const uint32_t r = wr0 + col;
-    const bool real = col < wrows;
+    const uint32_t fresh = afresh(tid & 63), r = wr0 + (fresh & 31);
+    const bool real = (fresh & 31) < wrows;
     const int32_t row_pos = real ? row_position(a, cu.q, r) : -1;
     bf16x8 qf[8][NS];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       float x[8] = {};
-      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * half, x);
+      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * (fresh >> 5), x);
       split_bf16<NS>(x, qf[j]);
     }
     f32x16 acc[4];
@@ -988,7 +1041,7 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
           }
         }
         if (cu.block == 0 && tid == 0)
-          a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, cu.seq, cu.head, cu.tile};
+          a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, min(cu.q.rows - cu.tile * R, uint32_t(R)), cu.head, cu.tile * R, cu.q.row0};
       }
     }
     left -= take;
@@ -1007,8 +1060,7 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const uint32_t w = blockIdx.x, tid = threadIdx.x;
   const Joint j = a.joints[w];
   if (j.n == 0) return;
-  const Seq q = read_seq(a, j.seq);
-  const uint32_t rows = min(q.rows - j.tile * R, R), r0 = blockIdx.y * 16;
+  const uint32_t rows = j.rows, r0 = blockIdx.y * 16;
   if (r0 >= rows) return;
   const uint32_t here = min(rows - r0, 16u);
   uint32_t slots = 1;
@@ -1022,20 +1074,43 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const bool real = r < rows;
   float mx = -INFINITY, sum = 0.f, o[8] = {};
   if (real) {
-#pragma unroll 4
-    for (uint32_t i = me; i < j.n; i += share)
-      mx = fmaxf(mx, a.parts[(2 * size_t(w + i) + (i == 0)) * slot + R * kPageDim + r]);
-#pragma unroll 4
-    for (uint32_t i = me; i < j.n; i += share) {
-      const float* part = a.parts + (2 * size_t(w + i) + (i == 0)) * slot;
-      const float f = rebase(part[R * kPageDim + r], mx);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(part + e0), y = *reinterpret_cast<const f32x4*>(part + e1);
-      sum = fmaf(part[R * kPageDim + R + r], f, sum);
+    // a few parts at a time, all their loads together
+    constexpr uint32_t AT = 4;
+    for (uint32_t i0 = me; i0 < j.n; i0 += AT * share) {
+      float pm[AT], pl[AT];
+      f32x4 x[AT], y[AT];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        o[e] = fmaf(x[e], f, o[e]);
-        o[e + 4] = fmaf(y[e], f, o[e + 4]);
+      for (uint32_t b = 0; b < AT; b++) {
+        const uint32_t i = i0 + b * share;
+        pm[b] = -INFINITY;
+        pl[b] = 0.f;
+        x[b] = y[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (i < j.n) {
+          const float* part = a.parts + (2 * size_t(w + i) + (i == 0)) * slot;
+          pm[b] = part[R * kPageDim + r];
+          pl[b] = part[R * kPageDim + R + r];
+          x[b] = *reinterpret_cast<const f32x4*>(part + e0);
+          y[b] = *reinterpret_cast<const f32x4*>(part + e1);
+        }
       }
+      float top = mx;
+#pragma unroll
+      for (uint32_t b = 0; b < AT; b++) top = fmaxf(top, pm[b]);
+      float f = rebase(mx, top);
+      sum *= f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] *= f;
+#pragma unroll
+      for (uint32_t b = 0; b < AT; b++) {
+        f = rebase(pm[b], top);
+        sum = fmaf(pl[b], f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          o[e] = fmaf(x[b][e], f, o[e]);
+          o[e + 4] = fmaf(y[b][e], f, o[e + 4]);
+        }
+      }
+      mx = top;
     }
   }
   if constexpr (!TILES) {
@@ -1069,7 +1144,9 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 8; e++) o[e] *= inv;
-  store_out8<BF16_ROWS>(a.out, row_element(a, q, j.head, j.tile * R + r, a.out_stride) + d, o);
+  Seq q;
+  q.row0 = j.row0;
+  store_out8<BF16_ROWS>(a.out, row_element(a, q, j.head, j.first + r, a.out_stride) + d, o);
 }
 
 constexpr uint32_t kWorkgroups = 512;  // two for each CU
@@ -1080,12 +1157,16 @@ constexpr uint32_t kWorkgroups = 512;  // two for each CU
 struct Cut {
   uint32_t rows, workgroups;
 };
-Cut cut_of(uint64_t max_new, uint64_t group, bool bf16) {
+Cut cut_of(uint64_t max_new, uint64_t group, bool bf16, uint64_t seq_heads) {
   const uint64_t most = max_new && max_new < 256 ? max_new * group : 256;
-  if (most <= 32) return {most <= 16 ? 16u : 32u, kWorkgroups};
+  // few rows: two workgroups for each CU where there are as many items (64 x 8 of 4.6k positions 113 us, so 117
+  // with one), one where items are cut up all the same (16 x 8: 39 us with two, so 29)
+  if (most <= 32) return {most <= 16 ? 16u : 32u, seq_heads >= kWorkgroups ? kWorkgroups : kWorkgroups / 2};
   if (!bf16) return {128, kWorkgroups / 2};
   return most <= 128 ? Cut{128, kWorkgroups} : Cut{256, kWorkgroups / 2};
 }
+// Up to so many positions in a table's row an item is not cut: no join.
+constexpr uint64_t kWholeItems = 512;
 
 }  // namespace
 }  // namespace qe
@@ -1096,7 +1177,7 @@ uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, 
   if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
   uint64_t rows = 0;  // of all workgroups
   for (bool bf16 : {false, true}) {
-    const qe::Cut c = qe::cut_of(max_new, n_heads / n_kv_heads, bf16);
+    const qe::Cut c = qe::cut_of(max_new, n_heads / n_kv_heads, bf16, ~0ull);
     rows = rows > uint64_t(c.rows) * c.workgroups ? rows : uint64_t(c.rows) * c.workgroups;
   }
   return rows * 2 * qe::kPartRow * 4 + qe::kWorkgroups * sizeof(qe::Joint);
@@ -1135,10 +1216,11 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   while ((1ull << a.group_shift) < a.group) a.group_shift++;
   a.group_magic = uint32_t(((1ull << (31 + a.group_shift)) + a.group - 1) / a.group);
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
-  a.min_blocks = 4;
+  a.whole_items = pages->table_stride * pages->page_size <= qe::kWholeItems;
+  a.min_blocks = a.whole_items ? 1 : 4;
   a.joints = static_cast<qe::Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
-  const qe::Cut c = qe::cut_of(max_new, a.group, bf16);
+  const qe::Cut c = qe::cut_of(max_new, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
   const uint32_t R = c.rows, grid = c.workgroups;
   auto go = [&](auto* kern) { kern<<<grid, R == 256 ? 512 : 256, 0, st>>>(a); };
   if (R == 256) {
@@ -1153,10 +1235,12 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
     if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 1> : qe::k_page_attn_rows<true, false, 1>);
     else go(bf16 ? qe::k_page_attn_rows<false, true, 1> : qe::k_page_attn_rows<false, false, 1>);
   }
-  const dim3 join(grid, R / 16);
-  auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
-  if (R >= 128) join_by(bf16 ? qe::k_page_join<true, true> : qe::k_page_join<false, true>);
-  else join_by(bf16 ? qe::k_page_join<true, false> : qe::k_page_join<false, false>);
+  if (!a.whole_items) {
+    const dim3 join(grid, R / 16);
+    auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
+    if (R >= 128) join_by(bf16 ? qe::k_page_join<true, true> : qe::k_page_join<false, true>);
+    else join_by(bf16 ? qe::k_page_join<true, false> : qe::k_page_join<false, false>);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page attention launch failed: %s", hipGetErrorString(e));
   return QE_OK;
