@@ -744,12 +744,6 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     const bool real = (fresh & 31) < wrows;
     const int32_t row_pos = real ? row_position(a, cu.q, r) : -1;
     bf16x8 qf[8][NS];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      float x[8] = {};
-      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * (fresh >> 5), x);
-      split_bf16<NS>(x, qf[j]);
-    }
     f32x16 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; t++)
@@ -946,11 +940,21 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     };
 
     __syncthreads();  // the buffers' last readers are done
+    // e4m3: block x is in LDS and x + 1 in registers when x is multiplied; bf16: STAGES - 1 are on their way.
+    // The first one's loads are under way while q is read.
     if (first < last) {
-      // e4m3: block x is in LDS and x + 1 in registers when x is multiplied; bf16: STAGES - 1 are on their way
       fetch(first, 0, page_at(first + 16 * run));
+      if (!FP8 && STAGES == 3 && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float x[8] = {};
+      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * (fresh >> 5), x);
+      split_bf16<NS>(x, qf[j]);
+    }
+    if (first < last) {
       widen(0);
-      if ((FP8 || STAGES == 3) && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
+      if (FP8 && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
       if (tid == 0) foul[0] = 0;
       constexpr uint32_t AHEAD = FP8 || STAGES == 3 ? 2 : 1;
       uint32_t b = 0, there = pages_there(first);
@@ -1075,7 +1079,7 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   float mx = -INFINITY, sum = 0.f, o[8] = {};
   if (real) {
     // a few parts at a time, all their loads together
-    constexpr uint32_t AT = 4;
+    constexpr uint32_t AT = TILES ? 8 : 4;
     for (uint32_t i0 = me; i0 < j.n; i0 += AT * share) {
       float pm[AT], pl[AT];
       f32x4 x[AT], y[AT];
