@@ -35,6 +35,7 @@ constexpr uint32_t kBlock = 64;    // positions
 // Weights are 2^(score - m) with m the largest score so far, or up to kSlack below it: sums are only put
 // on a new m when a score exceeds it by that much (in some row of 32 one is a little larger in most blocks).
 constexpr float kSlack = 8.f;
+constexpr uint32_t kWholeBlocks = 32;
 constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
@@ -48,8 +49,9 @@ struct AttnArgs {
   struct Joint* joints;           // [workgroup]
   uint32_t n_rows, n_heads, group;
   uint32_t group_magic, group_shift;  // r / group = (2 r * magic >> 32) >> shift for r < 2^31
-  uint32_t min_blocks;            // a workgroup takes at least so many
-  uint32_t whole_items;           // 1: an item counts as one block and is never cut
+  uint32_t whole_items;           // 1: an item counts as one block and is never cut (a call without a join says
+                                  // so; else each workgroup finds out by the lengths)
+  uint32_t join;                  // a join follows
   float c;                        // log2(e) / sqrt(128)
 };
 
@@ -171,29 +173,41 @@ __device__ __forceinline__ Cursor uniform(const Cursor& c) {
 // (0: none). (A part is far below 2^32 blocks: that many are 70 TB of K and V.) A wave finds it alone where a
 // lane can have a sequence each; else each thread sums a contiguous range of sequences, and the one whose
 // range holds the block walks it.
-__device__ __forceinline__ uint32_t find_part(const AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
+// Items that are short and about as many as the workgroups are not cut but dealt out whole: a second piece
+// costs a workgroup some 4 us (its q, its first loads, its sums through LDS and the join). The longest up to
+// 32 blocks and up to twice a workgroup's share: 32 x 8 heads of up to 1000 positions 24 us cut, so 14; up to
+// 2000 34 and 23; 4 x 8 of up to 2000 (13 times the share) 15 cut, 20 so; 64 x 8 of up to 4000 59 and 63.
+__device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
                                               uint32_t& per_out, Cursor& cu) {
   const uint32_t tid = threadIdx.x;
-  auto split = [&](uint64_t total) {
-    const uint64_t even = (total + W - 1) / W;
-    return even > a.min_blocks ? even : uint64_t(a.min_blocks);
-  };
+  auto split = [&](uint64_t total) { return (total + W - 1) / W; };
+  auto fits = [&](uint32_t longest, uint64_t total) { return longest <= kWholeBlocks && longest <= 2 * split(total); };
   if (a.p.n_seqs <= 64) {
     const uint32_t lane = tid & 63;
     Seq q{};
-    uint64_t one = 0;
+    uint64_t one = 0, up_to = 0, mine = 0, total = 0;
+    uint32_t longest = 0;
     if (lane < a.p.n_seqs) {
       q = read_seq(a, lane);
       one = seq_blocks(a, q, R);
+      if (q.rows) longest = tile_blocks(a, q, q.tiles(R) - 1, R);
     }
-    uint64_t up_to = one * a.p.n_kv;
-    const uint64_t mine = up_to;
+    auto sum = [&]() __attribute__((always_inline)) {
+      up_to = mine = one * a.p.n_kv;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint64_t v = __shfl_up(up_to, d);
-      if (int(lane) >= d) up_to += v;
+      for (int d = 1; d < 64; d *= 2) {
+        const uint64_t v = __shfl_up(up_to, d);
+        if (int(lane) >= d) up_to += v;
+      }
+      total = __shfl(up_to, 63);
+    };
+    sum();
+    if (!a.whole_items && !__any(!fits(longest, total))) {
+      a.whole_items = 1;
+      one = seq_blocks(a, q, R);
+      sum();
     }
-    const uint64_t total = __shfl(up_to, 63), per = split(total), at = w * per;
+    const uint64_t per = split(total), at = w * per;
     per_out = uniform(uint32_t(per));
     if (at >= total) return 0;
     const bool here = at < up_to && at >= up_to - mine;
@@ -213,17 +227,31 @@ __device__ __forceinline__ uint32_t find_part(const AttnArgs& a, uint32_t w, uin
   const uint32_t T = blockDim.x, each = (a.p.n_seqs + T - 1) / T;
   const uint32_t s0 = min(tid * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
   uint64_t mine = 0;
-  for (uint32_t s = s0; s < s1; s++) mine += seq_blocks(a, read_seq(a, s), R);
-  mine *= a.p.n_kv;
-  sh.sum[tid] = mine;
-  __syncthreads();
-  for (uint32_t d = 1; d < T; d *= 2) {
-    const uint64_t v = tid >= d ? sh.sum[tid - d] : 0;
+  uint32_t longest = 0;
+  auto sum = [&]() __attribute__((always_inline)) {
+    mine = 0;
+    for (uint32_t s = s0; s < s1; s++) {
+      const Seq q = read_seq(a, s);
+      mine += seq_blocks(a, q, R);
+      if (q.rows) longest = max(longest, tile_blocks(a, q, q.tiles(R) - 1, R));
+    }
+    mine *= a.p.n_kv;
+    sh.sum[tid] = mine;
     __syncthreads();
-    sh.sum[tid] += v;
-    __syncthreads();
+    for (uint32_t d = 1; d < T; d *= 2) {
+      const uint64_t v = tid >= d ? sh.sum[tid - d] : 0;
+      __syncthreads();
+      sh.sum[tid] += v;
+      __syncthreads();
+    }
+    return sh.sum[T - 1];
+  };
+  uint64_t total = sum();
+  if (!a.whole_items && !__syncthreads_or(!fits(longest, total))) {
+    a.whole_items = 1;
+    total = sum();
   }
-  const uint64_t total = sh.sum[T - 1], per = split(total), at = w * per;
+  const uint64_t per = split(total), at = w * per;
   uint64_t before = sh.sum[tid] - mine;
   if (at >= before && at < sh.sum[tid]) {
     for (uint32_t s = s0; s < s1; s++) {
@@ -419,7 +447,8 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
   uint32_t left = uniform(find_part(a, w, gridDim.x, R, sh, per, cu));
   cu = uniform(cu);
   per = uniform(per);
-  if (tid == 0 && !a.whole_items) a.joints[w].n = 0;
+  a.whole_items = uniform(a.whole_items);
+  if (tid == 0 && a.join) a.joints[w].n = 0;
   if (left == 0) return;
   const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
@@ -723,7 +752,8 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
   uint32_t left = uniform(find_part(a, w, gridDim.x, R, sh, per, cu));
   cu = uniform(cu);
   per = uniform(per);
-  if (tid == 0 && !a.whole_items) a.joints[w].n = 0;
+  a.whole_items = uniform(a.whole_items);
+  if (tid == 0 && a.join) a.joints[w].n = 0;
   if (left == 0) return;
   const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
@@ -1169,8 +1199,9 @@ Cut cut_of(uint64_t max_new, uint64_t group, bool bf16, uint64_t seq_heads) {
   if (!bf16) return {128, kWorkgroups / 2};
   return most <= 128 ? Cut{128, kWorkgroups} : Cut{256, kWorkgroups / 2};
 }
-// Up to so many positions in a table's row an item is not cut: no join.
-constexpr uint64_t kWholeItems = 512;
+// Up to so many positions in a table's row no item of few rows is cut, and no join follows (one row at 197
+// positions 9.0 us, so 10.6 with it; at 500 12.0 and 10.7; f32 tiles of 128 rows at 250 23 and 19).
+constexpr uint64_t kWholeItems = 256;
 
 }  // namespace
 }  // namespace qe
@@ -1220,12 +1251,12 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   while ((1ull << a.group_shift) < a.group) a.group_shift++;
   a.group_magic = uint32_t(((1ull << (31 + a.group_shift)) + a.group - 1) / a.group);
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
-  a.whole_items = pages->table_stride * pages->page_size <= qe::kWholeItems;
-  a.min_blocks = a.whole_items ? 1 : 4;
   a.joints = static_cast<qe::Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
   const qe::Cut c = qe::cut_of(max_new, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
   const uint32_t R = c.rows, grid = c.workgroups;
+  a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= qe::kWholeItems;
+  a.join = !a.whole_items;
   auto go = [&](auto* kern) { kern<<<grid, R == 256 ? 512 : 256, 0, st>>>(a); };
   if (R == 256) {
     go(fp8 ? qe::k_page_attn_tiles<true, true, 8> : qe::k_page_attn_tiles<false, true, 8>);
@@ -1239,7 +1270,7 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
     if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 1> : qe::k_page_attn_rows<true, false, 1>);
     else go(bf16 ? qe::k_page_attn_rows<false, true, 1> : qe::k_page_attn_rows<false, false, 1>);
   }
-  if (!a.whole_items) {
+  if (a.join) {
     const dim3 join(grid, R / 16);
     auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
     if (R >= 128) join_by(bf16 ? qe::k_page_join<true, true> : qe::k_page_join<false, true>);
