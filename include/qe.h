@@ -267,7 +267,8 @@ int qe_op_read_sum_nt(const float* src, uint64_t n, float* partial, uint32_t gri
  *   v [n_pages][n_kv_heads][page_size / 16][128][16]: each 16 positions transposed, the form in
  *     which the matrix cores take V
  * and, with QE_KV_FP8, one exponent byte e per position and KV head in k_exp and v_exp
- * [n_pages][n_kv_heads][page_size]: the row's values are the stored ones times 2^(e - 127).
+ * [n_pages][n_kv_heads][page_size]: the row's values are the stored ones times 2^(e - 127), e from
+ * 1 to 254.
  * The plan of a call is device memory too, read when the call runs: row s of `table` names the
  * pages of sequence s in order, lens[s] is its length with the call's new tokens, and the packed
  * rows starts[s] .. starts[s + 1] are its new tokens, the last of them at position lens[s] - 1
@@ -296,7 +297,7 @@ uint64_t qe_page_bytes(uint64_t n_pages, uint64_t page_size, uint64_t n_kv_heads
  * nearest value. e4m3 pages: the exponent is the smallest for which the row's largest finite
  * magnitude is at most 448 of its scale, the values are the nearest (ties to even), and infinities
  * and NaN become NaN. A position whose page is not there is not written. Two rows for one position
- * of one page: either may win. n_rows = 0 does nothing. */
+ * of one page: either may win. n_rows below 2^28; 0 does nothing. */
 int qe_op_page_append(const qe_pages* pages, const void* k, const void* v, uint64_t n_rows, uint64_t row_stride,
                       int dtype, void* stream);
 /* The same rows out of the pages (arguments as qe_op_page_append; k and v are written): zeros where
@@ -309,6 +310,8 @@ int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, ui
  * of `dtype` (QE_KV_F32 or QE_KV_BF16), rows q_stride and out_stride elements apart, 16-byte
  * aligned; out must not overlap q or the pages. n_heads is a multiple of n_kv_heads. Softmax and
  * sums are f32; f32 rows keep f32's precision, bf16 rows take the softmax weights rounded to bf16.
+ * A position that a row does not attend has no part in it, whatever K and V hold there; infinities
+ * and NaN where it does attend may make it either.
  * max_new: the most new tokens any sequence has (0: not known). It chooses how the work is cut up;
  * the results are right for any value. `work` is scratch memory of the call, overwritten by every
  * call: work_bytes at least what qe_op_page_attention_work_bytes gives for the same values. Calls

@@ -68,6 +68,7 @@ struct DraftArgs {
 constexpr int kThreads = 512;
 constexpr uint32_t kChunk = 2048, kNone = 0xFFFFFFFFu;
 constexpr uint32_t kMostVocab = kThreads * kChunk;  // a thread of a draw has one chunk: 2^20
+constexpr uint32_t kRowsAcross = 65535;              // a grid's limit in y and z
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -168,7 +169,7 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c0, uint32
 // A wave per (row, chunk).
 __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
   const uint32_t lane = threadIdx.x & 63;
-  const uint32_t c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), r = blockIdx.y + blockIdx.z * 32768;
+  const uint32_t c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), r = blockIdx.y + blockIdx.z * kRowsAcross;
   if (c >= a.chunks || r >= a.n_rows) return;
   float x[32];
   load_chunk(a.logits + r * a.stride, c * kChunk, a.vocab, -INFINITY, x);
@@ -526,8 +527,8 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t waves4 = qe::ceil_div(a.chunks, 4u);
   if (n_rows) {
-    const uint32_t y = a.n_rows < 32768 ? a.n_rows : 32768;
-    qe::k_draft_sums<<<dim3(waves4, y, qe::ceil_div(a.n_rows, 32768u)), 256, 0, st>>>(a);
+    const uint32_t y = a.n_rows < qe::kRowsAcross ? a.n_rows : qe::kRowsAcross;
+    qe::k_draft_sums<<<dim3(waves4, y, qe::ceil_div(a.n_rows, qe::kRowsAcross)), 256, 0, st>>>(a);
   }
   qe::k_draft_decide<<<a.n_seqs, qe::kThreads, 0, st>>>(a);
   if (a.probs && n_rows) {

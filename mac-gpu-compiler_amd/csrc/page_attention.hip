@@ -7,14 +7,14 @@
 // over the positions j whose page is there; a row that has none gives zeros.
 //
 // How the work is cut. The rows of a sequence and KV head are (token, q head) pairs, token first; an
-// item is one tile of them (16 to 128 rows) with its positions in blocks of 64, up to the last
+// item is one tile of them (16 to 256 rows) with its positions in blocks of 64, up to the last
 // position that any of its rows attends. The blocks of all items, in order (sequence, head, tile),
 // are dealt to a fixed number of workgroups in equal contiguous parts, whatever the lengths: the
 // lengths are device data, so the host cannot choose a split by them, and a batch of ragged lengths
 // keeps every CU busy to the end. A workgroup that holds all blocks of an item writes its rows out;
 // one that holds a part leaves the part's unnormalised sums, maxima and weight sums in `work`, and
-// k_page_join adds the parts of an item in order. The cut depends on the plan alone, so results are
-// the same every time.
+// k_page_join adds the parts of an item in order. (Short items are dealt out whole: find_part.) The
+// cut depends on the plan alone, so results are the same every time.
 #include "pages.h"
 
 #include "device_common.h"
@@ -47,7 +47,7 @@ struct AttnArgs {
   uint64_t q_stride, out_stride;  // elements
   float* parts;                   // [workgroup][2][rows of a tile][kPartRow]
   struct Joint* joints;           // [workgroup]
-  uint32_t n_rows, n_heads, group;
+  uint32_t n_rows, group;
   uint32_t group_magic, group_shift;  // r / group = (2 r * magic >> 32) >> shift for r < 2^31
   uint32_t whole_items;           // 1: an item counts as one block and is never cut (a call without a join says
                                   // so; else each workgroup finds out by the lengths)
@@ -1245,7 +1245,6 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   a.q_stride = q_stride;
   a.out_stride = out_stride;
   a.n_rows = uint32_t(n_rows);
-  a.n_heads = uint32_t(n_heads);
   a.group = uint32_t(n_heads / a.p.n_kv);
   // shift = ceil(log2 group), magic = ceil(2^(31 + shift) / group): exact below 2^31
   while ((1ull << a.group_shift) < a.group) a.group_shift++;
@@ -1253,7 +1252,9 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
   a.joints = static_cast<qe::Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
-  const qe::Cut c = qe::cut_of(max_new, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
+  // (fewer rows than max_new says need no more than the work that was asked for)
+  const uint64_t bound = max_new && max_new < n_rows ? max_new : n_rows;
+  const qe::Cut c = qe::cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
   const uint32_t R = c.rows, grid = c.workgroups;
   a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= qe::kWholeItems;
   a.join = !a.whole_items;

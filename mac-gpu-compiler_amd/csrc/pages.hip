@@ -342,6 +342,8 @@ int check_rows(const qe_pages* pages, const void* k, const void* v, uint64_t n_r
   if (!k || !v) return set_error(QE_ERR_ARG, "null argument");
   const uint64_t el = dtype == QE_KV_F32 ? 4 : 2;
   if (n_rows > 0x7FFFFFFFull / plan->n_kv) return set_error(QE_ERR_ARG, "need n_rows * n_kv_heads < 2^31");
+  // (a launch has fewer than 2^32 threads along x, 256 for each 16 rows)
+  if (n_rows >= 1ull << 28) return set_error(QE_ERR_ARG, "need n_rows < 2^28");
   if (stride < uint64_t(plan->n_kv) * kPageDim || stride > 0xFFFFFFFFull || stride * el % 16)
     return set_error(QE_ERR_ARG, "row_stride must be at least n_kv_heads * 128 elements and a multiple of 16 bytes");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16)

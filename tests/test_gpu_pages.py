@@ -323,3 +323,91 @@ def test_pages_past_32_bits(gpu):
     qe.op_page_attention(pages, q, o, work, 600)
     w = torch.softmax(q[599, 3].double() @ k[:, 3].double().T / math.sqrt(D), -1) @ v[:, 3].double()
     assert (o[599, 3].double() - w).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("n_seqs,most,longest", [(65, 1, 2000), (65, 3, 5000), (64, 2, 300), (1500, 2, 40), (70, 100, 30)])
+def test_attention_of_batches(gpu, n_seqs, most, longest, rows, kv):
+    """batches on both sides of what a wave plans alone, with sequences that have no new token; items dealt
+    out whole and, where one sequence is much longer than the rest, cut"""
+    new = [i % (most + 1) for i in range(n_seqs)]
+    ctx = [(i * 37) % 40 for i in range(n_seqs)]
+    ctx[n_seqs // 2] = longest
+    new[n_seqs // 2] = most
+    check_attention(Case(new, ctx, 32, 1, kv, seed=19, lead=3, tail=20), 2, rows, gap=8)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_append_to_many_sequences(gpu, kv):
+    """more sequences than the search keeps on chip"""
+    n_seqs = 1500
+    case = Case([i % 3 for i in range(n_seqs)], [(i * 11) % 30 for i in range(n_seqs)], 16, 1, kv, seed=20, lead=1, tail=9)
+    pages = case.pages()
+    x = torch.randn(case.total, 1, D, generator=torch.Generator().manual_seed(4))
+    k, v = (torch.full_like(x, 9.0).cuda() for _ in "kv")
+    qe.op_page_append(pages, x.cuda(), -x.cuda())
+    qe.op_page_read(pages, k, v)
+    if kv == "fp8":
+        y, e = pow2_rows(x.double())
+        y = (y * torch.exp2(e.double() - 127)[..., None]).float()
+    else:
+        y = x.bfloat16().float()
+    mine = slice(case.starts[0], case.starts[-1])
+    assert torch.equal(k.cpu()[mine], y[mine]) and torch.equal(v.cpu()[mine], -y[mine])
+    for t in (k, v):
+        assert (t[:case.starts[0]] == 9).all() and (t[case.starts[-1]:] == 9).all()
+
+
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("new,heads", [(6, 2), (100, 2)])
+def test_e4m3_values_that_are_masked(gpu, rows, new, heads):
+    """NaN in e4m3 pages at a later token reaches only the rows that attend it"""
+    case = Case([new], [40], 16, 1, "fp8", seed=16)
+    at = 40 + new // 2
+    page, off = int(case.host["table"][0, at // 16]), at % 16
+    q = torch.randn(new, heads, D, generator=torch.Generator().manual_seed(7)).to(rows)
+    want, worst, vmax = case.attention(q)
+    case.host["k"].view(torch.uint8)[page, 0, off, 5] = 0x7F
+    case.host["v"].view(torch.uint8)[page, 0, off // 16, 9, off % 16] = 0xFF
+    got = attend(case, q)
+    assert (got[:new // 2] - want[:new // 2]).abs().max() <= attention_tolerance(worst, vmax, rows)
+    assert torch.isnan(got[new // 2:]).any(-1).all()
+
+
+def test_calls_on_two_streams(gpu):
+    """two plans on two streams at once, each with work of its own, as eager calls and as graphs"""
+    cases = [Case([1, 3, 2], [900, 40, 333], 16, 2, "bf16", seed=23), Case([150, 20], [60, 700], 32, 2, "fp8", seed=24)]
+    qs = [torch.randn(c.total, 4, D, generator=torch.Generator().manual_seed(5)) for c in cases]
+    alone = [attend(c, q) for c, q in zip(cases, qs)]
+    pages, qd = [c.pages() for c in cases], [q.cuda() for q in qs]
+    outs = [torch.empty_like(q) for q in qd]
+    works = [torch.empty(qe.op_page_attention_work_bytes(4, 2, max(c.new)), dtype=torch.uint8, device="cuda") for c in cases]
+    streams, graphs = [torch.cuda.Stream() for _ in cases], []
+    torch.cuda.synchronize()
+
+    def call(i):
+        qe.op_page_attention(pages[i], qd[i], outs[i], works[i], max(cases[i].new))
+
+    def same():
+        torch.cuda.synchronize()
+        for o, a in zip(outs, alone):
+            assert torch.equal(o.cpu().double(), a)
+            o.zero_()
+        torch.cuda.synchronize()
+
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                call(i)
+    same()
+    for i, st in enumerate(streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=st):
+            call(i)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+        same()

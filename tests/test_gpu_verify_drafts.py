@@ -189,6 +189,44 @@ def test_what_is_emitted_follows_the_target(gpu, dense):
     assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / n) + 1e-9).all(), (share, p)
 
 
+@pytest.mark.parametrize("dense", [False, True])
+def test_long_runs_of_drafts(gpu, dense):
+    """sequences of more drafts than are looked at together, that stop at the border, behind it and not at all"""
+    rng = np.random.default_rng([5, dense])
+    rows_of, wrong = [150, 64, 65, 129, 200], [140, 63, 64, 999, 64]
+    starts = np.concatenate([[0], np.cumsum(rows_of)])
+    x = (rng.standard_normal((starts[-1], 40)) * 4).astype(np.float32)
+    drafts = x.argmax(-1).astype(np.uint32)
+    for s, w in enumerate(wrong):
+        if w < rows_of[s]:
+            drafts[starts[s] + w] = x[starts[s] + w].argmin()
+    probs = np.zeros_like(x) if dense else None
+    if dense:
+        probs[np.arange(len(x)), drafts] = 1.0
+    check(x, starts, drafts, probs, np.full(len(x), 0.5, np.float32), rng.random(5, np.float32), np.zeros(5, np.float32))
+
+
+def test_more_rows_than_a_grid_is_wide(gpu):
+    """70,002 rows: greedy, two a sequence"""
+    rng = np.random.default_rng(6)
+    n, vocab = 35001, 7
+    x = rng.standard_normal((2 * n, vocab)).astype(np.float32)
+    best = x.argmax(-1)
+    drafts = rng.integers(0, vocab, 2 * n)
+    yes = drafts[::2] == best[::2]
+    dev = lambda a, t: torch.from_numpy(a.astype(t)).cuda()  # noqa: E731
+    tokens = torch.zeros(2 * n, dtype=torch.int32, device="cuda")
+    count = torch.zeros(n, dtype=torch.int32, device="cuda")
+    work = torch.empty(qe.op_verify_drafts_work_bytes(2 * n, n, vocab), dtype=torch.uint8, device="cuda")
+    qe.op_verify_drafts(dev(x, np.float32), dev(np.arange(n + 1) * 2, np.int32), dev(drafts, np.int32),
+                        dev(np.full(2 * n, 0.5), np.float32), dev(np.full(n, 0.5), np.float32), tokens, count, work,
+                        temperature=torch.zeros(n, device="cuda"))
+    got = tokens.cpu().numpy()
+    np.testing.assert_array_equal(count.cpu().numpy(), 1 + yes)
+    np.testing.assert_array_equal(got[::2], best[::2])
+    np.testing.assert_array_equal(got[1::2], np.where(yes, best[1::2], -1))
+
+
 @pytest.mark.parametrize("kv,rows", [("fp8", torch.float32), ("bf16", torch.bfloat16)])
 def test_a_pass_of_speculative_serving_as_a_graph(gpu, kv, rows):
     """append, attention, projection to logits and the check of the drafts, captured once on a stream of
