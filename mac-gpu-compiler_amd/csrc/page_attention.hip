@@ -21,6 +21,8 @@
 #include "dma.h"
 #include "status.h"
 
+#include <type_traits>
+
 namespace qe {
 namespace {
 
@@ -296,6 +298,16 @@ __device__ __forceinline__ float add_groups(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// the same over the two halves of a wave
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
@@ -735,16 +747,19 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 // of 16, which lie in one page.
 // ---------------------------------------------------------------------------------------------
 template <bool FP8, bool BF16_ROWS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_tiles(AttnArgs a) {
-  constexpr int NS = BF16_ROWS ? 1 : 3, R = 32 * WAVES;
+__global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
+  static_assert(BF16_ROWS || WAVES == 8, "f32 rows: 8 waves of 16");
+  constexpr int NS = BF16_ROWS ? 1 : 3, WR = BF16_ROWS ? 32 : 16, R = WR * WAVES;
+  constexpr int NJ = BF16_ROWS ? 8 : 4, NSUM = BF16_ROWS ? 16 : 8;  // fragments of a row of q; 4 dims of the sums each
+  typedef typename std::conditional<BF16_ROWS, f32x16, f32x4>::type Acc;
   constexpr int PARTS = WAVES / 4, LOADS = 4 / PARTS;  // waves that share a run; 1 KB loads of K (and V) of each
-  constexpr int STAGES = !FP8 && (WAVES == 8 || !BF16_ROWS) ? 3 : 2;  // LDS of one workgroup on a CU holds 3
+  constexpr int STAGES = !FP8 && WAVES == 8 ? 3 : 2;  // LDS of one workgroup on a CU holds 3
   constexpr uint32_t TILE = kBlock * kPageDim * 2;  // bytes of K, and of V
   __shared__ __align__(16) uint8_t buf[STAGES][2 * TILE];
   __shared__ __align__(16) float vscale[2][FP8 ? kBlock : 4];
   __shared__ uint32_t foul[STAGES];
   __shared__ PlanShared sh;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & (WR - 1), grp = lane / WR;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t w = part_index();
   Cursor cu;
@@ -765,20 +780,28 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     const uint32_t first = cu.block * kBlock, last = a.whole_items ? limit : min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // this wave's rows, and the positions that all of them (free_to) and some of them (end) attend
-    const uint32_t wr0 = cu.tile * R + 32 * wave;
-    const uint32_t wrows = cu.q.rows > wr0 ? min(cu.q.rows - wr0, 32u) : 0;
+    const uint32_t wr0 = cu.tile * R + WR * wave;
+    const uint32_t wrows = cu.q.rows > wr0 ? min(cu.q.rows - wr0, uint32_t(WR)) : 0;
     const int32_t free_to = row_position(a, cu.q, wr0);
     const uint32_t end = wrows ? row_limit(a, cu.q, wr0 + wrows - 1) : 0;
     const int32_t tile_free = row_position(a, cu.q, cu.tile * R);  // all rows of the tile attend up to it
-    const uint32_t fresh = afresh(tid & 63), r = wr0 + (fresh & 31);
-    const bool real = (fresh & 31) < wrows;
+    const uint32_t fresh = afresh(tid & 63), r = wr0 + (fresh & (WR - 1));
+    const bool real = (fresh & (WR - 1)) < wrows;
     const int32_t row_pos = real ? row_position(a, cu.q, r) : -1;
-    bf16x8 qf[8][NS];
-    f32x16 acc[4];
+    bf16x8 qf[NJ][NS];
+    // sums of 4 dims each: n-th of them, and the first of its dims (of lane group g)
+    constexpr int NACC = BF16_ROWS ? 4 : 8, PER = NSUM / NACC;
+    Acc acc[NACC];
+    auto dim_of = [](int n, uint32_t g) __attribute__((always_inline)) {
+      return BF16_ROWS ? 32 * (n / 4) + 8 * (n % 4) + 4 * g : 16 * n + 4 * g;
+    };
+    auto sum_of = [&](int n) __attribute__((always_inline)) {
+      const Acc& v = acc[n / PER];
+      const int i = 4 * (n % PER);
+      return f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    };
 #pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) acc[t][i] = 0.f;
+    for (int t = 0; t < NACC; t++) acc[t] = 0.f;
     float m = -INFINITY, l = 0.f;
 
     const int32_t* const table = a.p.table + size_t(cu.seq) * a.p.table_stride;
@@ -791,6 +814,8 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     const uint32_t run = wave / PARTS, part_of = wave % PARTS;
     u32x4 rk[FP8 ? 2 / PARTS : 1], rv[FP8 ? 2 / PARTS : 1];  // e4m3: 16 bytes of K rows, the 16 positions of V's dims
     uint32_t ke[FP8 ? 2 / PARTS : 1] = {}, ve = 0;
+    // which place the 16-byte piece c of row p of K takes: c ^ swap(p), different for 16 rows that are read at once
+    auto swap = [](uint32_t p) __attribute__((always_inline)) { return BF16_ROWS ? p & 15 : (p & 3) | (p >> 1 & 12); };
     // starts the loads of this wave's part of the block at x (a page that is not there is read as page 0,
     // and what comes of it is masked)
     auto fetch = [&](uint32_t x, uint32_t b, int32_t page) __attribute__((always_inline)) {
@@ -809,7 +834,7 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
         const uint8_t *k = a.st.k + row * kPageDim * 2, *v = a.st.v + row * kPageDim * 2 + part_of * LOADS * 1024;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-          const uint32_t kr = 4 * (part_of * LOADS + i) + (lane >> 4), c = (lane & 15) ^ kr;  // row, piece of the row
+          const uint32_t kr = 4 * (part_of * LOADS + i) + (lane >> 4), c = (lane & 15) ^ swap(16 * run + kr);  // row, piece of the row
           dma16(dst + i * 1024, k + kr * kPageDim * 2 + c * 16);
         }
 #pragma unroll
@@ -828,15 +853,17 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
           const float ks = __uint_as_float(ke[i] << 23);
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            *reinterpret_cast<bf16x8*>(k + (((2 * (lane & 7) + e) ^ (kr & 15)) * 16)) = fp8_bf16(rk[i][2 * e], rk[i][2 * e + 1], ks);
+            *reinterpret_cast<bf16x8*>(k + (((2 * (lane & 7) + e) ^ swap(16 * run + kr)) * 16)) = fp8_bf16(rk[i][2 * e], rk[i][2 * e + 1], ks);
             *reinterpret_cast<bf16x8*>(v + ((e ^ (d >> 3 & 1)) * 16)) = fp8_bf16(rv[i][2 * e], rv[i][2 * e + 1], 1.f);
           }
         }
         if (part_of == 0 && lane < 16) vscale[b][16 * run + lane] = __uint_as_float(ve << 23);
       }
     };
-    auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {  // dims 32 t + col, positions 16 u + 8 half ..
-      return *reinterpret_cast<const u32x4*>(buf[b] + TILE + u * 4096 + (32 * t + col) * 32 + (half ^ (col >> 3 & 1)) * 16);
+    // V of positions 16 u + 8 (grp % 2) .., operand A of dims 32 t + col, or 16 t + col of positions 32 u + 8 grp ..
+    auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {
+      const uint32_t run = BF16_ROWS ? u : 2 * u + (grp >> 1), d = WR * t + col;
+      return *reinterpret_cast<const bf16x8*>(buf[b] + TILE + run * 4096 + d * 32 + ((grp & 1) ^ (col >> 3 & 1)) * 16);
     };
     // V of the block in buffer b as every row may multiply it: zeros at positions that no row of the tile
     // attends, which may hold anything (0 x NaN is NaN), and where it is not finite at one that only some
@@ -867,97 +894,121 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
     auto multiply = [&](uint32_t x, uint32_t b, uint32_t there) __attribute__((always_inline)) {
       // Fragments come from LDS four at a time, a group ahead of the products that use them; the scheduling
       // barriers keep it so (left alone the compiler waits for every read right behind it).
-      f32x16 s[2];
+      constexpr int NT = BF16_ROWS ? 2 : 4, PERS = BF16_ROWS ? 16 : 4;
+      Acc s[NT];
       bf16x8 kf[2][4];
-      // operand A's row `col` is position 32 u + kr of the block
-      const uint32_t kr = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
-      auto k_part = [&](int n) __attribute__((always_inline)) {  // fragment n: rows 32 (n / 8) .., dims 16 (n % 8) ..
-        return *reinterpret_cast<const bf16x8*>(buf[b] + (32 * (n / 8) + kr) * 256 +
-                                                (((2 * (n % 8) + half) ^ (kr & 15)) * 16));
+      // operand A's row `col` is position 32 t + kr of the block (f32 rows: kr of 32 (t / 2), 4 (t & 1) further)
+      const uint32_t kr = BF16_ROWS ? 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3)
+                                    : 8 * (col >> 2) + (col & 3);
+      // fragment n of group o: bf16 rows score tile o / 2, dims 16 (4 (o & 1) + n) ..; f32 rows score tile
+      // 2 (o / 2) + (n & 1), dims 32 (2 (o & 1) + n / 2) .., so that two sums take turns
+      auto tile_of = [](int o, int n) __attribute__((always_inline)) { return BF16_ROWS ? o / 2 : 2 * (o / 2) + (n & 1); };
+      auto dims_of = [](int o, int n) __attribute__((always_inline)) { return BF16_ROWS ? 4 * (o & 1) + n : 2 * (o & 1) + n / 2; };
+      auto k_part = [&](int o, int n) __attribute__((always_inline)) {
+        const int t = tile_of(o, n), j = dims_of(o, n);
+        const uint32_t p = BF16_ROWS ? 32 * t + kr : 32 * (t / 2) + 4 * (t & 1) + kr;
+        return *reinterpret_cast<const bf16x8*>(buf[b] + p * 256 + (((64 / WR * j + grp) ^ swap(p)) * 16));
       };
 #pragma unroll
-      for (int n = 0; n < 4; n++) kf[0][n] = k_part(n);
+      for (int n = 0; n < 4; n++) kf[0][n] = k_part(0, n);
 #pragma unroll
       for (int o = 0; o < 4; o++) {
         if (o < 3)
 #pragma unroll
-          for (int n = 0; n < 4; n++) kf[(o + 1) & 1][n] = k_part(4 * o + 4 + n);
+          for (int n = 0; n < 4; n++) kf[(o + 1) & 1][n] = k_part(o + 1, n);
         __builtin_amdgcn_sched_barrier(0);
+        if (!(o & 1))
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          const int u = o / 2, j = 4 * (o & 1) + n;
-          if (j == 0)
+          for (int t = tile_of(o, 0); t <= tile_of(o, 3); t++) s[t] = 0.f;
+        if constexpr (BF16_ROWS) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[u][i] = 0.f;
+          for (int n = 0; n < 4; n++)
+            s[o / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[o & 1][n], qf[dims_of(o, n)][0], s[o / 2], 0, 0, 0);
+        } else {
 #pragma unroll
-          for (int i = 0; i < NS; i++)
-            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[o & 1][n], qf[j][i], s[u], 0, 0, 0);
+          for (int n = 0; n < 4; n += 2)
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+              for (int e = n; e < n + 2; e++)
+                s[tile_of(o, e)] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[o & 1][e], qf[dims_of(o, e)][i], s[tile_of(o, e)], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      // score i of tile t: position in the block
+      auto position = [&](int t, int i) __attribute__((always_inline)) {
+        return BF16_ROWS ? 32 * t + 16 * (i >> 3) + 4 * ((i >> 2) & 1) + (i & 3) + 8 * grp
+                         : 32 * (t / 2) + 4 * (t & 1) + i + 8 * grp;
+      };
       const bool masked = int32_t(x + kBlock - 1) > free_to || there != 15;
       if (masked) {
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int in = 32 * u + 16 * (i >> 3) + 4 * ((i >> 2) & 1) + (i & 3);  // + 8 half
-            if (int32_t(x + in + 8 * half) > row_pos || !(there >> (in / 16) & 1)) s[u][i] = -INFINITY;
+          for (int i = 0; i < PERS; i++) {
+            const uint32_t in = position(t, i);
+            if (int32_t(x + in) > row_pos || !(there >> (in / 16) & 1)) s[t][i] = -INFINITY;
           }
       }
       float mx = s[0][0];
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
-      {
-        const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
-      }
-      mx = fmaxf(m, mx * a.c);
+        for (int i = 0; i < PERS; i++) mx = fmaxf(mx, s[t][i]);
+      mx = fmaxf(m, (BF16_ROWS ? max_halves(mx) : max_groups(mx)) * a.c);
       if (__any(mx > m + kSlack)) {
         const float f = rebase(m, mx);
         l *= f;
 #pragma unroll
-        for (int t = 0; t < 4; t++) acc[t] *= f;
+        for (int t = 0; t < NACC; t++) acc[t] *= f;
         m = mx;
       }
       const float ref = m == -INFINITY ? 0.f : m;
       bf16x8 pf[2][NS];
       bf16x8 vf[2][4];
-      // weights of positions 16 u + 8 half ..
+      // weights of positions 16 u + 8 grp .. (f32 rows: 32 u + 8 grp ..)
       auto weights = [&](int u, bf16x8 (&o)[NS]) __attribute__((always_inline)) {
         float e[8];
         f32x4 vs[2];
         if constexpr (FP8) {
-          vs[0] = *reinterpret_cast<const f32x4*>(&vscale[b][16 * u + 8 * half]);
-          vs[1] = *reinterpret_cast<const f32x4*>(&vscale[b][16 * u + 8 * half + 4]);
+          vs[0] = *reinterpret_cast<const f32x4*>(&vscale[b][(BF16_ROWS ? 16 : 32) * u + 8 * grp]);
+          vs[1] = *reinterpret_cast<const f32x4*>(&vscale[b][(BF16_ROWS ? 16 : 32) * u + 8 * grp + 4]);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          const float y = exp2_fast(fmaf(s[u / 2][8 * (u & 1) + i], a.c, -ref));
+          const float z = BF16_ROWS ? s[u / 2][8 * (u & 1) + i] : s[2 * u + i / 4][i & 3];
+          const float y = exp2_fast(fmaf(z, a.c, -ref));
           l += y;
           e[i] = y;
           if constexpr (FP8) e[i] *= vs[i / 4][i & 3];
         }
         split_bf16<NS>(e, o);
       };
+      // group o: bf16 rows 16 positions and all dims, f32 rows 32 positions and half of them
+      auto group = [&](int o, bf16x8 (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < 4; t++) vf[0][t] = __builtin_bit_cast(bf16x8, v_part(b, t, 0));
+        for (int t = 0; t < 4; t++) v[t] = BF16_ROWS ? v_part(b, t, o) : v_part(b, 4 * (o & 1) + t, o / 2);
+      };
+      group(0, vf[0]);
       weights(0, pf[0]);
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        if (u < 3)
-#pragma unroll
-          for (int t = 0; t < 4; t++) vf[(u + 1) & 1][t] = __builtin_bit_cast(bf16x8, v_part(b, t, u + 1));
+      for (int o = 0; o < 4; o++) {
+        if (o < 3) group(o + 1, vf[(o + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
         // products of these positions beside the next ones' weights
+        if constexpr (BF16_ROWS) {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+          for (int t = 0; t < 4; t++)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[o & 1][t], pf[o & 1][0], acc[t], 0, 0, 0);
+          if (o < 3) weights(o + 1, pf[(o + 1) & 1]);
+        } else {
 #pragma unroll
           for (int i = 0; i < NS; i++)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u & 1][t], pf[u & 1][i], acc[t], 0, 0, 0);
-        if (u < 3) weights(u + 1, pf[(u + 1) & 1]);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+              acc[4 * (o & 1) + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[o & 1][t], pf[o / 2][i], acc[4 * (o & 1) + t], 0, 0, 0);
+          if (o == 0) weights(1, pf[1]);
+        }
       }
       if (masked && foul_from == kNowhere && uniform(foul[b]) != 0) foul_from = x;
     };
@@ -977,9 +1028,9 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
       if (!FP8 && STAGES == 3 && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < NJ; j++) {
       float x[8] = {};
-      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + 16 * j + 8 * (fresh >> 5), x);
+      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + (512 / WR) * j + 8 * (fresh / WR), x);
       split_bf16<NS>(x, qf[j]);
     }
     if (first < last) {
@@ -1017,42 +1068,38 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
       if (!is_page(page)) continue;
       const size_t e = v_element(a.p, page, head, j & ps_mask);
 #pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int n = 0; n < NSUM; n++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float v = v_value<FP8>(a.st.v, e + 16 * (32 * t + 8 * (i / 4) + 4 * half + (i & 3)));
-          if (!(fabsf(v) < INFINITY) && int32_t(j) <= row_pos) acc[t][i] += v;
+        for (int i = 0; i < 4; i++) {
+          const float v = v_value<FP8>(a.st.v, e + 16 * (dim_of(n, grp) + i));
+          if (!(fabsf(v) < INFINITY) && int32_t(j) <= row_pos) acc[n / PER][4 * (n % PER) + i] += v;
         }
     }
-    {
-      const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-      l = __uint_as_float(z[0]) + __uint_as_float(z[1]);
-    }
+    l = BF16_ROWS ? add_halves(l) : add_groups(l);
     const bool whole = cu.block == 0 && take == cu.blocks;
     {
-      const uint32_t lane = afresh(tid & 63), col = lane & 31, half = lane >> 5;
+      const uint32_t lane = afresh(tid & 63), col = lane & (WR - 1), grp = lane / WR;
       if (whole) {
         // through LDS (each wave in its own part of the buffers), so that rows are stored in one piece
         const float inv = l == 0.f ? 0.f : 1.f / l;
         constexpr uint32_t ROW = kPageDim * (BF16_ROWS ? 2 : 4), PIECES = ROW / 16;
-        uint8_t* const rows_at = buf[0] + wave * 32 * ROW;
+        uint8_t* const rows_at = buf[0] + wave * WR * ROW;
         __syncthreads();  // the buffers' last readers are done
-  #pragma unroll
-        for (int t = 0; t < 4; t++)
-  #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const f32x4 v = f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * inv;
-            if constexpr (BF16_ROWS) {
-              uint2 u;
-              u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2));
-              u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2));
-              *reinterpret_cast<uint2*>(rows_at + col * ROW + (((4 * t + i) ^ (col & 15)) * 16) + 8 * half) = u;
-            } else {
-              *reinterpret_cast<f32x4*>(rows_at + col * ROW + (((8 * t + 2 * i + half) ^ col) * 16)) = v;
-            }
+#pragma unroll
+        for (int n = 0; n < NSUM; n++) {
+          const f32x4 v = sum_of(n) * inv;
+          const uint32_t d = dim_of(n, grp);
+          if constexpr (BF16_ROWS) {
+            uint2 u;
+            u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2));
+            u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2));
+            *reinterpret_cast<uint2*>(rows_at + col * ROW + ((d / 8 ^ (col & 15)) * 16) + 8 * grp) = u;
+          } else {
+            *reinterpret_cast<f32x4*>(rows_at + col * ROW + ((d / 4 ^ col) * 16)) = v;
           }
-  #pragma unroll
-        for (uint32_t i = 0; i < 32 * PIECES / 64; i++) {
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < WR * PIECES / 64; i++) {
           const uint32_t in = i * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
           if (in < wrows) {
             const u32x4 v = *reinterpret_cast<const u32x4*>(rows_at + in * ROW + ((piece ^ (in & (PIECES - 1))) * 16));
@@ -1060,18 +1107,18 @@ __global__ __launch_bounds__(64 * WAVES, BF16_ROWS ? 2 : 1) void k_page_attn_til
           }
         }
       } else {
-        // sums as the lanes hold them: [wave][8 dims][half][row of the 32][4 dims]
+        // sums as [32 rows][8 dims][half of them][row][4 dims]
         float* const part = my_parts + (cu.block == 0 ? size_t(R) * kPartRow : 0);
         if (wrows) {
-  #pragma unroll
-          for (int t = 0; t < 4; t++)
-  #pragma unroll
-            for (int i = 0; i < 4; i++)
-              *reinterpret_cast<f32x4*>(part + ((wave * 16 + 4 * t + i) * 64 + lane) * 4) =
-                  f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-          if (half == 0) {
-            part[R * kPageDim + 32 * wave + col] = m;
-            part[R * kPageDim + R + 32 * wave + col] = l;
+          const uint32_t in = WR * wave + col;
+#pragma unroll
+          for (int n = 0; n < NSUM; n++) {
+            const uint32_t d = dim_of(n, grp);
+            *reinterpret_cast<f32x4*>(part + ((in / 32 * 16 + d / 8) * 64 + (d / 4 & 1) * 32 + in % 32) * 4) = sum_of(n);
+          }
+          if (grp == 0) {
+            part[R * kPageDim + in] = m;
+            part[R * kPageDim + R + in] = l;
           }
         }
         if (cu.block == 0 && tid == 0)
@@ -1258,12 +1305,12 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   const uint32_t R = c.rows, grid = c.workgroups;
   a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= qe::kWholeItems;
   a.join = !a.whole_items;
-  auto go = [&](auto* kern) { kern<<<grid, R == 256 ? 512 : 256, 0, st>>>(a); };
+  auto go = [&](auto* kern) { kern<<<grid, R == 256 || (R == 128 && !bf16) ? 512 : 256, 0, st>>>(a); };
   if (R == 256) {
     go(fp8 ? qe::k_page_attn_tiles<true, true, 8> : qe::k_page_attn_tiles<false, true, 8>);
   } else if (R == 128) {
-    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true, 4> : qe::k_page_attn_tiles<true, false, 4>);
-    else go(bf16 ? qe::k_page_attn_tiles<false, true, 4> : qe::k_page_attn_tiles<false, false, 4>);
+    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true, 4> : qe::k_page_attn_tiles<true, false, 8>);
+    else go(bf16 ? qe::k_page_attn_tiles<false, true, 4> : qe::k_page_attn_tiles<false, false, 8>);
   } else if (R == 32) {
     if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 2> : qe::k_page_attn_rows<true, false, 2>);
     else go(bf16 ? qe::k_page_attn_rows<false, true, 2> : qe::k_page_attn_rows<false, false, 2>);
