@@ -816,6 +816,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
     uint32_t ke[FP8 ? 2 / PARTS : 1] = {}, ve = 0;
     // which place the 16-byte piece c of row p of K takes: c ^ swap(p), different for 16 rows that are read at once
     auto swap = [](uint32_t p) __attribute__((always_inline)) { return BF16_ROWS ? p & 15 : (p & 3) | (p >> 1 & 12); };
+    // whether the two pieces of dim d of a run of V change places
+    auto swap_v = [](uint32_t d) __attribute__((always_inline)) { return BF16_ROWS ? d >> 3 & 1 : 0; };
     // starts the loads of this wave's part of the block at x (a page that is not there is read as page 0,
     // and what comes of it is masked)
     auto fetch = [&](uint32_t x, uint32_t b, int32_t page) __attribute__((always_inline)) {
@@ -839,7 +841,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < LOADS; i++)
-          dma16(dst + TILE + i * 1024, v + i * 1024 + (lane ^ (lane >> 4 & 1)) * 16);
+          dma16(dst + TILE + i * 1024, v + i * 1024 + (lane ^ swap_v(lane >> 1)) * 16);
       }
     };
     // e4m3: what fetch loaded, widened, into LDS
@@ -854,7 +856,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             *reinterpret_cast<bf16x8*>(k + (((2 * (lane & 7) + e) ^ swap(16 * run + kr)) * 16)) = fp8_bf16(rk[i][2 * e], rk[i][2 * e + 1], ks);
-            *reinterpret_cast<bf16x8*>(v + ((e ^ (d >> 3 & 1)) * 16)) = fp8_bf16(rv[i][2 * e], rv[i][2 * e + 1], 1.f);
+            *reinterpret_cast<bf16x8*>(v + ((e ^ swap_v(d)) * 16)) = fp8_bf16(rv[i][2 * e], rv[i][2 * e + 1], 1.f);
           }
         }
         if (part_of == 0 && lane < 16) vscale[b][16 * run + lane] = __uint_as_float(ve << 23);
@@ -863,14 +865,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
     // V of positions 16 u + 8 (grp % 2) .., operand A of dims 32 t + col, or 16 t + col of positions 32 u + 8 grp ..
     auto v_part = [&](uint32_t b, int t, int u) __attribute__((always_inline)) {
       const uint32_t run = BF16_ROWS ? u : 2 * u + (grp >> 1), d = WR * t + col;
-      return *reinterpret_cast<const bf16x8*>(buf[b] + TILE + run * 4096 + d * 32 + ((grp & 1) ^ (col >> 3 & 1)) * 16);
+      return *reinterpret_cast<const bf16x8*>(buf[b] + TILE + run * 4096 + d * 32 + ((grp & 1) ^ swap_v(col)) * 16);
     };
     // V of the block in buffer b as every row may multiply it: zeros at positions that no row of the tile
     // attends, which may hold anything (0 x NaN is NaN), and where it is not finite at one that only some
     // attend (`foul`: those rows get it at the end). Each wave clears what it loaded.
     auto clear = [&](uint32_t x, uint32_t b, bool page) __attribute__((always_inline)) {
       // lane: 8 of the 16 positions at dims lane / 2, lane / 2 + 32, ... of its part
-      const uint32_t base = x + 16 * run + 8 * ((lane ^ (lane >> 4)) & 1), ok = page && limit > base ? limit - base : 0;
+      const uint32_t base = x + 16 * run + 8 * ((lane & 1) ^ swap_v(lane >> 1)), ok = page && limit > base ? limit - base : 0;
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
