@@ -37,7 +37,7 @@ constexpr uint32_t kBlock = 64;    // positions
 // Weights are 2^(score - m) with m the largest score so far, or up to kSlack below it: sums are only put
 // on a new m when a score exceeds it by that much (in some row of 32 one is a little larger in most blocks).
 constexpr float kSlack = 8.f;
-constexpr uint32_t kWholeBlocks = 32;
+constexpr uint32_t kWholeBlocks = 32, kSpare = 1;  // blocks: see find_part
 constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
@@ -174,46 +174,79 @@ __device__ __forceinline__ Cursor uniform(const Cursor& c) {
 // Workgroup w's part of the list, of W parts of `per` blocks: where it begins and how many blocks it has
 // (0: none). (A part is far below 2^32 blocks: that many are 70 TB of K and V.) A wave finds it alone where a
 // lane can have a sequence each; else each thread sums a contiguous range of sequences, and the one whose
-// range holds the block walks it.
-// Items that are short and about as many as the workgroups are not cut but dealt out whole: a second piece
-// costs a workgroup some 4 us (its q, its first loads, its sums through LDS and the join). The longest up to
-// 32 blocks and up to twice a workgroup's share: 32 x 8 heads of up to 1000 positions 24 us cut, so 14; up to
-// 2000 34 and 23; 4 x 8 of up to 2000 (13 times the share) 15 cut, 20 so; 64 x 8 of up to 4000 59 and 63.
+// range holds the block walks it. W is a power of two.
+//
+// A second piece costs a workgroup some 5 us (its q, its first loads, its sums through LDS and the join), so
+// parts keep to the items in two cases:
+// - Items that are short and about as many as the workgroups are not cut but dealt out whole: the longest up to
+//   32 blocks and up to twice a workgroup's share. 32 x 8 heads of up to 1000 positions 24 us cut, so 14; up to
+//   2000 34 and 23; 4 x 8 of up to 2000 (13 times the share) 15 cut, 20 so; 64 x 8 of up to 4000 59 and 63.
+// - Few items are cut into equally many parts each, where the longest part is at most a block over the even
+//   share: a chunk of 512 over 2048 positions 43.8 us dealt evenly, so 39.0 (bf16 rows 36.6 and 31.8); one row
+//   over 4225 positions 14.7 and 12.7; 3 chunks of up to 300, whose parts would be 2 to 4 blocks over, 43 and 47.
 __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
                                               uint32_t& per_out, Cursor& cu) {
-  const uint32_t tid = threadIdx.x;
-  auto split = [&](uint64_t total) { return (total + W - 1) / W; };
-  auto fits = [&](uint32_t longest, uint64_t total) { return longest <= kWholeBlocks && longest <= 2 * split(total); };
+  const uint32_t tid = threadIdx.x, log_w = 31 - __builtin_clz(W);
+  auto split = [&](uint64_t total) { return (total + W - 1) >> log_w; };
+  auto longest_whole = [&](uint64_t total) { return min(uint64_t(kWholeBlocks), 2 * split(total)); };
   if (a.p.n_seqs <= 64) {
     const uint32_t lane = tid & 63;
     Seq q{};
-    uint64_t one = 0, up_to = 0, mine = 0, total = 0;
-    uint32_t longest = 0;
+    uint64_t one = 0;
+    uint32_t longest = 0, tiles = 0;
     if (lane < a.p.n_seqs) {
       q = read_seq(a, lane);
       one = seq_blocks(a, q, R);
-      if (q.rows) longest = tile_blocks(a, q, q.tiles(R) - 1, R);
+      tiles = q.tiles(R);
+      if (tiles) longest = tile_blocks(a, q, tiles - 1, R);
     }
-    auto sum = [&]() __attribute__((always_inline)) {
-      up_to = mine = one * a.p.n_kv;
+    const uint64_t mine = one * a.p.n_kv;
+    const uint32_t my_items = tiles * a.p.n_kv;
+    uint64_t up_to = mine;  // blocks and items of the sequences up to the lane's
+    uint32_t up_items = my_items;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const uint64_t v = __shfl_up(up_to, d);
-        if (int(lane) >= d) up_to += v;
+    for (int d = 1; d < 64; d *= 2) {
+      const uint64_t v = __shfl_up(up_to, d);
+      const uint32_t i = __shfl_up(up_items, d);
+      if (int(lane) >= d) {
+        up_to += v;
+        up_items += i;
       }
-      total = __shfl(up_to, 63);
-    };
-    sum();
-    if (!a.whole_items && !__any(!fits(longest, total))) {
-      a.whole_items = 1;
-      one = seq_blocks(a, q, R);
-      sum();
     }
-    const uint64_t per = split(total), at = w * per;
+    const uint64_t total = __shfl(up_to, 63);
+    const uint32_t items = __shfl(up_items, 63);
+    uint64_t per = split(total), at = w * per;
+    uint32_t each = 0;  // parts of every item
+    if (!a.whole_items) {
+      if (!__any(longest > longest_whole(total))) a.whole_items = 1;
+      else if (items <= W) {
+        each = W / items;
+        if (__any(longest > each * (per + kSpare))) each = 0;
+      }
+    }
+    const bool by_items = each || a.whole_items;
+    if (by_items) {
+      per = each ? 1 : split(items);
+      at = each ? w / each : w * per;
+    }
+    const uint64_t end = by_items ? items : total;
     per_out = uniform(uint32_t(per));
-    if (at >= total) return 0;
-    const bool here = at < up_to && at >= up_to - mine;
-    if (here) cu = cursor_in(a, lane, q, one, at - (up_to - mine), R);
+    if (at >= end) return 0;
+    const uint64_t to = by_items ? up_items : up_to, from_here = by_items ? my_items : mine;
+    const bool here = at < to && at >= to - from_here;
+    if (here) {
+      if (by_items) {
+        const uint32_t in = uint32_t(at - (to - from_here));
+        cu.q = q;
+        cu.seq = lane;
+        cu.head = in / tiles;
+        cu.tile = in - cu.head * tiles;
+        cu.block = 0;
+        cu.blocks = 1;
+      } else {
+        cu = cursor_in(a, lane, q, one, at - (to - from_here), R);
+      }
+    }
     const uint32_t owner = uniform(uint32_t(__builtin_ctzll(__ballot(here))));
     auto from = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(owner))); };
     cu.q.first = int32_t(from(uint32_t(cu.q.first)));
@@ -224,7 +257,13 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
     cu.tile = from(cu.tile);
     cu.block = from(cu.block);
     cu.blocks = from(cu.blocks);
-    return uniform(uint32_t(per < total - at ? per : total - at));
+    if (each) {
+      cu.blocks = tile_blocks(a, cu.q, cu.tile, R);
+      per_out = uniform((cu.blocks + each - 1) / each);
+      cu.block = uniform((w % each) * per_out);
+      return cu.block < cu.blocks ? uniform(min(per_out, cu.blocks - cu.block)) : 0;
+    }
+    return uniform(uint32_t(per < end - at ? per : end - at));
   }
   const uint32_t T = blockDim.x, each = (a.p.n_seqs + T - 1) / T;
   const uint32_t s0 = min(tid * each, a.p.n_seqs), s1 = min(s0 + each, a.p.n_seqs);
@@ -249,7 +288,7 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
     return sh.sum[T - 1];
   };
   uint64_t total = sum();
-  if (!a.whole_items && !__syncthreads_or(!fits(longest, total))) {
+  if (!a.whole_items && !__syncthreads_or(longest > longest_whole(total))) {
     a.whole_items = 1;
     total = sum();
   }
@@ -1140,7 +1179,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 template <bool BF16_ROWS, bool TILES>
 __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
-  const uint32_t w = blockIdx.x, tid = threadIdx.x;
+  const uint32_t w = part_index(), tid = threadIdx.x;  // on the XCD that wrote the first part
   const Joint j = a.joints[w];
   if (j.n == 0) return;
   const uint32_t rows = j.rows, r0 = blockIdx.y * 16;
