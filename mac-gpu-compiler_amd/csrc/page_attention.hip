@@ -1061,22 +1061,36 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
       return bits;
     };
 
+    // Loads of q, then the first blocks', so that q is cut into its parts while those are under way (rows
+    // behind the sequence's last are read as that one and come to nothing).
+    constexpr int NQ = BF16_ROWS ? 1 : 2;
+    const int32_t page0 = page_at(first + 16 * run), page1 = page_at(first + kBlock + 16 * run);
+    u32x4 raw[NJ][NQ];
+    const uint8_t* const q_row = a.q + (row_element(a, cu.q, head, min(r, cu.q.rows - 1), a.q_stride) + 8 * (fresh / WR)) * (BF16_ROWS ? 2 : 4);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int i = 0; i < NQ; i++) raw[j][i] = *reinterpret_cast<const u32x4*>(q_row + (512 / WR) * (BF16_ROWS ? 2 : 4) * j + 16 * i);
     __syncthreads();  // the buffers' last readers are done
-    // e4m3: block x is in LDS and x + 1 in registers when x is multiplied; bf16: STAGES - 1 are on their way.
-    // The first one's loads are under way while q is read.
+    // e4m3: block x is in LDS and x + 1 in registers when x is multiplied; bf16: STAGES - 1 are on their way
     if (first < last) {
-      fetch(first, 0, page_at(first + 16 * run));
-      if (!FP8 && STAGES == 3 && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
+      fetch(first, 0, page0);
+      if (!FP8 && STAGES == 3 && first + kBlock < last) fetch(first + kBlock, 1, page1);
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-      float x[8] = {};
-      if (real) load_q8<BF16_ROWS>(a.q, row_element(a, cu.q, head, r, a.q_stride) + (512 / WR) * j + 8 * (fresh / WR), x);
-      split_bf16<NS>(x, qf[j]);
+      if constexpr (BF16_ROWS) {
+        qf[j][0] = __builtin_bit_cast(bf16x8, raw[j][0]);
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(raw[j][i / 4][i & 3]);
+        split_bf16<NS>(x, qf[j]);
+      }
     }
     if (first < last) {
       widen(0);
-      if (FP8 && first + kBlock < last) fetch(first + kBlock, 1, page_at(first + kBlock + 16 * run));
+      if (FP8 && first + kBlock < last) fetch(first + kBlock, 1, page1);
       if (tid == 0) foul[0] = 0;
       constexpr uint32_t AHEAD = FP8 || STAGES == 3 ? 2 : 1;
       uint32_t b = 0, there = pages_there(first);
