@@ -33,7 +33,7 @@ namespace qe {
 namespace {
 
 // What a chunk of a row adds up to: weights relative to its own largest logit.
-struct ChunkSum {
+struct alignas(16) ChunkSum {
   double sum;
   float top;      // -inf: nothing above -inf
   uint32_t best;  // first index of top, of greedy rows
@@ -123,11 +123,26 @@ __device__ __forceinline__ float log_weight(const DrawRow& d, float x, float t) 
   return float((x == d.top ? 0.0 : (double(x) - double(d.top)) / double(t)) - log(d.total));
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
+// Sums over a wave's lanes up to each, by lane shifts within rows of 16 and broadcasts of the rows' last
+// lanes (through LDS, as __shfl_up goes, the six steps take 0.4 us).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double shifted(double v) {  // 0 where nothing comes
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false);
+  return __hiloint2double(hi, lo);
 }
+__device__ __forceinline__ double wave_scan64(double v) {
+  v += shifted<0x111, 0xF>(v);
+  v += shifted<0x112, 0xF>(v);
+  v += shifted<0x114, 0xF>(v);
+  v += shifted<0x118, 0xF>(v);
+  v += shifted<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to the rows behind them
+  return v + shifted<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+__device__ __forceinline__ double wave_sum64(double v) { return from_lane(wave_scan64(v), 63); }
 
 // the row's sequence, or -1 (as paged rows are found: the last one that starts at or before it)
 __device__ __forceinline__ int32_t sequence(const DraftArgs& a, int32_t r) {
@@ -211,67 +226,26 @@ __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
 // ---- a workgroup's draw ----
 struct Scratch {
   double wave[kThreads / 64];
-  uint32_t owner, last;  // the thread whose items the aim falls into; one past the last thread with any weight
-  uint32_t pick;
-  double before;
+  uint64_t some[kThreads / 64], over[kThreads / 64];  // lanes with any weight; of them those the aim lies below
 };
 
-// Items lie in order, N to a thread, w their weights. The first whose running sum is above aim(sum of
-// all), and the running sum before it; if rounding leaves none, the last with any weight; kNone if
-// nothing has any.
-template <int N, class Aim>
-__device__ __forceinline__ uint32_t find(const double (&w)[N], Aim aim, Scratch& sc, double& before) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  double mine = 0.0;
+// Of N items with weights w: the first with some whose running sum, from `run` on, is above `to` (else the
+// last with some), and the running sum before it.
+template <int N>
+__device__ __forceinline__ uint32_t pick(const double (&w)[N], double run, double to, double& before) {
+  uint32_t at = 0;
+  bool found = false;
+  before = run;
 #pragma unroll
-  for (int i = 0; i < N; i++) mine += w[i];
-  double up_to = mine;  // over the wave's threads up to this one, then over all
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double u = __shfl_up(up_to, d);
-    if (int(lane) >= d) up_to += u;
-  }
-  __syncthreads();  // the draw before has been read
-  if (lane == 63) sc.wave[wave] = up_to;
-  if (tid == 0) {
-    sc.owner = kNone;
-    sc.last = 0;
-  }
-  __syncthreads();
-  double all = 0.0, base = 0.0;
-#pragma unroll
-  for (uint32_t i = 0; i < kThreads / 64; i++) {
-    if (i == wave) base = all;
-    all += sc.wave[i];
-  }
-  up_to += base;
-  const double to = aim(all);
-  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
-  if (lane == 0) {
-    if (some) atomicMax(&sc.last, wave * 64 + 64 - __builtin_clzll(some));
-    if (over) atomicMin(&sc.owner, wave * 64 + __builtin_ctzll(over));
-  }
-  __syncthreads();
-  const uint32_t owner = sc.owner != kNone ? sc.owner : sc.last - 1;  // (nothing at all: kNone)
-  if (tid == owner) {
-    double run = up_to - mine, from = run;
-    uint32_t at = 0;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      if (!found && w[i] > 0.0) {
-        at = i;
-        from = run;
-        found = run + w[i] > to;
-      }
-      run += w[i];
+  for (int i = 0; i < N; i++) {
+    if (!found && w[i] > 0.0) {
+      at = i;
+      before = run;
+      found = run + w[i] > to;
     }
-    sc.pick = tid * N + at;
-    sc.before = from;
+    run += w[i];
   }
-  __syncthreads();
-  before = sc.before;
-  return owner == kNone ? kNone : sc.pick;
+  return at;
 }
 
 // sum of the chunk's weights from one logit to another: the chunk's largest to the row's
@@ -279,51 +253,90 @@ __device__ __forceinline__ double chunk_scale(float from, float top, double k) {
   return from == top ? 1.0 : top == INFINITY ? 0.0 : exp2_64((double(from) - double(top)) * k);
 }
 
-// One token of row d.row: over the chunks by their sums (a thread each), then within a chunk (4 tokens a
-// thread). REST: from max(p - q, 0).
+// A row's chunks over the lanes of a wave: lane l has n = ceil(chunks / 64) of them from n l on.
+constexpr int kLaneChunks = kMostVocab / kChunk / 64;
+
+// The first chunk whose running sum is above aim(sum of all), and the running sum before it; if rounding leaves
+// none, the last with any weight; kNone if nothing has any. Every wave finds it for itself.
+template <class Aim>
+__device__ __forceinline__ uint32_t find_chunk(const double (&w)[kLaneChunks], uint32_t n, Aim aim, double& before) {
+  const uint32_t lane = threadIdx.x & 63;
+  double mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; i++) mine += w[i];
+  const double up_to = wave_scan64(mine), to = aim(from_lane(up_to, 63));
+  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
+  before = 0.0;
+  if (!some) return kNone;
+  const int owner = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+  const uint32_t at = lane * n + pick(w, up_to - mine, to, before);
+  before = from_lane(before, owner);
+  return __builtin_amdgcn_readlane(at, owner);
+}
+
+// The sums of max(p - q, 0) over a lane's chunks of sequence s.
+__device__ __forceinline__ void load_rests(const DraftArgs& a, uint32_t s, double (&w)[kLaneChunks]) {
+  const uint32_t n = (a.chunks + 63) / 64, c0 = (threadIdx.x & 63) * n;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; i++) w[i] = uint32_t(i) < n && c0 + i < a.chunks ? a.rests[size_t(s) * a.chunks + c0 + i] : 0.0;
+}
+
+// One token of row d.row: over the chunks by their sums, then within a chunk (4 tokens a thread). v, t: the
+// sequence's random number and temperature. REST: from max(p - q, 0), whose sums by chunk are w.
 template <bool REST>
-__device__ __forceinline__ void draw(const DraftArgs& a, uint32_t s, const DrawRow& d, bool last, Scratch& sc) {
+__device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool last, double v, float t, double (&w)[kLaneChunks],
+                                     Scratch& sc) {
   constexpr int N = kChunk / kThreads;
   const float* x = a.logits + d.row * a.stride;
-  const uint32_t tid = threadIdx.x;
+  const uint32_t tid = threadIdx.x, n = (a.chunks + 63) / 64, c0 = (tid & 63) * n;
   const uint32_t skip = last || a.probs ? kNone : d.draft;  // a drafted token that has all of q
-  const double v = double(a.sample[s]);
-  const float t = temperature(a, s);
   auto token_weight = [&](uint32_t i, float xi) -> double {
     return d.greedy ? (i == d.best ? 1.0 : 0.0) : weight(xi, d.top, d.k);
   };
-  auto plain_chunk = [&]() -> double {
-    if (tid >= a.chunks) return 0.0;
-    if (d.greedy) return d.best / kChunk == tid ? 1.0 : 0.0;
-    const ChunkSum p = a.sums[size_t(d.row) * a.chunks + tid];
-    return p.sum * chunk_scale(p.top, d.top, d.k);
+  auto plain_chunks = [&]() {
+    ChunkSum p[kLaneChunks];
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; i++)
+      if (uint32_t(i) < n) p[i] = a.sums[size_t(d.row) * a.chunks + min(c0 + i, a.chunks - 1)];
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; i++) {
+      w[i] = 0.0;
+      if (uint32_t(i) < n) {
+        if (d.greedy) w[i] = d.best / kChunk == c0 + i ? 1.0 : 0.0;
+        else if (c0 + i < a.chunks) w[i] = p[i].sum * chunk_scale(p[i].top, d.top, d.k);
+      }
+    }
   };
-  double w[1], before, aim = 0.0;
+  double before, aim = 0.0;
   auto share = [&](double all) { return aim = v * all; };
-  if constexpr (REST) {
-    w[0] = tid < a.chunks ? a.rests[size_t(s) * a.chunks + tid] : 0.0;
-  } else {
-    w[0] = plain_chunk();
+  if constexpr (!REST) {
+    const float drafted = skip < a.vocab ? x[skip] : 0.f;
+    plain_chunks();
     // (a draft is refused where u < 1 is at least p(d): what is left is 2^-24 of the row or more, and the
     // difference is off by 2^-29 of that at most)
-    if (skip < a.vocab && skip / kChunk == tid) w[0] = fmax(w[0] - token_weight(skip, x[skip]), 0.0);
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; i++)
+      if (uint32_t(i) < n && skip < a.vocab && skip / kChunk == c0 + i) w[i] = fmax(w[i] - token_weight(skip, drafted), 0.0);
   }
-  uint32_t c = find<1>(w, share, sc, before);
+  uint32_t c = find_chunk(w, n, share, before);
   bool plain = false;
   if (c == kNone) {  // nothing is left of p - q: from p
     plain = true;
-    w[0] = plain_chunk();
-    c = find<1>(w, share, sc, before);
+    plain_chunks();
+    c = find_chunk(w, n, share, before);
   }
-  double z[N], inner;
+  double z[N], mine = 0.0;
+  float y[N];
   const uint32_t i0 = c * kChunk + tid * N;
   const double to = aim - before;
 #pragma unroll
   for (int e = 0; e < N; e++) {
     z[e] = 0.0;
+    y[e] = 0.f;
     const uint32_t i = i0 + e;
     if (c != kNone && i < a.vocab) {
-      z[e] = token_weight(i, x[i]);
+      y[e] = x[i];
+      z[e] = token_weight(i, y[e]);
       if (!plain) {
         if (REST) {
           const float q = a.probs[d.row * a.probs_stride + i];
@@ -335,11 +348,42 @@ __device__ __forceinline__ void draw(const DraftArgs& a, uint32_t s, const DrawR
       }
     }
   }
-  const uint32_t in = find<N>(z, [&](double) { return to; }, sc, inner);
-  if (tid == 0) {
-    const uint32_t token = in == kNone ? d.best : c * kChunk + in;
+  // the token, by the thread that has it
+#pragma unroll
+  for (int e = 0; e < N; e++) mine += z[e];
+  const uint32_t lane = tid & 63, wave = tid >> 6;
+  double up_to = wave_scan64(mine);
+  if (lane == 63) sc.wave[wave] = up_to;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kThreads / 64 - 1; i++)
+    if (i < wave) up_to += sc.wave[i];
+  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
+  if (lane == 0) {
+    sc.some[wave] = some;
+    sc.over[wave] = over;
+  }
+  __syncthreads();
+  uint32_t first = kNone, final = kNone;
+#pragma unroll
+  for (uint32_t i = 0; i < kThreads / 64; i++) {
+    if (first == kNone && sc.over[i]) first = i * 64 + __builtin_ctzll(sc.over[i]);
+    if (sc.some[i]) final = i * 64 + 63 - __builtin_clzll(sc.some[i]);
+  }
+  const uint32_t owner = first != kNone ? first : final;
+  if (tid == (owner == kNone ? 0 : owner)) {
+    double inner;
+    uint32_t at = pick(z, up_to - mine, to, inner), token = i0 + at;
+    float logit = y[0];
+#pragma unroll
+    for (int e = 1; e < N; e++)
+      if (at == uint32_t(e)) logit = y[e];
+    if (owner == kNone) {
+      token = d.best;
+      logit = x[token];
+    }
     a.tokens[d.row] = token;
-    if (a.logprobs) a.logprobs[d.row] = log_weight(d, x[token], t);
+    if (a.logprobs) a.logprobs[d.row] = log_weight(d, logit, t);
   }
 }
 
@@ -352,7 +396,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   __shared__ uint32_t taken[BATCH];
   const uint32_t s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
-  const float t = temperature(a, s);
+  const float t = temperature(a, s), v = a.sample[s];
   if (r1 <= r0) {
     if (threadIdx.x == 0) {
       a.count[s] = 0;
@@ -366,6 +410,11 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
     const uint32_t n = uint32_t(min(r1 - b, int64_t(BATCH)));
     for (uint32_t i = wave; i < n; i += WAVES) {
       const uint32_t r = uint32_t(b) + i;
+      // (the loads that wait for nothing first)
+      const ChunkSum* const sums = a.sums + size_t(r) * a.chunks;
+      ChunkSum z[2];
+#pragma unroll
+      for (uint32_t e = 0; e < 2; e++) z[e] = sums[min(lane + 64 * e, a.chunks - 1)];
       DrawRow d;
       d.k = k;
       d.row = r;
@@ -378,8 +427,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
       float top = -INFINITY;
       uint32_t best = kNone;
       double sum = 0.0;
-      for (uint32_t c = lane; c < a.chunks; c += 64) {
-        const ChunkSum z = a.sums[size_t(r) * a.chunks + c];
+      auto join = [&](const ChunkSum& z) {
         if (z.top > top) {
           sum = sum * (sum == 0.0 ? 0.0 : chunk_scale(top, z.top, k)) + z.sum;
           top = z.top;
@@ -387,7 +435,11 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
         } else if (z.top > -INFINITY) {
           sum += z.sum * chunk_scale(z.top, top, k);
         }
-      }
+      };
+#pragma unroll
+      for (uint32_t e = 0; e < 2; e++)
+        if (lane + 64 * e < a.chunks) join(z[e]);
+      for (uint32_t c = lane + 128; c < a.chunks; c += 64) join(sums[c]);
       d.top = wave_max(top);
       d.greedy = !(t > 0.f) || !(d.top > -INFINITY);
       if (d.greedy) {
@@ -431,7 +483,10 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
       if (!rest) a.draws[s].row = kNone;
     }
   }
-  if (!rest) draw<false>(a, s, d, last, sc);
+  if (!rest) {
+    double w[kLaneChunks];
+    draw<false>(a, d, last, double(v), t, w, sc);
+  }
 }
 
 // A wave per (sequence, chunk): the sum of max(p - q, 0) over a chunk of the row that draws.
@@ -473,9 +528,12 @@ __global__ __launch_bounds__(256) void k_draft_rest(DraftArgs a) {
 __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
   __shared__ Scratch sc;
   const uint32_t s = blockIdx.x;
+  double w[kLaneChunks];  // (of no use, and of any value, where nothing is drawn)
+  load_rests(a, s, w);
+  const float t = temperature(a, s), v = a.sample[s];
   const DrawRow d = a.draws[s];
   if (d.row == kNone) return;
-  draw<true>(a, s, d, false, sc);
+  draw<true>(a, d, false, double(v), t, w, sc);
 }
 
 struct DraftWork {
