@@ -20,6 +20,11 @@
 // row that draws; with no draft probabilities the chunk sums already hold the running sum at chunk
 // borders, so it also draws, reading one chunk again. With them k_draft_rest sums max(p - q, 0) of the
 // drawing rows by chunks and k_draft_draw draws.
+//
+// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 60 us, of which
+// the sums take 32 (152 MB, 4.8 TB/s), decide 8.5, the rest 13 and the draw 6; 32 rows without drafts 16.7 (sums
+// 8, bound by the 64-bit exponentials; decide 8); 5 rows of one sequence 12.5. Decide and draw are chains: plan,
+// sums, the row's total, its chunk, the logits there, the token; 0.5 to 1.5 us a link.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -475,6 +475,10 @@ __device__ __forceinline__ uint64_t row_element(const AttnArgs& a, const Seq& q,
 // and A is 16 bytes of one line of the transposed V page. So K and V go from memory to registers to
 // the matrix cores, with no LDS, no exchange between lanes but the maximum, and no barrier until a
 // part's end. The loads of a step are issued a step ahead (the page numbers two).
+//
+// Measured: a row of each of 64 chats of up to 8192 positions, 32 over 8 heads, e4m3 (587 MB): 106 us, 5.5
+// TB/s (a large copy reads and writes 4.9); 5 rows of each of 16 chats of 2048, 16 over 8 heads, bf16 (95 MB):
+// 26 us; one row over 197 positions: 7.4 us, a launch and four load latencies (plan, page numbers, K and V, out).
 // ---------------------------------------------------------------------------------------------
 template <bool FP8>
 struct StepData {
@@ -769,21 +773,27 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 32 for each of the workgroup's 4 or 8 waves, which share blocks of 64 positions of K
-// and V through LDS: while one is multiplied the next (two, where LDS has room) are on their way.
+// Many rows: tiles of 32 rows (f32: 16) for each of the workgroup's waves, which share blocks of 64 positions
+// of K and V through LDS: while one is multiplied the next (two, where LDS has room) are on their way.
 //
-// Bound by the matrix cores: v_mfma_f32_32x32x16_bf16, transposed as above (a lane's 16 results of a
-// score tile are the weights of 8 consecutive positions in two groups of 16, operand B of
-// Out^T = V^T P^T as they stand), against the exponentials and their arithmetic on the vector unit, some
-// 1400 cycles a block beside 1024 of products, so two waves on each SIMD run one beside the other. bf16
-// rows go in tiles of 256 where there are so many: with 128 every CU pulls 32 KB from L2 for 2 MFLOP, and
-// with all of them loading L2 gives some 50 B/ns each, less than the products take. f32 rows take three
-// products for one, and their registers leave room for one wave on a SIMD: tiles of 128.
-// LDS: K [64][128] with the 16-byte piece c of row r at place c ^ (r & 15), V as it lies in memory
-// ([4][128][16]) with the two pieces of every second 8 dims exchanged: what 16 lanes read at once lies in
-// different banks. bf16 pages are loaded straight into it; e4m3 pages go through registers and are widened
-// once for all rows (K with its scale, V's scale is put on the weights). A wave loads positions of one run
-// of 16, which lie in one page.
+// Bound by the matrix cores and the vector unit, which hardly work at the same time (a 32x32x16 product takes
+// 36 cycles of a SIMD, of which 4 vector operations of its other wave hide behind it; each further one costs
+// 2.8). bf16 rows: v_mfma_f32_32x32x16_bf16, transposed as above (a lane's 16 results of a score tile are the
+// weights of 8 consecutive positions in two groups of 16, operand B of Out^T = V^T P^T as they stand): 32
+// products and some 240 vector operations a block and wave. They go in tiles of 256 where there are so many:
+// with 128 every CU pulls 32 KB from L2 for 2 MFLOP, and with all of them loading L2 gives some 50 B/ns each,
+// less than the products take. f32 rows take three products for one, and 32 rows of their parts fill the
+// registers of a SIMD: 16 rows by v_mfma_f32_16x16x32_bf16 (as in k_page_attn_rows) leave room for two waves
+// on each (32 rows and one wave 1696 us, 16 and two 1455, for 8 chunks of up to 2048 over 4096 positions).
+// Measured: those chunks, 32 over 8 heads, bf16 rows 700 us (e4m3 pages) and 675 (bf16), 860 and 890 TFLOP/s of
+// 1225 that a large library product reaches; matrix cores busy 38% of the time, vector unit 50%. A chunk of
+// 512 f32 rows over 2048 positions, 16 over 8 heads: 37.7 us, of which the plan takes 2, the first loads 3 to 4,
+// the products of 8 blocks 20 and the join 5.
+// LDS: K [64][128] with the 16-byte piece c of row r at place c ^ swap(r), V as it lies in memory
+// ([4][128][16]), for 32-row waves with the two pieces of every second 8 dims exchanged: the lanes that a
+// 16-byte read serves at once (0-3, 12-15, 20-23 and 24-27, and so on) find different banks. bf16 pages are
+// loaded straight into it; e4m3 pages go through registers and are widened once for all rows (K with its
+// scale, V's scale is put on the weights). A wave loads positions of one run of 16, which lie in one page.
 // ---------------------------------------------------------------------------------------------
 template <bool FP8, bool BF16_ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
@@ -1190,6 +1200,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
 // slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; with fewer than 16 of them
 // the threads also share the parts. TILES: parts as the tiles' lanes wrote them.
+// Bound by its launch and two load latencies: 4 to 5 us (15 for 2270 tiles of 256 rows). A workgroup runs on the
+// XCD that wrote the first part: with first parts at multiples of 8 and no such order all of it ran on one XCD,
+// 13 us more.
 // ---------------------------------------------------------------------------------------------
 template <bool BF16_ROWS, bool TILES>
 __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {

@@ -154,7 +154,10 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&o)
 }
 
 // A workgroup per (16 packed rows, KV head), see Rows: thread (tid / 16, tid % 16) has a row and 8 dims of it.
-// Bound by the rows read and written: 14,162 rows of 8 heads, f32 to e4m3 (145 MB), 48 us.
+// Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143
+// MB), 27 us alone and 36 back to back with other inputs (4.0 TB/s; a large copy 4.9); a row each of 48
+// sequences 5.0 us, a launch and the chain starts, lens, table, row. Reading 18,400 bf16 rows out of bf16 pages
+// (151 MB) 30 and 37 us.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, const uint8_t* k, const uint8_t* v,
                                                      uint32_t n_rows, uint64_t stride) {
