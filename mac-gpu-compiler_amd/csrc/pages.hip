@@ -104,10 +104,10 @@ __device__ __forceinline__ void store8(uint8_t* row, uint32_t d, const float (&x
     u32x4_t u;
 #pragma unroll
     for (int i = 0; i < 4; i++) u[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<u32x4_t*>(row + 2 * d) = u;
+    __builtin_nontemporal_store(u, reinterpret_cast<u32x4_t*>(row + 2 * d));
   } else {
-    *reinterpret_cast<f32x4*>(row + 4 * d) = f32x4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f32x4*>(row + 4 * d + 16) = f32x4{x[4], x[5], x[6], x[7]};
+    __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4*>(row + 4 * d));
+    __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4*>(row + 4 * d + 16));
   }
 }
 
@@ -156,8 +156,7 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&o)
 // A workgroup per (16 packed rows, KV head), see Rows: thread (tid / 16, tid % 16) has a row and 8 dims of it.
 // Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143
 // MB), 27 us alone and 36 back to back with other inputs (4.0 TB/s; a large copy 4.9); a row each of 48
-// sequences 5.0 us, a launch and the chain starts, lens, table, row. Reading 18,400 bf16 rows out of bf16 pages
-// (151 MB) 30 and 37 us.
+// sequences 5.0 us, a launch and the chain starts, lens, table, row.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, const uint8_t* k, const uint8_t* v,
                                                      uint32_t n_rows, uint64_t stride) {
@@ -219,7 +218,9 @@ __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, c
   }
 }
 
-// The same rows the other way; a position without a page reads as zeros.
+// The same rows the other way; a position without a page reads as zeros. Pages and rows pass by once, with
+// non-temporal loads and stores: 18,400 bf16 rows out of bf16 pages (151 MB) 39.3 us without, so 35.8 (4.2 TB/s).
+// (The rows that an append reads gain nothing by it, 39.5 and 40.8 us, and the pages it writes are read next.)
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_read(PagePlan p, PageStore st, uint8_t* k, uint8_t* v, uint32_t n_rows,
                                                    uint64_t stride) {
@@ -243,14 +244,14 @@ __global__ __launch_bounds__(256) void k_page_read(PagePlan p, PageStore st, uin
         ks = exp_scale(st.k_exp[slot]);
         vs = exp_scale(st.v_exp[slot]);
       } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(o);
-        kq[0] = u.x; kq[1] = u.y; kq[2] = u.z; kq[3] = u.w;
+        const u32x4_t u = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(o));
+        kq[0] = u[0]; kq[1] = u[1]; kq[2] = u[2]; kq[3] = u[3];
       }
     }
     if (r.whole) {
       const int64_t base = slot_of(r, 0);
       if (tid < sizeof(run) / 16)
-        reinterpret_cast<uint4*>(run)[tid] = reinterpret_cast<const uint4*>(st.v + size_t(base) * kPageDim * EL)[tid];
+        reinterpret_cast<u32x4_t*>(run)[tid] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(st.v + size_t(base) * kPageDim * EL) + tid);
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 8; e++) {
