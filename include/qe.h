@@ -297,7 +297,8 @@ uint64_t qe_page_bytes(uint64_t n_pages, uint64_t page_size, uint64_t n_kv_heads
  * nearest value. e4m3 pages: the exponent is the smallest for which the row's largest finite
  * magnitude is at most 448 of its scale, the values are the nearest (ties to even), and infinities
  * and NaN become NaN. A position whose page is not there is not written. Two rows for one position
- * of one page: either may win. n_rows below 2^28; 0 does nothing. */
+ * of one page: either may win. n_rows, rounded up to a multiple of 16, times n_kv_heads must be below
+ * 2^28; n_rows = 0 does nothing. */
 int qe_op_page_append(const qe_pages* pages, const void* k, const void* v, uint64_t n_rows, uint64_t row_stride,
                       int dtype, void* stream);
 /* The same rows out of the pages (arguments as qe_op_page_append; k and v are written): zeros where

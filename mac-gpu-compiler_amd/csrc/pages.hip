@@ -22,20 +22,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 // ---- which rows a workgroup takes ----
-// V lies transposed in runs of 16 positions, so the rows of one run are written together. Workgroup x
-// takes the runs whose first new row is one of the packed rows 16 x .. 16 x + 15: a window of a long
-// chunk is one whole run whatever the alignment of the chunk, a window of decode rows is 16 runs of one
-// row. Those rows are contiguous and at most 31.
+// V lies transposed in runs of 16 positions, so the rows of one run are written together. The workgroup of
+// window x (and a KV head) takes the runs whose first new row is one of the packed rows 16 x .. 16 x + 15: a
+// window of a long chunk is one whole run whatever the alignment of the chunk, a window of decode rows is 16
+// runs of one row. Those rows are contiguous and at most 31. The heads of a window come one after another:
+// their parts of the packed rows lie side by side (head after head over all rows, 143 MB took 39.5 us for 35.2).
 struct Rows {
-  uint32_t first, count;  // packed rows
-  bool whole;             // one run, all 16 positions of it
-  int64_t slot;           // of lane i < 32: where packed row 16 x + i lies (row index in the pages), -1 no page, -2 no sequence
+  uint32_t window, first, count;  // packed rows
+  bool whole;                     // one run, all 16 positions of it
+  int64_t slot;  // of lane i < 32: where packed row window + i lies (row index in the pages), -1 no page, -2 no sequence
 };
 
 constexpr uint32_t kStartsInLds = 1024;
 
-__device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, int32_t* starts) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, t0 = blockIdx.x * 16, t = t0 + (lane & 31);
+__device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, uint32_t window, uint32_t head, int32_t* starts) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, t0 = window * 16, t = t0 + (lane & 31);
   // the search in `starts` is a chain of loads: from LDS where it fits
   const bool in_lds = p.n_seqs < kStartsInLds;
   if (in_lds) {
@@ -60,7 +61,7 @@ __device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, int3
       r.slot = -1;
       if (pos >= 0 && pos < capacity_of(p)) {
         const int32_t page = page_of(p, lo, pos);
-        if (page >= 0) r.slot = int64_t(page_row(p, page, blockIdx.y, uint32_t(pos) & ((1u << p.page_shift) - 1)));
+        if (page >= 0) r.slot = int64_t(page_row(p, page, head, uint32_t(pos) & ((1u << p.page_shift) - 1)));
       }
     }
   }
@@ -69,6 +70,7 @@ __device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, int3
   // (of 16 consecutive rows one begins a run, so both are there; a plan whose starts decrease may lack it)
   const uint32_t from = here ? __builtin_ctz(here) : 16, to = 16 + (next ? __builtin_ctz(next) : 16);
   r.first = t0 + from;
+  r.window = t0;
   r.count = here ? min(to, n_rows > t0 ? n_rows - t0 : 0u) - min(from, n_rows > t0 ? n_rows - t0 : 0u) : 0;
   const int64_t s = __shfl(r.slot, from & 31);
   r.whole = __builtin_popcount(here) == 1 && r.count == 16 && s >= 0 && (s & (kPageRun - 1)) == 0;
@@ -76,7 +78,7 @@ __device__ __forceinline__ Rows rows_of(const PagePlan& p, uint32_t n_rows, int3
 }
 // slot of row i of r.first ..
 __device__ __forceinline__ int64_t slot_of(const Rows& r, uint32_t i) {
-  return __shfl(r.slot, int((r.first + i) & 31) - int((blockIdx.x * 16) & 31) & 31);
+  return __shfl(r.slot, int(r.first + i - r.window) & 31);
 }
 
 // ---- values ----
@@ -154,17 +156,16 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&o)
 }
 
 // A workgroup per (16 packed rows, KV head), see Rows: thread (tid / 16, tid % 16) has a row and 8 dims of it.
-// Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143
-// MB), 27 us alone and 36 back to back with other inputs (4.0 TB/s; a large copy 4.9); a row each of 48
-// sequences 5.0 us, a launch and the chain starts, lens, table, row.
+// Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143 MB), 33 to 35 us (4.1 to 4.3
+// TB/s; a large copy 4.9); a row each of 48 sequences 5.0 us, a launch and the chain starts, lens, table, row.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, const uint8_t* k, const uint8_t* v,
                                                      uint32_t n_rows, uint64_t stride) {
   constexpr uint32_t EL = FP8 ? 1 : 2, IN = BF16_ROWS ? 2 : 4;
   __shared__ int32_t starts[kStartsInLds + 1];
   __shared__ __align__(16) uint8_t run[kPageRun * kPageDim * EL];  // V of a run as it lies in the page
-  const uint32_t tid = threadIdx.x, head = blockIdx.y, d = (tid & 15) * 8;
-  const Rows r = rows_of(p, n_rows, starts);
+  const uint32_t tid = threadIdx.x, window = blockIdx.x / p.n_kv, head = blockIdx.x - window * p.n_kv, d = (tid & 15) * 8;
+  const Rows r = rows_of(p, n_rows, window, head, starts);
   for (uint32_t b = 0; b < r.count; b += 16) {
     const uint32_t i = b + tid / 16;
     const int64_t slot = slot_of(r, i);
@@ -227,8 +228,8 @@ __global__ __launch_bounds__(256) void k_page_read(PagePlan p, PageStore st, uin
   constexpr uint32_t EL = FP8 ? 1 : 2, OUT = BF16_ROWS ? 2 : 4;
   __shared__ int32_t starts[kStartsInLds + 1];
   __shared__ __align__(16) uint8_t run[kPageRun * kPageDim * EL];
-  const uint32_t tid = threadIdx.x, head = blockIdx.y, d = (tid & 15) * 8;
-  const Rows r = rows_of(p, n_rows, starts);
+  const uint32_t tid = threadIdx.x, window = blockIdx.x / p.n_kv, head = blockIdx.x - window * p.n_kv, d = (tid & 15) * 8;
+  const Rows r = rows_of(p, n_rows, window, head, starts);
   for (uint32_t b = 0; b < r.count; b += 16) {
     const uint32_t i = b + tid / 16;
     const int64_t slot = slot_of(r, i);
@@ -345,9 +346,9 @@ int check_rows(const qe_pages* pages, const void* k, const void* v, uint64_t n_r
   if (n_rows == 0) return QE_OK;
   if (!k || !v) return set_error(QE_ERR_ARG, "null argument");
   const uint64_t el = dtype == QE_KV_F32 ? 4 : 2;
-  if (n_rows > 0x7FFFFFFFull / plan->n_kv) return set_error(QE_ERR_ARG, "need n_rows * n_kv_heads < 2^31");
-  // (a launch has fewer than 2^32 threads along x, 256 for each 16 rows)
-  if (n_rows >= 1ull << 28) return set_error(QE_ERR_ARG, "need n_rows < 2^28");
+  // (a launch has fewer than 2^32 threads, 256 for each 16 rows of a head)
+  if (n_rows >= 1ull << 28 || ceil_div(uint32_t(n_rows), 16u) * uint64_t(plan->n_kv) >= 1ull << 24)
+    return set_error(QE_ERR_ARG, "need n_rows * n_kv_heads < 2^28, n_rows rounded up to a multiple of 16");
   if (stride < uint64_t(plan->n_kv) * kPageDim || stride > 0xFFFFFFFFull || stride * el % 16)
     return set_error(QE_ERR_ARG, "row_stride must be at least n_kv_heads * 128 elements and a multiple of 16 bytes");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16)
@@ -377,7 +378,7 @@ int qe_op_page_append(const qe_pages* pages, const void* k, const void* v, uint6
   qe::PageStore st;
   if (int rc = qe::check_rows(pages, k, v, n_rows, row_stride, dtype, &p, &st)) return rc;
   if (n_rows == 0) return QE_OK;
-  const dim3 grid(qe::ceil_div(uint32_t(n_rows), 16u), p.n_kv);
+  const uint32_t grid = qe::ceil_div(uint32_t(n_rows), 16u) * p.n_kv;
   const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
   auto* kern = fp8 ? (bf16 ? qe::k_page_append<true, true> : qe::k_page_append<true, false>)
                    : (bf16 ? qe::k_page_append<false, true> : qe::k_page_append<false, false>);
@@ -392,7 +393,7 @@ int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, ui
   qe::PageStore st;
   if (int rc = qe::check_rows(pages, k, v, n_rows, row_stride, dtype, &p, &st)) return rc;
   if (n_rows == 0) return QE_OK;
-  const dim3 grid(qe::ceil_div(uint32_t(n_rows), 16u), p.n_kv);
+  const uint32_t grid = qe::ceil_div(uint32_t(n_rows), 16u) * p.n_kv;
   const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
   auto* kern = fp8 ? (bf16 ? qe::k_page_read<true, true> : qe::k_page_read<true, false>)
                    : (bf16 ? qe::k_page_read<false, true> : qe::k_page_read<false, false>);

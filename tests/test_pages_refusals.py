@@ -41,6 +41,7 @@ def calls(pages, rows=4, k=ADDR, v=ADDR, stride=256, dtype=qe.QE_KV_F32):
 
 def test_more_rows_than_a_launch_takes():
     assert list(calls(c_pages(n_kv_heads=1), rows=1 << 28, dtype=qe.QE_KV_BF16)) == [qe.QE_ERR_ARG] * 2
+    assert list(calls(c_pages(n_kv_heads=1024), rows=(1 << 18) - 15, stride=1 << 17)) == [qe.QE_ERR_ARG] * 2
 
 
 def attend(pages, rows=4, heads=4, q=ADDR, out=ADDR + 65536, qs=512, os=512, new=1, dtype=qe.QE_KV_F32, work=ADDR,
