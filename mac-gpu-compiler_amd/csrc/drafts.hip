@@ -14,16 +14,16 @@
 // that f32 would give. Without a distribution to subtract a draw uses the weights as they are, so
 // equal ones are exactly equal.
 //
-// Bound by one read of the logits. k_draft_sums reads every row once, a wave per chunk of 2048 tokens,
+// Bound by one read of the logits. k_draft_sums reads every row once, in chunks of 2048 tokens,
 // and keeps each chunk's largest logit and its sum of weights relative to that one. k_draft_decide, a
 // workgroup per sequence, joins the chunks of each row, accepts drafts (a gather each) and finds the
 // row that draws; with no draft probabilities the chunk sums already hold the running sum at chunk
 // borders, so it also draws, reading one chunk again. With them k_draft_rest sums max(p - q, 0) of the
 // drawing rows by chunks and k_draft_draw draws.
 //
-// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 60 us, of which
-// the sums take 32 (152 MB, 4.8 TB/s), decide 8.5, the rest 13 and the draw 6; 32 rows without drafts 16.7 (sums
-// 8, bound by the 64-bit exponentials; decide 8); 5 rows of one sequence 12.5. Decide and draw are chains: plan,
+// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 59 us, of which
+// the sums take 32 (152 MB, 4.8 TB/s), decide 8.5, the rest 11 and the draw 6; 32 rows without drafts 16.6 (sums
+// 8, bound by the 64-bit exponentials; decide 8); 5 rows of one sequence 12.4. Decide and draw are chains: plan,
 // sums, the row's total, its chunk, the logits there, the token; 0.5 to 1.5 us a link.
 #include <hip/hip_runtime.h>
 
@@ -165,19 +165,20 @@ __device__ __forceinline__ float temperature(const DraftArgs& a, uint32_t s) {
 // log2(e) / T
 __device__ __forceinline__ double rate(float t) { return 1.4426950408889634 / double(t); }
 
-// 32 values of a chunk of a row of n: value 4 i + e of lane l is token c0 + 256 i + 4 l + e; `pad` behind the row
-__device__ __forceinline__ void load_chunk(const float* row, uint32_t c0, uint32_t n, float pad, float (&x)[32]) {
+// N values of a row of n from c0 on: value 4 i + e of lane l is token c0 + 256 i + 4 l + e; `pad` behind the row
+template <int N>
+__device__ __forceinline__ void load_values(const float* row, uint32_t c0, uint32_t n, float pad, float (&x)[N]) {
   const uint32_t lane = threadIdx.x & 63;
-  if (c0 + kChunk <= n) {
+  if (c0 + 64 * N <= n) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < N / 4; i++) {
       const f32x4u v = *reinterpret_cast<const f32x4u*>(row + c0 + 256 * i + 4 * lane);
 #pragma unroll
       for (int e = 0; e < 4; e++) x[4 * i + e] = v[e];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < N / 4; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const uint32_t t = c0 + 256 * i + 4 * lane + e;
@@ -186,27 +187,50 @@ __device__ __forceinline__ void load_chunk(const float* row, uint32_t c0, uint32
   }
 }
 
-// A wave per (row, chunk).
+// A chunk's work goes to one wave (WAVES = 1) or to the four waves of a workgroup, so that few chunks reach all
+// SIMDs: up to 4 for each of them (5 rows 13.4 us with one wave, 12.4 with four; the rests of 40 rows 61.0 and
+// 58.8; the sums of 250 rows, 18,750 chunks, 58.8 and 63.5).
+constexpr uint64_t kFewChunks = 4096;
+
+// The chunk's number, and the first token of the wave's share.
+template <int WAVES>
+__device__ __forceinline__ uint32_t chunk_of(uint32_t& c0) {
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t c = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  c0 = c * kChunk + (WAVES == 1 ? 0 : wave * (kChunk / WAVES));
+  return c;
+}
+
+// Row blockIdx.y + ..., a chunk of it.
+template <int WAVES>
 __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint32_t c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), r = blockIdx.y + blockIdx.z * kRowsAcross;
+  constexpr int N = 32 / WAVES;
+  __shared__ ChunkSum shares[WAVES];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y + blockIdx.z * kRowsAcross;
+  uint32_t c0;
+  const uint32_t c = chunk_of<WAVES>(c0);
   if (c >= a.chunks || r >= a.n_rows) return;
-  float x[32];
-  load_chunk(a.logits + r * a.stride, c * kChunk, a.vocab, -INFINITY, x);
+  float x[N];
+  load_values(a.logits + r * a.stride, c0, a.vocab, -INFINITY, x);
   const int32_t s = sequence(a, int32_t(r));
   if (s < 0) return;
   const float t = temperature(a, s);
   float m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 32; i++) m = fmaxf(m, x[i]);
+  for (int i = 0; i < N; i++) m = fmaxf(m, x[i]);
   m = wave_max(m);
+  if constexpr (WAVES > 1) {
+    if (lane == 0) shares[wave].top = m;
+    __syncthreads();
+    for (int i = 0; i < WAVES; i++) m = fmaxf(m, shares[i].top);
+  }
   double sum = 0.0;
   uint32_t at = kNone;
   if (t > 0.f && m > -INFINITY) {
     const double k = rate(t), top = double(m);
     if (m < INFINITY) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
+      for (int i = 0; i < N; i += 4) {
         double t4[4], w[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) t4[e] = (double(x[i + e]) - top) * k;
@@ -215,17 +239,29 @@ __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; i++) sum += x[i] == m ? 1.0 : 0.0;
+      for (int i = 0; i < N; i++) sum += x[i] == m ? 1.0 : 0.0;
     }
     sum = wave_sum64(sum);
   } else {  // greedy: the first place that holds the largest
 #pragma unroll
-    for (int i = 31; i >= 0; i--)
-      if (x[i] == m) at = c * kChunk + 256 * (i / 4) + 4 * lane + i % 4;
+    for (int i = N - 1; i >= 0; i--)
+      if (x[i] == m) at = c0 + 256 * (i / 4) + 4 * lane + i % 4;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) at = min(at, uint32_t(__shfl_xor(int(at), d)));
   }
-  if (lane == 0) a.sums[size_t(r) * a.chunks + c] = ChunkSum{sum, m, at};
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      shares[wave].sum = sum;
+      shares[wave].best = at;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int i = 1; i < WAVES; i++) {
+        sum += shares[i].sum;
+        at = min(at, shares[i].best);
+      }
+  }
+  if (lane == 0 && (WAVES == 1 || wave == 0)) a.sums[size_t(r) * a.chunks + c] = ChunkSum{sum, m, at};
 }
 
 // ---- a workgroup's draw ----
@@ -494,21 +530,25 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   }
 }
 
-// A wave per (sequence, chunk): the sum of max(p - q, 0) over a chunk of the row that draws.
+// The sum of max(p - q, 0) over a chunk of the row that sequence blockIdx.y draws from.
+template <int WAVES>
 __global__ __launch_bounds__(256) void k_draft_rest(DraftArgs a) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint32_t c = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), s = blockIdx.y;
+  constexpr int N = 32 / WAVES;
+  __shared__ double shares[WAVES];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.y;
+  uint32_t c0;
+  const uint32_t c = chunk_of<WAVES>(c0);
   if (c >= a.chunks) return;
   const DrawRow d = a.draws[s];
   if (d.row == kNone) return;
-  float x[32], q[32];
-  load_chunk(a.logits + d.row * a.stride, c * kChunk, a.vocab, -INFINITY, x);
-  load_chunk(a.probs + d.row * a.probs_stride, c * kChunk, a.vocab, 0.f, q);
+  float x[N], q[N];
+  load_values(a.logits + d.row * a.stride, c0, a.vocab, -INFINITY, x);
+  load_values(a.probs + d.row * a.probs_stride, c0, a.vocab, 0.f, q);
   double sum = 0.0;
   const uint32_t greedy = __builtin_amdgcn_readfirstlane(d.greedy);
   const bool usual = !greedy && d.top < INFINITY;
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < N; i += 4) {
     double w[4];
     if (usual) {
       double t4[4];
@@ -517,8 +557,7 @@ __global__ __launch_bounds__(256) void k_draft_rest(DraftArgs a) {
       exp2_64<4>(t4, w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        w[e] = (greedy ? c * kChunk + 64 * i + 4 * lane + e == d.best : x[i + e] == d.top) ? 1.0 : 0.0;
+      for (int e = 0; e < 4; e++) w[e] = (greedy ? c0 + 64 * i + 4 * lane + e == d.best : x[i + e] == d.top) ? 1.0 : 0.0;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -527,7 +566,13 @@ __global__ __launch_bounds__(256) void k_draft_rest(DraftArgs a) {
     }
   }
   sum = wave_sum64(sum);
-  if (lane == 0) a.rests[size_t(s) * a.chunks + c] = sum;
+  if constexpr (WAVES > 1) {
+    if (lane == 0) shares[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int i = 1; i < WAVES; i++) sum += shares[i];
+  }
+  if (lane == 0 && (WAVES == 1 || wave == 0)) a.rests[size_t(s) * a.chunks + c] = sum;
 }
 
 __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
@@ -589,13 +634,16 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
                   reinterpret_cast<qe::DrawRow*>(base + w.draws)};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t waves4 = qe::ceil_div(a.chunks, 4u);
+  // (`rows` rows of chunks at hand: four waves for each)
+  auto few = [&](uint64_t rows) { return rows * a.chunks <= qe::kFewChunks; };
   if (n_rows) {
     const uint32_t y = a.n_rows < qe::kRowsAcross ? a.n_rows : qe::kRowsAcross;
-    qe::k_draft_sums<<<dim3(waves4, y, qe::ceil_div(a.n_rows, qe::kRowsAcross)), 256, 0, st>>>(a);
+    const dim3 grid(few(a.n_rows) ? a.chunks : waves4, y, qe::ceil_div(a.n_rows, qe::kRowsAcross));
+    (few(a.n_rows) ? qe::k_draft_sums<4> : qe::k_draft_sums<1>)<<<grid, 256, 0, st>>>(a);
   }
   qe::k_draft_decide<<<a.n_seqs, qe::kThreads, 0, st>>>(a);
   if (a.probs && n_rows) {
-    qe::k_draft_rest<<<dim3(waves4, a.n_seqs), 256, 0, st>>>(a);
+    (few(a.n_seqs) ? qe::k_draft_rest<4> : qe::k_draft_rest<1>)<<<dim3(few(a.n_seqs) ? a.chunks : waves4, a.n_seqs), 256, 0, st>>>(a);
     qe::k_draft_draw<<<a.n_seqs, qe::kThreads, 0, st>>>(a);
   }
   const hipError_t e = hipGetLastError();
