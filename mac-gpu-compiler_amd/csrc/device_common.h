@@ -53,6 +53,37 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// Sums over the lanes of a wave up to each (32- and 64-bit types), by lane shifts within rows of 16 and
+// broadcasts of the rows' last lanes; lane 63 has the total.
+template <int CTRL, int ROW_MASK = 0xF, class T>
+__device__ __forceinline__ T shifted(T v) {  // 0 where nothing comes
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = shifted<CTRL, ROW_MASK>(uint32_t(u)), hi = shifted<CTRL, ROW_MASK>(uint32_t(u >> 32));
+    return __builtin_bit_cast(T, uint64_t(hi) << 32 | lo);
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xF, false));
+  }
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += shifted<0x111>(v);
+  v += shifted<0x112>(v);
+  v += shifted<0x114>(v);
+  v += shifted<0x118>(v);
+  v += shifted<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to the rows behind them
+  return v + shifted<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+}
+template <class T>
+__device__ __forceinline__ T from_lane(T v, int lane) {  // to all lanes
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(T, uint64_t(from_lane(uint32_t(u >> 32), lane)) << 32 | from_lane(uint32_t(u), lane));
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  }
+}
+
 // Sum over each aligned group of 8 lanes, returned to the 8 lanes of the group
 // (quad xor1, quad xor2, half-row mirror).
 __device__ __forceinline__ float sum8(float v) {

@@ -128,26 +128,7 @@ __device__ __forceinline__ float log_weight(const DrawRow& d, float x, float t) 
   return float((x == d.top ? 0.0 : (double(x) - double(d.top)) / double(t)) - log(d.total));
 }
 
-// Sums over a wave's lanes up to each, by lane shifts within rows of 16 and broadcasts of the rows' last
-// lanes (through LDS, as __shfl_up goes, the six steps take 0.4 us).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double shifted(double v) {  // 0 where nothing comes
-  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xF, false);
-  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xF, false);
-  return __hiloint2double(hi, lo);
-}
-__device__ __forceinline__ double wave_scan64(double v) {
-  v += shifted<0x111, 0xF>(v);
-  v += shifted<0x112, 0xF>(v);
-  v += shifted<0x114, 0xF>(v);
-  v += shifted<0x118, 0xF>(v);
-  v += shifted<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to the rows behind them
-  return v + shifted<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
-}
-__device__ __forceinline__ double from_lane(double v, int lane) {
-  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
-}
-__device__ __forceinline__ double wave_sum64(double v) { return from_lane(wave_scan64(v), 63); }
+__device__ __forceinline__ double wave_sum64(double v) { return from_lane(wave_scan(v), 63); }
 
 // the row's sequence, or -1 (as paged rows are found: the last one that starts at or before it)
 __device__ __forceinline__ int32_t sequence(const DraftArgs& a, int32_t r) {
@@ -306,14 +287,14 @@ __device__ __forceinline__ uint32_t find_chunk(const double (&w)[kLaneChunks], u
   double mine = 0.0;
 #pragma unroll
   for (int i = 0; i < kLaneChunks; i++) mine += w[i];
-  const double up_to = wave_scan64(mine), to = aim(from_lane(up_to, 63));
+  const double up_to = wave_scan(mine), to = aim(from_lane(up_to, 63));
   const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
   before = 0.0;
   if (!some) return kNone;
   const int owner = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
   const uint32_t at = lane * n + pick(w, up_to - mine, to, before);
   before = from_lane(before, owner);
-  return __builtin_amdgcn_readlane(at, owner);
+  return from_lane(at, owner);
 }
 
 // The sums of max(p - q, 0) over a lane's chunks of sequence s.
@@ -394,7 +375,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
 #pragma unroll
   for (int e = 0; e < N; e++) mine += z[e];
   const uint32_t lane = tid & 63, wave = tid >> 6;
-  double up_to = wave_scan64(mine);
+  double up_to = wave_scan(mine);
   if (lane == 63) sc.wave[wave] = up_to;
   __syncthreads();
 #pragma unroll

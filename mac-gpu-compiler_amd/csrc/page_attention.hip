@@ -37,7 +37,7 @@ constexpr uint32_t kBlock = 64;    // positions
 // Weights are 2^(score - m) with m the largest score so far, or up to kSlack below it: sums are only put
 // on a new m when a score exceeds it by that much (in some row of 32 one is a little larger in most blocks).
 constexpr float kSlack = 8.f;
-constexpr uint32_t kWholeBlocks = 32, kSpare = 1;  // blocks: see find_part
+constexpr uint32_t kWholeBlocks = 32, kSpare = 1, kSpareCut = 3, kFewTiles = 4;  // see find_part
 constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
@@ -171,19 +171,43 @@ __device__ __forceinline__ Cursor uniform(const Cursor& c) {
   return u;
 }
 
+// The cursor of the lane that has `here`, to all lanes.
+__device__ __forceinline__ void take_from(Cursor& cu, bool here) {
+  const uint32_t owner = uniform(uint32_t(__builtin_ctzll(__ballot(here))));
+  auto from = [&](uint32_t v) { return from_lane(v, int(owner)); };
+  cu.q.first = int32_t(from(uint32_t(cu.q.first)));
+  cu.q.row0 = int32_t(from(uint32_t(cu.q.row0)));
+  cu.q.rows = from(cu.q.rows);
+  cu.seq = from(cu.seq);
+  cu.head = from(cu.head);
+  cu.tile = from(cu.tile);
+  cu.block = from(cu.block);
+  cu.blocks = from(cu.blocks);
+}
+
+// How many parts of q blocks b blocks make. (b + q - 1/2) / q is at least 1/2q from a whole number, which f32's
+// rounding of it cannot reach for b up to 2^20 and q up to 2^20.
+__device__ __forceinline__ uint32_t parts_of(uint32_t b, uint32_t q) {
+  return uint32_t((float(b + q) - 0.5f) * __builtin_amdgcn_rcpf(float(q)));
+}
+
 // Workgroup w's part of the list, of W parts of `per` blocks: where it begins and how many blocks it has
 // (0: none). (A part is far below 2^32 blocks: that many are 70 TB of K and V.) A wave finds it alone where a
 // lane can have a sequence each; else each thread sums a contiguous range of sequences, and the one whose
 // range holds the block walks it. W is a power of two.
 //
 // A second piece costs a workgroup some 5 us (its q, its first loads, its sums through LDS and the join), so
-// parts keep to the items in two cases:
+// parts keep to the items in three cases:
 // - Items that are short and about as many as the workgroups are not cut but dealt out whole: the longest up to
 //   32 blocks and up to twice a workgroup's share. 32 x 8 heads of up to 1000 positions 24 us cut, so 14; up to
 //   2000 34 and 23; 4 x 8 of up to 2000 (13 times the share) 15 cut, 20 so; 64 x 8 of up to 4000 59 and 63.
 // - Few items are cut into equally many parts each, where the longest part is at most a block over the even
 //   share: a chunk of 512 over 2048 positions 43.8 us dealt evenly, so 39.0 (bf16 rows 36.6 and 31.8); one row
 //   over 4225 positions 14.7 and 12.7; 3 chunks of up to 300, whose parts would be 2 to 4 blocks over, 43 and 47.
+// - Else few items (of few tiles a sequence, so that counting is quick) are cut into parts of equally many blocks,
+//   with the last of an item shorter, where up to 3 blocks over the even share give no more parts than
+//   workgroups: 16 x 8 of up to 2048 positions, 5 rows each, e4m3 22.2 us dealt evenly, so 19.1 (12 rows 32.4 and
+//   29.1; bf16 pages 26.2 and 26.5); 10 x 8 of up to 3000, one row 23.3 and 21.9.
 __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
                                               uint32_t& per_out, Cursor& cu) {
   const uint32_t tid = threadIdx.x, log_w = 31 - __builtin_clz(W);
@@ -202,19 +226,8 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
     }
     const uint64_t mine = one * a.p.n_kv;
     const uint32_t my_items = tiles * a.p.n_kv;
-    uint64_t up_to = mine;  // blocks and items of the sequences up to the lane's
-    uint32_t up_items = my_items;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint64_t v = __shfl_up(up_to, d);
-      const uint32_t i = __shfl_up(up_items, d);
-      if (int(lane) >= d) {
-        up_to += v;
-        up_items += i;
-      }
-    }
-    const uint64_t total = __shfl(up_to, 63);
-    const uint32_t items = __shfl(up_items, 63);
+    const uint64_t up_to = wave_scan(mine), total = from_lane(up_to, 63);  // blocks of the sequences up to the lane's
+    const uint32_t up_items = wave_scan(my_items), items = from_lane(up_items, 63);
     uint64_t per = split(total), at = w * per;
     uint32_t each = 0;  // parts of every item
     if (!a.whole_items) {
@@ -222,6 +235,43 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
       else if (items <= W) {
         each = W / items;
         if (__any(longest > each * (per + kSpare))) each = 0;
+      }
+    }
+    uint32_t most = 0, parts = 0;  // blocks of a part at most; parts of a head of the lane's sequence
+    if (!a.whole_items && !each && items <= W && !__any(tiles > kFewTiles || longest > 1u << 20)) {
+      uint32_t cut[kSpareCut + 1] = {};
+      for (uint32_t i = 0; i < tiles; i++) {
+        const uint32_t b = tile_blocks(a, q, i, R);
+#pragma unroll
+        for (uint32_t c = 0; c <= kSpareCut; c++) cut[c] += parts_of(b, uint32_t(per) + c);
+      }
+#pragma unroll
+      for (int c = kSpareCut; c >= 0; c--) {
+        if (from_lane(wave_scan(cut[c] * a.p.n_kv), 63) <= W) {
+          most = uint32_t(per) + c;
+          parts = cut[c];
+        }
+      }
+      if (most) {
+        const uint32_t up_parts = wave_scan(parts * a.p.n_kv);
+        const bool here = w < up_parts && w >= up_parts - parts * a.p.n_kv;
+        if (w >= from_lane(up_parts, 63)) return 0;
+        if (here) {
+          uint32_t in = w - (up_parts - parts * a.p.n_kv), n;
+          cu.q = q;
+          cu.seq = lane;
+          cu.head = in / parts;
+          in -= cu.head * parts;
+          cu.tile = 0;
+          while (in >= (n = parts_of(cu.blocks = tile_blocks(a, q, cu.tile, R), most))) {
+            in -= n;
+            cu.tile++;
+          }
+          cu.block = in * most;
+        }
+        per_out = uniform(most);
+        take_from(cu, here);
+        return uniform(min(most, cu.blocks - cu.block));
       }
     }
     const bool by_items = each || a.whole_items;
@@ -247,16 +297,7 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
         cu = cursor_in(a, lane, q, one, at - (to - from_here), R);
       }
     }
-    const uint32_t owner = uniform(uint32_t(__builtin_ctzll(__ballot(here))));
-    auto from = [&](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(owner))); };
-    cu.q.first = int32_t(from(uint32_t(cu.q.first)));
-    cu.q.row0 = int32_t(from(uint32_t(cu.q.row0)));
-    cu.q.rows = from(cu.q.rows);
-    cu.seq = from(cu.seq);
-    cu.head = from(cu.head);
-    cu.tile = from(cu.tile);
-    cu.block = from(cu.block);
-    cu.blocks = from(cu.blocks);
+    take_from(cu, here);
     if (each) {
       cu.blocks = tile_blocks(a, cu.q, cu.tile, R);
       per_out = uniform((cu.blocks + each - 1) / each);
@@ -1309,7 +1350,7 @@ struct Cut {
 Cut cut_of(uint64_t max_new, uint64_t group, bool bf16, uint64_t seq_heads) {
   const uint64_t most = max_new && max_new < 256 ? max_new * group : 256;
   // few rows: two workgroups for each CU where there are as many items (64 x 8 of 4.6k positions 113 us, so 117
-  // with one), one where items are cut up all the same (16 x 8: 39 us with two, so 29)
+  // with one), one where items are cut up all the same (16 x 8: 29.6 us with two, so 26.8)
   if (most <= 32) return {most <= 16 ? 16u : 32u, seq_heads >= kWorkgroups ? kWorkgroups : kWorkgroups / 2};
   if (!bf16) return {128, kWorkgroups / 2};
   return most <= 128 ? Cut{128, kWorkgroups} : Cut{256, kWorkgroups / 2};

@@ -411,3 +411,13 @@ def test_calls_on_two_streams(gpu):
             with torch.cuda.stream(st):
                 graphs[i].replay()
         same()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("new,ctx", [([1 + i % 3 for i in range(40)], [(i * 397) % 3000 for i in range(40)]),
+                                     ([1, 0, 4, 1], [12000, 50, 700, 5000]),
+                                     ([190, 0, 70, 1, 120], [1500, 9, 100, 2500, 800])])
+def test_attention_of_ragged_batches(gpu, new, ctx, rows, kv):
+    """few sequences of very different lengths: parts of one size that end with their item"""
+    check_attention(Case(new, ctx, 64, 2, kv, seed=25, lead=2, tail=5), 4, rows, gap=8)
