@@ -305,10 +305,11 @@ __device__ __forceinline__ void load_rests(const DraftArgs& a, uint32_t s, doubl
 }
 
 // One token of row d.row: over the chunks by their sums, then within a chunk (4 tokens a thread). v, t: the
-// sequence's random number and temperature. REST: from max(p - q, 0), whose sums by chunk are w.
+// sequence's random number and temperature. REST: from max(p - q, 0), whose sums by chunk are w. Else: the logit of
+// the row's draft, and the row's sums by chunk relative to its largest logit where they are at hand (`kept`).
 template <bool REST>
 __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool last, double v, float t, double (&w)[kLaneChunks],
-                                     Scratch& sc) {
+                                     float drafted, const double* kept, Scratch& sc) {
   constexpr int N = kChunk / kThreads;
   const float* x = a.logits + d.row * a.stride;
   const uint32_t tid = threadIdx.x, n = (a.chunks + 63) / 64, c0 = (tid & 63) * n;
@@ -316,7 +317,12 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
   auto token_weight = [&](uint32_t i, float xi) -> double {
     return d.greedy ? (i == d.best ? 1.0 : 0.0) : weight(xi, d.top, d.k);
   };
-  auto plain_chunks = [&]() {
+  auto plain_chunks = [&](const double* kept) {
+    if (kept && !d.greedy) {
+#pragma unroll
+      for (int i = 0; i < kLaneChunks; i++) w[i] = uint32_t(i) < n && c0 + i < a.chunks ? kept[c0 + i] : 0.0;
+      return;
+    }
     ChunkSum p[kLaneChunks];
 #pragma unroll
     for (int i = 0; i < kLaneChunks; i++)
@@ -333,8 +339,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
   double before, aim = 0.0;
   auto share = [&](double all) { return aim = v * all; };
   if constexpr (!REST) {
-    const float drafted = skip < a.vocab ? x[skip] : 0.f;
-    plain_chunks();
+    plain_chunks(kept);
     // (a draft is refused where u < 1 is at least p(d): what is left is 2^-24 of the row or more, and the
     // difference is off by 2^-29 of that at most)
 #pragma unroll
@@ -345,7 +350,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
   bool plain = false;
   if (c == kNone) {  // nothing is left of p - q: from p
     plain = true;
-    plain_chunks();
+    plain_chunks(kept);
     c = find_chunk(w, n, share, before);
   }
   double z[N], mine = 0.0;
@@ -417,6 +422,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   __shared__ DrawRow rows[BATCH];
   __shared__ float drafted[BATCH];  // the draft's logit
   __shared__ uint32_t taken[BATCH];
+  __shared__ double kept[WAVES][128];  // of each wave's last row: its sums by chunk (the first 128)
   const uint32_t s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
   const float t = temperature(a, s), v = a.sample[s];
@@ -429,6 +435,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   }
   const double k = rate(t);
   int64_t stop = -1;
+  const double* at_hand = nullptr;
   for (int64_t b = r0; stop < 0; b += BATCH) {
     const uint32_t n = uint32_t(min(r1 - b, int64_t(BATCH)));
     for (uint32_t i = wave; i < n; i += WAVES) {
@@ -446,32 +453,37 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
       const float x = has ? a.logits[r * a.stride + d.draft] : 0.f, u = a.accept[r];
       float qd = 1.f;
       if (has && a.probs) qd = a.probs[r * a.probs_stride + d.draft];
-      // each lane joins its chunks as they come, then the lanes
       float top = -INFINITY;
-      uint32_t best = kNone;
-      double sum = 0.0;
-      auto join = [&](const ChunkSum& z) {
-        if (z.top > top) {
-          sum = sum * (sum == 0.0 ? 0.0 : chunk_scale(top, z.top, k)) + z.sum;
-          top = z.top;
-          best = z.best;
-        } else if (z.top > -INFINITY) {
-          sum += z.sum * chunk_scale(z.top, top, k);
-        }
-      };
 #pragma unroll
-      for (uint32_t e = 0; e < 2; e++)
-        if (lane + 64 * e < a.chunks) join(z[e]);
-      for (uint32_t c = lane + 128; c < a.chunks; c += 64) join(sums[c]);
+      for (uint32_t e = 0; e < 2; e++) {
+        if (lane + 64 * e >= a.chunks) z[e] = ChunkSum{0.0, -INFINITY, kNone};
+        top = fmaxf(top, z[e].top);
+      }
+      for (uint32_t c = lane + 128; c < a.chunks; c += 64) top = fmaxf(top, sums[c].top);
       d.top = wave_max(top);
       d.greedy = !(t > 0.f) || !(d.top > -INFINITY);
+      uint32_t best = kNone;
+      double sum = 1.0;
       if (d.greedy) {
-        if (top != d.top) best = kNone;
+        auto first = [&](const ChunkSum& z) {
+          if (z.top == d.top) best = min(best, z.best);
+        };
+#pragma unroll
+        for (uint32_t e = 0; e < 2; e++) first(z[e]);
+        for (uint32_t c = lane + 128; c < a.chunks; c += 64) first(sums[c]);
 #pragma unroll
         for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
-        sum = 1.0;
       } else {
-        sum = wave_sum64(sum == 0.0 ? 0.0 : sum * chunk_scale(top, d.top, k));
+        sum = 0.0;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; e++) {
+          const double w = z[e].top > -INFINITY ? z[e].sum * chunk_scale(z[e].top, d.top, k) : 0.0;
+          kept[wave][lane + 64 * e] = w;
+          sum += w;
+        }
+        for (uint32_t c = lane + 128; c < a.chunks; c += 64)
+          if (sums[c].top > -INFINITY) sum += sums[c].sum * chunk_scale(sums[c].top, d.top, k);
+        sum = wave_sum64(sum);
       }
       d.best = best < a.vocab && d.top > -INFINITY && d.greedy ? best : 0;
       d.total = sum;
@@ -490,8 +502,12 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
       a.tokens[b + threadIdx.x] = rows[threadIdx.x].draft;
       if (a.logprobs) a.logprobs[b + threadIdx.x] = log_weight(rows[threadIdx.x], drafted[threadIdx.x], t);
     }
-    if (first < n) stop = b + first;
-    else __syncthreads();
+    if (first < n) {
+      stop = b + first;
+      if (first + WAVES >= n && a.chunks <= 128) at_hand = kept[first % WAVES];
+    } else {
+      __syncthreads();
+    }
   }
   const DrawRow d = rows[(stop - r0) % BATCH];
   for (int64_t e = stop + 1 + threadIdx.x; e < r1; e += kThreads) {
@@ -508,7 +524,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_decide(DraftArgs a) {
   }
   if (!rest) {
     double w[kLaneChunks];
-    draw<false>(a, d, last, double(v), t, w, sc);
+    draw<false>(a, d, last, double(v), t, w, drafted[(stop - r0) % BATCH], at_hand, sc);
   }
 }
 
@@ -565,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
   const float t = temperature(a, s), v = a.sample[s];
   const DrawRow d = a.draws[s];
   if (d.row == kNone) return;
-  draw<true>(a, d, false, double(v), t, w, sc);
+  draw<true>(a, d, false, double(v), t, w, 0.f, nullptr, sc);
 }
 
 struct DraftWork {
