@@ -828,7 +828,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 // on each (32 rows and one wave 1696 us, 16 and two 1455, for 8 chunks of up to 2048 over 4096 positions).
 // Measured: those chunks, 32 over 8 heads, bf16 rows 700 us (e4m3 pages) and 675 (bf16), 860 and 890 TFLOP/s of
 // 1225 that a large library product reaches; matrix cores busy 38% of the time, vector unit 50%. A chunk of
-// 512 f32 rows over 2048 positions, 16 over 8 heads: 37.7 us, of which the plan takes 2, the first loads 3 to 4,
+// 512 f32 rows over 2048 positions, 16 over 8 heads: 33.8 us, of which the plan takes 2, the first loads 3 to 4,
 // the products of 8 blocks 20 and the join 5.
 // LDS: K [64][128] with the 16-byte piece c of row r at place c ^ swap(r), V as it lies in memory
 // ([4][128][16]), for 32-row waves with the two pieces of every second 8 dims exchanged: the lanes that a
@@ -1241,7 +1241,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
 // slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; with fewer than 16 of them
 // the threads also share the parts. TILES: parts as the tiles' lanes wrote them.
-// Bound by its launch and two load latencies: 4 to 5 us (15 for 2270 tiles of 256 rows). A workgroup runs on the
+// Bound by its launch and two load latencies: 4 to 5 us (15 where 256 items of 256 rows are cut). A workgroup runs on the
 // XCD that wrote the first part: with first parts at multiples of 8 and no such order all of it ran on one XCD,
 // 13 us more.
 // ---------------------------------------------------------------------------------------------
