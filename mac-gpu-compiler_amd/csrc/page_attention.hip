@@ -57,10 +57,13 @@ struct AttnArgs {
   float c;                        // log2(e) / sqrt(128)
 };
 
-// An item whose first part is the last one of a workgroup: parts of `n` workgroups from there.
+// An item whose first part is the last one of a workgroup: parts of `n` workgroups from there (0: none). And the
+// workgroup of the first part of the item that this one's first part goes on with, where it helps to join it
+// (else kNowhere).
 struct Joint {
   uint32_t n, rows, head, first;  // rows of the tile; the first of them among its sequence's rows
   int32_t row0;                   // first packed row of the sequence
+  uint32_t from;
 };
 
 __device__ __forceinline__ uint32_t token_of(const AttnArgs& a, uint32_t r) {  // r / group
@@ -353,6 +356,28 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
   return uniform(uint32_t(per < total - at ? per : total - at));
 }
 
+// Whether the workgroups of an item's n parts share its rows when it is joined: where a row's 16 threads would
+// have more than two rounds of parts.
+__device__ __forceinline__ bool joined_by_all(uint32_t n, uint32_t rows) { return n * min(rows, 16u) > 128; }
+
+// The joint of workgroup w before it has begun an item of its own: its first part is at cu, if it has one (`left`).
+__device__ __forceinline__ void goes_on(Joint& j, uint32_t w, uint32_t left, uint32_t per, const Cursor& cu, uint32_t R) {
+  j.n = 0;
+  j.from = kNowhere;
+  if (left && cu.block) {
+    const uint32_t before = (cu.block + per - 1) / per, n = before + (cu.blocks - cu.block + per - 1) / per;
+    if (joined_by_all(n, min(cu.q.rows - cu.tile * R, R))) j.from = w - before;
+  }
+}
+// the item at cu begins a joint of n workgroups (`from` stays)
+__device__ __forceinline__ void begin_joint(Joint& j, uint32_t n, const Cursor& cu, uint32_t R) {
+  j.n = n;
+  j.rows = min(cu.q.rows - cu.tile * R, R);
+  j.head = cu.head;
+  j.first = cu.tile * R;
+  j.row0 = cu.q.row0;
+}
+
 // a workgroup's place in the list: consecutive parts on one XCD (workgroups go to the 8 XCDs in turn)
 __device__ __forceinline__ uint32_t part_index() {
   const uint32_t n = gridDim.x;
@@ -544,7 +569,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
   cu = uniform(cu);
   per = uniform(per);
   a.whole_items = uniform(a.whole_items);
-  if (tid == 0 && a.join) a.joints[w].n = 0;
+  if (tid == 0 && a.join) goes_on(a.joints[w], w, left, per, cu, R);
   if (left == 0) return;
   const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
@@ -806,7 +831,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
         }
       }
       if (!whole && cu.block == 0 && tid == 0)  // the item's last block is in the part (...) / per after this one
-        a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, min(cu.q.rows - cu.tile * R, uint32_t(R)), cu.head, cu.tile * R, cu.q.row0};
+        begin_joint(a.joints[w], (whole_part - left + cu.blocks - 1) / per + 1, cu, R);
     }
     left -= take;
     if (left == 0 || !next_tile(a, cu, R)) break;
@@ -858,7 +883,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
   cu = uniform(cu);
   per = uniform(per);
   a.whole_items = uniform(a.whole_items);
-  if (tid == 0 && a.join) a.joints[w].n = 0;
+  if (tid == 0 && a.join) goes_on(a.joints[w], w, left, per, cu, R);
   if (left == 0) return;
   const uint32_t whole_part = left;
   const uint32_t ps_mask = (1u << a.p.page_shift) - 1;
@@ -1228,7 +1253,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
           }
         }
         if (cu.block == 0 && tid == 0)
-          a.joints[w] = Joint{(whole_part - left + cu.blocks - 1) / per + 1, min(cu.q.rows - cu.tile * R, uint32_t(R)), cu.head, cu.tile * R, cu.q.row0};
+          begin_joint(a.joints[w], (whole_part - left + cu.blocks - 1) / per + 1, cu, R);
       }
     }
     left -= take;
@@ -1239,29 +1264,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Joins the parts of the items that more than one workgroup attended: workgroup (w, y) the item whose
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
-// slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; with fewer than 16 of them
-// the threads also share the parts. TILES: parts as the tiles' lanes wrote them.
+// slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; where they are many, their
+// workgroups share the rows (a row over 31,180 positions, 16 over 1 heads: 16 rows of 244 parts, 53 us with one of
+// them, so 17; 64 x 8 items of two parts 106 us with one, 110 so), and with fewer than 16 rows a workgroup's threads
+// the parts. TILES: parts as the tiles' lanes wrote them.
 // Bound by its launch and two load latencies: 4 to 5 us (15 where 256 items of 256 rows are cut). A workgroup runs on the
 // XCD that wrote the first part: with first parts at multiples of 8 and no such order all of it ran on one XCD,
 // 13 us more.
 // ---------------------------------------------------------------------------------------------
+// The share of workgroup w + who, who in 0 .. n - 1, in joining the item that begins in workgroup w, joint j.
 template <bool BF16_ROWS, bool TILES>
-__global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
-  const uint32_t w = part_index(), tid = threadIdx.x;  // on the XCD that wrote the first part
-  const Joint j = a.joints[w];
-  if (j.n == 0) return;
+__device__ __forceinline__ void join_item(const AttnArgs& a, uint32_t R, const Joint& j, uint32_t w, uint32_t who) {
+  const uint32_t tid = threadIdx.x;
   const uint32_t rows = j.rows, r0 = blockIdx.y * 16;
   if (r0 >= rows) return;
-  const uint32_t here = min(rows - r0, 16u);
+  const uint32_t here = min(rows - r0, 16u), helpers = !TILES && joined_by_all(j.n, rows) ? min(j.n, here) : 1;
+  if (who >= helpers) return;
+  const uint32_t mine = (here - who + helpers - 1) / helpers;  // rows r0 + who, + helpers, ...
   uint32_t slots = 1;
-  while (slots < here) slots *= 2;  // rows side by side; 16 / slots threads share a row's parts
+  while (slots < mine) slots *= 2;  // rows side by side; 16 / slots threads share a row's parts
   if (TILES) slots = 16;
   // neighbouring threads read what lies together: 8 dims after another of a row, or one row after another
   const uint32_t u = TILES ? tid % 16 : tid / 16, d = (TILES ? tid / 16 : tid % 16) * 8;
-  const uint32_t share = 16 / slots, me = u / slots, r = r0 + u % slots;
+  const uint32_t share = 16 / slots, me = u / slots, r = r0 + who + helpers * (u % slots);
   const uint32_t e0 = TILES ? ((r / 32 * 16 + d / 8) * 64 + r % 32) * 4 : r * kPageDim + d, e1 = e0 + (TILES ? 128 : 4);
   const size_t slot = size_t(R) * kPartRow;
-  const bool real = r < rows;
+  const bool real = r < r0 + here;
   float mx = -INFINITY, sum = 0.f, o[8] = {};
   if (real) {
     // a few parts at a time, all their loads together
@@ -1307,6 +1335,7 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
     __shared__ __align__(16) float sums[16][kPageDim];
     __shared__ float top[16], mass[16];
     if (share > 1) {  // in order of the shares
+      __syncthreads();  // the item before has been read
 #pragma unroll
       for (int e = 0; e < 8; e++) sums[u][d + e] = o[e];
       if (d == 0) {
@@ -1337,6 +1366,15 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   Seq q;
   q.row0 = j.row0;
   store_out8<BF16_ROWS>(a.out, row_element(a, q, j.head, j.first + r, a.out_stride) + d, o);
+}
+
+template <bool BF16_ROWS, bool TILES>
+__global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
+  const uint32_t x = part_index();  // on the XCD that wrote the part
+  const Joint j = a.joints[x];
+  if (j.n) join_item<BF16_ROWS, TILES>(a, R, j, x, 0);
+  if constexpr (!TILES)
+    if (j.from != kNowhere) join_item<BF16_ROWS, TILES>(a, R, a.joints[j.from], j.from, x - j.from);
 }
 
 constexpr uint32_t kWorkgroups = 512;  // two for each CU

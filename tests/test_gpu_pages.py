@@ -421,3 +421,11 @@ def test_calls_on_two_streams(gpu):
 def test_attention_of_ragged_batches(gpu, new, ctx, rows, kv):
     """few sequences of very different lengths: parts of one size that end with their item"""
     check_attention(Case(new, ctx, 64, 2, kv, seed=25, lead=2, tail=5), 4, rows, gap=8)
+
+
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("new,ctx,n_kv,heads", [([1], [9000], 1, 16), ([12], [7000], 1, 2), ([2, 1, 1], [6000, 20, 300], 2, 12),
+                                                ([20, 1], [5000, 900], 1, 8)])
+def test_attention_of_many_parts(gpu, new, ctx, n_kv, heads, rows):
+    """a long axis and many q heads of a KV head: parts that the workgroups join together"""
+    check_attention(Case(new, ctx, 64, n_kv, "bf16", seed=26, lead=1), heads, rows)
