@@ -356,9 +356,12 @@ __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t 
   return uniform(uint32_t(per < total - at ? per : total - at));
 }
 
-// Whether the workgroups of an item's n parts share its rows when it is joined: where a row's 16 threads would
-// have more than two rounds of parts.
-__device__ __forceinline__ bool joined_by_all(uint32_t n, uint32_t rows) { return n * min(rows, 16u) > 128; }
+// How many of the workgroups of an item's n parts join it: more than one where a row's 16 threads would have more
+// than two rounds of parts. Small tiles: they share the rows; large ones (R >= 128): the dims, a power of two of them.
+__device__ __forceinline__ uint32_t joiners(uint32_t n, uint32_t rows, uint32_t R) {
+  if (R < 128) return n * min(rows, 16u) > 128 ? min(n, 16u) : 1;
+  return n > 64 ? 16 : n > 32 ? 8 : n > 16 ? 4 : 1;
+}
 
 // The joint of workgroup w before it has begun an item of its own: its first part is at cu, if it has one (`left`).
 __device__ __forceinline__ void goes_on(Joint& j, uint32_t w, uint32_t left, uint32_t per, const Cursor& cu, uint32_t R) {
@@ -366,7 +369,7 @@ __device__ __forceinline__ void goes_on(Joint& j, uint32_t w, uint32_t left, uin
   j.from = kNowhere;
   if (left && cu.block) {
     const uint32_t before = (cu.block + per - 1) / per, n = before + (cu.blocks - cu.block + per - 1) / per;
-    if (joined_by_all(n, min(cu.q.rows - cu.tile * R, R))) j.from = w - before;
+    if (joiners(n, min(cu.q.rows - cu.tile * R, R), R) > 1) j.from = w - before;
   }
 }
 // the item at cu begins a joint of n workgroups (`from` stays)
@@ -1264,13 +1267,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Joins the parts of the items that more than one workgroup attended: workgroup (w, y) the item whose
 // first part is slot 1 of workgroup w, 16 of its rows at a time; the parts that follow it are the
-// slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; where they are many, their
-// workgroups share the rows (a row over 31,180 positions, 16 over 1 heads: 16 rows of 244 parts, 53 us with one of
-// them, so 17; 64 x 8 items of two parts 106 us with one, 110 so), and with fewer than 16 rows a workgroup's threads
-// the parts. TILES: parts as the tiles' lanes wrote them.
-// Bound by its launch and two load latencies: 4 to 5 us (15 where 256 items of 256 rows are cut). A workgroup runs on the
-// XCD that wrote the first part: with first parts at multiples of 8 and no such order all of it ran on one XCD,
-// 13 us more.
+// slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; TILES: 32 rows side by side.
+// Bound by its launch and two load latencies: 4 to 5 us (15 where 256 items of 256 rows are cut), as long as a
+// thread has one or two rounds of parts. Where there would be more the workgroups of the parts share an item: a
+// row over 31,180 positions, 16 over 1 heads (16 rows of 244 parts) 53 us with one workgroup, so 17; 20 rows over
+// 20,000 (320 rows, 128 parts, f32 and bf16) 52 and 58 us, so 31 and 36; 64 x 8 items of two parts 106 us with
+// one, 110 so. A workgroup runs on the XCD that wrote its part: with first parts at multiples of 8 and no such
+// order all of it ran on one XCD, 13 us more.
 // ---------------------------------------------------------------------------------------------
 // The share of workgroup w + who, who in 0 .. n - 1, in joining the item that begins in workgroup w, joint j.
 template <bool BF16_ROWS, bool TILES>
@@ -1278,15 +1281,18 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint32_t R, const J
   const uint32_t tid = threadIdx.x;
   const uint32_t rows = j.rows, r0 = blockIdx.y * 16;
   if (r0 >= rows) return;
-  const uint32_t here = min(rows - r0, 16u), helpers = !TILES && joined_by_all(j.n, rows) ? min(j.n, here) : 1;
+  const uint32_t here = min(rows - r0, 16u), most = joiners(j.n, rows, R);
+  const uint32_t helpers = TILES ? most : min(most, here);
   if (who >= helpers) return;
-  const uint32_t mine = (here - who + helpers - 1) / helpers;  // rows r0 + who, + helpers, ...
-  uint32_t slots = 1;
-  while (slots < mine) slots *= 2;  // rows side by side; 16 / slots threads share a row's parts
-  if (TILES) slots = 16;
-  // neighbouring threads read what lies together: 8 dims after another of a row, or one row after another
-  const uint32_t u = TILES ? tid % 16 : tid / 16, d = (TILES ? tid / 16 : tid % 16) * 8;
-  const uint32_t share = 16 / slots, me = u / slots, r = r0 + who + helpers * (u % slots);
+  // Small tiles: rows r0 + who, + helpers, ..., `slots` of them side by side, a thread 8 dims after another; the
+  // 16 / slots threads of a row's dims share its parts. Large ones: 16 rows after another, a thread each, and
+  // `slots` times 8 dims; the threads that have the same share the parts.
+  uint32_t slots = TILES ? 16 / helpers : 1;
+  if (!TILES)
+    while (slots * helpers < here - who) slots *= 2;
+  const uint32_t u = tid / 16, share = 16 / slots, me = u / slots;
+  const uint32_t d = (TILES ? who * slots + u % slots : tid % 16) * 8;
+  const uint32_t r = r0 + (TILES ? tid % 16 : who + helpers * (u % slots));
   const uint32_t e0 = TILES ? ((r / 32 * 16 + d / 8) * 64 + r % 32) * 4 : r * kPageDim + d, e1 = e0 + (TILES ? 128 : 4);
   const size_t slot = size_t(R) * kPartRow;
   const bool real = r < r0 + here;
@@ -1331,32 +1337,28 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint32_t R, const J
       mx = top;
     }
   }
-  if constexpr (!TILES) {
-    __shared__ __align__(16) float sums[16][kPageDim];
-    __shared__ float top[16], mass[16];
-    if (share > 1) {  // in order of the shares
-      __syncthreads();  // the item before has been read
+  if (share > 1) {  // in order of the shares
+    __shared__ __align__(16) float sums[256 * 8];
+    __shared__ float top[256], mass[256];
+    __syncthreads();  // the item before has been read
 #pragma unroll
-      for (int e = 0; e < 8; e++) sums[u][d + e] = o[e];
-      if (d == 0) {
-        top[u] = mx;
-        mass[u] = sum;
-      }
-      __syncthreads();
-      if (me != 0) return;
-      float all = mx;
-      for (uint32_t i = 1; i < share; i++) all = fmaxf(all, top[u + i * slots]);
-      float f = rebase(mx, all);
-      sum *= f;
+    for (int e = 0; e < 8; e++) sums[tid * 8 + e] = o[e];
+    top[tid] = mx;
+    mass[tid] = sum;
+    __syncthreads();
+    if (me != 0) return;
+    float all = mx;
+    for (uint32_t i = 1; i < share; i++) all = fmaxf(all, top[tid + i * slots * 16]);
+    float f = rebase(mx, all);
+    sum *= f;
 #pragma unroll
-      for (int e = 0; e < 8; e++) o[e] *= f;
-      for (uint32_t i = 1; i < share; i++) {
-        const uint32_t k = u + i * slots;
-        f = rebase(top[k], all);
-        sum = fmaf(mass[k], f, sum);
+    for (int e = 0; e < 8; e++) o[e] *= f;
+    for (uint32_t i = 1; i < share; i++) {
+      const uint32_t k = tid + i * slots * 16;
+      f = rebase(top[k], all);
+      sum = fmaf(mass[k], f, sum);
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = fmaf(sums[k][d + e], f, o[e]);
-      }
+      for (int e = 0; e < 8; e++) o[e] = fmaf(sums[k * 8 + e], f, o[e]);
     }
   }
   if (!real) return;
@@ -1373,8 +1375,7 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   const uint32_t x = part_index();  // on the XCD that wrote the part
   const Joint j = a.joints[x];
   if (j.n) join_item<BF16_ROWS, TILES>(a, R, j, x, 0);
-  if constexpr (!TILES)
-    if (j.from != kNowhere) join_item<BF16_ROWS, TILES>(a, R, a.joints[j.from], j.from, x - j.from);
+  if (j.from != kNowhere) join_item<BF16_ROWS, TILES>(a, R, a.joints[j.from], j.from, x - j.from);
 }
 
 constexpr uint32_t kWorkgroups = 512;  // two for each CU

@@ -425,7 +425,7 @@ def test_attention_of_ragged_batches(gpu, new, ctx, rows, kv):
 
 @pytest.mark.parametrize("rows", [F32, BF16])
 @pytest.mark.parametrize("new,ctx,n_kv,heads", [([1], [9000], 1, 16), ([12], [7000], 1, 2), ([2, 1, 1], [6000, 20, 300], 2, 12),
-                                                ([20, 1], [5000, 900], 1, 8)])
+                                                ([20, 1], [5000, 900], 1, 8), ([20], [9000], 1, 16), ([40, 3], [3000, 100], 1, 8)])
 def test_attention_of_many_parts(gpu, new, ctx, n_kv, heads, rows):
     """a long axis and many q heads of a KV head: parts that the workgroups join together"""
     check_attention(Case(new, ctx, 64, n_kv, "bf16", seed=26, lead=1), heads, rows)
