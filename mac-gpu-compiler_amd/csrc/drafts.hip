@@ -21,7 +21,7 @@
 // borders, so it also draws, reading one chunk again. With them k_draft_rest sums max(p - q, 0) of the
 // drawing rows by chunks and k_draft_draw draws.
 //
-// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 54 to 59 us,
+// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 52 to 59 us,
 // of which the sums take 30 to 35 (152 MB, 4.3 to 5 TB/s), decide 7.4, the rest 10 and the draw 5; 32 rows without
 // drafts 14.0 (sums 8, bound by the 64-bit exponentials; decide 7); 5 rows of one sequence 11.5. Decide and draw
 // are chains: plan, sums, the row's total, its chunk, the logits there, the token; 0.5 to 1.5 us a link.
