@@ -90,14 +90,15 @@ __device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
   return q;
 }
 
-// Position of row r of a sequence's rows.
+// The last position that row r of a sequence's rows attends: its own, or the table's last where it lies behind
+// that (what a step or block holds past the table is masked by it, like any later position); negative: none.
 __device__ __forceinline__ int32_t row_position(const AttnArgs& a, const Seq& q, uint32_t r) {
-  return q.first + int32_t(token_of(a, r));
+  return min(q.first + int32_t(token_of(a, r)), int32_t((a.p.table_stride << a.p.page_shift) - 1));
 }
-// Positions that rows up to r attend: 0 .. limit - 1 (within the table).
+// Positions that rows up to r attend: 0 .. limit - 1.
 __device__ __forceinline__ uint32_t row_limit(const AttnArgs& a, const Seq& q, uint32_t r) {
   const int32_t pos = row_position(a, q, r);
-  return pos < 0 ? 0 : min(uint32_t(pos) + 1, a.p.table_stride << a.p.page_shift);
+  return pos < 0 ? 0 : uint32_t(pos) + 1;
 }
 __device__ __forceinline__ uint32_t tile_limit(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
   return row_limit(a, q, min((tile + 1) * R, q.rows) - 1);
