@@ -1011,8 +1011,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
         if (part_of == 0 && lane < 16 && !(page && x + 16 * run + lane < limit)) vscale[b][16 * run + lane] = 0.f;
     };
     uint32_t foul_from = kNowhere;  // the first block that `clear` cleared something of
-    // this wave's rows against the block at x in buffer b; there: which of its four pages are
-    auto multiply = [&](uint32_t x, uint32_t b, uint32_t there) __attribute__((always_inline)) {
+    // this wave's rows against the block at x in buffer b; there: which of its four pages are; cleared: by `clear`
+    auto multiply = [&](uint32_t x, uint32_t b, uint32_t there, bool cleared) __attribute__((always_inline)) {
       // Fragments come from LDS four at a time, a group ahead of the products that use them; the scheduling
       // barriers keep it so (left alone the compiler waits for every read right behind it).
       constexpr int NT = BF16_ROWS ? 2 : 4, PERS = BF16_ROWS ? 16 : 4;
@@ -1131,7 +1131,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
           if (o == 0) weights(1, pf[1]);
         }
       }
-      if (masked && foul_from == kNowhere && uniform(foul[b]) != 0) foul_from = x;
+      // (not only where this wave masks: `clear` is for the whole tile, whose first rows attend less)
+      if (cleared && foul_from == kNowhere && uniform(foul[b]) != 0) foul_from = x;
     };
     // which of a block's four runs of 16 positions have a page
     auto pages_there = [&](uint32_t x) __attribute__((always_inline)) {
@@ -1181,7 +1182,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
           else wait_dma<0>();
         }
         __syncthreads();  // block x is in LDS; the readers of the block before are done
-        if (int32_t(x + kBlock - 1) > tile_free || there != 15) {
+        const bool cleared = int32_t(x + kBlock - 1) > tile_free || there != 15;
+        if (cleared) {
           clear(x, b, there >> run & 1);
           __syncthreads();
         }
@@ -1190,7 +1192,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
         if (x + AHEAD * kBlock < last) fetch(x + AHEAD * kBlock, STAGES == 3 ? b2 : b1, page);
         const uint32_t there_next = pages_there(x + kBlock);
         page = page_at(x + (AHEAD + 1) * kBlock + 16 * run);
-        if (x < end) multiply(x, b, there);
+        if (x < end) multiply(x, b, there, cleared);
         if (tid == 0) foul[b1] = 0;  // (its last readers are done; its next writers come after a barrier)
         there = there_next;
         b = b1;
