@@ -309,8 +309,8 @@ int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, ui
  * out[t][h] = softmax over j <= position of t of (q[t][h] . k[j] / sqrt(128)), times v[j], over the
  * positions whose page is there; zeros for a row that has none. q and out are [n_rows][n_heads][128]
  * of `dtype` (QE_KV_F32 or QE_KV_BF16), rows q_stride and out_stride elements apart, 16-byte
- * aligned; out must not overlap q or the pages. n_heads is a multiple of n_kv_heads. Softmax and
- * sums are f32; f32 rows keep f32's precision, bf16 rows take the softmax weights rounded to bf16.
+ * aligned; an out that overlaps q or the pages is refused (rows of out may lie between those of q).
+ * n_heads is a multiple of n_kv_heads. Softmax and sums are f32; f32 rows keep f32's precision, bf16 rows take the softmax weights rounded to bf16.
  * A position that a row does not attend has no part in it, whatever K and V hold there; infinities
  * and NaN where it does attend may make it either.
  * max_new: the most new tokens any sequence has (0: not known). It chooses how the work is cut up;

@@ -1401,6 +1401,30 @@ Cut cut_of(uint64_t max_new, uint64_t group, bool bf16, uint64_t seq_heads) {
 // positions 9.0 us, so 10.6 with it; at 500 12.0 and 10.7; f32 tiles of 128 rows at 250 23 and 19).
 constexpr uint64_t kWholeItems = 256;
 
+// n rows of `width` bytes, `stride` (at least width) bytes apart; addresses in more than 64 bits, as the last
+// row's may be.
+struct RowSpan {
+  __int128 base, stride, width, n;
+  __int128 end() const { return base + (n - 1) * stride + width; }
+  // the first row that ends behind `at`
+  __int128 behind(__int128 at) const { return at < base + width ? 0 : (at - base - width) / stride + 1; }
+  __int128 row(__int128 i) const { return base + i * stride; }
+};
+// Whether a row of either shares memory with one of the other; rows may lie between each other's.
+bool overlap(const RowSpan& a, const RowSpan& b) {
+  if (a.end() <= b.base || b.end() <= a.base) return false;
+  if (a.stride == b.stride && a.n == b.n) {  // every row of `hi` lies to the rows of `lo` as its first does
+    const RowSpan &lo = a.base <= b.base ? a : b, &hi = a.base <= b.base ? b : a;
+    return lo.row(lo.behind(hi.base)) < hi.base + hi.width;
+  }
+  for (__int128 i = a.behind(b.base), j = 0; i < a.n && j < b.n;) {
+    if (b.row(j) + b.width <= a.row(i)) j = b.behind(a.row(i));
+    else if (a.row(i) + a.width <= b.row(j)) i = a.behind(b.row(j));
+    else return true;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace qe
 
@@ -1436,8 +1460,18 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   if (work_bytes < qe_op_page_attention_work_bytes(n_heads, a.p.n_kv, max_new))
     return qe::set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_page_attention_work_bytes gives",
                          (unsigned long long)work_bytes);
+  const bool fp8 = pages->kv_dtype == QE_KV_FP8;
+  auto span = [](const void* p, uint64_t stride, uint64_t width, uint64_t n) {
+    return qe::RowSpan{__int128(reinterpret_cast<uintptr_t>(p)), __int128(stride), __int128(width), __int128(n)};
+  };
+  const qe::RowSpan rows = span(out, out_stride * el, n_heads * qe::kPageDim * el, n_rows);
+  const uint64_t page_rows = pages->n_pages * pages->n_kv_heads, kv_bytes = pages->page_size * qe::kPageDim * (fp8 ? 1 : 2);
+  auto over = [&](const void* p, uint64_t bytes) { return qe::overlap(rows, span(p, bytes, bytes, page_rows)); };
+  if (qe::overlap(rows, span(q, q_stride * el, n_heads * qe::kPageDim * el, n_rows)) || over(pages->k, kv_bytes) ||
+      over(pages->v, kv_bytes) || (fp8 && (over(pages->k_exp, pages->page_size) || over(pages->v_exp, pages->page_size))))
+    return qe::set_error(QE_ERR_ARG, "out must not overlap q or the pages");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool fp8 = pages->kv_dtype == QE_KV_FP8, bf16 = dtype == QE_KV_BF16;
+  const bool bf16 = dtype == QE_KV_BF16;
   a.q = static_cast<const uint8_t*>(q);
   a.out = static_cast<uint8_t*>(out);
   a.q_stride = q_stride;
