@@ -310,11 +310,16 @@ int qe_op_page_read(const qe_pages* pages, void* k, void* v, uint64_t n_rows, ui
  * positions whose page is there; zeros for a row that has none. q and out are [n_rows][n_heads][128]
  * of `dtype` (QE_KV_F32 or QE_KV_BF16), rows q_stride and out_stride elements apart, 16-byte
  * aligned; an out that overlaps q or the pages is refused (rows of out may lie between those of q).
- * n_heads is a multiple of n_kv_heads. Softmax and sums are f32; f32 rows keep f32's precision, bf16 rows take the softmax weights rounded to bf16.
- * A position that a row does not attend has no part in it, whatever K and V hold there; infinities
- * and NaN where it does attend may make it either.
+ * n_heads is a multiple of n_kv_heads. Softmax and sums are f32; f32 rows keep f32's precision, bf16
+ * rows take the softmax weights (e4m3 pages: times V's scale) rounded to bf16, each by at most 2^-8 of
+ * itself. Weights are up to 2^8 before the division by their sum, so sums over V of magnitudes up to
+ * 2^88 stay finite at any length; far larger ones may become infinite. A position that a row does not
+ * attend has no part in it, whatever K and V hold there; infinities and NaN where it does attend may
+ * make it either.
  * max_new: the most new tokens any sequence has (0: not known). It chooses how the work is cut up;
- * the results are right for any value. `work` is scratch memory of the call, overwritten by every
+ * the results are right for any value, but the tiles are as large as the longest sequence wants: a call
+ * of a long chunk beside many sequences of one token takes longer than one call for each kind, and one
+ * with 0 may take longer than with the right value. `work` is scratch memory of the call, overwritten by every
  * call: work_bytes at least what qe_op_page_attention_work_bytes gives for the same values. Calls
  * that may overlap need one each. n_rows = 0 does nothing. */
 uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new);

@@ -36,6 +36,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kBlock = 64;    // positions
 // Weights are 2^(score - m) with m the largest score so far, or up to kSlack below it: sums are only put
 // on a new m when a score exceeds it by that much (in some row of 32 one is a little larger in most blocks).
+// So a weight is up to 2^8, and sums over up to 2^31 positions hold V up to 2^88 in f32.
 constexpr float kSlack = 8.f;
 constexpr uint32_t kWholeBlocks = 32, kSpare = 1, kSpareCut = 3, kFewTiles = 4;  // see find_part
 constexpr uint32_t kNowhere = 0xFFFFFFFFu;
