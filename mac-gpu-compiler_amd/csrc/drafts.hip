@@ -21,9 +21,9 @@
 // borders, so it also draws, reading one chunk again. With them k_draft_rest sums max(p - q, 0) of the
 // drawing rows by chunks and k_draft_draw draws.
 //
-// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 52 to 59 us,
-// of which the sums take 30 to 35 (152 MB, 4.3 to 5 TB/s), decide 7.4, the rest 10 and the draw 5; 32 rows without
-// drafts 14.0 (sums 8, bound by the 64-bit exponentials; decide 7); 5 rows of one sequence 11.5. Decide and draw
+// Measured: 250 rows of 151,936 logits with draft probabilities, 40 sequences of up to 7 drafts, 55 to 61 us,
+// of which the sums take 31 to 35 (152 MB, 4.3 to 5 TB/s), decide 7.5, the rest 10 and the draw 5; 32 rows without
+// drafts 14.0 (sums 8, bound by the 64-bit exponentials; decide 7); 5 rows of one sequence 11.4 in a graph. Decide and draw
 // are chains: plan, sums, the row's total, its chunk, the logits there, the token; 0.5 to 1.5 us a link.
 #include <hip/hip_runtime.h>
 
@@ -147,7 +147,8 @@ __device__ __forceinline__ float temperature(const DraftArgs& a, uint32_t s) {
 __device__ __forceinline__ double rate(float t) { return 1.4426950408889634 / double(t); }
 
 // N values of a row of n from c0 on: value 4 i + e of lane l is token c0 + 256 i + 4 l + e; `pad` behind the row.
-// Non-temporal: 40 sequences of up to 7 drafts 62.3 us without, so 58.9; 32 rows 18.2 and 16.5.
+// Non-temporal (four inputs in turn in a graph): 40 sequences of up to 7 drafts 62.6 us without, so 57.5; 32 rows
+// 17.8 and 15.6.
 template <int N>
 __device__ __forceinline__ void load_values(const float* row, uint32_t c0, uint32_t n, float pad, float (&x)[N]) {
   const uint32_t lane = threadIdx.x & 63;
@@ -170,8 +171,9 @@ __device__ __forceinline__ void load_values(const float* row, uint32_t c0, uint3
 }
 
 // A chunk's work goes to one wave (WAVES = 1) or to the four waves of a workgroup, so that few chunks reach all
-// SIMDs: up to 4 for each of them (5 rows 13.4 us with one wave, 12.4 with four; the rests of 40 rows 61.0 and
-// 58.8; the sums of 250 rows, 18,750 chunks, 58.8 and 63.5).
+// SIMDs: up to 4 for each of them (four inputs in turn in a graph: 5 rows 12.5 us with one wave, 11.4 with four; the
+// whole of 40 x 7 with the rests of 40 rows by one 61.5, by four 57.5; with the sums of its 250 rows, 18,750
+// chunks, by four 62.7).
 constexpr uint64_t kFewChunks = 4096;
 
 // The chunk's number, and the first token of the wave's share.

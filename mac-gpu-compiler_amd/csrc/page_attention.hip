@@ -202,17 +202,19 @@ __device__ __forceinline__ uint32_t parts_of(uint32_t b, uint32_t q) {
 // range holds the block walks it. W is a power of two.
 //
 // A second piece costs a workgroup some 5 us (its q, its first loads, its sums through LDS and the join), so
-// parts keep to the items in three cases:
+// parts keep to the items in three cases (times in a graph; f32 rows over bf16 pages, 16 over 8 heads, where not
+// said otherwise):
 // - Items that are short and about as many as the workgroups are not cut but dealt out whole: the longest up to
-//   32 blocks and up to twice a workgroup's share. 32 x 8 heads of up to 1000 positions 24 us cut, so 14; up to
-//   2000 34 and 23; 4 x 8 of up to 2000 (13 times the share) 15 cut, 20 so; 64 x 8 of up to 4000 59 and 63.
+//   32 blocks and up to twice a workgroup's share. bf16 rows over e4m3 pages, 32 over 8 heads: 32 sequences of up
+//   to 1000 positions 24 us cut, so 15; up to 2000 34 and 24; 4 of up to 2000 (13 times the share) 12 cut, 21
+//   whole; 64 of up to 4000 60 cut, 63 whole.
 // - Few items are cut into equally many parts each, where the longest part is at most a block over the even
-//   share: a chunk of 512 over 2048 positions 43.8 us dealt evenly, so 39.0 (bf16 rows 36.6 and 31.8); one row
-//   over 4225 positions 14.7 and 12.7; 3 chunks of up to 300, whose parts would be 2 to 4 blocks over, 43 and 47.
+//   share: a chunk of 512 over 2048 positions 42.8 us dealt evenly, so 38.3 (bf16 rows 33.0 and 30.1); one row
+//   over 4225 positions 13.9 and 12.1; 3 chunks of up to 300, whose parts would be 2 to 4 blocks over, 41 and 46.
 // - Else few items (of few tiles a sequence, so that counting is quick) are cut into parts of equally many blocks,
 //   with the last of an item shorter, where up to 3 blocks over the even share give no more parts than
-//   workgroups: 16 x 8 of up to 2048 positions, 5 rows each, e4m3 22.2 us dealt evenly, so 19.1 (12 rows 32.4 and
-//   29.1; bf16 pages 26.2 and 26.5); 10 x 8 of up to 3000, one row 23.3 and 21.9.
+//   workgroups: 16 x 8 of up to 2048 positions, 5 rows each, e4m3 21.9 us dealt evenly, so 18.9 (12 rows 33.7 and
+//   30.0; bf16 pages 26.6 and 26.4); 10 x 8 of up to 3000, one row 23.2 and 21.7.
 __device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
                                               uint32_t& per_out, Cursor& cu) {
   const uint32_t tid = threadIdx.x, log_w = 31 - __builtin_clz(W);
@@ -428,7 +430,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rebase(float from, float to) { return from == to ? 1.f : exp2_fast(from - to); }
 
 // 8 floats as NS bf16 parts that add up to them: 1 rounded to nearest, or 3 cut (8 + 8 + 8 of f32's 24
-// bits: nothing is lost), so that NS matrix products against bf16 values keep f32's precision.
+// bits: nothing is lost), so that NS matrix products against bf16 values keep f32's precision. bf16 rows take
+// their weights as 1: each is off by at most 2^-8 of itself, as every value of their q and out is, and a second
+// part would double the products of P V. Against 64 bits the result is off by 0.0023 (relative, 64 chats of up to
+// 8192 positions); f32 weights with the same rounding of out leave 0.0017.
 template <int NS>
 __device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&o)[NS]) {
   if constexpr (NS == 1) {
@@ -548,8 +553,8 @@ __device__ __forceinline__ uint64_t row_element(const AttnArgs& a, const Seq& q,
 // part's end. The loads of a step are issued a step ahead (the page numbers two).
 //
 // Measured: a row of each of 64 chats of up to 8192 positions, 32 over 8 heads, e4m3 (587 MB): 106 us, 5.5
-// TB/s (a large copy reads and writes 4.9); 5 rows of each of 16 chats of 2048, 16 over 8 heads, bf16 (95 MB):
-// 26 us; one row over 197 positions: 7.4 us, a launch and four load latencies (plan, page numbers, K and V, out).
+// TB/s, with the join 112 (a large copy reads and writes 4.9; V without non-temporal loads 10 more); 5 rows of each of 16 chats of 2048, 16 over 8 heads, bf16 (95 MB):
+// 26 us; one row over 197 positions: 7.3 us, a launch and four load latencies (plan, page numbers, K and V, out).
 // ---------------------------------------------------------------------------------------------
 template <bool FP8>
 struct StepData {
@@ -856,9 +861,9 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 // less than the products take. f32 rows take three products for one, and 32 rows of their parts fill the
 // registers of a SIMD: 16 rows by v_mfma_f32_16x16x32_bf16 (as in k_page_attn_rows) leave room for two waves
 // on each (32 rows and one wave 1696 us, 16 and two 1455, for 8 chunks of up to 2048 over 4096 positions).
-// Measured: those chunks, 32 over 8 heads, bf16 rows 700 us (e4m3 pages) and 675 (bf16), 860 and 890 TFLOP/s of
+// Measured: those chunks, 32 over 8 heads, bf16 rows 680 to 705 us (e4m3 pages) and 650 to 675 (bf16), 850 to 920 TFLOP/s of
 // 1225 that a large library product reaches; matrix cores busy 38% of the time, vector unit 50%. A chunk of
-// 512 f32 rows over 2048 positions, 16 over 8 heads: 33.8 us, of which the plan takes 2, the first loads 3 to 4,
+// 512 f32 rows over 2048 positions, 16 over 8 heads: 34.0 us, of which the plan takes 2, the first loads 3 to 4,
 // the products of 8 blocks 20 and the join 5.
 // LDS: K [64][128] with the 16-byte piece c of row r at place c ^ swap(r), V as it lies in memory
 // ([4][128][16]), for 32-row waves with the two pieces of every second 8 dims exchanged: the lanes that a
@@ -1274,9 +1279,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 // slots 0 of the workgroups after w. Small tiles' parts are rows of 128 sums; TILES: 32 rows side by side.
 // Bound by its launch and two load latencies: 4 to 5 us (15 where 256 items of 256 rows are cut), as long as a
 // thread has one or two rounds of parts. Where there would be more the workgroups of the parts share an item: a
-// row over 31,180 positions, 16 over 1 heads (16 rows of 244 parts) 53 us with one workgroup, so 17; 20 rows over
-// 20,000 (320 rows, 128 parts, f32 and bf16) 52 and 58 us, so 31 and 36; 64 x 8 items of two parts 106 us with
-// one, 110 so. A workgroup runs on the XCD that wrote its part: with first parts at multiples of 8 and no such
+// row over 31,180 positions, 16 over 1 heads (16 rows of 244 parts) 54 us with one workgroup, so 17; 20 rows over
+// 20,000 (320 rows, 128 parts, f32 and bf16) 52 and 56 us, so 31 and 36; 64 x 8 items of two parts 108 us with
+// one, 113 so. A workgroup runs on the XCD that wrote its part: with first parts at multiples of 8 and no such
 // order all of it ran on one XCD, 13 us more.
 // ---------------------------------------------------------------------------------------------
 // The share of workgroup w + who, who in 0 .. n - 1, in joining the item that begins in workgroup w, joint j.
@@ -1392,14 +1397,14 @@ struct Cut {
 };
 Cut cut_of(uint64_t max_new, uint64_t group, bool bf16, uint64_t seq_heads) {
   const uint64_t most = max_new && max_new < 256 ? max_new * group : 256;
-  // few rows: two workgroups for each CU where there are as many items (64 x 8 of 4.6k positions 113 us, so 117
-  // with one), one where items are cut up all the same (16 x 8: 29.6 us with two, so 26.8)
+  // few rows: two workgroups for each CU where there are as many items (64 x 8 of 4.6k positions 108 us in a graph,
+  // 114 with one), one where items are cut up all the same (16 x 8: 27.8 us with two, so 26.6)
   if (most <= 32) return {most <= 16 ? 16u : 32u, seq_heads >= kWorkgroups ? kWorkgroups : kWorkgroups / 2};
   if (!bf16) return {128, kWorkgroups / 2};
   return most <= 128 ? Cut{128, kWorkgroups} : Cut{256, kWorkgroups / 2};
 }
 // Up to so many positions in a table's row no item of few rows is cut, and no join follows (one row at 197
-// positions 9.0 us, so 10.6 with it; at 500 12.0 and 10.7; f32 tiles of 128 rows at 250 23 and 19).
+// positions 8.8 us in a graph, 10.2 with it; at 500 11.5 whole, so 10.2; f32 tiles of 128 rows at 250 17.9 and 14.5).
 constexpr uint64_t kWholeItems = 256;
 
 // n rows of `width` bytes, `stride` (at least width) bytes apart; addresses in more than 64 bits, as the last

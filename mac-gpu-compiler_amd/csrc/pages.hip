@@ -26,7 +26,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // window x (and a KV head) takes the runs whose first new row is one of the packed rows 16 x .. 16 x + 15: a
 // window of a long chunk is one whole run whatever the alignment of the chunk, a window of decode rows is 16
 // runs of one row. Those rows are contiguous and at most 31. The heads of a window come one after another:
-// their parts of the packed rows lie side by side (head after head over all rows, 143 MB took 39.5 us for 35.2).
+// their parts of the packed rows lie side by side (head after head over all rows, 143 MB
+// took 39.4 us for 35.2, four inputs in turn in a graph).
 struct Rows {
   uint32_t window, first, count;  // packed rows
   bool whole;                     // one run, all 16 positions of it
@@ -156,8 +157,8 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&o)
 }
 
 // A workgroup per (16 packed rows, KV head), see Rows: thread (tid / 16, tid % 16) has a row and 8 dims of it.
-// Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143 MB), 33 to 35 us (4.1 to 4.3
-// TB/s; a large copy 4.9); a row each of 48 sequences 5.0 us, a launch and the chain starts, lens, table, row.
+// Bound by the rows read and written: 13,900 rows of 8 heads, f32 to e4m3 (143 MB), 33.1 us (4.3 TB/s; a large
+// copy 4.9); a row each of 48 sequences 5.0 us, a launch and the chain starts, lens, table, row.
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, const uint8_t* k, const uint8_t* v,
                                                      uint32_t n_rows, uint64_t stride) {
@@ -220,8 +221,9 @@ __global__ __launch_bounds__(256) void k_page_append(PagePlan p, PageStore st, c
 }
 
 // The same rows the other way; a position without a page reads as zeros. Pages and rows pass by once, with
-// non-temporal loads and stores: 18,400 bf16 rows out of bf16 pages (151 MB) 39.3 us without, so 35.8 (4.2 TB/s).
-// (The rows that an append reads gain nothing by it, 39.5 and 40.8 us, and the pages it writes are read next.)
+// non-temporal loads and stores: 18,400 bf16 rows out of bf16 pages (151 MB) 33.7 us (4.5 TB/s);
+// four inputs in turn in a graph 38.8 without, so 35.5. (The rows that an append reads lose by it, 35.2 and 37.6 us,
+// and the pages it writes are read next.)
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_page_read(PagePlan p, PageStore st, uint8_t* k, uint8_t* v, uint32_t n_rows,
                                                    uint64_t stride) {
