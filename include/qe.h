@@ -326,6 +326,55 @@ uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, 
 int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
                          uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work,
                          uint64_t work_bytes, void* stream);
+/* The same for trees of drafted tokens: the new tokens of a sequence are the nodes of a tree (or of
+ * several), at most QE_TREE_NODES of them, appended like any new tokens: node i at position
+ * lens[s] - new + i. parents [n_rows] (int32): which of its sequence's rows a node's parent is, an
+ * earlier one (0 .. i - 1); any other value: it has none. A node attends the positions before the new
+ * tokens, its ancestors and itself; what the others hold has no part in it. A row behind its sequence's
+ * first QE_TREE_NODES is zeros. max_new: at most QE_TREE_NODES; work_bytes and all else as
+ * qe_op_page_attention, and out must not overlap parents either. */
+#define QE_TREE_NODES 64
+int qe_op_page_tree_attention(const qe_pages* pages, const int32_t* parents, const void* q, void* out, uint64_t n_rows,
+                              uint64_t n_heads, uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype,
+                              void* work, uint64_t work_bytes, void* stream);
+
+/* ---- a cache of bounded size: which positions get attention, which to keep, and the move of kept rows
+ *      to the front. No reference counterpart. ----
+ * mass [n_seqs][n_kv_heads][mass_stride] (f32) belongs to the sequences of a plan: entry j of a sequence
+ * and KV head is the softmax weight that position j got so far. */
+/* Adds to mass the weights that the new tokens give: mass[s][h][j] += sum over rows t of sequence s and q
+ * heads g of KV head h of the softmax weight of position j in (t, g), as qe_op_page_attention weighs
+ * them (causal; a position whose page is not there gets nothing). Arguments as there: the rows are the
+ * last tokens of their sequences, so a call may also take only the last few of a prompt. mass_stride is
+ * at least table_stride * page_size. Weights and sums are f32, of rows of either type; the sums are the
+ * same every time. A row with a score that is not finite may make any position it attends NaN. mass
+ * must not overlap q, the pages or work. */
+uint64_t qe_op_page_weigh_work_bytes(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv_heads, uint64_t n_seqs,
+                                     uint64_t positions, uint64_t max_new);
+int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint64_t n_heads, uint64_t q_stride,
+                     uint64_t max_new, int dtype, float* mass, uint64_t mass_stride, void* work, uint64_t work_bytes,
+                     void* stream);
+/* Picks the positions that each KV head of a sequence keeps, by mass: count[s] = min(lens[s], keep) of
+ * 0 .. lens[s] - 1 (lens below 0 counts as 0, above mass_stride as mass_stride), the first `sinks` and the
+ * last `recent` of them always (sinks + recent at most keep), the others by the largest mass, the lowest
+ * position on ties; NaN counts as the smallest, -0 as 0. kept [n_seqs][n_kv_heads][kept_stride]: the
+ * positions, ascending, then -1 up to `keep` (1 .. kept_stride; the rest of a row is left as it was).
+ * mass_stride and kept_stride below 2^31, n_seqs * n_kv_heads below 2^22. Outputs must not overlap the inputs. */
+int qe_op_page_keep(const float* mass, uint64_t mass_stride, const int32_t* lens, uint64_t n_seqs, uint64_t n_kv_heads,
+                    uint64_t keep, uint64_t sinks, uint64_t recent, int32_t* kept, uint64_t kept_stride,
+                    int32_t* count, void* stream);
+/* Moves rows of the pages to the front, in place, K, V and their exponents: position first[s] + i of
+ * sequence s takes the row at first[s] + src[s][h][i], for i < count[s]. src [n_seqs][src_heads][src_stride]
+ * (int32): src_heads is 1 (all KV heads alike) or n_kv_heads; a row of it ascends, with src[i] >= i. So
+ * qe_op_page_keep's positions pack what was kept (first NULL: 0), and qe_op_verify_tree's path puts the
+ * accepted nodes one after another (first: lens before the nodes). mass (nullable) moves along, and is
+ * 0 from first[s] + count[s] to lens[s]; lens itself is the caller's to change. A row whose source or
+ * destination is not there (a page that is not, a position past the table or, for mass, mass_stride) is
+ * left as it was; src that does not ascend or has src[i] < i leaves some of the rows moved undefined, and no
+ * others. count above src_stride counts as src_stride. A page that two sequences share is moved by both:
+ * not for shared pages. src_stride and mass_stride are below 2^31. */
+int qe_op_page_move(const qe_pages* pages, const int32_t* src, uint64_t src_heads, uint64_t src_stride,
+                    const int32_t* count, const int32_t* first, float* mass, uint64_t mass_stride, void* stream);
 
 /* ---- drafted tokens against the target's probabilities, from given random numbers: the sampled
  *      form of qe_verify_greedy's rule, on device memory. No reference counterpart. ----
@@ -351,6 +400,29 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
                         uint64_t probs_stride, const float* accept, const float* sample, const float* temperature,
                         uint32_t* tokens_out, uint32_t* count_out, float* logprobs_out, void* work,
                         uint64_t work_bytes, void* stream);
+
+
+/* The same for a tree of drafts. Rows starts[s] .. starts[s + 1] are the nodes of sequence s's tree, row
+ * starts[s] its root: the last token that is certain. The logits of a row are the target's after the tokens
+ * from the root to it; nodes[r] is its own token (the root's is not read) and parents[r] says which of
+ * the sequence's rows it follows, as in qe_op_page_tree_attention; a node without a parent other than
+ * the root, and a row behind the first QE_TREE_NODES, is never reached. From the root on: with p = softmax(logits
+ * of the node / temperature[s]), the node's children are tried in the order of their rows; child c is accepted
+ * while accept[c] * (1 - sum of the p of those tried before) < p[nodes[c]], a token that was tried before
+ * having no p left. The walk goes on from the first accepted child. Where none is, or max_depth drafts
+ * (0: no bound) have been accepted, the last token is drawn from p without the tokens tried (of a node at
+ * max_depth none are) by sample[s]. What is emitted follows the target's distribution whatever the tree is.
+ * accept [n_rows] and sample [n_seqs] are numbers in [0, 1). Logits, temperature, draws, logprobs_out and work
+ * as in qe_op_verify_drafts; tokens_out [n_rows]: the accepted nodes' tokens, then the drawn one, then
+ * 0xFFFFFFFF; path_out [n_seqs][QE_TREE_NODES] (int32): 0 for the root, the accepted nodes' rows counted from
+ * starts[s], then -1; count_out [n_seqs]: how many tokens, and rows on the path, that is (0 for a sequence
+ * without rows). So path_out and count_out are the src and count of qe_op_page_move. */
+uint64_t qe_op_verify_tree_work_bytes(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab);
+int qe_op_verify_tree(const float* logits, uint64_t n_rows, uint64_t vocab, uint64_t row_stride, const int32_t* starts,
+                      uint64_t n_seqs, const int32_t* parents, const uint32_t* nodes, const float* accept,
+                      const float* sample, const float* temperature, uint64_t max_depth, uint32_t* tokens_out,
+                      int32_t* path_out, uint32_t* count_out, float* logprobs_out, void* work, uint64_t work_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

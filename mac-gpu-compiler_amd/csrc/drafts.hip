@@ -306,6 +306,52 @@ __device__ __forceinline__ void load_rests(const DraftArgs& a, uint32_t s, doubl
   for (int i = 0; i < kLaneChunks; i++) w[i] = uint32_t(i) < n && c0 + i < a.chunks ? a.rests[size_t(s) * a.chunks + c0 + i] : 0.0;
 }
 
+// The token of row d.row whose running weight goes above `to`, by the thread that has it, into packed row
+// at_row; a thread has N tokens from i0 on, with weights z and logits y.
+template <int N>
+__device__ __forceinline__ void place_token(const DraftArgs& a, const DrawRow& d, uint32_t at_row, uint32_t i0, const double (&z)[N],
+                                            const float (&y)[N], double to, float t, Scratch& sc) {
+  const float* x = a.logits + d.row * a.stride;
+  const uint32_t tid = threadIdx.x;
+  double mine = 0.0;
+#pragma unroll
+  for (int e = 0; e < N; e++) mine += z[e];
+  const uint32_t lane = tid & 63, wave = tid >> 6;
+  double up_to = wave_scan(mine);
+  if (lane == 63) sc.wave[wave] = up_to;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kThreads / 64 - 1; i++)
+    if (i < wave) up_to += sc.wave[i];
+  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
+  if (lane == 0) {
+    sc.some[wave] = some;
+    sc.over[wave] = over;
+  }
+  __syncthreads();
+  uint32_t first = kNone, final = kNone;
+#pragma unroll
+  for (uint32_t i = 0; i < kThreads / 64; i++) {
+    if (first == kNone && sc.over[i]) first = i * 64 + __builtin_ctzll(sc.over[i]);
+    if (sc.some[i]) final = i * 64 + 63 - __builtin_clzll(sc.some[i]);
+  }
+  const uint32_t owner = first != kNone ? first : final;
+  if (tid == (owner == kNone ? 0 : owner)) {
+    double inner;
+    uint32_t at = pick(z, up_to - mine, to, inner), token = i0 + at;
+    float logit = y[0];
+#pragma unroll
+    for (int e = 1; e < N; e++)
+      if (at == uint32_t(e)) logit = y[e];
+    if (owner == kNone) {
+      token = d.best;
+      logit = x[token];
+    }
+    a.tokens[at_row] = token;
+    if (a.logprobs) a.logprobs[at_row] = log_weight(d, logit, t);
+  }
+}
+
 // One token of row d.row: over the chunks by their sums, then within a chunk (4 tokens a thread). v, t: the
 // sequence's random number and temperature. REST: from max(p - q, 0), whose sums by chunk are w. Else: the logit of
 // the row's draft, and the row's sums by chunk relative to its largest logit where they are at hand (`kept`).
@@ -355,7 +401,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
     plain_chunks(kept);
     c = find_chunk(w, n, share, before);
   }
-  double z[N], mine = 0.0;
+  double z[N];
   float y[N];
   const uint32_t i0 = c * kChunk + tid * N;
   const double to = aim - before;
@@ -378,43 +424,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
       }
     }
   }
-  // the token, by the thread that has it
-#pragma unroll
-  for (int e = 0; e < N; e++) mine += z[e];
-  const uint32_t lane = tid & 63, wave = tid >> 6;
-  double up_to = wave_scan(mine);
-  if (lane == 63) sc.wave[wave] = up_to;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t i = 0; i < kThreads / 64 - 1; i++)
-    if (i < wave) up_to += sc.wave[i];
-  const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && up_to > to);
-  if (lane == 0) {
-    sc.some[wave] = some;
-    sc.over[wave] = over;
-  }
-  __syncthreads();
-  uint32_t first = kNone, final = kNone;
-#pragma unroll
-  for (uint32_t i = 0; i < kThreads / 64; i++) {
-    if (first == kNone && sc.over[i]) first = i * 64 + __builtin_ctzll(sc.over[i]);
-    if (sc.some[i]) final = i * 64 + 63 - __builtin_clzll(sc.some[i]);
-  }
-  const uint32_t owner = first != kNone ? first : final;
-  if (tid == (owner == kNone ? 0 : owner)) {
-    double inner;
-    uint32_t at = pick(z, up_to - mine, to, inner), token = i0 + at;
-    float logit = y[0];
-#pragma unroll
-    for (int e = 1; e < N; e++)
-      if (at == uint32_t(e)) logit = y[e];
-    if (owner == kNone) {
-      token = d.best;
-      logit = x[token];
-    }
-    a.tokens[d.row] = token;
-    if (a.logprobs) a.logprobs[d.row] = log_weight(d, logit, t);
-  }
+  place_token(a, d, d.row, i0, z, y, to, t, sc);
 }
 
 // A workgroup per sequence: a wave joins the chunks of one row after another.
@@ -586,6 +596,159 @@ __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
   draw<true>(a, d, false, double(v), t, w, 0.f, nullptr, sc);
 }
 
+// ---- trees ----
+struct TreeArgs {
+  DraftArgs d;  // drafts: the nodes' tokens
+  const int32_t* parents;
+  int32_t* path;  // [n_seqs][QE_TREE_NODES]
+  uint32_t max_depth;
+};
+
+// The sum of a row's weights from its chunks' sums, and what a draw needs of it, by each wave for itself.
+__device__ __forceinline__ DrawRow row_of(const DraftArgs& a, uint32_t r, float t) {
+  const uint32_t lane = threadIdx.x & 63;
+  const ChunkSum* const sums = a.sums + size_t(r) * a.chunks;
+  DrawRow d;
+  d.k = rate(t);
+  d.row = r;
+  d.draft = kNone;
+  float top = -INFINITY;
+  for (uint32_t c = lane; c < a.chunks; c += 64) top = fmaxf(top, sums[c].top);
+  d.top = wave_max(top);
+  d.greedy = !(t > 0.f) || !(d.top > -INFINITY);
+  uint32_t best = kNone;
+  double sum = 0.0;
+  for (uint32_t c = lane; c < a.chunks; c += 64) {
+    const ChunkSum z = sums[c];
+    if (d.greedy) {
+      if (z.top == d.top) best = min(best, z.best);
+    } else if (z.top > -INFINITY) {
+      sum += z.sum * chunk_scale(z.top, d.top, d.k);
+    }
+  }
+#pragma unroll
+  for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
+  d.best = best < a.vocab && d.top > -INFINITY && d.greedy ? best : 0;
+  d.total = d.greedy ? 1.0 : wave_sum64(sum);
+  d.inv_total = 1.0 / d.total;
+  return d;
+}
+
+// The weight of token i, whose logit is x, in row d (its share times d.total)
+__device__ __forceinline__ double row_weight(const DrawRow& d, uint32_t i, float x) {
+  return d.greedy ? (i == d.best ? 1.0 : 0.0) : weight(x, d.top, d.k);
+}
+
+// A workgroup per sequence walks its tree: every wave has a node a lane and walks for itself, and all of them
+// draw at the end.
+__global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree) {
+  constexpr int N = kChunk / kThreads;
+  __shared__ Scratch sc;
+  const DraftArgs& a = tree.d;
+  const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
+  int32_t* const path = tree.path + size_t(s) * QE_TREE_NODES;
+  if (r1 <= r0) {
+    if (tid == 0) a.count[s] = 0;
+    if (tid < QE_TREE_NODES) path[tid] = -1;
+    return;
+  }
+  const float t = temperature(a, s);
+  const bool node = lane < r1 - r0;
+  const int32_t parent = node ? tree.parents[r0 + lane] : -1;
+  const uint32_t token = node ? a.drafts[r0 + lane] : kNone;
+  const float accept = node ? a.accept[r0 + lane] : 0.f;
+  uint32_t cur = 0, depth = 0, mine = lane == 0 ? 0u : kNone;  // mine: the path's row at depth `lane`
+  DrawRow d;
+  uint64_t tried;  // children of the last node
+  double w = 0.0;  // their tokens' weights, 0 for a token tried before
+  while (true) {
+    d = row_of(a, uint32_t(r0) + cur, t);
+    const bool child = depth < tree.max_depth && lane > cur && parent == int32_t(cur);
+    tried = __ballot(child);
+    if (!tried) break;
+    w = child && token < a.vocab ? row_weight(d, token, a.logits[d.row * a.stride + token]) : 0.0;
+    double left = 1.0;
+    uint32_t next = kNone;
+    for (uint64_t rest = tried; rest; rest &= rest - 1) {
+      const int c = __builtin_ctzll(rest);
+      const uint32_t is = from_lane(token, c);
+      const uint64_t before = __ballot(child && token == is) & ((1ull << c) - 1);
+      if (before && int(lane) == c) w = 0.0;
+      const double p = from_lane(w, c) * d.inv_total;
+      if (double(from_lane(accept, c)) * left < p) {
+        next = uint32_t(c);
+        break;
+      }
+      left -= p;
+    }
+    if (next == kNone) break;
+    const float x = a.logits[d.row * a.stride + from_lane(token, int(next))];
+    if (tid == 0) {
+      a.tokens[r0 + depth] = from_lane(token, int(next));
+      if (a.logprobs) a.logprobs[r0 + depth] = log_weight(d, x, t);
+    }
+    depth++;
+    if (lane == depth) mine = next;
+    cur = next;
+  }
+  if (tid < QE_TREE_NODES) path[tid] = int32_t(mine);
+  if (tid == 0) a.count[s] = depth + 1;
+  for (int64_t e = r0 + depth + 1 + tid; e < r1; e += kThreads) {
+    a.tokens[e] = kNone;
+    if (a.logprobs) a.logprobs[e] = 0.f;
+  }
+  // the draw: the chunks' sums without the tokens tried, then a chunk's tokens
+  const uint32_t n = (a.chunks + 63) / 64, c0 = lane * n;
+  double chunk[kLaneChunks], before, aim = 0.0;
+  auto plain_chunks = [&] {
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; i++) {
+      chunk[i] = 0.0;
+      if (uint32_t(i) < n && c0 + i < a.chunks) {
+        const ChunkSum z = a.sums[size_t(d.row) * a.chunks + c0 + i];
+        if (d.greedy) chunk[i] = d.best / kChunk == c0 + i ? 1.0 : 0.0;
+        else chunk[i] = z.sum * chunk_scale(z.top, d.top, d.k);
+      }
+    }
+  };
+  auto share = [&](double all) { return aim = double(a.sample[s]) * all; };
+  plain_chunks();
+  for (uint64_t rest = tried; rest; rest &= rest - 1) {
+    const int c = __builtin_ctzll(rest);
+    const uint32_t is = from_lane(token, c);
+    const double less = from_lane(w, c);
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; i++)
+      if (uint32_t(i) < n && is < a.vocab && is / kChunk == c0 + i) chunk[i] = fmax(chunk[i] - less, 0.0);
+  }
+  uint32_t c = find_chunk(chunk, n, share, before);
+  if (c == kNone) {  // nothing is left: from p
+    tried = 0;
+    plain_chunks();
+    c = find_chunk(chunk, n, share, before);
+  }
+  double z[N];
+  float y[N];
+  const uint32_t i0 = c * kChunk + tid * N;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    z[e] = 0.0;
+    y[e] = 0.f;
+    if (c != kNone && i0 + e < a.vocab) {
+      y[e] = a.logits[d.row * a.stride + i0 + e];
+      z[e] = row_weight(d, i0 + e, y[e]);
+    }
+  }
+  for (uint64_t rest = tried; rest; rest &= rest - 1) {
+    const uint32_t is = from_lane(token, __builtin_ctzll(rest));
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (is == i0 + e) z[e] = 0.0;
+  }
+  place_token(a, d, uint32_t(r0) + depth, i0, z, y, aim - before, t, sc);
+}
+
 struct DraftWork {
   uint64_t chunks, sums, rests, draws, bytes;  // byte offsets
 };
@@ -648,6 +811,75 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "verify drafts launch failed: %s", hipGetErrorString(e));
+  return QE_OK;
+}
+
+uint64_t qe_op_verify_tree_work_bytes(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab) {
+  return qe_op_verify_drafts_work_bytes(n_rows, n_seqs, vocab);
+}
+
+int qe_op_verify_tree(const float* logits, uint64_t n_rows, uint64_t vocab, uint64_t row_stride, const int32_t* starts,
+                      uint64_t n_seqs, const int32_t* parents, const uint32_t* nodes, const float* accept,
+                      const float* sample, const float* temperature, uint64_t max_depth, uint32_t* tokens_out,
+                      int32_t* path_out, uint32_t* count_out, float* logprobs_out, void* work, uint64_t work_bytes,
+                      void* stream) {
+  if (!starts || !sample || !count_out || !path_out || !work) return qe::set_error(QE_ERR_ARG, "null argument");
+  if (n_seqs == 0 || n_seqs > 65535) return qe::set_error(QE_ERR_ARG, "n_seqs must be 1..65535");
+  if (n_rows > 0x7FFFFFFFull) return qe::set_error(QE_ERR_ARG, "need n_rows < 2^31");
+  if (n_rows && (!logits || !parents || !nodes || !accept || !tokens_out)) return qe::set_error(QE_ERR_ARG, "null argument");
+  if (vocab == 0 || vocab > qe::kMostVocab) return qe::set_error(QE_ERR_ARG, "vocab must be 1..%u", qe::kMostVocab);
+  if (row_stride < vocab || row_stride > 0xFFFFFFFFull)
+    return qe::set_error(QE_ERR_ARG, "row_stride must be at least vocab and below 2^32");
+  if (work_bytes < qe_op_verify_tree_work_bytes(n_rows, n_seqs, vocab))
+    return qe::set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_verify_tree_work_bytes gives",
+                         (unsigned long long)work_bytes);
+  if (reinterpret_cast<uintptr_t>(work) % 16) return qe::set_error(QE_ERR_ARG, "work must be 16-byte aligned");
+  for (const void* p : {(const void*)logits, (const void*)starts, (const void*)parents, (const void*)nodes, (const void*)accept,
+                        (const void*)sample, (const void*)temperature, (const void*)tokens_out, (const void*)path_out,
+                        (const void*)count_out, (const void*)logprobs_out})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return qe::set_error(QE_ERR_ARG, "arrays must be 4-byte aligned");
+  const qe::Bytes out[] = {{tokens_out, 4 * n_rows}, {path_out, 4 * QE_TREE_NODES * n_seqs}, {count_out, 4 * n_seqs},
+                           {logprobs_out, 4 * n_rows}, {work, work_bytes}};
+  const qe::Bytes in[] = {{logits, n_rows ? 4 * ((n_rows - 1) * row_stride + vocab) : 0}, {starts, 4 * (n_seqs + 1)},
+                          {parents, 4 * n_rows}, {nodes, 4 * n_rows}, {accept, 4 * n_rows}, {sample, 4 * n_seqs},
+                          {temperature, 4 * n_seqs}};
+  for (int i = 0; i < 5; i++) {
+    for (const qe::Bytes& b : in)
+      if (out[i].meets(b)) return qe::set_error(QE_ERR_ARG, "outputs and work must not overlap the inputs");
+    for (int j = 0; j < i; j++)
+      if (out[i].meets(out[j])) return qe::set_error(QE_ERR_ARG, "outputs and work must not overlap each other");
+  }
+  const qe::DraftWork w = qe::draft_work(n_rows, n_seqs, vocab);
+  uint8_t* const base = static_cast<uint8_t*>(work);
+  qe::TreeArgs a{};
+  a.d.logits = logits;
+  a.d.starts = starts;
+  a.d.drafts = nodes;
+  a.d.accept = accept;
+  a.d.sample = sample;
+  a.d.temperature = temperature;
+  a.d.tokens = tokens_out;
+  a.d.count = count_out;
+  a.d.logprobs = logprobs_out;
+  a.d.stride = row_stride;
+  a.d.n_rows = uint32_t(n_rows);
+  a.d.n_seqs = uint32_t(n_seqs);
+  a.d.vocab = uint32_t(vocab);
+  a.d.chunks = uint32_t(w.chunks);
+  a.d.sums = reinterpret_cast<qe::ChunkSum*>(base);
+  a.parents = parents;
+  a.path = path_out;
+  a.max_depth = max_depth && max_depth < QE_TREE_NODES ? uint32_t(max_depth) : QE_TREE_NODES - 1;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n_rows) {
+    const bool few = n_rows * w.chunks <= qe::kFewChunks;
+    const uint32_t y = a.d.n_rows < qe::kRowsAcross ? a.d.n_rows : qe::kRowsAcross;
+    const dim3 grid(few ? a.d.chunks : qe::ceil_div(a.d.chunks, 4u), y, qe::ceil_div(a.d.n_rows, qe::kRowsAcross));
+    (few ? qe::k_draft_sums<4> : qe::k_draft_sums<1>)<<<grid, 256, 0, st>>>(a.d);
+  }
+  qe::k_tree_decide<<<a.d.n_seqs, qe::kThreads, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "verify tree launch failed: %s", hipGetErrorString(e));
   return QE_OK;
 }
 

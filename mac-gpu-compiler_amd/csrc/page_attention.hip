@@ -1387,6 +1387,76 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   if (j.from != kNowhere) join_item<BF16_ROWS, TILES>(a, R, a.joints[j.from], j.from, x - j.from);
 }
 
+// ---------------------------------------------------------------------------------------------
+// Trees: row t of a sequence's rows is a node, whose K and V lie at position first + t; it attends the
+// positions before `first`, its ancestors and itself. A wave for each row and q head: a lane a position's
+// score, then each lane 2 dims of the sum.
+// ---------------------------------------------------------------------------------------------
+template <bool FP8, bool BF16_ROWS>
+__global__ __launch_bounds__(64) void k_page_tree(AttnArgs a, const int32_t* parents) {
+  constexpr int EL = FP8 ? 1 : 2;
+  __shared__ float qs[kPageDim], weight[kBlock];
+  const uint32_t heads = a.group * a.p.n_kv, t = blockIdx.x / heads, h = blockIdx.x - t * heads, lane = threadIdx.x, kv = h / a.group;
+  uint32_t lo = 0, hi = a.p.n_seqs;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.p.starts[mid] <= int32_t(t)) lo = mid;
+    else hi = mid;
+  }
+  if (a.p.starts[lo] > int32_t(t) || int32_t(t) >= a.p.starts[lo + 1]) return;
+  const Seq q = read_seq(a, lo);
+  const uint32_t node = t - uint32_t(q.row0);
+  uint64_t family = 0;
+  if (node < 64) {
+    family = 1ull << node;
+    for (int32_t at = int32_t(node), p; (p = parents[q.row0 + at]) >= 0 && p < at; at = p) family |= 1ull << p;
+  }
+  for (int i = 0; i < 2; i++) {
+    const uint64_t e = uint64_t(t) * a.q_stride + h * kPageDim + 2 * lane + i;
+    qs[2 * lane + i] = BF16_ROWS ? bf16f(reinterpret_cast<const uint16_t*>(a.q)[e]) : reinterpret_cast<const float*>(a.q)[e];
+  }
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, o[2] = {};
+  const int64_t capacity = capacity_of(a.p), end = min(int64_t(q.first) + int64_t(node) + 1, capacity);
+  for (int64_t x = 0; x < end && node < 64; x += kBlock) {
+    const int64_t j = x + lane, in = j - q.first;
+    const int32_t page = j < capacity ? page_of(a.p, lo, j) : -1;
+    const uint32_t off = uint32_t(j) & ((1u << a.p.page_shift) - 1);
+    float s = -INFINITY;
+    if (page >= 0 && (in < 0 || (in < 64 && (family >> in & 1)))) {
+      const size_t row = page_row(a.p, page, kv, off);
+      s = 0.f;
+      for (uint32_t d = 0; d < kPageDim; d++) s = fmaf(qs[d], v_value<FP8>(a.st.k, row * kPageDim + d), s);
+      if (FP8) s *= exp_scale(a.st.k_exp[row]);
+      s *= a.c;
+    }
+    const float top = fmaxf(m, wave_max(s));
+    const float w = s == -INFINITY ? 0.f : exp2f(s - top);
+    const float f = m == top ? 1.f : exp2f(m - top);
+    m = top;
+    l = l * f + wave_sum(w);
+    o[0] *= f;
+    o[1] *= f;
+    weight[lane] = w;
+    __syncthreads();
+    for (uint32_t i = 0; i < kBlock; i++) {
+      if (weight[i] == 0.f) continue;
+      const int32_t at = page_of(a.p, lo, x + i);
+      const uint32_t off = uint32_t(x + i) & ((1u << a.p.page_shift) - 1);
+      const float scale = FP8 ? exp_scale(a.st.v_exp[page_row(a.p, at, kv, off)]) : 1.f;
+      const size_t e = v_element(a.p, at, kv, off);
+      for (int d = 0; d < 2; d++) o[d] = fmaf(weight[i] * scale, v_value<FP8>(a.st.v, e + 16 * (2 * lane + d)), o[d]);
+    }
+    __syncthreads();
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int d = 0; d < 2; d++) {
+    const uint64_t e = uint64_t(t) * a.out_stride + h * kPageDim + 2 * lane + d;
+    if (BF16_ROWS) reinterpret_cast<uint16_t*>(a.out)[e] = f32_to_bf16(o[d] * inv);
+    else reinterpret_cast<float*>(a.out)[e] = o[d] * inv;
+  }
+}
+
 constexpr uint32_t kWorkgroups = 512;  // two for each CU
 
 // How calls are cut, by the most rows (new tokens x q heads of a KV head) a sequence can have: tiles of 16
@@ -1431,51 +1501,49 @@ bool overlap(const RowSpan& a, const RowSpan& b) {
   return false;
 }
 
-}  // namespace
-}  // namespace qe
-
-extern "C" {
-
-uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
+uint64_t attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
   if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
   uint64_t rows = 0;  // of all workgroups
   for (bool bf16 : {false, true}) {
-    const qe::Cut c = qe::cut_of(max_new, n_heads / n_kv_heads, bf16, ~0ull);
+    const Cut c = cut_of(max_new, n_heads / n_kv_heads, bf16, ~0ull);
     rows = rows > uint64_t(c.rows) * c.workgroups ? rows : uint64_t(c.rows) * c.workgroups;
   }
-  return rows * 2 * qe::kPartRow * 4 + qe::kWorkgroups * sizeof(qe::Joint);
+  return rows * 2 * kPartRow * 4 + kWorkgroups * sizeof(Joint);
 }
 
-int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
-                         uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work,
-                         uint64_t work_bytes, void* stream) {
-  qe::AttnArgs a{};
-  if (int rc = qe::check_pages(pages, &a.p, &a.st)) return rc;
-  if (dtype != QE_KV_F32 && dtype != QE_KV_BF16) return qe::set_error(QE_ERR_ARG, "rows are QE_KV_F32 or QE_KV_BF16");
+// Causal attention (parents null), or of trees.
+int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
+           uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work, uint64_t work_bytes,
+           void* stream) {
+  AttnArgs a{};
+  if (int rc = check_pages(pages, &a.p, &a.st)) return rc;
+  if (dtype != QE_KV_F32 && dtype != QE_KV_BF16) return set_error(QE_ERR_ARG, "rows are QE_KV_F32 or QE_KV_BF16");
   if (n_heads == 0 || n_heads % a.p.n_kv || n_heads > 65536)
-    return qe::set_error(QE_ERR_ARG, "n_heads must be a multiple of n_kv_heads, at most 65536");
+    return set_error(QE_ERR_ARG, "n_heads must be a multiple of n_kv_heads, at most 65536");
   if (n_rows == 0) return QE_OK;
-  if (!q || !out || !work) return qe::set_error(QE_ERR_ARG, "null argument");
-  if (n_rows > 0x7FFFFFFFull / n_heads) return qe::set_error(QE_ERR_ARG, "need n_rows * n_heads < 2^31");
+  if (!q || !out || !work) return set_error(QE_ERR_ARG, "null argument");
+  if (n_rows > 0x7FFFFFFFull / n_heads) return set_error(QE_ERR_ARG, "need n_rows * n_heads < 2^31");
   const uint64_t el = dtype == QE_KV_F32 ? 4 : 2;
   for (uint64_t stride : {q_stride, out_stride})
-    if (stride < n_heads * qe::kPageDim || stride > 0xFFFFFFFFull || stride * el % 16)
-      return qe::set_error(QE_ERR_ARG, "row strides must be at least n_heads * 128 elements and multiples of 16 bytes");
+    if (stride < n_heads * kPageDim || stride > 0xFFFFFFFFull || stride * el % 16)
+      return set_error(QE_ERR_ARG, "row strides must be at least n_heads * 128 elements and multiples of 16 bytes");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) % 16)
-    return qe::set_error(QE_ERR_ARG, "q, out and work must be 16-byte aligned");
-  if (work_bytes < qe_op_page_attention_work_bytes(n_heads, a.p.n_kv, max_new))
-    return qe::set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_page_attention_work_bytes gives",
+    return set_error(QE_ERR_ARG, "q, out and work must be 16-byte aligned");
+  if (work_bytes < attention_work_bytes(n_heads, a.p.n_kv, max_new))
+    return set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_page_attention_work_bytes gives",
                          (unsigned long long)work_bytes);
   const bool fp8 = pages->kv_dtype == QE_KV_FP8;
   auto span = [](const void* p, uint64_t stride, uint64_t width, uint64_t n) {
-    return qe::RowSpan{__int128(reinterpret_cast<uintptr_t>(p)), __int128(stride), __int128(width), __int128(n)};
+    return RowSpan{__int128(reinterpret_cast<uintptr_t>(p)), __int128(stride), __int128(width), __int128(n)};
   };
-  const qe::RowSpan rows = span(out, out_stride * el, n_heads * qe::kPageDim * el, n_rows);
-  const uint64_t page_rows = pages->n_pages * pages->n_kv_heads, kv_bytes = pages->page_size * qe::kPageDim * (fp8 ? 1 : 2);
-  auto over = [&](const void* p, uint64_t bytes) { return qe::overlap(rows, span(p, bytes, bytes, page_rows)); };
-  if (qe::overlap(rows, span(q, q_stride * el, n_heads * qe::kPageDim * el, n_rows)) || over(pages->k, kv_bytes) ||
+  const RowSpan rows = span(out, out_stride * el, n_heads * kPageDim * el, n_rows);
+  const uint64_t page_rows = pages->n_pages * pages->n_kv_heads, kv_bytes = pages->page_size * kPageDim * (fp8 ? 1 : 2);
+  auto over = [&](const void* p, uint64_t bytes) { return overlap(rows, span(p, bytes, bytes, page_rows)); };
+  if (overlap(rows, span(q, q_stride * el, n_heads * kPageDim * el, n_rows)) || over(pages->k, kv_bytes) ||
       over(pages->v, kv_bytes) || (fp8 && (over(pages->k_exp, pages->page_size) || over(pages->v_exp, pages->page_size))))
-    return qe::set_error(QE_ERR_ARG, "out must not overlap q or the pages");
+    return set_error(QE_ERR_ARG, "out must not overlap q or the pages");
+  if (parents && overlap(rows, span(parents, 4 * n_rows, 4 * n_rows, 1)))
+    return set_error(QE_ERR_ARG, "out must not overlap parents");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == QE_KV_BF16;
   a.q = static_cast<const uint8_t*>(q);
@@ -1487,37 +1555,70 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
   // shift = ceil(log2 group), magic = ceil(2^(31 + shift) / group): exact below 2^31
   while ((1ull << a.group_shift) < a.group) a.group_shift++;
   a.group_magic = uint32_t(((1ull << (31 + a.group_shift)) + a.group - 1) / a.group);
-  a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
-  a.joints = static_cast<qe::Joint*>(work);
-  a.parts = reinterpret_cast<float*>(a.joints + qe::kWorkgroups);
+  a.c = 1.44269504f / sqrtf(float(kPageDim));
+  a.joints = static_cast<Joint*>(work);
+  a.parts = reinterpret_cast<float*>(a.joints + kWorkgroups);
+  if (parents) {
+    auto go = [&](auto* kern) { kern<<<uint32_t(n_rows * n_heads), 64, 0, st>>>(a, parents); };
+    if (fp8) go(bf16 ? k_page_tree<true, true> : k_page_tree<true, false>);
+    else go(bf16 ? k_page_tree<false, true> : k_page_tree<false, false>);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(QE_ERR_HIP, "page tree attention launch failed: %s", hipGetErrorString(e));
+    return QE_OK;
+  }
   // (fewer rows than max_new says need no more than the work that was asked for)
   const uint64_t bound = max_new && max_new < n_rows ? max_new : n_rows;
-  const qe::Cut c = qe::cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
+  const Cut c = cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
   const uint32_t R = c.rows, grid = c.workgroups;
-  a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= qe::kWholeItems;
+  a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= kWholeItems;
   a.join = !a.whole_items;
   auto go = [&](auto* kern) { kern<<<grid, R == 256 || (R == 128 && !bf16) ? 512 : 256, 0, st>>>(a); };
   if (R == 256) {
-    go(fp8 ? qe::k_page_attn_tiles<true, true, 8> : qe::k_page_attn_tiles<false, true, 8>);
+    go(fp8 ? k_page_attn_tiles<true, true, 8> : k_page_attn_tiles<false, true, 8>);
   } else if (R == 128) {
-    if (fp8) go(bf16 ? qe::k_page_attn_tiles<true, true, 4> : qe::k_page_attn_tiles<true, false, 8>);
-    else go(bf16 ? qe::k_page_attn_tiles<false, true, 4> : qe::k_page_attn_tiles<false, false, 8>);
+    if (fp8) go(bf16 ? k_page_attn_tiles<true, true, 4> : k_page_attn_tiles<true, false, 8>);
+    else go(bf16 ? k_page_attn_tiles<false, true, 4> : k_page_attn_tiles<false, false, 8>);
   } else if (R == 32) {
-    if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 2> : qe::k_page_attn_rows<true, false, 2>);
-    else go(bf16 ? qe::k_page_attn_rows<false, true, 2> : qe::k_page_attn_rows<false, false, 2>);
+    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 2> : k_page_attn_rows<true, false, 2>);
+    else go(bf16 ? k_page_attn_rows<false, true, 2> : k_page_attn_rows<false, false, 2>);
   } else {
-    if (fp8) go(bf16 ? qe::k_page_attn_rows<true, true, 1> : qe::k_page_attn_rows<true, false, 1>);
-    else go(bf16 ? qe::k_page_attn_rows<false, true, 1> : qe::k_page_attn_rows<false, false, 1>);
+    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 1> : k_page_attn_rows<true, false, 1>);
+    else go(bf16 ? k_page_attn_rows<false, true, 1> : k_page_attn_rows<false, false, 1>);
   }
   if (a.join) {
     const dim3 join(grid, R / 16);
     auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
-    if (R >= 128) join_by(bf16 ? qe::k_page_join<true, true> : qe::k_page_join<false, true>);
-    else join_by(bf16 ? qe::k_page_join<true, false> : qe::k_page_join<false, false>);
+    if (R >= 128) join_by(bf16 ? k_page_join<true, true> : k_page_join<false, true>);
+    else join_by(bf16 ? k_page_join<true, false> : k_page_join<false, false>);
   }
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page attention launch failed: %s", hipGetErrorString(e));
+  if (e != hipSuccess) return set_error(QE_ERR_HIP, "page attention launch failed: %s", hipGetErrorString(e));
   return QE_OK;
+}
+
+}  // namespace
+}  // namespace qe
+
+extern "C" {
+
+uint64_t qe_op_page_attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t max_new) {
+  return qe::attention_work_bytes(n_heads, n_kv_heads, max_new);
+}
+
+int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
+                         uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work,
+                         uint64_t work_bytes, void* stream) {
+  return qe::attend(pages, nullptr, q, out, n_rows, n_heads, q_stride, out_stride, max_new, dtype, work, work_bytes, stream);
+}
+
+int qe_op_page_tree_attention(const qe_pages* pages, const int32_t* parents, const void* q, void* out, uint64_t n_rows,
+                              uint64_t n_heads, uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype,
+                              void* work, uint64_t work_bytes, void* stream) {
+  if (n_rows && !parents) return qe::set_error(QE_ERR_ARG, "null argument");
+  if (reinterpret_cast<uintptr_t>(parents) % 4) return qe::set_error(QE_ERR_ARG, "parents must be 4-byte aligned");
+  if (max_new > QE_TREE_NODES) return qe::set_error(QE_ERR_ARG, "max_new must be at most %u", unsigned(QE_TREE_NODES));
+  return qe::attend(pages, parents, q, out, n_rows, n_heads, q_stride, out_stride, max_new ? max_new : QE_TREE_NODES, dtype,
+                    work, work_bytes, stream);
 }
 
 }  // extern "C"

@@ -229,6 +229,13 @@ def lib() -> ctypes.CDLL:
         "qe_op_page_attention": (i32, [ctypes.POINTER(_CPages), vp, vp, u64, u64, u64, u64, u64, i32, vp, u64, vp]),
         "qe_op_verify_drafts_work_bytes": (u64, [u64, u64, u64]),
         "qe_op_verify_drafts": (i32, [vp, u64, u64, u64, vp, u64, vp, vp, u64, vp, vp, vp, vp, vp, vp, vp, u64, vp]),
+        "qe_op_page_tree_attention": (i32, [ctypes.POINTER(_CPages), vp, vp, vp, u64, u64, u64, u64, u64, i32, vp, u64, vp]),
+        "qe_op_page_weigh_work_bytes": (u64, [u64, u64, u64, u64, u64, u64]),
+        "qe_op_page_weigh": (i32, [ctypes.POINTER(_CPages), vp, u64, u64, u64, u64, i32, vp, u64, vp, u64, vp]),
+        "qe_op_page_keep": (i32, [vp, u64, vp, u64, u64, u64, u64, u64, vp, u64, vp, vp]),
+        "qe_op_page_move": (i32, [ctypes.POINTER(_CPages), vp, u64, u64, vp, vp, vp, u64, vp]),
+        "qe_op_verify_tree_work_bytes": (u64, [u64, u64, u64]),
+        "qe_op_verify_tree": (i32, [vp, u64, u64, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp, vp, vp, vp, vp, u64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -713,3 +720,137 @@ def op_verify_drafts(logits, starts, drafts, accept, sample, tokens, count, work
     _check(lib().qe_op_verify_drafts(_ptr(logits), rows, vocab, strides[0], _ptr(starts), n_seqs, _ptr(drafts), opt[0],
                                      strides[1], _ptr(accept), _ptr(sample), opt[1], _ptr(tokens), _ptr(count), opt[2],
                                      _ptr(work), work.nbytes, _on_stream(stream, at)))
+
+
+# ---- trees of drafts, and a cache of bounded size ----
+
+QE_TREE_NODES = 64  # nodes of a tree at most
+
+
+def op_page_tree_attention(pages: Pages, parents, q, out, work, max_new: int = 0, stream=None) -> None:
+    """op_page_attention for trees of drafted tokens (qe_op_page_tree_attention): the new tokens of a
+    sequence are nodes, parents [rows] (int32) names each one's parent among its sequence's rows (an
+    earlier one, else none), and a node attends the positions before them, its ancestors and itself.
+    work: op_page_attention_work_bytes() device bytes; max_new: at most QE_TREE_NODES (0: not known)."""
+    dtype = _row_dtype("q", q)
+    heads = int(q.shape[1]) if q.dim() == 3 else 0
+    if out.dtype != q.dtype or out.shape != q.shape:
+        _refuse("q and out must have the same type and shape")
+    _dense("parents", parents, (_torch().int32,), q.shape[:1])
+    if not work.is_contiguous():
+        _refuse("work must be contiguous")
+    if max_new < 0:
+        _refuse("max_new must not be negative")
+    at = _same_device(q, out, work, pages.k, parents)
+    _check(lib().qe_op_page_tree_attention(pages._ref, _ptr(parents), _ptr(q), _ptr(out), q.shape[0], heads,
+                                           _row_stride("q", q, heads), _row_stride("out", out, heads), max_new, dtype,
+                                           _ptr(work), work.nbytes, _on_stream(stream, at)))
+
+
+def op_verify_tree_work_bytes(n_rows: int, n_seqs: int, vocab: int) -> int:
+    return int(lib().qe_op_verify_tree_work_bytes(n_rows, n_seqs, vocab))
+
+
+def op_verify_tree(logits, starts, parents, nodes, accept, sample, tokens, path, count, work, temperature=None,
+                   logprobs=None, max_depth: int = 0, stream=None) -> None:
+    """Checks a tree of drafts for each sequence against softmax(logits [rows, vocab] / temperature)
+    (qe_op_verify_tree): nodes and parents [rows] are the tree, accept [rows] and sample [n_seqs] random
+    numbers; tokens [rows], path [n_seqs, QE_TREE_NODES], count [n_seqs] and logprobs [rows] are written.
+    max_depth: the most drafts that are accepted (0: no bound). work: op_verify_tree_work_bytes() device
+    bytes."""
+    torch = _torch()
+    f32, whole = (torch.float32,), (torch.int32, torch.uint32)
+    if logits.dim() != 2 or starts.dim() != 1 or starts.shape[0] < 2:
+        _refuse("need logits [rows, vocab] and starts [n_seqs + 1]")
+    (rows, vocab), n_seqs = logits.shape, starts.shape[0] - 1
+    if logits.dtype != torch.float32 or (vocab > 1 and rows and logits.stride(1) != 1):
+        _refuse(f"logits: need float32 [{rows}, {vocab}] with each row's values one after the other")
+    _dense("starts", starts, (torch.int32,), (n_seqs + 1,))
+    _dense("parents", parents, (torch.int32,), (rows,))
+    _dense("nodes", nodes, whole, (rows,))
+    _dense("accept", accept, f32, (rows,))
+    _dense("sample", sample, f32, (n_seqs,))
+    _dense("tokens", tokens, whole, (rows,))
+    _dense("path", path, (torch.int32,), (n_seqs, QE_TREE_NODES))
+    _dense("count", count, whole, (n_seqs,))
+    if temperature is not None:
+        _dense("temperature", temperature, f32, (n_seqs,))
+    if logprobs is not None:
+        _dense("logprobs", logprobs, f32, (rows,))
+    if not work.is_contiguous():
+        _refuse("work must be contiguous")
+    if max_depth < 0:
+        _refuse("max_depth must not be negative")
+    at = _same_device(logits, starts, parents, nodes, accept, sample, tokens, path, count, work, temperature, logprobs)
+    _check(lib().qe_op_verify_tree(_ptr(logits), rows, vocab, int(logits.stride(0)) if rows > 1 else vocab, _ptr(starts),
+                                   n_seqs, _ptr(parents), _ptr(nodes), _ptr(accept), _ptr(sample),
+                                   None if temperature is None else _ptr(temperature), max_depth, _ptr(tokens),
+                                   _ptr(path), _ptr(count), None if logprobs is None else _ptr(logprobs), _ptr(work),
+                                   work.nbytes, _on_stream(stream, at)))
+
+
+def _mass_stride(name: str, t, n_seqs: int, n_kv: int) -> int:
+    """entries of a row of t [n_seqs, n_kv, entries]"""
+    if t.dim() != 3:
+        _refuse(f"{name}: need [{n_seqs}, {n_kv}, positions], got {tuple(t.shape)}")
+    _dense(name, t, (_torch().float32,), (n_seqs, n_kv, t.shape[2]))
+    return int(t.shape[2])
+
+
+def op_page_weigh_work_bytes(n_rows: int, n_heads: int, n_kv_heads: int, n_seqs: int, positions: int,
+                             max_new: int = 0) -> int:
+    """positions: what a row of the plan's table holds (its pages times the page size)"""
+    return int(lib().qe_op_page_weigh_work_bytes(n_rows, n_heads, n_kv_heads, n_seqs, positions, max_new))
+
+
+def op_page_weigh(pages: Pages, q, mass, work, max_new: int = 0, stream=None) -> None:
+    """Adds to mass [n_seqs, n_kv, positions] (float32) the softmax weight that each position gets from the
+    new tokens q [rows, n_heads, 128] (qe_op_page_weigh). work: op_page_weigh_work_bytes() device bytes."""
+    dtype = _row_dtype("q", q)
+    heads = int(q.shape[1]) if q.dim() == 3 else 0
+    stride = _mass_stride("mass", mass, int(pages.lens.shape[0]), pages.n_kv_heads)
+    if not work.is_contiguous():
+        _refuse("work must be contiguous")
+    if max_new < 0:
+        _refuse("max_new must not be negative")
+    at = _same_device(q, mass, work, pages.k)
+    _check(lib().qe_op_page_weigh(pages._ref, _ptr(q), q.shape[0], heads, _row_stride("q", q, heads), max_new, dtype,
+                                  _ptr(mass), stride, _ptr(work), work.nbytes, _on_stream(stream, at)))
+
+
+def op_page_keep(mass, lens, kept, count, keep: int, sinks: int = 0, recent: int = 0, stream=None) -> None:
+    """Picks the positions that each KV head keeps by mass [n_seqs, n_kv, positions] (qe_op_page_keep): kept
+    [n_seqs, n_kv, keep or more] and count [n_seqs] (int32) are written."""
+    torch = _torch()
+    if mass.dim() != 3 or kept.dim() != 3:
+        _refuse("need mass [n_seqs, n_kv, positions] and kept [n_seqs, n_kv, keep or more]")
+    n_seqs, n_kv = (int(n) for n in mass.shape[:2])
+    stride = _mass_stride("mass", mass, n_seqs, n_kv)
+    _dense("lens", lens, (torch.int32,), (n_seqs,))
+    _dense("kept", kept, (torch.int32,), (n_seqs, n_kv, kept.shape[2]))
+    _dense("count", count, (torch.int32,), (n_seqs,))
+    if min(keep, sinks, recent) < 0:
+        _refuse("keep, sinks and recent must not be negative")
+    at = _same_device(mass, lens, kept, count)
+    _check(lib().qe_op_page_keep(_ptr(mass), stride, _ptr(lens), n_seqs, n_kv, keep, sinks, recent, _ptr(kept),
+                                 int(kept.shape[2]), _ptr(count), _on_stream(stream, at)))
+
+
+def op_page_move(pages: Pages, src, count, first=None, mass=None, stream=None) -> None:
+    """Moves rows of the pages (and of mass) to the front, in place (qe_op_page_move): position first[s] + i
+    takes the row at first[s] + src[s, h, i], i < count[s]. src: [n_seqs, n] for all KV heads alike, or
+    [n_seqs, n_kv, n]; first None: 0."""
+    torch = _torch()
+    n_seqs, n_kv = int(pages.lens.shape[0]), pages.n_kv_heads
+    heads = 1 if src.dim() == 2 else n_kv
+    if src.dim() not in (2, 3):
+        _refuse("src must be [n_seqs, rows] or [n_seqs, n_kv, rows]")
+    _dense("src", src, (torch.int32,), (n_seqs, src.shape[1]) if src.dim() == 2 else (n_seqs, n_kv, src.shape[2]))
+    _dense("count", count, (torch.int32, torch.uint32), (n_seqs,))
+    if first is not None:
+        _dense("first", first, (torch.int32,), (n_seqs,))
+    stride = 0 if mass is None else _mass_stride("mass", mass, n_seqs, n_kv)
+    at = _same_device(src, count, first, mass, pages.k)
+    _check(lib().qe_op_page_move(pages._ref, _ptr(src), heads, int(src.shape[-1]), _ptr(count),
+                                 None if first is None else _ptr(first), None if mass is None else _ptr(mass), stride,
+                                 _on_stream(stream, at)))

@@ -26,6 +26,9 @@ pub const QE_KV_F32: c_int = 0;
 pub const QE_KV_BF16: c_int = 1;
 pub const QE_KV_FP8: c_int = 2;
 
+/// Nodes of a tree of drafts at most.
+pub const QE_TREE_NODES: u32 = 64;
+
 /// A draft source's failure return (qe_draft_fn).
 pub const QE_DRAFT_ERROR: u32 = 0xFFFF_FFFF;
 
@@ -182,4 +185,27 @@ extern "C" {
                                accept: *const f32, sample: *const f32, temperature: *const f32,
                                tokens_out: *mut u32, count_out: *mut u32, logprobs_out: *mut f32,
                                work: *mut c_void, work_bytes: u64, stream: *mut c_void) -> c_int;
+
+    // trees of drafts, and a cache of bounded size (no reference counterpart)
+    pub fn qe_op_page_tree_attention(pages: *const qe_pages, parents: *const i32, q: *const c_void,
+                                     out: *mut c_void, n_rows: u64, n_heads: u64, q_stride: u64, out_stride: u64,
+                                     max_new: u64, dtype: c_int, work: *mut c_void, work_bytes: u64,
+                                     stream: *mut c_void) -> c_int;
+    pub fn qe_op_page_weigh_work_bytes(n_rows: u64, n_heads: u64, n_kv_heads: u64, n_seqs: u64, positions: u64,
+                                       max_new: u64) -> u64;
+    pub fn qe_op_page_weigh(pages: *const qe_pages, q: *const c_void, n_rows: u64, n_heads: u64, q_stride: u64,
+                            max_new: u64, dtype: c_int, mass: *mut f32, mass_stride: u64, work: *mut c_void,
+                            work_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn qe_op_page_keep(mass: *const f32, mass_stride: u64, lens: *const i32, n_seqs: u64, n_kv_heads: u64,
+                           keep: u64, sinks: u64, recent: u64, kept: *mut i32, kept_stride: u64, count: *mut i32,
+                           stream: *mut c_void) -> c_int;
+    pub fn qe_op_page_move(pages: *const qe_pages, src: *const i32, src_heads: u64, src_stride: u64,
+                           count: *const i32, first: *const i32, mass: *mut f32, mass_stride: u64,
+                           stream: *mut c_void) -> c_int;
+    pub fn qe_op_verify_tree_work_bytes(n_rows: u64, n_seqs: u64, vocab: u64) -> u64;
+    pub fn qe_op_verify_tree(logits: *const f32, n_rows: u64, vocab: u64, row_stride: u64, starts: *const i32,
+                             n_seqs: u64, parents: *const i32, nodes: *const u32, accept: *const f32,
+                             sample: *const f32, temperature: *const f32, max_depth: u64, tokens_out: *mut u32,
+                             path_out: *mut i32, count_out: *mut u32, logprobs_out: *mut f32, work: *mut c_void,
+                             work_bytes: u64, stream: *mut c_void) -> c_int;
 }

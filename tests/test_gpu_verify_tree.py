@@ -1,0 +1,216 @@
+"""qe_op_verify_tree against the rule in numpy's 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import qe
+from test_gpu_verify_drafts import NONE, settle, target
+from tree_cases import random_tree
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(logits, starts, parents, nodes, accept, sample, temps, max_depth=0):
+    rows, vocab = logits.shape
+    n = len(starts) - 1
+    tokens, lps = np.full(rows, 77, np.int64), np.full(rows, 5.0)
+    path, count, drawn = np.full((n, 64), -1, np.int64), np.zeros(n, np.int64), {}
+    for s in range(n):
+        a, b = starts[s], starts[s + 1]
+        if b <= a:
+            continue
+        tokens[a:b], lps[a:b] = NONE, 0.0
+        at, way = a, [0]
+        while True:
+            lp = target(logits[a + way[-1]], temps[s])
+            p = np.exp(lp)
+            q, left, taken = p.copy(), 1.0, None
+            for c in range(way[-1] + 1, min(b - a, 64)):
+                if parents[a + c] != way[-1] or (max_depth and len(way) > max_depth):
+                    continue
+                d = int(nodes[a + c])
+                mine = q[d] if d < vocab else 0.0
+                if np.float64(accept[a + c]) * left < mine:
+                    taken = c
+                    break
+                left -= mine
+                if d < vocab:
+                    q[d] = 0.0
+            if taken is None:
+                break
+            tokens[at], lps[at] = nodes[a + taken], lp[nodes[a + taken]]
+            way.append(taken)
+            at += 1
+        if not q.sum() > 0:
+            q = p
+        c = np.cumsum(q)
+        hit = np.nonzero((c > np.float64(sample[s]) * c[-1]) & (q > 0))[0]
+        tok = int(hit[0]) if len(hit) else int(np.nonzero(q > 0)[0][-1])
+        tokens[at], lps[at], count[s] = tok, lp[tok], len(way)
+        path[s, :len(way)] = way
+        drawn[at] = q, np.float64(sample[s]) * c[-1], lp
+    return tokens, path, count, lps, drawn
+
+
+def call(logits, starts, parents, nodes, accept, sample, temps, max_depth=0, gap=0):
+    rows, vocab = logits.shape
+    n = len(starts) - 1
+    base = torch.full((rows, vocab + gap), math.inf, device="cuda")
+    base[:, :vocab] = torch.from_numpy(logits)
+    dev = lambda x, t: torch.from_numpy(np.ascontiguousarray(x).astype(t)).cuda()  # noqa: E731
+    tokens, count = (torch.full((m,), 77, dtype=torch.int32, device="cuda") for m in (rows, n))
+    path, lps = torch.full((n, 64), 77, dtype=torch.int32, device="cuda"), torch.full((rows,), 5.0, device="cuda")
+    work = torch.empty(qe.op_verify_tree_work_bytes(rows, n, vocab), dtype=torch.uint8, device="cuda")
+    work.fill_(0xFF)
+    qe.op_verify_tree(base[:, :vocab], dev(starts, np.int32), dev(parents, np.int32),
+                      dev(np.asarray(nodes, np.uint32).view(np.int32), np.int32), dev(accept, np.float32),
+                      dev(sample, np.float32), tokens, path, count, work,
+                      temperature=None if temps is None else dev(temps, np.float32), logprobs=lps, max_depth=max_depth)
+    return (tokens.cpu().numpy().view(np.uint32).astype(np.int64), path.cpu().numpy(), count.cpu().numpy(),
+            lps.cpu().numpy().astype(np.float64))
+
+
+def check(logits, starts, parents, nodes, accept, sample, temps=None, max_depth=0, gap=0):
+    n = len(starts) - 1
+    tokens, path, count, lps, drawn = reference(logits, starts, parents, nodes, accept, sample,
+                                                np.ones(n) if temps is None else temps, max_depth)
+    got = call(logits, starts, parents, nodes, accept, sample, temps, max_depth, gap)
+    np.testing.assert_array_equal(got[1], path)
+    np.testing.assert_array_equal(got[2], count)
+    settle(got[0], tokens, lps, drawn)
+    np.testing.assert_array_equal(got[0], tokens)
+    # log p in 64 bits, rounded once to f32: half a step, plus 64-bit noise
+    np.testing.assert_allclose(got[3], lps, rtol=2.0 ** -23, atol=1e-12)
+    return count
+
+
+def likely(rng, logits, starts, parents, share=0.85):
+    """nodes' tokens: a parent's likeliest in the order of its children, some at random"""
+    rows, vocab = logits.shape
+    nodes = rng.integers(0, vocab, rows).astype(np.uint32)
+    for a, b in zip(starts[:-1], starts[1:]):
+        seen = {}
+        for i in range(a, b):
+            p = parents[i]
+            if 0 <= p < i - a:
+                rank = seen[p] = seen.get(p, -1) + 1
+                if rng.random() < share:
+                    nodes[i] = np.argsort(-logits[a + p])[min(rank, vocab - 1)]
+    return nodes
+
+
+@pytest.mark.parametrize("max_depth", [0, 2, 63])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 4097, 33001, 151936])
+def test_against_the_rule(gpu, vocab, max_depth):
+    rng = np.random.default_rng([vocab, 3])
+    sizes = [1, 13, 0, 2, 64, 1, 3, 30, 5]
+    starts = np.concatenate([[2], 2 + np.cumsum(sizes)])
+    rows = starts[-1] + 1
+    parents = np.full(rows, -1)
+    for s, m in enumerate(sizes):
+        parents[starts[s]:starts[s] + m] = random_tree(m, s)
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    temps = np.array([1.0, 0.7, 1.0, 0.0, 1.5, 0.3, 1.0, 0.9, 1.0], np.float32)
+    check(x, starts, parents, likely(rng, x, starts, parents), rng.random(rows, np.float32), rng.random(len(sizes), np.float32),
+          temps, max_depth, gap=5)
+
+
+def test_rows_at_the_edges(gpu):
+    """NaN, infinities, nothing above -inf, ties, tokens out of range or impossible, the same token twice,
+    numbers 0 and just below 1, temperatures that are not above 0, tiny and infinite"""
+    vocab = 3001
+    rng = np.random.default_rng(8)
+    base = rng.standard_normal(vocab).astype(np.float32)
+    kinds = []
+    r = base.copy(); r[::3] = np.nan; kinds.append(r)
+    kinds.append(np.full(vocab, -np.inf, np.float32))
+    kinds.append(np.full(vocab, np.nan, np.float32))
+    r = base.copy(); r[[7, 2900]] = np.inf; kinds.append(r)
+    r = np.full(vocab, -np.inf, np.float32); r[2999] = -3.0; kinds.append(r)
+    kinds.append(np.zeros(vocab, np.float32))
+    r = base.copy(); r[[5, 1800]] = 40.0; kinds.append(r)
+    r = base.copy(); r[11] = 200.0; kinds.append(r)  # p is 1 there and nothing elsewhere
+    kinds.append((base * 1e30).astype(np.float32))
+    u_last = np.nextafter(np.float32(1), np.float32(0))
+    logits, starts, parents, nodes, accept, sample, temps = [], [0], [], [], [], [], []
+    for k in kinds:
+        for family in ((0, 5, 11), (11, 11, 2999), (2999, vocab, NONE), (7, 2900, 7), (5, 1800, 0)):
+            for u, v in ((0.0, 0.0), (0.5, u_last), (u_last, 0.5)):
+                for t in (1.0, 0.0, -1.0, np.nan, np.inf, 1e-38):
+                    logits += [k, base, k, base]
+                    parents += [-1, 0, 0, 0]
+                    nodes += [0, *family]
+                    accept += [u] * 4
+                    sample.append(v)
+                    temps.append(t)
+                    starts.append(len(logits))
+    check(np.stack(logits), np.array(starts), np.array(parents), np.array(nodes, np.uint32), np.array(accept, np.float32),
+          np.array(sample, np.float32), np.array(temps, np.float32))
+
+
+def test_what_is_emitted_follows_the_target(gpu):
+    """the first token of 60,000 trees has the target's distribution, whatever the children, and the second
+    that of the row it follows"""
+    n, vocab = 60000, 11
+    rng = np.random.default_rng(12)
+    x = (rng.standard_normal((4, vocab)) * 1.2).astype(np.float32)
+    # root, three children (tokens 4, 9, 4 again), the last two rows below the first child
+    parents, nodes = [-1, 0, 0, 0, 1, 1], [0, 4, 9, 4, 2, 7]
+    rows = np.stack([x[0], x[1], x[2], x[2], x[3], x[3]])
+    got = call(np.tile(rows, (n, 1)), np.arange(n + 1) * 6, np.tile(parents, n), np.tile(nodes, n),
+               rng.random(6 * n, np.float32), rng.random(n, np.float32), None)
+    tokens = got[0].reshape(n, 6)
+    for seen, row in ((tokens[:, 0], x[0]), (tokens[got[1][:, 1] == 1, 1], x[1])):
+        p = np.exp(target(row, 1.0))
+        share = np.bincount(seen, minlength=vocab) / len(seen)
+        # 5 standard deviations of a share of that many draws
+        assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / len(seen)) + 1e-9).all(), (share, p)
+
+
+@pytest.mark.parametrize("depth", [0, 1, 40, 63])
+def test_long_paths(gpu, depth):
+    """greedy chains and combs of 64 nodes that are accepted to the end, or to max_depth; rows behind the
+    first 64 are never reached"""
+    rng = np.random.default_rng(5)
+    sizes = [64, 64, 80, 63]
+    starts = np.concatenate([[0], np.cumsum(sizes)])
+    parents = np.concatenate([np.arange(-1, 63), [i - 2 if i > 1 else i - 1 for i in range(64)], np.arange(-1, 79),
+                              np.arange(-1, 62)])
+    x = (rng.standard_normal((starts[-1], 40)) * 4).astype(np.float32)
+    nodes = np.zeros(starts[-1], np.uint32)
+    for s in range(4):
+        for i in range(1, sizes[s]):
+            nodes[starts[s] + i] = x[starts[s] + parents[starts[s] + i]].argmax()
+    count = check(x, starts, parents, nodes, np.full(len(x), 0.5, np.float32), rng.random(4, np.float32),
+                  np.zeros(4, np.float32), depth)
+    np.testing.assert_array_equal(count, np.minimum([64, 33, 64, 63], depth + 1 if depth else 99))
+
+
+def test_trees_that_are_not(gpu):
+    """parents that are no earlier node: such nodes are never reached; a second root is not either"""
+    rng = np.random.default_rng(6)
+    parents = np.array([5, 0, 2, 3, 4, 99, -1, 6, 1, 1 << 30, 0, 0])
+    x = (rng.standard_normal((24, 50)) * 2).astype(np.float32)
+    starts = np.array([0, 12, 24])
+    both = np.concatenate([parents, parents])
+    for u in (0.0, 0.3, 0.9):
+        nodes = np.array([x[max(0, min(int(p), 11)) + 12 * (i // 12)].argmax() for i, p in enumerate(both)], np.uint32)
+        check(x, starts, both, nodes, np.full(24, u, np.float32), np.array([0.2, 0.8], np.float32))
+
+
+def test_many_trees(gpu):
+    """more rows than a grid is wide, and more sequences than there are CUs"""
+    rng = np.random.default_rng(7)
+    n, vocab = 22000, 7
+    x = rng.standard_normal((3 * n, vocab)).astype(np.float32)
+    parents = np.tile([-1, 0, 0], n)
+    nodes = rng.integers(0, vocab, 3 * n).astype(np.uint32)
+    got = call(x, np.arange(n + 1) * 3, parents, nodes, np.full(3 * n, 0.5), np.full(n, 0.5), np.zeros(n))
+    best = x.argmax(-1)
+    one, two = nodes[1::3] == best[::3], nodes[2::3] == best[::3]
+    np.testing.assert_array_equal(got[2], 1 + (one | two))
+    np.testing.assert_array_equal(got[1][:, 1], np.where(one, 1, np.where(two, 2, -1)))
+    np.testing.assert_array_equal(got[0][::3], best[::3])
+    np.testing.assert_array_equal(got[0][1::3], np.where(one, best[1::3], np.where(two, best[2::3], NONE)))
