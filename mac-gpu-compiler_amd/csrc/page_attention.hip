@@ -43,6 +43,7 @@ constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 constexpr uint32_t kPartRow = 130; // floats of a part's row: 128 sums, then (apart) the maximum and the weight sum
 
 struct AttnArgs {
+  static constexpr bool kTree = false;
   PagePlan p;
   PageStore st;
   const uint8_t* q;
@@ -58,6 +59,15 @@ struct AttnArgs {
   float c;                        // log2(e) / sqrt(128)
 };
 
+// Trees: row t of a sequence's new tokens is a node, stored at position first + t as ever. It attends the positions
+// before `first`, its ancestors and itself, all of them positions that it attends as a causal row too: blocks
+// that begin behind `first` are masked by `family`, all else is as for causal rows. Rows from kNodes on attend nothing.
+struct TreeAttnArgs : AttnArgs {
+  static constexpr bool kTree = true;
+  const int32_t* parents;  // [n_rows]
+};
+constexpr uint32_t kNodes = QE_TREE_NODES;
+
 // An item whose first part is the last one of a workgroup: parts of `n` workgroups from there (0: none). And the
 // workgroup of the first part of the item that this one's first part goes on with, where it helps to join it
 // (else kNowhere).
@@ -67,7 +77,8 @@ struct Joint {
   uint32_t from;
 };
 
-__device__ __forceinline__ uint32_t token_of(const AttnArgs& a, uint32_t r) {  // r / group
+template <class A>
+__device__ __forceinline__ uint32_t token_of(const A& a, uint32_t r) {  // r / group
   return __umulhi(2 * r, a.group_magic) >> a.group_shift;
 }
 
@@ -79,7 +90,8 @@ struct Seq {
   __device__ uint32_t tiles(uint32_t R) const { return (rows + R - 1) / R; }
 };
 
-__device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
+template <class A>
+__device__ __forceinline__ Seq read_seq(const A& a, uint32_t s) {
   const int64_t b = a.p.starts[s], e = a.p.starts[s + 1];
   const int64_t lo = b < 0 ? 0 : b, hi = e < int64_t(a.n_rows) ? e : int64_t(a.n_rows);
   Seq q;
@@ -93,22 +105,77 @@ __device__ __forceinline__ Seq read_seq(const AttnArgs& a, uint32_t s) {
 
 // The last position that row r of a sequence's rows attends: its own, or the table's last where it lies behind
 // that (what a step or block holds past the table is masked by it, like any later position); negative: none.
-__device__ __forceinline__ int32_t row_position(const AttnArgs& a, const Seq& q, uint32_t r) {
+template <class A>
+__device__ __forceinline__ int32_t row_position(const A& a, const Seq& q, uint32_t r) {
   return min(q.first + int32_t(token_of(a, r)), int32_t((a.p.table_stride << a.p.page_shift) - 1));
 }
 // Positions that rows up to r attend: 0 .. limit - 1.
-__device__ __forceinline__ uint32_t row_limit(const AttnArgs& a, const Seq& q, uint32_t r) {
+template <class A>
+__device__ __forceinline__ uint32_t row_limit(const A& a, const Seq& q, uint32_t r) {
   const int32_t pos = row_position(a, q, r);
   return pos < 0 ? 0 : uint32_t(pos) + 1;
 }
-__device__ __forceinline__ uint32_t tile_limit(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
-  return row_limit(a, q, min((tile + 1) * R, q.rows) - 1);
+template <class A>
+__device__ __forceinline__ uint32_t rows_limit(const A& a, const Seq& q, uint32_t r0, uint32_t r1) {  // of rows r0 .. r1 - 1
+  if constexpr (A::kTree) {
+    if (r0 >= kNodes * a.group) return 0;
+    r1 = min(r1, kNodes * a.group);
+  }
+  return row_limit(a, q, r1 - 1);
+}
+template <class A>
+__device__ __forceinline__ uint32_t tile_limit(const A& a, const Seq& q, uint32_t tile, uint32_t R) {
+  return rows_limit(a, q, tile * R, min((tile + 1) * R, q.rows));
+}
+// The last position up to which all of rows r0 .. r1 - 1 attend everything (negative: none).
+template <class A>
+__device__ __forceinline__ int32_t free_position(const A& a, const Seq& q, uint32_t r0, uint32_t r1) {
+  if constexpr (A::kTree) {
+    const int32_t before = min(max(q.first, 0) - 1, int32_t((a.p.table_stride << a.p.page_shift) - 1));
+    return r1 > kNodes * a.group ? -1 : before;
+  }
+  return row_position(a, q, r0);
+}
+// row_position of a row of a tile (a tree's rows behind its last node: none)
+template <class A>
+__device__ __forceinline__ int32_t tile_row_position(const A& a, const Seq& q, uint32_t r) {
+  if constexpr (A::kTree)
+    if (r >= kNodes * a.group) return -1;
+  return row_position(a, q, r);
+}
+
+// ---- trees ----
+// Of each node of sequence q, bit i: node i is the node itself or one of its ancestors; into kin[kNodes] of the calling
+// wave. Lane i has node i: after n rounds its word holds its 2^n nearest, and `at` is the next one above.
+__device__ __forceinline__ void find_families(const TreeAttnArgs& a, const Seq& q, uint64_t* kin) {
+  const uint32_t lane = threadIdx.x & 63, n = token_of(a, q.rows);
+  uint32_t at = lane;
+  if (lane < n) {
+    const int32_t parent = a.parents[uint32_t(q.row0) + lane];
+    if (uint32_t(parent) < lane) at = uint32_t(parent);
+  }
+  uint32_t lo = lane < 32 ? 1u << lane : 0, hi = lane < 32 ? 0 : 1u << (lane - 32);
+#pragma unroll
+  for (int i = 0; i < 6; i++) {
+    lo |= uint32_t(__shfl(int(lo), int(at)));
+    hi |= uint32_t(__shfl(int(hi), int(at)));
+    at = uint32_t(__shfl(int(at), int(at)));
+  }
+  kin[lane] = uint64_t(hi) << 32 | lo;
+}
+// Bit i: whether a node with this family attends position x + i (as far as the tree says).
+__device__ __forceinline__ uint64_t attended(uint64_t family, const Seq& q, uint32_t x) {
+  const int64_t d = int64_t(x) - q.first;
+  if (d >= 0) return d < 64 ? family >> d : 0;
+  return d > -64 ? family << -d | ((1ull << -d) - 1) : ~0ull;
 }
 // A tile that attends nothing still counts one block: its rows are zeros that someone writes.
-__device__ __forceinline__ uint32_t tile_blocks(const AttnArgs& a, const Seq& q, uint32_t tile, uint32_t R) {
+template <class A>
+__device__ __forceinline__ uint32_t tile_blocks(const A& a, const Seq& q, uint32_t tile, uint32_t R) {
   return a.whole_items ? 1 : max((tile_limit(a, q, tile, R) + kBlock - 1) / kBlock, 1u);
 }
-__device__ uint64_t seq_blocks(const AttnArgs& a, const Seq& q, uint32_t R) {
+template <class A>
+__device__ uint64_t seq_blocks(const A& a, const Seq& q, uint32_t R) {
   uint64_t n = 0;
   const uint32_t t = q.tiles(R);
   if (a.whole_items) return t;
@@ -128,7 +195,8 @@ struct PlanShared {
 };
 
 // The next tile with rows after `cu`'s (false: there is none).
-__device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_t R) {
+template <class A>
+__device__ __forceinline__ bool next_tile(const A& a, Cursor& cu, uint32_t R) {
   cu.block = 0;
   if (++cu.tile >= cu.q.tiles(R)) {
     cu.tile = 0;
@@ -145,7 +213,8 @@ __device__ __forceinline__ bool next_tile(const AttnArgs& a, Cursor& cu, uint32_
 }
 
 // The block `at` blocks into the list of sequence s's.
-__device__ __forceinline__ Cursor cursor_in(const AttnArgs& a, uint32_t s, const Seq& q, uint64_t one, uint64_t at, uint32_t R) {
+template <class A>
+__device__ __forceinline__ Cursor cursor_in(const A& a, uint32_t s, const Seq& q, uint64_t one, uint64_t at, uint32_t R) {
   Cursor cu;
   cu.q = q;
   cu.seq = s;
@@ -215,7 +284,8 @@ __device__ __forceinline__ uint32_t parts_of(uint32_t b, uint32_t q) {
 //   with the last of an item shorter, where up to 3 blocks over the even share give no more parts than
 //   workgroups: 16 x 8 of up to 2048 positions, 5 rows each, e4m3 21.9 us dealt evenly, so 18.9 (12 rows 33.7 and
 //   30.0; bf16 pages 26.6 and 26.4); 10 x 8 of up to 3000, one row 23.2 and 21.7.
-__device__ __forceinline__ uint32_t find_part(AttnArgs& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
+template <class A>
+__device__ __forceinline__ uint32_t find_part(A& a, uint32_t w, uint32_t W, uint32_t R, PlanShared& sh,
                                               uint32_t& per_out, Cursor& cu) {
   const uint32_t tid = threadIdx.x, log_w = 31 - __builtin_clz(W);
   auto split = [&](uint64_t total) { return (total + W - 1) >> log_w; };
@@ -532,7 +602,8 @@ __device__ __forceinline__ void store_out8(uint8_t* out, uint64_t element, const
   }
 }
 // element of row r of a tile's item in rows of `stride` elements
-__device__ __forceinline__ uint64_t row_element(const AttnArgs& a, const Seq& q, uint32_t head, uint32_t r,
+template <class A>
+__device__ __forceinline__ uint64_t row_element(const A& a, const Seq& q, uint32_t head, uint32_t r,
                                                 uint64_t stride) {
   const uint32_t t = token_of(a, r);
   return (uint64_t(q.row0) + t) * stride + (head * a.group + (r - t * a.group)) * kPageDim;
@@ -563,13 +634,15 @@ struct StepData {
   bool there;       // the page of the lane's V (and scores) is
 };
 
-template <bool FP8, bool BF16_ROWS, int NQ>
-__global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn_rows(AttnArgs a) {
+template <bool FP8, bool BF16_ROWS, int NQ, class A>
+__global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn_rows(A a) {
+  constexpr bool TREE = A::kTree;
   constexpr int NS = BF16_ROWS ? 1 : 3, R = 16 * NQ, KEYS = FP8 ? 64 : 32, NT = KEYS / 16, EL = FP8 ? 1 : 2;
   constexpr int LDO = 132;  // floats of a row's sums in LDS
   __shared__ PlanShared sh;
   __shared__ __align__(16) float sums[4][R][LDO];
   __shared__ float top[4][R], mass[4][R];
+  __shared__ uint64_t kin[TREE ? 4 : 1][TREE ? kNodes : 1];  // each wave's own
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t w = part_index();
@@ -593,8 +666,12 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     const uint32_t first = cu.block * kBlock, last = a.whole_items ? limit : min((cu.block + take) * kBlock, limit);
     const uint32_t head = cu.head;
     // the least position any row attends up to: below it no score is masked
-    const int32_t free_to = row_position(a, cu.q, cu.tile * R);
+    const int32_t free_to = free_position(a, cu.q, cu.tile * R, cu.tile * R + rows);
     const bool one_token = token_of(a, cu.tile * R) == token_of(a, cu.tile * R + rows - 1);
+    if constexpr (TREE) find_families(a, cu.q, kin[wave]);
+    auto family_of = [&](int n) __attribute__((always_inline)) {  // of the lane's row of group n (those that attend nothing: any)
+      return kin[TREE ? wave : 0][TREE ? min(token_of(a, cu.tile * R + 16 * n + col), kNodes - 1) : 0];
+    };
     int32_t row_pos[NQ];
     bf16x8 qf[NQ][4][NS];
 #pragma unroll
@@ -602,7 +679,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
       const uint32_t lane = afresh(tid & 63), col = lane & 15, g = lane >> 4;
       const uint32_t r = cu.tile * R + 16 * n + col;
       const bool real = r < cu.q.rows;
-      row_pos[n] = real ? row_position(a, cu.q, r) : -1;
+      row_pos[n] = real ? tile_row_position(a, cu.q, r) : -1;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const uint32_t d = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
@@ -679,12 +756,15 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
       uint32_t foul = 0;  // V is not finite at a position that only some rows of the tile attend
       if (masked) {
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
+        for (int n = 0; n < NQ; n++) {
+          uint32_t sees = ~0u;
+          if constexpr (TREE) sees = uint32_t(attended(family_of(n), cu.q, base));
 #pragma unroll
           for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-              if (int32_t(base + 4 * t + i) > row_pos[n] || !d.there) s[n][t][i] = -INFINITY;
+              if (int32_t(base + 4 * t + i) > row_pos[n] || !d.there || (TREE && !(sees >> (4 * t + i) & 1))) s[n][t][i] = -INFINITY;
+        }
         // V at positions no row attends may hold anything: 0 x NaN is NaN
         const uint32_t ok = d.there && limit > base ? min(limit - base, uint32_t(KEYS / 4)) : 0;
 #pragma unroll
@@ -696,7 +776,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
           for (int t = 0; t < 8; t++) d.v[t][i] &= bits;
           if constexpr (FP8) d.ve[i] &= bits;
         }
-        if (!one_token) {
+        if (TREE || !one_token) {
 #pragma unroll
           for (int t = 0; t < 8; t++)
 #pragma unroll
@@ -789,7 +869,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
             if (!(fabsf(v) < INFINITY))
 #pragma unroll
               for (int n = 0; n < NQ; n++)
-                if (int32_t(j) <= row_pos[n]) acc[n][t][i] += v;
+                if (int32_t(j) <= row_pos[n] && (!TREE || (attended(family_of(n), cu.q, j) & 1))) acc[n][t][i] += v;
           }
       }
     }
@@ -871,8 +951,9 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 // loaded straight into it; e4m3 pages go through registers and are widened once for all rows (K with its
 // scale, V's scale is put on the weights). A wave loads positions of one run of 16, which lie in one page.
 // ---------------------------------------------------------------------------------------------
-template <bool FP8, bool BF16_ROWS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
+template <bool FP8, bool BF16_ROWS, int WAVES, class A>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(A a) {
+  constexpr bool TREE = A::kTree;
   static_assert(BF16_ROWS || WAVES == 8, "f32 rows: 8 waves of 16");
   constexpr int NS = BF16_ROWS ? 1 : 3, WR = BF16_ROWS ? 32 : 16, R = WR * WAVES;
   constexpr int NJ = BF16_ROWS ? 8 : 4, NSUM = BF16_ROWS ? 16 : 8;  // fragments of a row of q; 4 dims of the sums each
@@ -883,6 +964,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
   __shared__ __align__(16) uint8_t buf[STAGES][2 * TILE];
   __shared__ __align__(16) float vscale[2][FP8 ? kBlock : 4];
   __shared__ uint32_t foul[STAGES];
+  __shared__ uint64_t kin[TREE ? WAVES : 1][TREE ? kNodes : 1];  // each wave's own
   __shared__ PlanShared sh;
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & (WR - 1), grp = lane / WR;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -907,12 +989,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
     // this wave's rows, and the positions that all of them (free_to) and some of them (end) attend
     const uint32_t wr0 = cu.tile * R + WR * wave;
     const uint32_t wrows = cu.q.rows > wr0 ? min(cu.q.rows - wr0, uint32_t(WR)) : 0;
-    const int32_t free_to = row_position(a, cu.q, wr0);
-    const uint32_t end = wrows ? row_limit(a, cu.q, wr0 + wrows - 1) : 0;
-    const int32_t tile_free = row_position(a, cu.q, cu.tile * R);  // all rows of the tile attend up to it
+    const int32_t free_to = free_position(a, cu.q, wr0, wr0 + wrows);
+    const uint32_t end = wrows ? rows_limit(a, cu.q, wr0, wr0 + wrows) : 0;
+    // all rows of the tile attend up to it
+    const int32_t tile_free = free_position(a, cu.q, cu.tile * R, min((cu.tile + 1) * R, cu.q.rows));
     const uint32_t fresh = afresh(tid & 63), r = wr0 + (fresh & (WR - 1));
     const bool real = (fresh & (WR - 1)) < wrows;
-    const int32_t row_pos = real ? row_position(a, cu.q, r) : -1;
+    const int32_t row_pos = real ? tile_row_position(a, cu.q, r) : -1;
+    if constexpr (TREE) find_families(a, cu.q, kin[wave]);
+    auto family = [&] __attribute__((always_inline)) {  // of the lane's row (one that attends nothing: any)
+      return kin[TREE ? wave : 0][TREE ? min(token_of(a, wr0 + (afresh(tid) & (WR - 1))), kNodes - 1) : 0];
+    };
     bf16x8 qf[NJ][NS];
     // sums of 4 dims each: n-th of them, and the first of its dims (of lane group g)
     constexpr int NACC = BF16_ROWS ? 4 : 8, PER = NSUM / NACC;
@@ -1016,6 +1103,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
       if constexpr (FP8)
         if (part_of == 0 && lane < 16 && !(page && x + 16 * run + lane < limit)) vscale[b][16 * run + lane] = 0.f;
     };
+    auto pages_bits = [&](uint32_t there) __attribute__((always_inline)) {  // 16 for each of four
+      return uint64_t((there & 1 ? 0xFFFFu : 0) | (there & 2 ? 0xFFFF0000u : 0)) |
+             uint64_t((there & 4 ? 0xFFFFu : 0) | (there & 8 ? 0xFFFF0000u : 0)) << 32;
+    };
     uint32_t foul_from = kNowhere;  // the first block that `clear` cleared something of
     // this wave's rows against the block at x in buffer b; there: which of its four pages are; cleared: by `clear`
     auto multiply = [&](uint32_t x, uint32_t b, uint32_t there, bool cleared) __attribute__((always_inline)) {
@@ -1069,13 +1160,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
       };
       const bool masked = int32_t(x + kBlock - 1) > free_to || there != 15;
       if (masked) {
+        if constexpr (TREE) {
+          // what the lane's row sees of the block, of which the lane has the positions 8 grp .. behind each 16
+          const int32_t ok = row_pos - int32_t(x) + 1;
+          uint64_t sees = attended(family(), cu.q, x) & pages_bits(there);
+          sees = (ok <= 0 ? 0 : ok < 64 ? sees & ((1ull << ok) - 1) : sees) >> (8 * grp);
+          const uint32_t half[2] = {uint32_t(sees), uint32_t(sees >> 32)};
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+          for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int i = 0; i < PERS; i++) {
-            const uint32_t in = position(t, i);
-            if (int32_t(x + in) > row_pos || !(there >> (in / 16) & 1)) s[t][i] = -INFINITY;
-          }
+            for (int i = 0; i < PERS; i++)
+              if (!(half[BF16_ROWS ? t : t / 2] >> (BF16_ROWS ? 16 * (i >> 3) + (i & 7) : 4 * (t & 1) + i) & 1)) s[t][i] = -INFINITY;
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < PERS; i++) {
+              const uint32_t in = position(t, i);
+              if (int32_t(x + in) > row_pos || !(there >> (in / 16) & 1)) s[t][i] = -INFINITY;
+            }
+        }
       }
       float mx = s[0][0];
 #pragma unroll
@@ -1215,7 +1319,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float v = v_value<FP8>(a.st.v, e + 16 * (dim_of(n, grp) + i));
-          if (!(fabsf(v) < INFINITY) && int32_t(j) <= row_pos) acc[n / PER][4 * (n % PER) + i] += v;
+          if (!(fabsf(v) < INFINITY) && int32_t(j) <= row_pos && (!TREE || (attended(family(), cu.q, j) & 1))) acc[n / PER][4 * (n % PER) + i] += v;
         }
     }
     l = BF16_ROWS ? add_halves(l) : add_groups(l);
@@ -1387,76 +1491,6 @@ __global__ __launch_bounds__(256) void k_page_join(AttnArgs a, uint32_t R) {
   if (j.from != kNowhere) join_item<BF16_ROWS, TILES>(a, R, a.joints[j.from], j.from, x - j.from);
 }
 
-// ---------------------------------------------------------------------------------------------
-// Trees: row t of a sequence's rows is a node, whose K and V lie at position first + t; it attends the
-// positions before `first`, its ancestors and itself. A wave for each row and q head: a lane a position's
-// score, then each lane 2 dims of the sum.
-// ---------------------------------------------------------------------------------------------
-template <bool FP8, bool BF16_ROWS>
-__global__ __launch_bounds__(64) void k_page_tree(AttnArgs a, const int32_t* parents) {
-  constexpr int EL = FP8 ? 1 : 2;
-  __shared__ float qs[kPageDim], weight[kBlock];
-  const uint32_t heads = a.group * a.p.n_kv, t = blockIdx.x / heads, h = blockIdx.x - t * heads, lane = threadIdx.x, kv = h / a.group;
-  uint32_t lo = 0, hi = a.p.n_seqs;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.p.starts[mid] <= int32_t(t)) lo = mid;
-    else hi = mid;
-  }
-  if (a.p.starts[lo] > int32_t(t) || int32_t(t) >= a.p.starts[lo + 1]) return;
-  const Seq q = read_seq(a, lo);
-  const uint32_t node = t - uint32_t(q.row0);
-  uint64_t family = 0;
-  if (node < 64) {
-    family = 1ull << node;
-    for (int32_t at = int32_t(node), p; (p = parents[q.row0 + at]) >= 0 && p < at; at = p) family |= 1ull << p;
-  }
-  for (int i = 0; i < 2; i++) {
-    const uint64_t e = uint64_t(t) * a.q_stride + h * kPageDim + 2 * lane + i;
-    qs[2 * lane + i] = BF16_ROWS ? bf16f(reinterpret_cast<const uint16_t*>(a.q)[e]) : reinterpret_cast<const float*>(a.q)[e];
-  }
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[2] = {};
-  const int64_t capacity = capacity_of(a.p), end = min(int64_t(q.first) + int64_t(node) + 1, capacity);
-  for (int64_t x = 0; x < end && node < 64; x += kBlock) {
-    const int64_t j = x + lane, in = j - q.first;
-    const int32_t page = j < capacity ? page_of(a.p, lo, j) : -1;
-    const uint32_t off = uint32_t(j) & ((1u << a.p.page_shift) - 1);
-    float s = -INFINITY;
-    if (page >= 0 && (in < 0 || (in < 64 && (family >> in & 1)))) {
-      const size_t row = page_row(a.p, page, kv, off);
-      s = 0.f;
-      for (uint32_t d = 0; d < kPageDim; d++) s = fmaf(qs[d], v_value<FP8>(a.st.k, row * kPageDim + d), s);
-      if (FP8) s *= exp_scale(a.st.k_exp[row]);
-      s *= a.c;
-    }
-    const float top = fmaxf(m, wave_max(s));
-    const float w = s == -INFINITY ? 0.f : exp2f(s - top);
-    const float f = m == top ? 1.f : exp2f(m - top);
-    m = top;
-    l = l * f + wave_sum(w);
-    o[0] *= f;
-    o[1] *= f;
-    weight[lane] = w;
-    __syncthreads();
-    for (uint32_t i = 0; i < kBlock; i++) {
-      if (weight[i] == 0.f) continue;
-      const int32_t at = page_of(a.p, lo, x + i);
-      const uint32_t off = uint32_t(x + i) & ((1u << a.p.page_shift) - 1);
-      const float scale = FP8 ? exp_scale(a.st.v_exp[page_row(a.p, at, kv, off)]) : 1.f;
-      const size_t e = v_element(a.p, at, kv, off);
-      for (int d = 0; d < 2; d++) o[d] = fmaf(weight[i] * scale, v_value<FP8>(a.st.v, e + 16 * (2 * lane + d)), o[d]);
-    }
-    __syncthreads();
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int d = 0; d < 2; d++) {
-    const uint64_t e = uint64_t(t) * a.out_stride + h * kPageDim + 2 * lane + d;
-    if (BF16_ROWS) reinterpret_cast<uint16_t*>(a.out)[e] = f32_to_bf16(o[d] * inv);
-    else reinterpret_cast<float*>(a.out)[e] = o[d] * inv;
-  }
-}
-
 constexpr uint32_t kWorkgroups = 512;  // two for each CU
 
 // How calls are cut, by the most rows (new tokens x q heads of a KV head) a sequence can have: tiles of 16
@@ -1511,6 +1545,23 @@ uint64_t attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t ma
   return rows * 2 * kPartRow * 4 + kWorkgroups * sizeof(Joint);
 }
 
+template <class A>
+void launch(const A& a, uint32_t R, uint32_t grid, bool fp8, bool bf16, hipStream_t st) {
+  auto go = [&](auto* kern) { kern<<<grid, R == 256 || (R == 128 && !bf16) ? 512 : 256, 0, st>>>(a); };
+  if (R == 256) {
+    go(fp8 ? k_page_attn_tiles<true, true, 8, A> : k_page_attn_tiles<false, true, 8, A>);
+  } else if (R == 128) {
+    if (fp8) go(bf16 ? k_page_attn_tiles<true, true, 4, A> : k_page_attn_tiles<true, false, 8, A>);
+    else go(bf16 ? k_page_attn_tiles<false, true, 4, A> : k_page_attn_tiles<false, false, 8, A>);
+  } else if (R == 32) {
+    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 2, A> : k_page_attn_rows<true, false, 2, A>);
+    else go(bf16 ? k_page_attn_rows<false, true, 2, A> : k_page_attn_rows<false, false, 2, A>);
+  } else {
+    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 1, A> : k_page_attn_rows<true, false, 1, A>);
+    else go(bf16 ? k_page_attn_rows<false, true, 1, A> : k_page_attn_rows<false, false, 1, A>);
+  }
+}
+
 // Causal attention (parents null), or of trees.
 int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* out, uint64_t n_rows, uint64_t n_heads,
            uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype, void* work, uint64_t work_bytes,
@@ -1558,32 +1609,18 @@ int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* o
   a.c = 1.44269504f / sqrtf(float(kPageDim));
   a.joints = static_cast<Joint*>(work);
   a.parts = reinterpret_cast<float*>(a.joints + kWorkgroups);
-  if (parents) {
-    auto go = [&](auto* kern) { kern<<<uint32_t(n_rows * n_heads), 64, 0, st>>>(a, parents); };
-    if (fp8) go(bf16 ? k_page_tree<true, true> : k_page_tree<true, false>);
-    else go(bf16 ? k_page_tree<false, true> : k_page_tree<false, false>);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return set_error(QE_ERR_HIP, "page tree attention launch failed: %s", hipGetErrorString(e));
-    return QE_OK;
-  }
   // (fewer rows than max_new says need no more than the work that was asked for)
   const uint64_t bound = max_new && max_new < n_rows ? max_new : n_rows;
   const Cut c = cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
   const uint32_t R = c.rows, grid = c.workgroups;
   a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= kWholeItems;
   a.join = !a.whole_items;
-  auto go = [&](auto* kern) { kern<<<grid, R == 256 || (R == 128 && !bf16) ? 512 : 256, 0, st>>>(a); };
-  if (R == 256) {
-    go(fp8 ? k_page_attn_tiles<true, true, 8> : k_page_attn_tiles<false, true, 8>);
-  } else if (R == 128) {
-    if (fp8) go(bf16 ? k_page_attn_tiles<true, true, 4> : k_page_attn_tiles<true, false, 8>);
-    else go(bf16 ? k_page_attn_tiles<false, true, 4> : k_page_attn_tiles<false, false, 8>);
-  } else if (R == 32) {
-    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 2> : k_page_attn_rows<true, false, 2>);
-    else go(bf16 ? k_page_attn_rows<false, true, 2> : k_page_attn_rows<false, false, 2>);
+  if (parents) {
+    TreeAttnArgs tree{a};
+    tree.parents = parents;
+    launch(tree, R, grid, fp8, bf16, st);
   } else {
-    if (fp8) go(bf16 ? k_page_attn_rows<true, true, 1> : k_page_attn_rows<true, false, 1>);
-    else go(bf16 ? k_page_attn_rows<false, true, 1> : k_page_attn_rows<false, false, 1>);
+    launch(a, R, grid, fp8, bf16, st);
   }
   if (a.join) {
     const dim3 join(grid, R / 16);
