@@ -348,7 +348,8 @@ int qe_op_page_tree_attention(const qe_pages* pages, const int32_t* parents, con
  * last tokens of their sequences, so a call may also take only the last few of a prompt. mass_stride is
  * at least table_stride * page_size. Weights and sums are f32, of rows of either type; the sums are the
  * same every time. A row with a score that is not finite may make any position it attends NaN. mass
- * must not overlap q, the pages or work. */
+ * must not overlap q, the pages or work. n_rows * n_heads is below 2^28, and n_seqs * n_kv_heads times the
+ * positions of a table's row / 256 below 2^24. */
 uint64_t qe_op_page_weigh_work_bytes(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv_heads, uint64_t n_seqs,
                                      uint64_t positions, uint64_t max_new);
 int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint64_t n_heads, uint64_t q_stride,
@@ -372,7 +373,7 @@ int qe_op_page_keep(const float* mass, uint64_t mass_stride, const int32_t* lens
  * destination is not there (a page that is not, a position past the table or, for mass, mass_stride) is
  * left as it was; src that does not ascend or has src[i] < i leaves some of the rows moved undefined, and no
  * others. count above src_stride counts as src_stride. A page that two sequences share is moved by both:
- * not for shared pages. src_stride and mass_stride are below 2^31. */
+ * not for shared pages. src_stride and mass_stride are below 2^31, n_seqs * n_kv_heads below 2^19. */
 int qe_op_page_move(const qe_pages* pages, const int32_t* src, uint64_t src_heads, uint64_t src_stride,
                     const int32_t* count, const int32_t* first, float* mass, uint64_t mass_stride, void* stream);
 

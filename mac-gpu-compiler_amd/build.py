@@ -52,6 +52,7 @@ SOURCE_FLAGS = {"batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-am
                 "fused_timed.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
                 # page_attention.hip: as batch.hip (its f32 kernels then keep their sums out of scratch memory)
                 "page_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "page_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                 # batch.hip (its leading plain arguments), attention.hip: the same
                 "attention.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
                 # kernels.hip: the same for k_matvec (the lm_head) and k_argmax

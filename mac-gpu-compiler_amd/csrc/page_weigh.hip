@@ -4,8 +4,15 @@
 //   mass[s][h][j] += sum over rows t, q heads g of KV head h of w_tg(j),
 //   w_tg(j) = exp(x_tg(j) - m_tg) / sum_i exp(x_tg(i) - m_tg),  x_tg(j) = q[t][g] . k_j / sqrt(128)
 //
-// k_weigh_rows takes each row's maximum and sum, k_weigh_mass each position's weights, in row order:
-// one thread owns an entry of mass, so sums are the same every time.
+// A weight needs its row's sum over all positions, so the scores are computed twice: k_weigh<false> leaves
+// each row's maximum and sum over each block of positions, k_weigh_rows joins them, and k_weigh<true> adds
+// up the weights. (Kept scores would be 4 bytes a row and position, where K has 256 for all rows.)
+//
+// Both passes hold K still: a workgroup has 256 positions of a sequence and KV head, 64 a wave, as operand
+// A of v_mfma_f32_32x32x16_bf16 in registers, and passes the rows by, 32 at a time through LDS. So K is read
+// once a pass and a position's sum belongs to one wave: nothing is added in an order that changes. Where the
+// positions make few workgroups the rows are split among several, whose sums k_weigh_add adds in order.
+// f32 rows as three bf16 parts that add up exactly.
 #include "pages.h"
 
 #include "device_common.h"
@@ -16,6 +23,14 @@
 namespace qe {
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kSpan = 256;   // positions of a workgroup
+constexpr uint32_t kTile = 32;    // rows that pass by together
+
 struct WeighArgs {
   PagePlan p;
   PageStore st;
@@ -23,37 +38,273 @@ struct WeighArgs {
   uint64_t q_stride;
   float* mass;
   uint64_t mass_stride;
-  float2* rows;  // [n_rows][heads]: maximum, 1 / sum
-  uint32_t n_rows, group;
+  float2* parts;  // [n_rows][heads][blocks]: maximum, sum over a block
+  float2* rows;   // [n_rows][heads]: maximum, 1 / sum
+  float* sums;    // [splits][n_seqs][n_kv][blocks][kSpan], where splits > 1
+  uint32_t n_rows, group, blocks, splits;
   float c;  // log2(e) / sqrt(128)
 };
 
+// The rows of a sequence: (token, q head) pairs of a KV head, token first.
 struct Span {
-  int64_t first;      // position of its first row
-  int32_t row0, rows;  // packed rows
+  int64_t first;        // position of its first token
+  uint32_t row0, rows;  // first packed row; tokens * group
+  uint32_t end;         // positions that any of them attends: 0 .. end - 1
 };
 __device__ __forceinline__ Span span_of(const WeighArgs& a, uint32_t s) {
   const int64_t b = a.p.starts[s], e = a.p.starts[s + 1], lo = b < 0 ? 0 : b, hi = e < a.n_rows ? e : a.n_rows;
-  return {int64_t(a.p.lens[s]) - (e - lo), int32_t(lo), hi > lo ? int32_t(hi - lo) : 0};
+  Span q;
+  q.first = int64_t(a.p.lens[s]) - (e - lo);
+  q.row0 = uint32_t(lo);
+  const int64_t n = hi > lo ? hi - lo : 0;
+  q.rows = uint32_t(n) * a.group;
+  q.end = uint32_t(max(min(q.first + n, capacity_of(a.p)), int64_t(0)));
+  if (n == 0) q.end = 0;
+  return q;
 }
 
-template <bool FP8, bool BF16_ROWS>
-__device__ float score(const WeighArgs& a, uint32_t t, uint32_t h, size_t row) {
-  float s = 0.f;
-  const uint64_t e = uint64_t(t) * a.q_stride + h * kPageDim;
-  for (uint32_t d = 0; d < kPageDim; d++) {
-    const float q = BF16_ROWS ? bf16f(reinterpret_cast<const uint16_t*>(a.q)[e + d]) : reinterpret_cast<const float*>(a.q)[e + d];
-    const float k = FP8 ? __builtin_amdgcn_cvt_f32_fp8(a.st.k[row * kPageDim + d], 0)
-                        : bf16f(reinterpret_cast<const uint16_t*>(a.st.k)[row * kPageDim + d]);
-    s = fmaf(q, k, s);
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rebase(float from, float to) { return from == to ? 1.f : exp2_fast(from - to); }
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sum over each half of the wave, in lanes 31 and 63.
+__device__ __forceinline__ float sum_half(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  v += dpp<0x140>(v);
+  return v + dpp<0x142, 0xA>(v);
+}
+
+// 8 e4m3 values (two words) as bf16 times a power of two
+__device__ __forceinline__ bf16x8 fp8_bf16(uint32_t a, uint32_t b, float scale) {
+  u32x4 u;
+  u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false));
+  u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true));
+  u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false));
+  u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true));
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+// What passes by: a tile of rows of q in LDS, each of NS bf16 parts; the 16-byte piece c of row r at place
+// c ^ (r & 15), so that the 32 rows that are read at once lie in different banks.
+template <bool BF16_ROWS>
+struct RowTile {
+  static constexpr int NS = BF16_ROWS ? 1 : 3, LOADS = BF16_ROWS ? 2 : 4;
+  u32x4 raw[LOADS];
+  // thread: 16 dims of row tid / 8 (rows behind the last are read as that one)
+  __device__ __forceinline__ void load(const WeighArgs& a, const Span& q, uint32_t head, uint32_t r0) {
+    const uint32_t r = min(r0 + threadIdx.x / 8, q.rows - 1), t = r / a.group;
+    const uint64_t e = (uint64_t(q.row0) + t) * a.q_stride + (head * a.group + (r - t * a.group)) * kPageDim + (threadIdx.x & 7) * 16;
+    const u32x4* p = reinterpret_cast<const u32x4*>(a.q + e * (BF16_ROWS ? 2 : 4));
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) raw[i] = p[i];
   }
-  return (FP8 ? s * exp_scale(a.st.k_exp[row]) : s) * a.c;
+  __device__ __forceinline__ void store(uint8_t (*buf)[kTile * 256]) const {
+    const uint32_t r = threadIdx.x / 8;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t at = r * 256 + (((threadIdx.x & 7) * 2 + i) ^ (r & 15)) * 16;
+      if constexpr (BF16_ROWS) {
+        *reinterpret_cast<u32x4*>(buf[0] + at) = raw[i];
+      } else {
+        u32x4 part[3];  // cut: 8 + 8 + 8 of f32's 24 bits, so nothing is lost
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          uint32_t w[2][3];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float v = __uint_as_float(raw[2 * i + k / 2][2 * (k & 1) + e]);
+            w[e][0] = __float_as_uint(v);
+            const float rest = v - __uint_as_float(w[e][0] & 0xFFFF0000u);
+            w[e][1] = __float_as_uint(rest);
+            w[e][2] = __float_as_uint(rest - __uint_as_float(w[e][1] & 0xFFFF0000u));
+          }
+#pragma unroll
+          for (int n = 0; n < 3; n++) part[n][k] = __builtin_amdgcn_perm(w[1][n], w[0][n], 0x07060302u);
+        }
+#pragma unroll
+        for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(buf[n] + at) = part[n];
+      }
+    }
+  }
+};
+
+template <bool FP8, bool BF16_ROWS, bool SUMS>
+__global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
+  constexpr int NS = BF16_ROWS ? 1 : 3, EL = FP8 ? 1 : 2;
+  __shared__ __align__(16) uint8_t buf[2][NS][kTile * 256];
+  __shared__ float2 stat[SUMS ? 1 : 2][SUMS ? 1 : 4][SUMS ? 1 : kTile];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t at = blockIdx.x;
+  const uint32_t head = at % a.p.n_kv;
+  at /= a.p.n_kv;
+  const uint32_t split = at % a.splits;
+  at /= a.splits;
+  const uint32_t block = at % a.blocks, s = at / a.blocks;
+  const Span q = span_of(a, s);
+  if (block * kSpan >= q.end) return;
+  // the tiles of rows that attend any of the positions, and of them this workgroup's
+  const uint32_t tiles = (q.rows + kTile - 1) / kTile;
+  const int64_t token0 = int64_t(block * kSpan) - q.first;
+  const uint32_t tile0 = token0 > 0 ? uint32_t(token0) * a.group / kTile : 0;
+  const uint32_t from = tile0 + uint32_t(uint64_t(tiles - tile0) * split / a.splits);
+  const uint32_t to = tile0 + uint32_t(uint64_t(tiles - tile0) * (split + 1) / a.splits);
+  const uint32_t x = block * kSpan + 64 * wave;  // this wave's positions
+
+  // K, 32 positions at a time: operand A's lane has row `col` and, of dims in 8 steps, 8 a step
+  const int32_t* const table = a.p.table + size_t(s) * a.p.table_stride;
+  const uint32_t mask = (1u << a.p.page_shift) - 1;
+  int32_t page[4];
+  uint32_t there = 0;  // which of the four runs of 16 positions have a page
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    page[i] = table[min((x + 16 * i) >> a.p.page_shift, a.p.table_stride - 1)];
+    if (uint32_t(page[i]) < a.p.n_pages) there |= 1u << i;
+    else page[i] = 0;  // read as page 0, and what comes of it is masked
+  }
+  bf16x8 k[2][8];
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int32_t one = page[2 * u], two = page[2 * u + 1];
+    const size_t row = page_row(a.p, col < 16 ? one : two, head, (x + 32 * u + col) & mask);
+    if constexpr (FP8) {
+      u32x4 raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) raw[i] = *reinterpret_cast<const u32x4*>(a.st.k + row * kPageDim + 32 * i + 16 * half);
+      const float scale = exp_scale(a.st.k_exp[row]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) k[u][j] = fp8_bf16(raw[j / 2][2 * (j & 1)], raw[j / 2][2 * (j & 1) + 1], scale);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        k[u][j] = *reinterpret_cast<const bf16x8*>(a.st.k + (row * kPageDim + 16 * j + 8 * half) * EL);
+    }
+  }
+
+  f32x16 sum[2];
+  sum[0] = 0.f;
+  sum[1] = 0.f;
+  RowTile<BF16_ROWS> rows;
+  if (from < to) {
+    rows.load(a, q, head, from * kTile);
+    rows.store(buf[from & 1]);
+    if (from + 1 < to) rows.load(a, q, head, (from + 1) * kTile);
+  }
+  __syncthreads();
+  for (uint32_t i = from; i < to; i++) {
+    const uint32_t r = i * kTile + col, token = r / a.group;  // this lane's row
+    const bool real = r < q.rows;
+    const int32_t last = real ? int32_t(max(min(q.first + token, capacity_of(a.p) - 1), int64_t(-1))) : -1;  // the last position it attends
+    const uint64_t stat_at = (uint64_t(q.row0) + token) * a.group * a.p.n_kv + head * a.group + (r - token * a.group);
+    float2 rs = make_float2(0.f, 0.f);
+    if constexpr (SUMS)
+      if (real) rs = a.rows[stat_at];
+    f32x16 v[2];
+    v[0] = 0.f;
+    v[1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      // dims of step j: bf16 16 j + 8 half .., e4m3 32 (j / 2) + 16 half + 8 (j & 1) ..
+      const uint32_t piece = FP8 ? 4 * (j / 2) + 2 * half + (j & 1) : 2 * j + half;
+#pragma unroll
+      for (int n = NS - 1; n >= 0; n--) {
+        const bf16x8 f = *reinterpret_cast<const bf16x8*>(buf[i & 1][n] + col * 256 + ((piece ^ (col & 15)) * 16));
+#pragma unroll
+        for (int u = 0; u < 2; u++) v[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[u][j], f, v[u], 0, 0, 0);
+      }
+    }
+    // element e of tile u: position x + 32 u + 8 (e / 4) + 4 half + e % 4
+    const int64_t free_to = q.first + i * kTile / a.group;  // the least position that any of the tile's rows attends
+    const bool masked = int64_t(x) + 63 > min(free_to, capacity_of(a.p) - 1) || (i + 1) * kTile > q.rows || there != 15;
+    auto hidden = [&](int u, int e) __attribute__((always_inline)) {
+      const uint32_t in = 32 * u + 8 * (e / 4) + (e & 3);
+      return int32_t(x + in + 4 * half) > last || !(there >> (2 * u + e / 8) & 1);
+    };
+    if constexpr (SUMS) {
+      const float ref = rs.x == -INFINITY ? 0.f : rs.x;
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float w = exp2_fast(fmaf(v[u][e], a.c, -ref)) * rs.y;
+            sum[u][e] += hidden(u, e) ? 0.f : w;
+          }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) sum[u][e] = fmaf(exp2_fast(fmaf(v[u][e], a.c, -ref)), rs.y, sum[u][e]);
+      }
+    } else {
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (hidden(u, e)) v[u][e] = -INFINITY;
+      }
+      float m = v[0][0], l = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) m = fmaxf(m, v[u][e]);
+      m = max_halves(m) * a.c;
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) l += exp2_fast(fmaf(v[u][e], a.c, -ref));
+      l = add_halves(l);
+      if (half == 0) stat[i & 1][wave][col] = make_float2(m, l);
+    }
+    if (i + 1 < to) {
+      rows.store(buf[(i + 1) & 1]);
+      if (i + 2 < to) rows.load(a, q, head, (i + 2) * kTile);
+    }
+    __syncthreads();
+    if constexpr (!SUMS) {
+      if (tid < kTile && real) {  // (wave 0, whose lane has this row)
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) m = fmaxf(m, stat[i & 1][w][col].x);
+#pragma unroll
+        for (int w = 0; w < 4; w++) l = fmaf(stat[i & 1][w][col].y, rebase(stat[i & 1][w][col].x, m), l);
+        a.parts[stat_at * a.blocks + block] = make_float2(m, l);
+      }
+    }
+  }
+  if constexpr (SUMS) {
+    float* const mass = a.mass + (uint64_t(s) * a.p.n_kv + head) * a.mass_stride;
+    float* const part = a.sums + (((uint64_t(split) * a.p.n_seqs + s) * a.p.n_kv + head) * a.blocks + block) * kSpan;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const float v = sum_half(sum[u][e]);
+        const uint32_t in = 64 * wave + 32 * u + 8 * (e / 4) + 4 * half + (e & 3);
+        if (col == 31) {
+          if (a.splits > 1) part[in] = v;
+          else if (block * kSpan + in < q.end && !(v == 0.f)) mass[block * kSpan + in] += v;
+        }
+      }
+  }
 }
 
-// a wave for each row and q head
-template <bool FP8, bool BF16_ROWS>
-__global__ __launch_bounds__(64) void k_weigh_rows(WeighArgs a) {
-  const uint32_t heads = a.group * a.p.n_kv, t = blockIdx.x / heads, h = blockIdx.x - t * heads, lane = threadIdx.x;
+// Joins a row's maxima and sums over its blocks, 16 lanes a row.
+__global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs a) {
+  const uint32_t heads = a.group * a.p.n_kv, lane = threadIdx.x & 15;
+  const uint64_t r = uint64_t(blockIdx.x) * 16 + threadIdx.x / 16;
+  const uint32_t t = uint32_t(r / heads);
+  if (t >= a.n_rows) return;
   uint32_t lo = 0, hi = a.p.n_seqs;
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
@@ -61,40 +312,56 @@ __global__ __launch_bounds__(64) void k_weigh_rows(WeighArgs a) {
     else hi = mid;
   }
   const Span q = span_of(a, lo);
-  if (int32_t(t) < q.row0 || int32_t(t) >= q.row0 + q.rows) return;
-  const int64_t end = min(q.first + (int32_t(t) - q.row0) + 1, capacity_of(a.p));
+  if (t < q.row0 || t - q.row0 >= q.rows / a.group) return;
+  const int64_t last = min(q.first + (t - q.row0), capacity_of(a.p) - 1);
+  const uint32_t n = last < 0 ? 0 : uint32_t(last) / kSpan + 1;
+  const float2* parts = a.parts + r * a.blocks;
   float m = -INFINITY, l = 0.f;
-  for (int64_t x = 0; x < end; x += 64) {
-    const int64_t j = x + lane;
-    const int32_t page = j < end ? page_of(a.p, lo, j) : -1;
-    float s = -INFINITY;
-    if (page >= 0) s = score<FP8, BF16_ROWS>(a, t, h, page_row(a.p, page, h / a.group, uint32_t(j) & ((1u << a.p.page_shift) - 1)));
-    const float top = fmaxf(m, wave_max(s));
-    l = l * (m == top ? 1.f : exp2f(m - top)) + wave_sum(s == -INFINITY ? 0.f : exp2f(s - top));
+  for (uint32_t i = lane; i < n; i += 16) {
+    const float2 p = parts[i];
+    const float top = fmaxf(m, p.x);
+    l = l * rebase(m, top) + p.y * rebase(p.x, top);
     m = top;
   }
-  if (lane == 0) a.rows[uint64_t(t) * heads + h] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+    const float om = __shfl_xor(m, d), ol = __shfl_xor(l, d), top = fmaxf(m, om);
+    l = l * rebase(m, top) + ol * rebase(om, top);
+    m = top;
+  }
+  if (lane == 0) a.rows[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
 }
 
-// a thread for each position of a sequence and KV head
-template <bool FP8, bool BF16_ROWS>
-__global__ __launch_bounds__(256) void k_weigh_mass(WeighArgs a, uint32_t blocks) {
-  const uint32_t item = blockIdx.x / blocks, s = item / a.p.n_kv, kv = item - s * a.p.n_kv;
-  const int64_t j = int64_t(blockIdx.x - item * blocks) * 256 + threadIdx.x;
+// Adds the sums of the splits to mass, in order.
+__global__ __launch_bounds__(256) void k_weigh_add(WeighArgs a) {
+  const uint32_t item = blockIdx.x / a.blocks, block = blockIdx.x - item * a.blocks, s = item / a.p.n_kv;
+  const uint32_t j = block * kSpan + threadIdx.x;
   const Span q = span_of(a, s);
-  if (j >= capacity_of(a.p) || j >= q.first + q.rows) return;
-  const int32_t page = page_of(a.p, s, j);
-  if (page < 0) return;
-  const size_t row = page_row(a.p, page, kv, uint32_t(j) & ((1u << a.p.page_shift) - 1));
-  float sum = 0.f;
-  for (int32_t i = j < q.first ? 0 : int32_t(j - q.first); i < q.rows; i++)
-    for (uint32_t g = 0; g < a.group; g++) {
-      const uint32_t t = uint32_t(q.row0 + i), h = kv * a.group + g;
-      const float2 r = a.rows[uint64_t(t) * a.group * a.p.n_kv + h];
-      const float x = score<FP8, BF16_ROWS>(a, t, h, row);
-      sum += x == -INFINITY && r.x == -INFINITY ? 0.f : exp2f(x - r.x) * r.y;
-    }
-  a.mass[(uint64_t(s) * a.p.n_kv + kv) * a.mass_stride + j] += sum;
+  if (j >= q.end) return;
+  float v = 0.f;
+  for (uint32_t i = 0; i < a.splits; i++)
+    v += a.sums[((uint64_t(i) * a.p.n_seqs * a.p.n_kv + item) * a.blocks + block) * kSpan + threadIdx.x];
+  if (!(v == 0.f)) a.mass[uint64_t(item) * a.mass_stride + j] += v;
+}
+
+// How a call is cut up, and what its work holds.
+struct WeighCut {
+  uint64_t blocks, splits, parts, rows, sums;  // byte sizes of the last three
+  uint64_t bytes() const { return parts + rows + sums; }
+};
+// Rows are split where the positions alone make fewer than four workgroups a CU, into parts of at least four tiles.
+WeighCut weigh_cut(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv, uint64_t n_seqs, uint64_t positions, uint64_t max_new) {
+  WeighCut c{};
+  c.blocks = (positions + kSpan - 1) / kSpan;
+  const uint64_t most = max_new && max_new < n_rows ? max_new : n_rows;
+  const uint64_t tiles = (most * (n_heads / n_kv) + kTile - 1) / kTile, items = n_seqs * n_kv * c.blocks;
+  c.splits = (1024 + items - 1) / items;
+  if (c.splits > tiles / 4) c.splits = tiles / 4;
+  if (c.splits < 1) c.splits = 1;
+  c.parts = n_rows * n_heads * c.blocks * sizeof(float2);
+  c.rows = (n_rows * n_heads * sizeof(float2) + 15) / 16 * 16;
+  c.sums = c.splits > 1 ? c.splits * items * kSpan * sizeof(float) : 0;
+  return c;
 }
 
 }  // namespace
@@ -104,8 +371,10 @@ extern "C" {
 
 uint64_t qe_op_page_weigh_work_bytes(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv_heads, uint64_t n_seqs,
                                      uint64_t positions, uint64_t max_new) {
-  if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return 0;
-  return n_rows * n_heads * sizeof(float2);
+  if (!n_kv_heads || !n_heads || n_heads % n_kv_heads || !n_seqs || !positions || n_seqs > 65536 || n_kv_heads > 1024 ||
+      n_heads > 65536 || positions > 0x7FFFFFFFull || n_rows >= (1ull << 28) / n_heads)
+    return 0;
+  return qe::weigh_cut(n_rows, n_heads, n_kv_heads, n_seqs, positions, max_new).bytes();
 }
 
 int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint64_t n_heads, uint64_t q_stride,
@@ -118,7 +387,7 @@ int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint
     return qe::set_error(QE_ERR_ARG, "n_heads must be a multiple of n_kv_heads, at most 65536");
   if (n_rows == 0) return QE_OK;
   if (!q || !mass || !work) return qe::set_error(QE_ERR_ARG, "null argument");
-  if (n_rows > 0x7FFFFFFFull / n_heads) return qe::set_error(QE_ERR_ARG, "need n_rows * n_heads < 2^31");
+  if (n_rows >= (1ull << 28) / n_heads) return qe::set_error(QE_ERR_ARG, "need n_rows * n_heads < 2^28");
   const uint64_t el = dtype == QE_KV_F32 ? 4 : 2, capacity = pages->table_stride * pages->page_size;
   if (q_stride < n_heads * qe::kPageDim || q_stride > 0xFFFFFFFFull || q_stride * el % 16)
     return qe::set_error(QE_ERR_ARG, "q_stride must be at least n_heads * 128 elements and a multiple of 16 bytes");
@@ -126,7 +395,11 @@ int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint
     return qe::set_error(QE_ERR_ARG, "mass_stride must be at least table_stride * page_size, and below 2^31");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(work)) % 16 || reinterpret_cast<uintptr_t>(mass) % 4)
     return qe::set_error(QE_ERR_ARG, "q and work must be 16-byte aligned, mass 4-byte");
-  if (work_bytes < qe_op_page_weigh_work_bytes(n_rows, n_heads, a.p.n_kv, a.p.n_seqs, capacity, max_new))
+  const qe::WeighCut cut = qe::weigh_cut(n_rows, n_heads, a.p.n_kv, a.p.n_seqs, capacity, max_new);
+  const uint64_t items = uint64_t(a.p.n_seqs) * a.p.n_kv * cut.blocks;
+  if (items * cut.splits >= 1u << 24)
+    return qe::set_error(QE_ERR_ARG, "need n_seqs * n_kv_heads * (positions of a table's row / 256) < 2^24");
+  if (work_bytes < cut.bytes())
     return qe::set_error(QE_ERR_ARG, "work holds %llu bytes, fewer than qe_op_page_weigh_work_bytes gives",
                          (unsigned long long)work_bytes);
   const qe::Bytes to{mass, 4 * mass_stride * a.p.n_seqs * a.p.n_kv};
@@ -140,21 +413,28 @@ int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint
   a.q_stride = q_stride;
   a.mass = mass;
   a.mass_stride = mass_stride;
-  a.rows = static_cast<float2*>(work);
+  uint8_t* const base = static_cast<uint8_t*>(work);
+  a.rows = reinterpret_cast<float2*>(base);
+  a.parts = reinterpret_cast<float2*>(base + cut.rows);
+  a.sums = reinterpret_cast<float*>(base + cut.rows + cut.parts);
   a.n_rows = uint32_t(n_rows);
   a.group = uint32_t(n_heads / a.p.n_kv);
+  a.blocks = uint32_t(cut.blocks);
+  a.splits = uint32_t(cut.splits);
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const uint32_t blocks = uint32_t((capacity + 255) / 256);
-  auto go = [&](auto* rows, auto* sums) {
-    rows<<<uint32_t(n_rows * n_heads), 64, 0, st>>>(a);
-    sums<<<blocks * a.p.n_seqs * a.p.n_kv, 256, 0, st>>>(a, blocks);
+  const uint32_t grid = uint32_t(items * cut.splits);
+  auto go = [&](auto* first, auto* second) {
+    first<<<grid, 256, 0, st>>>(a);
+    qe::k_weigh_rows<<<uint32_t((n_rows * n_heads + 15) / 16), 256, 0, st>>>(a);
+    second<<<grid, 256, 0, st>>>(a);
+    if (a.splits > 1) qe::k_weigh_add<<<uint32_t(items), 256, 0, st>>>(a);
   };
   const bool bf16 = dtype == QE_KV_BF16;
-  if (fp8 && bf16) go(qe::k_weigh_rows<true, true>, qe::k_weigh_mass<true, true>);
-  else if (fp8) go(qe::k_weigh_rows<true, false>, qe::k_weigh_mass<true, false>);
-  else if (bf16) go(qe::k_weigh_rows<false, true>, qe::k_weigh_mass<false, true>);
-  else go(qe::k_weigh_rows<false, false>, qe::k_weigh_mass<false, false>);
+  if (fp8 && bf16) go(qe::k_weigh<true, true, false>, qe::k_weigh<true, true, true>);
+  else if (fp8) go(qe::k_weigh<true, false, false>, qe::k_weigh<true, false, true>);
+  else if (bf16) go(qe::k_weigh<false, true, false>, qe::k_weigh<false, true, true>);
+  else go(qe::k_weigh<false, false, false>, qe::k_weigh<false, false, true>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page weigh launch failed: %s", hipGetErrorString(e));
   return QE_OK;
