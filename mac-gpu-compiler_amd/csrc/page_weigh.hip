@@ -73,13 +73,28 @@ __device__ __forceinline__ float add_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// Sum over each half of the wave, in lanes 31 and 63.
-__device__ __forceinline__ float sum_half(float v) {
-  v += dpp<0xB1>(v);
-  v += dpp<0x4E>(v);
-  v += dpp<0x141>(v);
-  v += dpp<0x140>(v);
-  return v + dpp<0x142, 0xA>(v);
+// Sums of 32 values over the 32 lanes of each half of the wave, value i to lane i: each step adds two values'
+// halves up, one for the lanes whose bit is clear and one for the others.
+template <int CTRL, int N>
+__device__ __forceinline__ void halve(float (&v)[32], bool upper) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float keep = upper ? v[i + N] : v[i], send = upper ? v[i] : v[i + N];
+    v[i] = keep + dpp<CTRL>(send);
+  }
+}
+__device__ __forceinline__ float sums_of_halves(float (&v)[32]) {
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 16]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  halve<0x128, 8>(v, lane & 8);  // with lane ^ 8 of its row
+  halve<0x141, 4>(v, lane & 4);  // 7 - lane of its 8
+  halve<0x4E, 2>(v, lane & 2);   // lane ^ 2
+  halve<0xB1, 1>(v, lane & 1);   // lane ^ 1
+  return v[0];
 }
 
 // 8 e4m3 values (two words) as bf16 times a power of two
@@ -283,19 +298,14 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
     }
   }
   if constexpr (SUMS) {
-    float* const mass = a.mass + (uint64_t(s) * a.p.n_kv + head) * a.mass_stride;
-    float* const part = a.sums + (((uint64_t(split) * a.p.n_seqs + s) * a.p.n_kv + head) * a.blocks + block) * kSpan;
+    float all[32];
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const float v = sum_half(sum[u][e]);
-        const uint32_t in = 64 * wave + 32 * u + 8 * (e / 4) + 4 * half + (e & 3);
-        if (col == 31) {
-          if (a.splits > 1) part[in] = v;
-          else if (block * kSpan + in < q.end && !(v == 0.f)) mass[block * kSpan + in] += v;
-        }
-      }
+    for (int i = 0; i < 32; i++) all[i] = sum[i / 16][i % 16];
+    const float v = sums_of_halves(all);  // of element lane % 16 of tile lane / 16 % 2
+    const uint32_t in = 64 * wave + 32 * (lane >> 4 & 1) + 8 * (lane >> 2 & 3) + 4 * half + (lane & 3), j = block * kSpan + in;
+    const uint64_t item = uint64_t(s) * a.p.n_kv + head;
+    if (a.splits > 1) a.sums[((uint64_t(split) * a.p.n_seqs * a.p.n_kv + item) * a.blocks + block) * kSpan + in] = v;
+    else if (j < q.end && !(v == 0.f)) a.mass[item * a.mass_stride + j] += v;
   }
 }
 
