@@ -4,11 +4,12 @@
 //   mass[s][h][j] += sum over rows t, q heads g of KV head h of w_tg(j),
 //   w_tg(j) = exp(x_tg(j) - m_tg) / sum_i exp(x_tg(i) - m_tg),  x_tg(j) = q[t][g] . k_j / sqrt(128)
 //
-// A weight needs its row's sum over all positions, so the scores are computed twice: k_weigh<false> leaves
-// each row's maximum and sum over each block of positions, k_weigh_rows joins them, and k_weigh<true> adds
-// up the weights. (Kept scores would be 4 bytes a row and position, where K has 256 for all rows.)
+// A weight needs its row's sum over all positions. Up to 16 rows (tokens x q heads) of a sequence and KV head:
+// k_weigh_few leaves the scores, 4 bytes a row and position where K has 128 or 256 for all rows, and k_weigh_kept makes
+// weights of them. More rows: the scores are computed twice. k_weigh<false> leaves each row's maximum and sum over
+// each block of positions, k_weigh_rows joins them, and k_weigh<true> adds up the weights.
 //
-// Both passes hold K still: a workgroup has 256 positions of a sequence and KV head, 64 a wave, as operand
+// Those two passes hold K still: a workgroup has 256 positions of a sequence and KV head, 64 a wave, as operand
 // A of v_mfma_f32_32x32x16_bf16 in registers, and passes the rows by, 32 at a time through LDS. So K is read
 // once a pass and a position's sum belongs to one wave: nothing is added in an order that changes. Where the
 // positions make few workgroups the rows are split among several, whose sums k_weigh_add adds in order.
@@ -30,6 +31,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kSpan = 256;   // positions of a workgroup
 constexpr uint32_t kTile = 32;    // rows that pass by together
+constexpr uint32_t kFewRows = 16;
 
 struct WeighArgs {
   PagePlan p;
@@ -38,10 +40,12 @@ struct WeighArgs {
   uint64_t q_stride;
   float* mass;
   uint64_t mass_stride;
-  float2* parts;  // [n_rows][heads][blocks]: maximum, sum over a block
+  float2* parts;  // [n_rows][heads][blocks]: maximum, sum over a block; few rows: [n_seqs][n_kv][few][blocks]
   float2* rows;   // [n_rows][heads]: maximum, 1 / sum
   float* sums;    // [splits][n_seqs][n_kv][blocks][kSpan], where splits > 1
+  float* scores;  // few rows: [n_seqs][n_kv][few][blocks * span], -inf where a row does not attend
   uint32_t n_rows, group, blocks, splits;
+  uint32_t few, span;  // rows of a sequence and KV head that scores are kept of (0: none); positions of a workgroup
   float c;  // log2(e) / sqrt(128)
 };
 
@@ -107,6 +111,24 @@ __device__ __forceinline__ bf16x8 fp8_bf16(uint32_t a, uint32_t b, float scale) 
   return __builtin_bit_cast(bf16x8, u);
 }
 
+// 8 floats as three bf16 parts that add up to them: 8 + 8 + 8 of f32's 24 bits, so nothing is lost
+__device__ __forceinline__ void cut_f32(const u32x4 (&x)[2], u32x4 (&part)[3]) {
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    uint32_t w[2][3];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const float v = __uint_as_float(x[k / 2][2 * (k & 1) + e]);
+      w[e][0] = __float_as_uint(v);
+      const float rest = v - __uint_as_float(w[e][0] & 0xFFFF0000u);
+      w[e][1] = __float_as_uint(rest);
+      w[e][2] = __float_as_uint(rest - __uint_as_float(w[e][1] & 0xFFFF0000u));
+    }
+#pragma unroll
+    for (int n = 0; n < 3; n++) part[n][k] = __builtin_amdgcn_perm(w[1][n], w[0][n], 0x07060302u);  // upper halves
+  }
+}
+
 // What passes by: a tile of rows of q in LDS, each of NS bf16 parts; the 16-byte piece c of row r at place
 // c ^ (r & 15), so that the 32 rows that are read at once lie in different banks.
 template <bool BF16_ROWS>
@@ -129,21 +151,9 @@ struct RowTile {
       if constexpr (BF16_ROWS) {
         *reinterpret_cast<u32x4*>(buf[0] + at) = raw[i];
       } else {
-        u32x4 part[3];  // cut: 8 + 8 + 8 of f32's 24 bits, so nothing is lost
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          uint32_t w[2][3];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float v = __uint_as_float(raw[2 * i + k / 2][2 * (k & 1) + e]);
-            w[e][0] = __float_as_uint(v);
-            const float rest = v - __uint_as_float(w[e][0] & 0xFFFF0000u);
-            w[e][1] = __float_as_uint(rest);
-            w[e][2] = __float_as_uint(rest - __uint_as_float(w[e][1] & 0xFFFF0000u));
-          }
-#pragma unroll
-          for (int n = 0; n < 3; n++) part[n][k] = __builtin_amdgcn_perm(w[1][n], w[0][n], 0x07060302u);
-        }
+        u32x4 part[3];
+        const u32x4 two[2] = {raw[2 * i], raw[2 * i + 1]};
+        cut_f32(two, part);
 #pragma unroll
         for (int n = 0; n < 3; n++) *reinterpret_cast<u32x4*>(buf[n] + at) = part[n];
       }
@@ -173,6 +183,8 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
   const uint32_t from = tile0 + uint32_t(uint64_t(tiles - tile0) * split / a.splits);
   const uint32_t to = tile0 + uint32_t(uint64_t(tiles - tile0) * (split + 1) / a.splits);
   const uint32_t x = block * kSpan + 64 * wave;  // this wave's positions
+  RowTile<BF16_ROWS> rows;
+  if (from < to) rows.load(a, q, head, from * kTile);
 
   // K, 32 positions at a time: operand A's lane has row `col` and, of dims in 8 steps, 8 a step
   const int32_t* const table = a.p.table + size_t(s) * a.p.table_stride;
@@ -207,9 +219,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
   f32x16 sum[2];
   sum[0] = 0.f;
   sum[1] = 0.f;
-  RowTile<BF16_ROWS> rows;
   if (from < to) {
-    rows.load(a, q, head, from * kTile);
     rows.store(buf[from & 1]);
     if (from + 1 < to) rows.load(a, q, head, (from + 1) * kTile);
   }
@@ -309,6 +319,227 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
   }
 }
 
+// ---- few rows: up to 16 of a sequence and KV head ----
+// K goes by once, in steps of 64 positions a wave, against the rows in registers (operand B of
+// v_mfma_f32_16x16x32_bf16), and the scores are kept, which is less than a second read of K. A
+// step's loads are issued a step ahead.
+template <bool FP8>
+struct KStep {
+  u32x4 k[FP8 ? 8 : 16];
+  uint32_t exp[4];
+};
+
+template <bool FP8, bool BF16_ROWS>
+__global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
+  constexpr int NS = BF16_ROWS ? 1 : 3, EL = FP8 ? 1 : 2;
+  __shared__ float2 stat[4][kFewRows];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t head = blockIdx.x % a.p.n_kv, block = blockIdx.x / a.p.n_kv % a.blocks, s = blockIdx.x / a.p.n_kv / a.blocks;
+  const Span q = span_of(a, s);
+  const uint32_t x0 = block * a.span, x1 = min(x0 + a.span, q.end);
+  if (x0 >= q.end || q.rows > a.few) return;  // (more rows than there was room for: k_weigh_kept sees to them)
+  const int32_t* const table = a.p.table + size_t(s) * a.p.table_stride;
+  const uint32_t mask = (1u << a.p.page_shift) - 1;
+  // K of positions x .. x + 63 in tiles of 16: operand A's lane has row `col` of a tile and, of dims, 8 in each of
+  // 4 steps: bf16 32 j + 8 g .., e4m3 64 (j / 2) + 16 g + 8 (j & 1) ..
+  auto fetch = [&](KStep<FP8>& d, uint32_t x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const int32_t page = table[min((x + 16 * t) >> a.p.page_shift, a.p.table_stride - 1)];
+      const size_t row = page_row(a.p, uint32_t(page) < a.p.n_pages ? page : 0, head, (x + 16 * t + col) & mask);
+      const uint8_t* p = a.st.k + row * kPageDim * EL + 16 * g;
+#pragma unroll
+      for (int i = 0; i < (FP8 ? 2 : 4); i++) d.k[(FP8 ? 2 : 4) * t + i] = *reinterpret_cast<const u32x4*>(p + 64 * i);
+      if constexpr (FP8) d.exp[t] = a.st.k_exp[row];
+    }
+  };
+  const uint32_t r = min(col, q.rows - 1), token = r / a.group;
+  const int32_t last = col < q.rows ? int32_t(max(min(q.first + token, capacity_of(a.p) - 1), int64_t(-1))) : -1;
+  const int32_t free_to = int32_t(max(min(q.first, capacity_of(a.p) - 1), int64_t(-1)));
+  const uint64_t e0 = (uint64_t(q.row0) + token) * a.q_stride + (head * a.group + (r - token * a.group)) * kPageDim;
+  bf16x8 f[4][NS];
+  u32x4 raw[4][BF16_ROWS ? 1 : 2];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t d = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j & 1) : 32 * j + 8 * g;
+#pragma unroll
+    for (int i = 0; i < (BF16_ROWS ? 1 : 2); i++)
+      raw[j][i] = *reinterpret_cast<const u32x4*>(a.q + (e0 + d) * (BF16_ROWS ? 2 : 4) + 16 * i);
+  }
+  KStep<FP8> d0, d1;
+  uint32_t x = x0 + 64 * wave;
+  fetch(d0, x);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if constexpr (BF16_ROWS) {
+      f[j][0] = __builtin_bit_cast(bf16x8, raw[j][0]);
+    } else {
+      u32x4 part[3];
+      cut_f32(raw[j], part);
+#pragma unroll
+      for (int n = 0; n < 3; n++) f[j][n] = __builtin_bit_cast(bf16x8, part[n]);
+    }
+  }
+  float* const kept = a.scores + ((uint64_t(s) * a.p.n_kv + head) * a.few + r) * (uint64_t(a.blocks) * a.span);
+  float m = -INFINITY, l = 0.f;
+  auto step = [&](const KStep<FP8>& d, uint32_t x) __attribute__((always_inline)) {
+    f32x4 v[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      v[t] = 0.f;
+      const float scale = FP8 ? exp_scale(d.exp[t]) : 1.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        bf16x8 k;
+        if constexpr (FP8) k = fp8_bf16(d.k[2 * t + j / 2][2 * (j & 1)], d.k[2 * t + j / 2][2 * (j & 1) + 1], scale);
+        else k = __builtin_bit_cast(bf16x8, d.k[4 * t + j]);
+#pragma unroll
+        for (int n = NS - 1; n >= 0; n--) v[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, f[j][n], v[t], 0, 0, 0);
+      }
+      const int32_t page = table[min((x + 16 * t) >> a.p.page_shift, a.p.table_stride - 1)];
+      const bool there = uint32_t(page) < a.p.n_pages;
+      if (int32_t(x + 16 * t + 15) > free_to || !there) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (int32_t(x + 16 * t + 4 * g + e) > last || !there) v[t][e] = -INFINITY;
+      }
+      if (col < q.rows) *reinterpret_cast<f32x4*>(kept + x + 16 * t + 4 * g) = v[t];
+    }
+    float top = v[0][0];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) top = fmaxf(top, v[t][e]);
+    top = fmaxf(m, top * a.c);
+    const float ref = top == -INFINITY ? 0.f : top;
+    l *= rebase(m, top);
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) l += exp2_fast(fmaf(v[t][e], a.c, -ref));
+    m = top;
+  };
+  while (x < x1) {
+    fetch(d1, min(x + 256, x1 - 1) & ~63u);  // (past the end: positions that are there, unused)
+    step(d0, x);
+    x += 256;
+    if (x >= x1) break;
+    fetch(d0, min(x + 256, x1 - 1) & ~63u);
+    step(d1, x);
+    x += 256;
+  }
+  // the four groups of lanes, then the four waves
+#pragma unroll
+  for (int d = 16; d < 64; d *= 2) {
+    const float om = __shfl_xor(m, d), ol = __shfl_xor(l, d), top = fmaxf(m, om);
+    l = l * rebase(m, top) + ol * rebase(om, top);
+    m = top;
+  }
+  if (g == 0) stat[wave][col] = make_float2(m, l);
+  __syncthreads();
+  if (tid < q.rows) {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) m = fmaxf(m, stat[w][tid].x);
+#pragma unroll
+    for (int w = 0; w < 4; w++) l = fmaf(stat[w][tid].y, rebase(stat[w][tid].x, m), l);
+    a.parts[((uint64_t(s) * a.p.n_kv + head) * a.few + tid) * a.blocks + block] = make_float2(m, l);
+  }
+}
+
+// The weight of the rows' kept scores, 1024 positions a workgroup: the rows' maxima and sums first, 16 lanes a row.
+template <bool FP8, bool BF16_ROWS>
+__global__ __launch_bounds__(256) void k_weigh_kept(WeighArgs a, uint32_t blocks) {
+  __shared__ float2 stat[kFewRows];
+  const uint32_t tid = threadIdx.x, item = blockIdx.x / blocks, s = item / a.p.n_kv, head = item - s * a.p.n_kv;
+  const Span q = span_of(a, s);
+  const uint32_t x0 = (blockIdx.x - item * blocks) * 1024, j = x0 + 4 * tid;
+  if (x0 >= q.end) return;
+  float* const mass = a.mass + uint64_t(item) * a.mass_stride;
+  if (q.rows > a.few) {
+    // more rows than max_new says: a row after another, its maximum, its sum, its weights, by plain sums
+    __shared__ float2 part[256];
+    const int32_t* const table = a.p.table + size_t(s) * a.p.table_stride;
+    float sum[4] = {};
+    for (uint32_t r = 0; r < q.rows; r++) {
+      const uint32_t token = r / a.group;
+      const uint64_t e = (uint64_t(q.row0) + token) * a.q_stride + (head * a.group + (r - token * a.group)) * kPageDim;
+      const uint32_t end = uint32_t(max(min(q.first + token + 1, capacity_of(a.p)), int64_t(0)));
+      auto score = [&](uint32_t p) {
+        const int32_t page = p < end ? table[p >> a.p.page_shift] : -1;
+        if (uint32_t(page) >= a.p.n_pages) return -INFINITY;
+        const size_t row = page_row(a.p, page, head, p & ((1u << a.p.page_shift) - 1));
+        float v = 0.f;
+        for (uint32_t d = 0; d < kPageDim; d++) {
+          const float x = BF16_ROWS ? bf16f(reinterpret_cast<const uint16_t*>(a.q)[e + d]) : reinterpret_cast<const float*>(a.q)[e + d];
+          const float k = FP8 ? __builtin_amdgcn_cvt_f32_fp8(a.st.k[row * kPageDim + d], 0)
+                              : bf16f(reinterpret_cast<const uint16_t*>(a.st.k)[row * kPageDim + d]);
+          v = fmaf(x, k, v);
+        }
+        return (FP8 ? v * exp_scale(a.st.k_exp[row]) : v) * a.c;
+      };
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t p = tid; p < end; p += 256) {
+        const float v = score(p), top = fmaxf(m, v);
+        l = l * rebase(m, top) + (v == -INFINITY ? 0.f : exp2_fast(v - top));
+        m = top;
+      }
+      __syncthreads();
+      part[tid] = make_float2(m, l);
+      __syncthreads();
+      m = -INFINITY, l = 0.f;
+      for (int i = 0; i < 256; i++) m = fmaxf(m, part[i].x);
+      for (int i = 0; i < 256; i++) l = fmaf(part[i].y, rebase(part[i].x, m), l);
+      for (int i = 0; i < 4; i++) {
+        const float v = j + i < end ? score(j + i) : -INFINITY;
+        if (v != -INFINITY) sum[i] += exp2_fast(v - m) / l;
+      }
+    }
+    for (int i = 0; i < 4; i++)
+      if (j + i < q.end && !(sum[i] == 0.f)) mass[j + i] += sum[i];
+    return;
+  }
+  {
+    const uint32_t r = tid / 16, lane = tid & 15;
+    float m = -INFINITY, l = 0.f;
+    if (r < q.rows) {
+      const int64_t last = min(q.first + r / a.group, capacity_of(a.p) - 1);
+      const uint32_t n = last < 0 ? 0 : uint32_t(last) / a.span + 1;
+      const float2* parts = a.parts + (uint64_t(item) * a.few + r) * a.blocks;
+      for (uint32_t i = lane; i < n; i += 16) {
+        const float2 p = parts[i];
+        const float top = fmaxf(m, p.x);
+        l = l * rebase(m, top) + p.y * rebase(p.x, top);
+        m = top;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      const float om = __shfl_xor(m, d), ol = __shfl_xor(l, d), top = fmaxf(m, om);
+      l = l * rebase(m, top) + ol * rebase(om, top);
+      m = top;
+    }
+    if (lane == 0) stat[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+  }
+  __syncthreads();
+  if (j >= q.end) return;
+  const uint64_t stride = uint64_t(a.blocks) * a.span;
+  const float* kept = a.scores + uint64_t(item) * a.few * stride + j;
+  float sum[4] = {};
+#pragma unroll 4
+  for (uint32_t r = 0; r < q.rows; r++) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(kept + r * stride);
+    const float2 rs = stat[r];
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] += v[i] == -INFINITY ? 0.f : exp2_fast(fmaf(v[i], a.c, -rs.x)) * rs.y;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (j + i < q.end && !(sum[i] == 0.f)) mass[j + i] += sum[i];
+}
+
+// ---- more rows ----
 // Joins a row's maxima and sums over its blocks, 16 lanes a row.
 __global__ __launch_bounds__(256) void k_weigh_rows(WeighArgs a) {
   const uint32_t heads = a.group * a.p.n_kv, lane = threadIdx.x & 15;
@@ -356,21 +587,35 @@ __global__ __launch_bounds__(256) void k_weigh_add(WeighArgs a) {
 
 // How a call is cut up, and what its work holds.
 struct WeighCut {
-  uint64_t blocks, splits, parts, rows, sums;  // byte sizes of the last three
-  uint64_t bytes() const { return parts + rows + sums; }
+  uint64_t few, span, blocks, splits, parts, rows, sums, scores;  // the last four in bytes
+  uint64_t bytes() const { return parts + rows + sums + scores; }
 };
-// Rows are split where the positions alone make fewer than four workgroups a CU, into parts of at least four tiles.
 WeighCut weigh_cut(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv, uint64_t n_seqs, uint64_t positions, uint64_t max_new) {
   WeighCut c{};
-  c.blocks = (positions + kSpan - 1) / kSpan;
-  const uint64_t most = max_new && max_new < n_rows ? max_new : n_rows;
-  const uint64_t tiles = (most * (n_heads / n_kv) + kTile - 1) / kTile, items = n_seqs * n_kv * c.blocks;
-  c.splits = (1024 + items - 1) / items;
+  const uint64_t most = max_new && max_new < n_rows ? max_new : n_rows, items = n_seqs * n_kv;
+  const uint64_t rows = max_new ? most * (n_heads / n_kv) : ~0ull;
+  if (rows <= kFewRows) {
+    c.few = rows ? rows : 1;
+    c.span = 1024;
+    while (c.span > kSpan && items * ((positions + c.span - 1) / c.span) < 512) c.span /= 2;
+  } else {
+    c.span = kSpan;
+  }
+  c.blocks = (positions + c.span - 1) / c.span;
+  c.splits = 1;
+  if (c.few) {
+    c.parts = (items * c.few * c.blocks * sizeof(float2) + 15) / 16 * 16;
+    c.scores = items * c.few * c.blocks * c.span * sizeof(float);
+    return c;
+  }
+  // rows are split where the positions alone make fewer than four workgroups a CU, into parts of at least four tiles
+  const uint64_t tiles = (most * (n_heads / n_kv) + kTile - 1) / kTile;
+  c.splits = (1024 + items * c.blocks - 1) / (items * c.blocks);
   if (c.splits > tiles / 4) c.splits = tiles / 4;
   if (c.splits < 1) c.splits = 1;
-  c.parts = n_rows * n_heads * c.blocks * sizeof(float2);
+  c.parts = (n_rows * n_heads * c.blocks * sizeof(float2) + 15) / 16 * 16;
   c.rows = (n_rows * n_heads * sizeof(float2) + 15) / 16 * 16;
-  c.sums = c.splits > 1 ? c.splits * items * kSpan * sizeof(float) : 0;
+  c.sums = c.splits > 1 ? c.splits * items * c.blocks * kSpan * sizeof(float) : 0;
   return c;
 }
 
@@ -424,27 +669,38 @@ int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint
   a.mass = mass;
   a.mass_stride = mass_stride;
   uint8_t* const base = static_cast<uint8_t*>(work);
-  a.rows = reinterpret_cast<float2*>(base);
-  a.parts = reinterpret_cast<float2*>(base + cut.rows);
-  a.sums = reinterpret_cast<float*>(base + cut.rows + cut.parts);
+  a.parts = reinterpret_cast<float2*>(base);
+  a.rows = reinterpret_cast<float2*>(base + cut.parts);
+  a.sums = reinterpret_cast<float*>(base + cut.parts + cut.rows);
+  a.scores = a.sums;
   a.n_rows = uint32_t(n_rows);
   a.group = uint32_t(n_heads / a.p.n_kv);
   a.blocks = uint32_t(cut.blocks);
   a.splits = uint32_t(cut.splits);
+  a.few = uint32_t(cut.few);
+  a.span = uint32_t(cut.span);
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t grid = uint32_t(items * cut.splits);
-  auto go = [&](auto* first, auto* second) {
+  auto go = [&](auto* few, auto* kept, auto* first, auto* second) {
+    if (a.few) {
+      const uint32_t blocks = uint32_t((capacity + 1023) / 1024);
+      few<<<grid, 256, 0, st>>>(a);
+      kept<<<blocks * a.p.n_seqs * a.p.n_kv, 256, 0, st>>>(a, blocks);
+      return;
+    }
     first<<<grid, 256, 0, st>>>(a);
     qe::k_weigh_rows<<<uint32_t((n_rows * n_heads + 15) / 16), 256, 0, st>>>(a);
     second<<<grid, 256, 0, st>>>(a);
     if (a.splits > 1) qe::k_weigh_add<<<uint32_t(items), 256, 0, st>>>(a);
   };
+#define QE_WEIGH(F, B) go(qe::k_weigh_few<F, B>, qe::k_weigh_kept<F, B>, qe::k_weigh<F, B, false>, qe::k_weigh<F, B, true>)
   const bool bf16 = dtype == QE_KV_BF16;
-  if (fp8 && bf16) go(qe::k_weigh<true, true, false>, qe::k_weigh<true, true, true>);
-  else if (fp8) go(qe::k_weigh<true, false, false>, qe::k_weigh<true, false, true>);
-  else if (bf16) go(qe::k_weigh<false, true, false>, qe::k_weigh<false, true, true>);
-  else go(qe::k_weigh<false, false, false>, qe::k_weigh<false, false, true>);
+  if (fp8 && bf16) QE_WEIGH(true, true);
+  else if (fp8) QE_WEIGH(true, false);
+  else if (bf16) QE_WEIGH(false, true);
+  else QE_WEIGH(false, false);
+#undef QE_WEIGH
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page weigh launch failed: %s", hipGetErrorString(e));
   return QE_OK;
