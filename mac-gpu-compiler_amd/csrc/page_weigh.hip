@@ -326,13 +326,15 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
 template <bool FP8>
 struct KStep {
   u32x4 k[FP8 ? 8 : 16];
-  uint32_t exp[4];
+  u32x4 exp;      // e4m3: of the run that the lane's rows of K lie in
+  uint32_t there;  // which of the four runs of 16 positions have a page
 };
 
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
   constexpr int NS = BF16_ROWS ? 1 : 3, EL = FP8 ? 1 : 2;
   __shared__ float2 stat[4][kFewRows];
+  __shared__ __align__(16) float out[4][kFewRows][68];  // each wave's own
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t head = blockIdx.x % a.p.n_kv, block = blockIdx.x / a.p.n_kv % a.blocks, s = blockIdx.x / a.p.n_kv / a.blocks;
@@ -341,18 +343,28 @@ __global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
   if (x0 >= q.end || q.rows > a.few) return;  // (more rows than there was room for: k_weigh_kept sees to them)
   const int32_t* const table = a.p.table + size_t(s) * a.p.table_stride;
   const uint32_t mask = (1u << a.p.page_shift) - 1;
-  // K of positions x .. x + 63 in tiles of 16: operand A's lane has row `col` of a tile and, of dims, 8 in each of
+  // K of positions x .. x + 63: operand A's row `col` of tile t is position 16 (col / 4) + 4 t + col % 4, so that a
+  // lane's results of the four tiles are those of the 16 positions from 16 g; and of dims a lane has 8 in each of
   // 4 steps: bf16 32 j + 8 g .., e4m3 64 (j / 2) + 16 g + 8 (j & 1) ..
   auto fetch = [&](KStep<FP8>& d, uint32_t x) __attribute__((always_inline)) {
+    int32_t page[4];
+    d.there = 0;
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const int32_t page = table[min((x + 16 * t) >> a.p.page_shift, a.p.table_stride - 1)];
-      const size_t row = page_row(a.p, uint32_t(page) < a.p.n_pages ? page : 0, head, (x + 16 * t + col) & mask);
-      const uint8_t* p = a.st.k + row * kPageDim * EL + 16 * g;
-#pragma unroll
-      for (int i = 0; i < (FP8 ? 2 : 4); i++) d.k[(FP8 ? 2 : 4) * t + i] = *reinterpret_cast<const u32x4*>(p + 64 * i);
-      if constexpr (FP8) d.exp[t] = a.st.k_exp[row];
+    for (int i = 0; i < 4; i++) {
+      page[i] = table[min((x + 16 * i) >> a.p.page_shift, a.p.table_stride - 1)];
+      if (uint32_t(page[i]) < a.p.n_pages) d.there |= 1u << i;
+      else page[i] = 0;  // read as page 0, and what comes of it is masked
     }
+    const int32_t p0 = page[0], p1 = page[1], p2 = page[2], p3 = page[3];
+    const int32_t mine = col & 8 ? (col & 4 ? p3 : p2) : (col & 4 ? p1 : p0);
+    const size_t run = page_row(a.p, mine, head, (x + 16 * (col >> 2)) & mask);
+    const uint8_t* p = a.st.k + (run + (col & 3)) * kPageDim * EL + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < (FP8 ? 2 : 4); i++)
+        d.k[(FP8 ? 2 : 4) * t + i] = *reinterpret_cast<const u32x4*>(p + 4 * t * kPageDim * EL + 64 * i);
+    if constexpr (FP8) d.exp = *reinterpret_cast<const u32x4*>(a.st.k_exp + run);
   };
   const uint32_t r = min(col, q.rows - 1), token = r / a.group;
   const int32_t last = col < q.rows ? int32_t(max(min(q.first + token, capacity_of(a.p) - 1), int64_t(-1))) : -1;
@@ -381,14 +393,16 @@ __global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
       for (int n = 0; n < 3; n++) f[j][n] = __builtin_bit_cast(bf16x8, part[n]);
     }
   }
-  float* const kept = a.scores + ((uint64_t(s) * a.p.n_kv + head) * a.few + r) * (uint64_t(a.blocks) * a.span);
+  const uint64_t stride = uint64_t(a.blocks) * a.span;
+  float* const kept = a.scores + (uint64_t(s) * a.p.n_kv + head) * a.few * stride;
   float m = -INFINITY, l = 0.f;
   auto step = [&](const KStep<FP8>& d, uint32_t x) __attribute__((always_inline)) {
     f32x4 v[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       v[t] = 0.f;
-      const float scale = FP8 ? exp_scale(d.exp[t]) : 1.f;
+      float scale = 1.f;
+      if constexpr (FP8) scale = exp_scale(d.exp[t] >> (8 * (col & 3)) & 0xFFu);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         bf16x8 k;
@@ -397,15 +411,21 @@ __global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
 #pragma unroll
         for (int n = NS - 1; n >= 0; n--) v[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, f[j][n], v[t], 0, 0, 0);
       }
-      const int32_t page = table[min((x + 16 * t) >> a.p.page_shift, a.p.table_stride - 1)];
-      const bool there = uint32_t(page) < a.p.n_pages;
-      if (int32_t(x + 16 * t + 15) > free_to || !there) {
+    }
+    if (int32_t(x + 63) > free_to || d.there != 15) {
+      const bool there = d.there >> g & 1;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (int32_t(x + 16 * t + 4 * g + e) > last || !there) v[t][e] = -INFINITY;
-      }
-      if (col < q.rows) *reinterpret_cast<f32x4*>(kept + x + 16 * t + 4 * g) = v[t];
+          if (int32_t(x + 16 * g + 4 * t + e) > last || !there) v[t][e] = -INFINITY;
     }
+    // through LDS, so that each store instruction writes whole rows of 64 positions
+    if (col < q.rows)
+#pragma unroll
+      for (int t = 0; t < 4; t++) *reinterpret_cast<f32x4*>(&out[wave][col][16 * g + 4 * t]) = v[t];
+    for (uint32_t i = lane >> 4; i < q.rows; i += 4)
+      *reinterpret_cast<f32x4*>(kept + i * stride + x + 4 * col) = *reinterpret_cast<const f32x4*>(&out[wave][i][4 * col]);
     float top = v[0][0];
 #pragma unroll
     for (int t = 0; t < 4; t++)
@@ -452,9 +472,10 @@ __global__ __launch_bounds__(256, 2) void k_weigh_few(WeighArgs a) {
 template <bool FP8, bool BF16_ROWS>
 __global__ __launch_bounds__(256) void k_weigh_kept(WeighArgs a, uint32_t blocks) {
   __shared__ float2 stat[kFewRows];
-  const uint32_t tid = threadIdx.x, item = blockIdx.x / blocks, s = item / a.p.n_kv, head = item - s * a.p.n_kv;
+  const uint32_t tid = threadIdx.x, head = blockIdx.x % a.p.n_kv, s = blockIdx.x / a.p.n_kv / blocks;
+  const uint32_t item = s * a.p.n_kv + head;
   const Span q = span_of(a, s);
-  const uint32_t x0 = (blockIdx.x - item * blocks) * 1024, j = x0 + 4 * tid;
+  const uint32_t x0 = blockIdx.x / a.p.n_kv % blocks * 1024, j = x0 + 4 * tid;
   if (x0 >= q.end) return;
   float* const mass = a.mass + uint64_t(item) * a.mass_stride;
   if (q.rows > a.few) {
@@ -500,6 +521,16 @@ __global__ __launch_bounds__(256) void k_weigh_kept(WeighArgs a, uint32_t blocks
       if (j + i < q.end && !(sum[i] == 0.f)) mass[j + i] += sum[i];
     return;
   }
+  const uint64_t stride = uint64_t(a.blocks) * a.span;
+  const float* kept = a.scores + uint64_t(item) * a.few * stride + j;
+  constexpr uint32_t AT = 4;  // rows whose scores are loaded together, the first of them before the sums are joined
+  f32x4 v[AT];
+  auto load = [&](uint32_t r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < AT; i++)
+      if (r0 + i < q.rows && j < q.end) v[i] = *reinterpret_cast<const f32x4*>(kept + (r0 + i) * stride);
+  };
+  load(0);
   {
     const uint32_t r = tid / 16, lane = tid & 15;
     float m = -INFINITY, l = 0.f;
@@ -524,15 +555,16 @@ __global__ __launch_bounds__(256) void k_weigh_kept(WeighArgs a, uint32_t blocks
   }
   __syncthreads();
   if (j >= q.end) return;
-  const uint64_t stride = uint64_t(a.blocks) * a.span;
-  const float* kept = a.scores + uint64_t(item) * a.few * stride + j;
   float sum[4] = {};
-#pragma unroll 4
-  for (uint32_t r = 0; r < q.rows; r++) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(kept + r * stride);
-    const float2 rs = stat[r];
+  for (uint32_t r0 = 0; r0 < q.rows; r0 += AT) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum[i] += v[i] == -INFINITY ? 0.f : exp2_fast(fmaf(v[i], a.c, -rs.x)) * rs.y;
+    for (uint32_t n = 0; n < AT; n++) {
+      if (r0 + n >= q.rows) break;
+      const float2 rs = stat[r0 + n];
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[i] += v[n][i] == -INFINITY ? 0.f : exp2_fast(fmaf(v[n][i], a.c, -rs.x)) * rs.y;
+    }
+    load(r0 + AT);
   }
 #pragma unroll
   for (int i = 0; i < 4; i++)
