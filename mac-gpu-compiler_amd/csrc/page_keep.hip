@@ -26,73 +26,156 @@ struct KeepArgs {
   uint32_t n_kv, keep, sinks, recent;
 };
 
-// Sum over the workgroup's threads up to each, without its own; `all`: of all of them.
-__device__ uint32_t scan_below(uint32_t v, uint32_t* waves, uint32_t& all) {
-  const uint32_t wave = threadIdx.x >> 6, up = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) waves[wave] = up;
-  __syncthreads();
-  uint32_t below = up - v;
-  all = 0;
-  for (uint32_t i = 0; i < kKeepThreads / 64; i++) {
-    if (i < wave) below += waves[i];
-    all += waves[i];
-  }
-  return below;
-}
+// A wave has a contiguous part of the row, in groups of 256 positions, a lane 4 consecutive ones of each.
+constexpr uint32_t kGroup = 256, kGroupsInRegs = 8, kWaves = kKeepThreads / 64;
+constexpr uint32_t kInRegs = kWaves * kGroupsInRegs * kGroup;  // positions of a row that fit in registers
+constexpr uint32_t kDigits = 2048, kCopies = 4;
 
-// A workgroup for each sequence and KV head: the `need`-th largest of the middle by its digits of 8 bits
-// from the top (a count of each digit among the values that agree so far), then everything above it and the
-// first of what equals it.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// A workgroup for each sequence and KV head. The value that the `need`-th largest of the middle has is found by its
+// digits from the top, 11, 11 and 10 bits: the values that agree so far are counted by their next digit in LDS (the
+// first time in four copies, since masses share few exponents), and the digit is where the count from above
+// reaches `need`. Then everything above that value is kept, and of what equals it the first.
+// Bound by latency, not by the 4 bytes a position: some ten barriers, and LDS counts that meet in one place.
+template <bool REGS>
 __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
-  __shared__ uint32_t digits[256], waves[kKeepThreads / 64], found[2];
-  const uint32_t tid = threadIdx.x, s = blockIdx.x / a.n_kv, h = blockIdx.x - s * a.n_kv;
+  __shared__ uint32_t digits[(kCopies + 2) * kDigits];
+  __shared__ uint32_t waves[3][kWaves], found[3][2], above[kWaves], equal[kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t s = blockIdx.x / a.n_kv, h = blockIdx.x - s * a.n_kv;
   const uint32_t len = uint32_t(min(int64_t(max(a.lens[s], 0)), int64_t(a.mass_stride)));
   const uint32_t keep = min(len, a.keep), sinks = min(a.sinks, keep), recent = min(a.recent, keep - sinks);
-  const uint32_t from = sinks, to = len - recent;
+  const uint32_t from = sinks, to = len - recent, want = keep - sinks - recent;  // `want` of from .. to - 1
   const float* mass = a.mass + uint64_t(blockIdx.x) * a.mass_stride;
   int32_t* kept = a.kept + uint64_t(blockIdx.x) * a.kept_stride;
-  uint32_t need = keep - sinks - recent;  // of from .. to - 1
-  uint32_t prefix = 0;
-  const bool choose = need < to - from;
-  if (choose && need)
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) digits[tid] = 0;
-      __syncthreads();
-      for (uint32_t j = from + tid; j < to; j += kKeepThreads) {
-        const uint32_t key = order_of(mass[j]);
-        if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&digits[key >> shift & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t d = 255, above = 0;
-        while (above + digits[d] < need) above += digits[d--];
-        found[0] = d;
-        found[1] = above;
-      }
-      __syncthreads();
-      prefix |= found[0] << shift;
-      need -= found[1];
-    }
-  uint32_t at = 0, ties = 0;
-  for (uint32_t x = 0; x < len; x += kKeepThreads) {
-    const uint32_t j = x + tid;
-    bool in = j < len, tie = false;
-    if (in && choose && j >= from && j < to) {
-      const uint32_t key = order_of(mass[j]);
-      tie = need && key == prefix;
-      in = keep - sinks - recent && key > prefix;
-    }
-    uint32_t all;
-    const uint32_t rank = ties + scan_below(tie, waves, all);
-    ties += all;
-    in = in || (tie && rank < need);
-    const uint32_t place = at + scan_below(in, waves, all);
-    at += all;
-    if (in) kept[place] = int32_t(j);
-  }
   for (uint32_t i = keep + tid; i < a.keep; i += kKeepThreads) kept[i] = -1;
   if (h == 0 && tid == 0) a.count[s] = int32_t(keep);
+  if (want == to - from) {  // all of them
+    for (uint32_t j = tid; j < len; j += kKeepThreads) kept[j] = int32_t(j);
+    return;
+  }
+  const uint32_t groups = (len + kWaves * kGroup - 1) / (kWaves * kGroup), j0 = wave * groups * kGroup + 4 * lane;
+  auto load = [&](uint32_t g, uint32_t (&key)[4]) __attribute__((always_inline)) {
+    const uint32_t j = j0 + g * kGroup;
+    if (uint64_t(j) + 3 < a.mass_stride) {
+      const f32x4u x = *reinterpret_cast<const f32x4u*>(mass + j);
+#pragma unroll
+      for (int e = 0; e < 4; e++) key[e] = order_of(x[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) key[e] = j + e < a.mass_stride ? order_of(mass[j + e]) : 0;
+    }
+  };
+  uint32_t keys[REGS ? kGroupsInRegs : 1][4];
+  if constexpr (REGS) {
+#pragma unroll
+    for (uint32_t g = 0; g < kGroupsInRegs; g++)
+      if (g < groups) load(g, keys[g]);
+  }
+  // f(first position, keys) of each group
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (REGS) {
+#pragma unroll
+      for (uint32_t g = 0; g < kGroupsInRegs; g++)
+        if (g < groups) f(j0 + g * kGroup, keys[g]);
+    } else {
+      for (uint32_t g = 0; g < groups; g++) {
+        load(g, keys[0]);
+        f(j0 + g * kGroup, keys[0]);
+      }
+    }
+  };
+  uint32_t prefix = 0, need = want;  // the digits so far; how many of the values that have them are kept
+  if (want) {
+    for (uint32_t i = tid; i < (kCopies + 2) * kDigits; i += kKeepThreads) digits[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, high = pass == 1 ? 21 : 10;  // of the digit; of those before
+      const uint32_t n = pass == 2 ? 1024 : 2048;
+      uint32_t* const bins = digits + (pass == 0 ? (wave % kCopies) * kDigits : (kCopies + pass - 1) * kDigits);
+      each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (j + e >= from && j + e < to && (pass == 0 || key[e] >> high == prefix >> high))
+            atomicAdd(&bins[key[e] >> shift & (n - 1)], 1u);
+      });
+      __syncthreads();
+      // from above: thread t has the digits n - 1 - 2 t and n - 2 - 2 t
+      uint32_t c[2] = {};
+      if (2 * tid < n)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (uint32_t k = 0; k < (pass == 0 ? kCopies : 1); k++)
+            c[i] += digits[(pass == 0 ? k : kCopies + pass - 1) * kDigits + n - 1 - 2 * tid - i];
+      uint32_t upto = wave_scan(c[0] + c[1]);
+      if (lane == 63) waves[pass][wave] = upto;
+      __syncthreads();
+      for (uint32_t w = 0; w < wave; w++) upto += waves[pass][w];
+      const uint32_t before = upto - c[0] - c[1];
+      if (before < need && upto >= need) {
+        const bool second = before + c[0] < need;
+        found[pass][0] = n - 1 - 2 * tid - second;
+        found[pass][1] = before + (second ? c[0] : 0);
+      }
+      __syncthreads();
+      prefix |= found[pass][0] << shift;
+      need -= found[pass][1];
+    }
+  }
+  // which are kept: always, above the value, or equal to it among the first
+  auto always = [&](uint32_t j) { return j < from || (j >= to && j < len); };
+  auto is_above = [&](uint32_t j, uint32_t key) { return always(j) || (want && j < to && key > prefix); };
+  auto is_equal = [&](uint32_t j, uint32_t key) { return want && j >= from && j < to && key == prefix; };
+  uint32_t n_above = 0, n_equal = 0;
+  each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      n_above += __builtin_popcountll(__ballot(is_above(j + e, key[e])));
+      n_equal += __builtin_popcountll(__ballot(is_equal(j + e, key[e])));
+    }
+  });
+  if (lane == 0) {
+    above[wave] = n_above;
+    equal[wave] = n_equal;
+  }
+  __syncthreads();
+  uint32_t at = 0, ties = 0;  // kept before this wave's positions; equal ones there
+  for (uint32_t w = 0; w < wave; w++) {
+    at += above[w];
+    ties += equal[w];
+  }
+  at += min(ties, need);
+  // (rank of a lane's position among those of a group: the lanes before it, then its own)
+  auto below = [&](uint64_t m) { return __builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0)); };
+  each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
+    bool in[4], tie[4];
+    uint32_t rank = ties, here = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      tie[e] = is_equal(j + e, key[e]);
+      const uint64_t m = __ballot(tie[e]);
+      rank += below(m);
+      here += __builtin_popcountll(m);
+    }
+    ties += here;
+    uint32_t place = at;
+    here = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      in[e] = is_above(j + e, key[e]) || (tie[e] && rank < need);
+      rank += tie[e];
+      const uint64_t m = __ballot(in[e]);
+      place += below(m);
+      here += __builtin_popcountll(m);
+    }
+    at += here;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (in[e]) kept[place++] = int32_t(j + e);
+  });
 }
 
 // ---- the move ----
@@ -206,7 +289,8 @@ int qe_op_page_keep(const float* mass, uint64_t mass_stride, const int32_t* lens
   if (k.meets(m) || k.meets(l) || k.meets(c) || c.meets(m) || c.meets(l))
     return qe::set_error(QE_ERR_ARG, "kept and count must not overlap each other, mass or lens");
   qe::KeepArgs a{mass, lens, kept, count, mass_stride, kept_stride, uint32_t(n_kv_heads), uint32_t(keep), uint32_t(sinks), uint32_t(recent)};
-  qe::k_page_keep<<<uint32_t(rows), qe::kKeepThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  (mass_stride <= qe::kInRegs ? qe::k_page_keep<true> : qe::k_page_keep<false>)<<<uint32_t(rows), qe::kKeepThreads, 0,
+                                                                                  static_cast<hipStream_t>(stream)>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page keep launch failed: %s", hipGetErrorString(e));
   return QE_OK;
