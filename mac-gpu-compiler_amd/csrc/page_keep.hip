@@ -9,9 +9,11 @@ namespace qe {
 namespace {
 
 // ---- the choice ----
-// A float as a whole number that orders as it does: NaN (0) below all, -0 as 0.
+// A float as a whole number that orders as it does: NaN below all, -0 as 0. What is always kept is above them, what
+// is not there below.
+constexpr uint32_t kAlways = 0xFFFFFFFFu, kNever = 0;
 __device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0;
+  if (x != x) return 1;
   const uint32_t u = x == 0.f ? 0 : __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -32,6 +34,12 @@ constexpr uint32_t kInRegs = kWaves * kGroupsInRegs * kGroup;  // positions of a
 constexpr uint32_t kDigits = 2048, kCopies = 4;
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// The sum of the waves' values before `wave`.
+__device__ __forceinline__ uint32_t sum_below(const uint32_t* waves, uint32_t wave) {
+  const uint32_t lane = threadIdx.x & 63, v = waves[lane < kWaves ? lane : 0];
+  return from_lane(wave_scan(lane < wave ? v : 0), 63);
+}
 
 // A workgroup for each sequence and KV head. The value that the `need`-th largest of the middle has is found by its
 // digits from the top, 11, 11 and 10 bits: the values that agree so far are counted by their next digit in LDS (the
@@ -58,14 +66,18 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
   const uint32_t groups = (len + kWaves * kGroup - 1) / (kWaves * kGroup), j0 = wave * groups * kGroup + 4 * lane;
   auto load = [&](uint32_t g, uint32_t (&key)[4]) __attribute__((always_inline)) {
     const uint32_t j = j0 + g * kGroup;
-    if (uint64_t(j) + 3 < a.mass_stride) {
+    if (j + 3 < len) {
       const f32x4u x = *reinterpret_cast<const f32x4u*>(mass + j);
 #pragma unroll
       for (int e = 0; e < 4; e++) key[e] = order_of(x[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) key[e] = j + e < a.mass_stride ? order_of(mass[j + e]) : 0;
+      for (int e = 0; e < 4; e++) key[e] = j + e < len ? order_of(mass[j + e]) : kNever;
     }
+    if (j < from || j + 3 >= to)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (j + e < len && (j + e < from || j + e >= to)) key[e] = kAlways;
   };
   uint32_t keys[REGS ? kGroupsInRegs : 1][4];
   if constexpr (REGS) {
@@ -98,7 +110,7 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
       each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (j + e >= from && j + e < to && (pass == 0 || key[e] >> high == prefix >> high))
+          if (pass == 0 ? key[e] - 1 < kAlways - 1 : key[e] >> high == prefix >> high)
             atomicAdd(&bins[key[e] >> shift & (n - 1)], 1u);
       });
       __syncthreads();
@@ -113,7 +125,7 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
       uint32_t upto = wave_scan(c[0] + c[1]);
       if (lane == 63) waves[pass][wave] = upto;
       __syncthreads();
-      for (uint32_t w = 0; w < wave; w++) upto += waves[pass][w];
+      upto += sum_below(waves[pass], wave);
       const uint32_t before = upto - c[0] - c[1];
       if (before < need && upto >= need) {
         const bool second = before + c[0] < need;
@@ -125,16 +137,14 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
       need -= found[pass][1];
     }
   }
-  // which are kept: always, above the value, or equal to it among the first
-  auto always = [&](uint32_t j) { return j < from || (j >= to && j < len); };
-  auto is_above = [&](uint32_t j, uint32_t key) { return always(j) || (want && j < to && key > prefix); };
-  auto is_equal = [&](uint32_t j, uint32_t key) { return want && j >= from && j < to && key == prefix; };
+  else prefix = kAlways - 1;
+  // which are kept: what is above the value, and of what equals it the first
   uint32_t n_above = 0, n_equal = 0;
-  each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
+  each([&](uint32_t, const uint32_t (&key)[4]) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      n_above += __builtin_popcountll(__ballot(is_above(j + e, key[e])));
-      n_equal += __builtin_popcountll(__ballot(is_equal(j + e, key[e])));
+      n_above += __builtin_popcountll(__ballot(key[e] > prefix));
+      n_equal += __builtin_popcountll(__ballot(key[e] == prefix));
     }
   });
   if (lane == 0) {
@@ -142,40 +152,48 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
     equal[wave] = n_equal;
   }
   __syncthreads();
-  uint32_t at = 0, ties = 0;  // kept before this wave's positions; equal ones there
-  for (uint32_t w = 0; w < wave; w++) {
-    at += above[w];
-    ties += equal[w];
-  }
-  at += min(ties, need);
+  uint32_t ties = sum_below(equal, wave), at = sum_below(above, wave) + min(ties, need);  // equal, and kept, before this wave's positions
+  // positions go through LDS, where the counts were, if they fit: stored in order then
+  int32_t* const stage = reinterpret_cast<int32_t*>(digits);
+  const bool staged = keep <= (kCopies + 2) * kDigits;
   // (rank of a lane's position among those of a group: the lanes before it, then its own)
   auto below = [&](uint64_t m) { return __builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0)); };
-  each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
-    bool in[4], tie[4];
-    uint32_t rank = ties, here = 0;
+  auto places = [&](int32_t* to) __attribute__((always_inline)) {
+    each([&](uint32_t j, const uint32_t (&key)[4]) __attribute__((always_inline)) {
+      bool in[4];
+      uint64_t m[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      tie[e] = is_equal(j + e, key[e]);
-      const uint64_t m = __ballot(tie[e]);
-      rank += below(m);
-      here += __builtin_popcountll(m);
-    }
-    ties += here;
-    uint32_t place = at;
-    here = 0;
+      for (int e = 0; e < 4; e++) m[e] = __ballot(in[e] = key[e] > prefix);
+      uint64_t tie[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      in[e] = is_above(j + e, key[e]) || (tie[e] && rank < need);
-      rank += tie[e];
-      const uint64_t m = __ballot(in[e]);
-      place += below(m);
-      here += __builtin_popcountll(m);
-    }
-    at += here;
+      for (int e = 0; e < 4; e++) tie[e] = __ballot(key[e] == prefix);
+      if (tie[0] | tie[1] | tie[2] | tie[3]) {
+        uint32_t rank = ties;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (in[e]) kept[place++] = int32_t(j + e);
-  });
+        for (int e = 0; e < 4; e++) rank += below(tie[e]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          ties += __builtin_popcountll(tie[e]);
+          if (key[e] == prefix) in[e] = rank++ < need;
+          m[e] = __ballot(in[e]);
+        }
+      }
+      uint32_t place = at;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        place += below(m[e]);
+        at += __builtin_popcountll(m[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (in[e]) to[place++] = int32_t(j + e);
+    });
+  };
+  if (staged) places(stage);
+  else places(kept);
+  if (!staged) return;
+  __syncthreads();
+  for (uint32_t i = tid; i < keep; i += kKeepThreads) kept[i] = stage[i];
 }
 
 // ---- the move ----
