@@ -373,7 +373,8 @@ int qe_op_page_keep(const float* mass, uint64_t mass_stride, const int32_t* lens
  * destination is not there (a page that is not, a position past the table or, for mass, mass_stride) is
  * left as it was; src that does not ascend or has src[i] < i leaves some of the rows moved undefined, and no
  * others. count above src_stride counts as src_stride. A page that two sequences share is moved by both:
- * not for shared pages. src_stride and mass_stride are below 2^31, n_seqs * n_kv_heads below 2^19. */
+ * not for shared pages. src_stride and mass_stride are below 2^31, n_seqs * n_kv_heads below 2^19,
+ * the rows of all pages (n_pages * n_kv_heads * page_size) below 2^32 - 1. */
 int qe_op_page_move(const qe_pages* pages, const int32_t* src, uint64_t src_heads, uint64_t src_stride,
                     const int32_t* count, const int32_t* first, float* mass, uint64_t mass_stride, void* stream);
 

@@ -5,6 +5,8 @@
 #include "device_common.h"
 #include "status.h"
 
+#include <type_traits>
+
 namespace qe {
 namespace {
 
@@ -206,80 +208,259 @@ struct MoveArgs {
   uint32_t src_heads, src_stride;
 };
 
-constexpr uint32_t kMoveThreads = 256;
-enum Part { kMoveK, kMoveV, kMoveRest };
+constexpr uint32_t kMoveThreads = 256, kNoSlot = 0xFFFFFFFFu;
 
-// A workgroup for a part of every row of a sequence and KV head: slices of 16 dims of K and of V, and what
-// there is one of for a row (exponents, mass). Rows ascend and only ever move to the front, so what a chunk
-// of rows writes no later chunk reads: within one, everything is read before anything is written.
+// The moves of a sequence and KV head. Slots are row indexes in the pages (below 2^32 - 1, as the host checks).
+struct Moves {
+  const int32_t* src;
+  int64_t first;
+  uint32_t s, head, count;
+};
+__device__ __forceinline__ Moves moves_of(const MoveArgs& a, uint32_t item) {
+  Moves m;
+  m.s = item / a.p.n_kv;
+  m.head = item - m.s * a.p.n_kv;
+  m.first = a.first ? a.first[m.s] : 0;
+  m.count = uint32_t(min(int64_t(max(a.count[m.s], 0)), int64_t(a.src_stride)));
+  m.src = a.src + (uint64_t(m.s) * a.src_heads + (a.src_heads == 1 ? 0 : m.head)) * a.src_stride;
+  return m;
+}
+__device__ __forceinline__ uint32_t slot_of(const MoveArgs& a, const Moves& m, int64_t pos) {
+  if (pos < 0 || pos >= capacity_of(a.p)) return kNoSlot;
+  const int32_t page = page_of(a.p, m.s, pos);
+  return page < 0 ? kNoSlot : uint32_t(page_row(a.p, page, m.head, uint32_t(pos) & ((1u << a.p.page_shift) - 1)));
+}
+// Where row i comes from and goes to; neither, unless both are there and differ.
+struct Move {
+  uint32_t from, to;
+};
+__device__ __forceinline__ Move move_of(const MoveArgs& a, const Moves& m, uint32_t i) {
+  Move v{kNoSlot, kNoSlot};
+  if (i >= m.count) return v;
+  const int32_t at = m.src[i];
+  if (at < 0 || at == int32_t(i)) return v;
+  v.from = slot_of(a, m, m.first + at);
+  v.to = slot_of(a, m, m.first + i);
+  if (v.from == kNoSlot || v.to == kNoSlot) v.from = v.to = kNoSlot;
+  return v;
+}
+// The wave's loads have arrived: no wave of the workgroup writes before all of them, behind a barrier, are done.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 template <bool FP8>
-__global__ __launch_bounds__(kMoveThreads) void k_page_move(MoveArgs a) {
-  constexpr uint32_t EL = FP8 ? 1 : 2, SLICES = 8;
-  const uint32_t tid = threadIdx.x, item = blockIdx.x / (2 * SLICES + 1), part = blockIdx.x - item * (2 * SLICES + 1);
-  const uint32_t s = item / a.p.n_kv, h = item - s * a.p.n_kv;
-  const int64_t first = a.first ? a.first[s] : 0, capacity = capacity_of(a.p);
-  const uint32_t count = uint32_t(min(int64_t(max(a.count[s], 0)), int64_t(a.src_stride)));
-  const int32_t* src = a.src + (uint64_t(s) * a.src_heads + (a.src_heads == 1 ? 0 : h)) * a.src_stride;
-  const uint32_t mask = (1u << a.p.page_shift) - 1;
-  auto slot_of = [&](int64_t pos) -> int64_t {  // row index in the pages, -1: not there
-    if (pos < 0 || pos >= capacity) return -1;
-    const int32_t page = page_of(a.p, s, pos);
-    return page < 0 ? -1 : int64_t(page_row(a.p, page, h, uint32_t(pos) & mask));
-  };
-  if (part < 2 * SLICES) {
-    const bool k = part < SLICES;
-    const uint32_t d = (part % SLICES) * 16 + (tid & 15);
-    for (uint32_t i0 = 0; i0 < count; i0 += kMoveThreads / 16) {
-      const uint32_t i = i0 + tid / 16;
-      uint8_t* to = nullptr;
-      uint32_t v = 0;
-      if (i < count && src[i] != int32_t(i) && src[i] >= 0) {
-        const int64_t x = slot_of(first + src[i]), y = slot_of(first + i);
-        if (x >= 0 && y >= 0) {
-          auto at = [&](int64_t r) {
-            return k ? a.st.k + (size_t(r) * kPageDim + d) * EL
-                     : a.st.v + (size_t(r & ~int64_t(kPageRun - 1)) * kPageDim + (r & (kPageRun - 1)) + d * kPageRun) * EL;
-          };
-          v = FP8 ? *at(x) : *reinterpret_cast<const uint16_t*>(at(x));
-          to = at(y);
+struct Element {
+  typedef typename std::conditional<FP8, uint8_t, uint16_t>::type type;
+};
+// V of row `slot`, dim d, in elements
+__device__ __forceinline__ size_t v_at(uint32_t slot, uint32_t d) {
+  return size_t(slot & ~(kPageRun - 1)) * kPageDim + d * kPageRun + (slot & (kPageRun - 1));
+}
+
+// mass of the rows moved, and 0 behind them; the exponents. Row i is thread i % 256's.
+template <bool FP8, int N>
+__device__ __forceinline__ void move_rest(const MoveArgs& a, const Moves& m, uint32_t item) {
+  const uint32_t tid = threadIdx.x;
+  float* const mass = a.mass ? a.mass + uint64_t(item) * a.mass_stride : nullptr;
+  if (!FP8 && !mass) return;
+  for (uint32_t i0 = 0; i0 < m.count; i0 += kMoveThreads * N) {
+    uint32_t to[N], ke[N], ve[N];
+    int64_t place[N];
+    float v[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const uint32_t i = i0 + n * kMoveThreads + tid;
+      to[n] = kNoSlot;
+      place[n] = -1;
+      ke[n] = ve[n] = 0;
+      v[n] = 0.f;
+      if (FP8) {
+        const Move w = move_of(a, m, i);
+        to[n] = w.to;
+        if (w.from != kNoSlot) {
+          ke[n] = a.st.k_exp[w.from];
+          ve[n] = a.st.v_exp[w.from];
         }
       }
-      __syncthreads();
-      if (to) {
-        if (FP8) *to = uint8_t(v);
-        else *reinterpret_cast<uint16_t*>(to) = uint16_t(v);
+      if (mass && i < m.count) {
+        const int32_t at = m.src[i];
+        const int64_t x = m.first + at, y = m.first + i;
+        if (at >= 0 && x >= 0 && y >= 0 && x < int64_t(a.mass_stride) && y < int64_t(a.mass_stride)) {
+          place[n] = y;
+          v[n] = mass[x];
+        }
       }
     }
-    return;
-  }
-  float* mass = a.mass ? a.mass + uint64_t(item) * a.mass_stride : nullptr;
-  for (uint32_t i0 = 0; i0 < count; i0 += kMoveThreads) {
-    const uint32_t i = i0 + tid;
-    int64_t to = -1, place = -1;
-    uint32_t ke = 0, ve = 0;
-    float m = 0.f;
-    if (i < count && src[i] != int32_t(i) && src[i] >= 0) {
-      const int64_t x = first + src[i], y = first + i, from = slot_of(x);
-      if (FP8 && from >= 0 && (to = slot_of(y)) >= 0) {
-        ke = a.st.k_exp[from];
-        ve = a.st.v_exp[from];
-      }
-      if (mass && x >= 0 && y >= 0 && x < int64_t(a.mass_stride) && y < int64_t(a.mass_stride)) {
-        place = y;
-        m = mass[x];
-      }
-    }
+    wait_loads();
     __syncthreads();
-    if (to >= 0) {
-      a.st.k_exp[to] = uint8_t(ke);
-      a.st.v_exp[to] = uint8_t(ve);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      if (FP8 && to[n] != kNoSlot) {
+        a.st.k_exp[to[n]] = uint8_t(ke[n]);
+        a.st.v_exp[to[n]] = uint8_t(ve[n]);
+      }
+      if (place[n] >= 0) mass[place[n]] = v[n];
     }
-    if (place >= 0) mass[place] = m;
   }
   if (mass) {
     __syncthreads();
-    const int64_t end = min(int64_t(a.p.lens[s]), int64_t(a.mass_stride));
-    for (int64_t j = max(first + count, int64_t(0)) + tid; j < end; j += kMoveThreads) mass[j] = 0.f;
+    const int64_t end = min(int64_t(a.p.lens[m.s]), int64_t(a.mass_stride));
+    for (int64_t j = max(m.first + m.count, int64_t(0)) + tid; j < end; j += kMoveThreads) mass[j] = 0.f;
+  }
+}
+
+// Up to 64 rows of a sequence and KV head, as a path has them: a workgroup reads all of them and writes them.
+// Bound by its chain: count, src, table, rows.
+constexpr uint32_t kFewMoves = 64;
+template <bool FP8>
+__global__ __launch_bounds__(kMoveThreads) void k_page_move_few(MoveArgs a) {
+  typedef typename Element<FP8>::type T;
+  constexpr uint32_t ROW = kPageDim * sizeof(T), PIECES = ROW / 16, ROWS = kMoveThreads / PIECES, NK = kFewMoves / ROWS;
+  constexpr uint32_t NV = kFewMoves * kPageDim / kMoveThreads;
+  __shared__ Move moves[kFewMoves];
+  const uint32_t tid = threadIdx.x, item = blockIdx.x;
+  const Moves m = moves_of(a, item);
+  if (tid < kFewMoves) moves[tid] = move_of(a, m, tid);
+  __syncthreads();
+  u32x4_t k[NK];
+#pragma unroll
+  for (uint32_t n = 0; n < NK; n++) {
+    const uint32_t i = n * ROWS + tid / PIECES;
+    if (n * ROWS < m.count && moves[i].from != kNoSlot)
+      k[n] = *reinterpret_cast<const u32x4_t*>(a.st.k + size_t(moves[i].from) * ROW + (tid % PIECES) * 16);
+  }
+  T* const pages = reinterpret_cast<T*>(a.st.v);
+  T v[NV];
+#pragma unroll
+  for (uint32_t n = 0; n < NV; n++) {
+    const uint32_t i = 2 * n + tid / kPageDim;
+    if (2 * n < m.count && moves[i].from != kNoSlot) v[n] = pages[v_at(moves[i].from, tid % kPageDim)];
+  }
+  wait_loads();
+  __syncthreads();
+#pragma unroll
+  for (uint32_t n = 0; n < NK; n++) {
+    const uint32_t i = n * ROWS + tid / PIECES;
+    if (n * ROWS < m.count && moves[i].from != kNoSlot)
+      *reinterpret_cast<u32x4_t*>(a.st.k + size_t(moves[i].to) * ROW + (tid % PIECES) * 16) = k[n];
+  }
+#pragma unroll
+  for (uint32_t n = 0; n < NV; n++) {
+    const uint32_t i = 2 * n + tid / kPageDim;
+    if (2 * n < m.count && moves[i].from != kNoSlot) pages[v_at(moves[i].to, tid % kPageDim)] = v[n];
+  }
+  move_rest<FP8, 1>(a, m, item);
+}
+
+// Many rows. Dims do not meet, so a sequence and KV head is shared by workgroups that have 64 bytes of each K row, or
+// 16 dims of V; one has what there is one of for a row. Rows ascend and only ever move to the front, so what a chunk
+// of rows writes no later chunk reads: within one everything is read before anything is written, and the next one's
+// reads are under way while it is written. Where the rows lie is found for 2048 of them at a time (src, then the
+// table: two load latencies, which a chunk would otherwise wait for). Workgroup (part, item): the parts of an item share
+// an XCD where the items are a multiple of 8.
+constexpr uint32_t kPlan = 2048, kChunk = 256, kSliceV = 16;
+template <bool FP8>
+constexpr uint32_t move_parts() { return kPageDim * (FP8 ? 1 : 2) / 64 + kPageDim / kSliceV + 1; }
+
+template <bool FP8>
+__global__ __launch_bounds__(kMoveThreads) void k_page_move(MoveArgs a, uint32_t items) {
+  typedef typename Element<FP8>::type T;
+  constexpr uint32_t ROW = kPageDim * sizeof(T), K_PARTS = ROW / 64, V_PARTS = kPageDim / kSliceV;
+  __shared__ uint32_t from[kPlan], to[kPlan];
+  const uint32_t tid = threadIdx.x, part = blockIdx.x / items, item = blockIdx.x - part * items;
+  const Moves m = moves_of(a, item);
+  // Rows p0 - lead .. of the plan, in chunks that are read one ahead.
+  auto run = [&](uint32_t lead, auto&& read, auto&& write, auto& v0, auto& v1) __attribute__((always_inline)) {
+    const uint32_t total = m.count + lead;
+    for (uint32_t p0 = 0; p0 < total; p0 += kPlan) {
+#pragma unroll
+      for (uint32_t n = 0; n < kPlan / kMoveThreads; n++) {
+        const uint32_t p = n * kMoveThreads + tid;
+        const Move w = p0 + p >= lead ? move_of(a, m, p0 + p - lead) : Move{kNoSlot, kNoSlot};
+        from[p] = w.from;
+        to[p] = w.to;
+      }
+      __syncthreads();
+      const uint32_t n = (min(total - p0, kPlan) + kChunk - 1) / kChunk;
+      read(v0, 0);
+      for (uint32_t c = 0; c < n; c += 2) {
+        wait_loads();
+        __syncthreads();  // chunk c has been read
+        if (c + 1 < n) read(v1, (c + 1) * kChunk);
+        write(v0, c * kChunk);
+        if (c + 1 == n) break;
+        wait_loads();
+        __syncthreads();
+        if (c + 2 < n) read(v0, (c + 2) * kChunk);
+        write(v1, (c + 1) * kChunk);
+      }
+      __syncthreads();  // the plan has been read
+    }
+  };
+  if (part < K_PARTS) {
+    constexpr uint32_t ROWS = kMoveThreads / 4, N = kChunk / ROWS;
+    uint8_t* const pages = a.st.k + part * 64 + (tid & 3) * 16;
+    struct Rows {
+      u32x4_t v[N];
+    } v0, v1;
+    run(0, [&](Rows& r, uint32_t at) __attribute__((always_inline)) {
+#pragma unroll
+          for (uint32_t n = 0; n < N; n++) {
+            const uint32_t x = from[at + n * ROWS + tid / 4];
+            if (x != kNoSlot) r.v[n] = *reinterpret_cast<const u32x4_t*>(pages + size_t(x) * ROW);
+          }
+        },
+        [&](const Rows& r, uint32_t at) __attribute__((always_inline)) {
+#pragma unroll
+          for (uint32_t n = 0; n < N; n++) {
+            const uint32_t x = to[at + n * ROWS + tid / 4];
+            if (x != kNoSlot) *reinterpret_cast<u32x4_t*>(pages + size_t(x) * ROW) = r.v[n];
+          }
+        }, v0, v1);
+  } else if (part < K_PARTS + V_PARTS) {
+    // runs of 16 positions as they lie in the pages: a thread has a dim of a run
+    const uint32_t at = tid / kSliceV * kPageRun, d = (part - K_PARTS) * kSliceV + tid % kSliceV;
+    T* const pages = reinterpret_cast<T*>(a.st.v);
+    struct Run {
+      T v[kPageRun];
+    } v0, v1;
+    run(uint32_t(m.first) & (kPageRun - 1),  // positions of the first run before the rows
+        [&](Run& r, uint32_t p) __attribute__((always_inline)) {
+#pragma unroll
+          for (uint32_t k = 0; k < kPageRun; k++) {
+            const uint32_t x = from[p + at + k];
+            r.v[k] = pages[v_at(x != kNoSlot ? x : 0, d)];
+          }
+        },
+        [&](const Run& r, uint32_t p) __attribute__((always_inline)) {
+          uint32_t have = 0, first = 0;
+#pragma unroll
+          for (uint32_t k = 0; k < kPageRun; k++) {
+            const uint32_t x = to[p + at + k];
+            if (x != kNoSlot) {
+              have |= 1u << k;
+              first = x & ~(kPageRun - 1);
+            }
+          }
+          if (!have) return;
+          T* const o = pages + v_at(first, d);
+          if (have == (1u << kPageRun) - 1) {
+            u32x4_t w[kPageRun * sizeof(T) / 16];
+#pragma unroll
+            for (uint32_t i = 0; i < kPageRun * sizeof(T) / 4; i++) {
+              w[i / 4][i % 4] = 0;
+#pragma unroll
+              for (uint32_t e = 0; e < 4 / sizeof(T); e++) w[i / 4][i % 4] |= uint32_t(r.v[i * (4 / sizeof(T)) + e]) << (8 * sizeof(T) * e);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kPageRun * sizeof(T) / 16; i++) reinterpret_cast<u32x4_t*>(o)[i] = w[i];
+          } else {
+#pragma unroll
+            for (uint32_t k = 0; k < kPageRun; k++)
+              if (have >> k & 1) o[k] = r.v[k];
+          }
+        }, v0, v1);
+  } else {
+    move_rest<FP8, 8>(a, m, item);
   }
 }
 
@@ -322,6 +503,8 @@ int qe_op_page_move(const qe_pages* pages, const int32_t* src, uint64_t src_head
   if (src_heads != 1 && src_heads != a.p.n_kv) return qe::set_error(QE_ERR_ARG, "src_heads must be 1 or n_kv_heads");
   if (src_stride == 0 || src_stride > 0x7FFFFFFFull || mass_stride > 0x7FFFFFFFull || (mass && mass_stride == 0))
     return qe::set_error(QE_ERR_ARG, "src_stride and mass_stride must be above 0 and below 2^31");
+  if (pages->n_pages > 0xFFFFFFFEull / (pages->page_size * pages->n_kv_heads))
+    return qe::set_error(QE_ERR_ARG, "need n_pages * n_kv_heads * page_size < 2^32 - 1");
   if (uint64_t(a.p.n_seqs) * a.p.n_kv >= 1u << 19) return qe::set_error(QE_ERR_ARG, "need n_seqs * n_kv_heads < 2^19");
   if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(count) | reinterpret_cast<uintptr_t>(first) |
        reinterpret_cast<uintptr_t>(mass)) % 4)
@@ -344,9 +527,14 @@ int qe_op_page_move(const qe_pages* pages, const int32_t* src, uint64_t src_head
   a.mass_stride = mass_stride;
   a.src_heads = uint32_t(src_heads);
   a.src_stride = uint32_t(src_stride);
-  const uint32_t grid = uint32_t(items) * 17;
-  (pages->kv_dtype == QE_KV_FP8 ? qe::k_page_move<true> : qe::k_page_move<false>)<<<grid, qe::kMoveThreads, 0,
-                                                                                     static_cast<hipStream_t>(stream)>>>(a);
+  const bool fp8 = pages->kv_dtype == QE_KV_FP8;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (src_stride <= qe::kFewMoves) {
+    (fp8 ? qe::k_page_move_few<true> : qe::k_page_move_few<false>)<<<uint32_t(items), qe::kMoveThreads, 0, st>>>(a);
+  } else {
+    const uint32_t grid = uint32_t(items) * (fp8 ? qe::move_parts<true>() : qe::move_parts<false>());
+    (fp8 ? qe::k_page_move<true> : qe::k_page_move<false>)<<<grid, qe::kMoveThreads, 0, st>>>(a, uint32_t(items));
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page move launch failed: %s", hipGetErrorString(e));
   return QE_OK;
