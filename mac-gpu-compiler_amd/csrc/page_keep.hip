@@ -352,12 +352,12 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move_few(MoveArgs a) {
 }
 
 // Many rows. Dims do not meet, so a sequence and KV head is shared by workgroups that have 64 bytes of each K row, or
-// 16 dims of V; one has what there is one of for a row. Rows ascend and only ever move to the front, so what a chunk
+// 8 dims of V; one has what there is one of for a row. Rows ascend and only ever move to the front, so what a chunk
 // of rows writes no later chunk reads: within one everything is read before anything is written, and the next one's
 // reads are under way while it is written. Where the rows lie is found for 2048 of them at a time (src, then the
 // table: two load latencies, which a chunk would otherwise wait for). Workgroup (part, item): the parts of an item share
 // an XCD where the items are a multiple of 8.
-constexpr uint32_t kPlan = 2048, kChunk = 256, kSliceV = 16;
+constexpr uint32_t kPlan = 2048, kSliceV = 8;
 template <bool FP8>
 constexpr uint32_t move_parts() { return kPageDim * (FP8 ? 1 : 2) / 64 + kPageDim / kSliceV + 1; }
 
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move(MoveArgs a, uint32_t
   const uint32_t tid = threadIdx.x, part = blockIdx.x / items, item = blockIdx.x - part * items;
   const Moves m = moves_of(a, item);
   // Rows p0 - lead .. of the plan, in chunks that are read one ahead.
-  auto run = [&](uint32_t lead, auto&& read, auto&& write, auto& v0, auto& v1) __attribute__((always_inline)) {
+  auto run = [&](uint32_t lead, uint32_t chunk, auto&& read, auto&& write, auto& v0, auto& v1) __attribute__((always_inline)) {
     const uint32_t total = m.count + lead;
     for (uint32_t p0 = 0; p0 < total; p0 += kPlan) {
 #pragma unroll
@@ -380,29 +380,29 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move(MoveArgs a, uint32_t
         to[p] = w.to;
       }
       __syncthreads();
-      const uint32_t n = (min(total - p0, kPlan) + kChunk - 1) / kChunk;
+      const uint32_t n = (min(total - p0, kPlan) + chunk - 1) / chunk;
       read(v0, 0);
       for (uint32_t c = 0; c < n; c += 2) {
         wait_loads();
         __syncthreads();  // chunk c has been read
-        if (c + 1 < n) read(v1, (c + 1) * kChunk);
-        write(v0, c * kChunk);
+        if (c + 1 < n) read(v1, (c + 1) * chunk);
+        write(v0, c * chunk);
         if (c + 1 == n) break;
         wait_loads();
         __syncthreads();
-        if (c + 2 < n) read(v0, (c + 2) * kChunk);
-        write(v1, (c + 1) * kChunk);
+        if (c + 2 < n) read(v0, (c + 2) * chunk);
+        write(v1, (c + 1) * chunk);
       }
       __syncthreads();  // the plan has been read
     }
   };
   if (part < K_PARTS) {
-    constexpr uint32_t ROWS = kMoveThreads / 4, N = kChunk / ROWS;
+    constexpr uint32_t ROWS = kMoveThreads / 4, N = 4;
     uint8_t* const pages = a.st.k + part * 64 + (tid & 3) * 16;
     struct Rows {
       u32x4_t v[N];
     } v0, v1;
-    run(0, [&](Rows& r, uint32_t at) __attribute__((always_inline)) {
+    run(0, ROWS * N, [&](Rows& r, uint32_t at) __attribute__((always_inline)) {
 #pragma unroll
           for (uint32_t n = 0; n < N; n++) {
             const uint32_t x = from[at + n * ROWS + tid / 4];
@@ -424,6 +424,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move(MoveArgs a, uint32_t
       T v[kPageRun];
     } v0, v1;
     run(uint32_t(m.first) & (kPageRun - 1),  // positions of the first run before the rows
+        kMoveThreads / kSliceV * kPageRun,
         [&](Run& r, uint32_t p) __attribute__((always_inline)) {
 #pragma unroll
           for (uint32_t k = 0; k < kPageRun; k++) {
