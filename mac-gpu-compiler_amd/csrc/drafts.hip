@@ -185,20 +185,10 @@ __device__ __forceinline__ uint32_t chunk_of(uint32_t& c0) {
   return c;
 }
 
-// Row blockIdx.y + ..., a chunk of it.
-template <int WAVES>
-__global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
-  constexpr int N = 32 / WAVES;
-  __shared__ ChunkSum shares[WAVES];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y + blockIdx.z * kRowsAcross;
-  uint32_t c0;
-  const uint32_t c = chunk_of<WAVES>(c0);
-  if (c >= a.chunks || r >= a.n_rows) return;
-  float x[N];
-  load_values(a.logits + r * a.stride, c0, a.vocab, -INFINITY, x);
-  const int32_t s = sequence(a, int32_t(r));
-  if (s < 0) return;
-  const float t = temperature(a, s);
+// What the wave's values x (of WAVES = 4: with the workgroup's other three waves') add up to; of wave 0.
+template <int WAVES, int N>
+__device__ __forceinline__ ChunkSum chunk_sum(const float (&x)[N], uint32_t c0, float t, ChunkSum* shares) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < N; i++) m = fmaxf(m, x[i]);
@@ -245,7 +235,24 @@ __global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
         at = min(at, shares[i].best);
       }
   }
-  if (lane == 0 && (WAVES == 1 || wave == 0)) a.sums[size_t(r) * a.chunks + c] = ChunkSum{sum, m, at};
+  return ChunkSum{sum, m, at};
+}
+
+// Row blockIdx.y + ..., a chunk of it.
+template <int WAVES>
+__global__ __launch_bounds__(256) void k_draft_sums(DraftArgs a) {
+  constexpr int N = 32 / WAVES;
+  __shared__ ChunkSum shares[WAVES];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.y + blockIdx.z * kRowsAcross;
+  uint32_t c0;
+  const uint32_t c = chunk_of<WAVES>(c0);
+  if (c >= a.chunks || r >= a.n_rows) return;
+  float x[N];
+  load_values(a.logits + r * a.stride, c0, a.vocab, -INFINITY, x);
+  const int32_t s = sequence(a, int32_t(r));
+  if (s < 0) return;
+  const ChunkSum sum = chunk_sum<WAVES>(x, c0, temperature(a, s), shares);
+  if (lane == 0 && (WAVES == 1 || wave == 0)) a.sums[size_t(r) * a.chunks + c] = sum;
 }
 
 // ---- a workgroup's draw ----
@@ -308,9 +315,11 @@ __device__ __forceinline__ void load_rests(const DraftArgs& a, uint32_t s, doubl
 
 // The token of row d.row whose running weight goes above `to`, by the thread that has it, into packed row
 // at_row; a thread has N tokens from i0 on, with weights z and logits y.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <int N>
 __device__ __forceinline__ void place_token(const DraftArgs& a, const DrawRow& d, uint32_t at_row, uint32_t i0, const double (&z)[N],
-                                            const float (&y)[N], double to, float t, Scratch& sc) {
+                                            f32x4 y, double to, float t, Scratch& sc) {
+  static_assert(N == 4, "y holds 4");
   const float* x = a.logits + d.row * a.stride;
   const uint32_t tid = threadIdx.x;
   double mine = 0.0;
@@ -338,11 +347,9 @@ __device__ __forceinline__ void place_token(const DraftArgs& a, const DrawRow& d
   const uint32_t owner = first != kNone ? first : final;
   if (tid == (owner == kNone ? 0 : owner)) {
     double inner;
-    uint32_t at = pick(z, up_to - mine, to, inner), token = i0 + at;
-    float logit = y[0];
-#pragma unroll
-    for (int e = 1; e < N; e++)
-      if (at == uint32_t(e)) logit = y[e];
+    const uint32_t at = pick(z, up_to - mine, to, inner);
+    uint32_t token = i0 + at;
+    float logit = at == 0 ? y[0] : at == 1 ? y[1] : at == 2 ? y[2] : y[3];
     if (owner == kNone) {
       token = d.best;
       logit = x[token];
@@ -402,7 +409,7 @@ __device__ __forceinline__ void draw(const DraftArgs& a, const DrawRow& d, bool 
     c = find_chunk(w, n, share, before);
   }
   double z[N];
-  float y[N];
+  f32x4 y;
   const uint32_t i0 = c * kChunk + tid * N;
   const double to = aim - before;
 #pragma unroll
@@ -597,17 +604,21 @@ __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
 }
 
 // ---- trees ----
+// Where a walk is: at node `cur` of depth `depth`, or (done) it ended there.
+struct Walk {
+  uint32_t cur, depth, done, pad;
+};
 struct TreeArgs {
-  DraftArgs d;  // drafts: the nodes' tokens
+  DraftArgs d;  // drafts: the nodes' tokens; sums: [n_rows][chunks], or by level: [2][n_seqs][chunks]
   const int32_t* parents;
   int32_t* path;  // [n_seqs][QE_TREE_NODES]
+  Walk* walks;    // by level: [2][n_seqs]
   uint32_t max_depth;
 };
 
 // The sum of a row's weights from its chunks' sums, and what a draw needs of it, by each wave for itself.
-__device__ __forceinline__ DrawRow row_of(const DraftArgs& a, uint32_t r, float t) {
+__device__ __forceinline__ DrawRow row_of(const DraftArgs& a, const ChunkSum* sums, uint32_t r, float t) {
   const uint32_t lane = threadIdx.x & 63;
-  const ChunkSum* const sums = a.sums + size_t(r) * a.chunks;
   DrawRow d;
   d.k = rate(t);
   d.row = r;
@@ -639,59 +650,137 @@ __device__ __forceinline__ double row_weight(const DrawRow& d, uint32_t i, float
   return d.greedy ? (i == d.best ? 1.0 : 0.0) : weight(x, d.top, d.k);
 }
 
-// A workgroup per sequence walks its tree: every wave has a node a lane and walks for itself, and all of them
-// draw at the end.
-__global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree) {
+// The nodes of a sequence, one a lane; rows r0 .. r1 - 1.
+struct Nodes {
+  int64_t r0, r1;
+  int32_t parent;
+  uint32_t token;
+  float accept, t;  // t: the sequence's temperature
+};
+__device__ __forceinline__ Nodes nodes_of(const TreeArgs& tree, uint32_t s) {
+  const DraftArgs& a = tree.d;
+  const uint32_t lane = threadIdx.x & 63;
+  Nodes n;
+  n.r0 = max(a.starts[s], 0);
+  n.r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
+  const bool node = lane < n.r1 - n.r0;
+  n.parent = node ? tree.parents[n.r0 + lane] : -1;
+  n.token = node ? a.drafts[n.r0 + lane] : kNone;
+  n.accept = node ? a.accept[n.r0 + lane] : 0.f;
+  n.t = temperature(a, s);
+  return n;
+}
+
+// One step of a walk by each wave for itself: the first child of node `cur` that is accepted, or kNone. d: cur's row;
+// tried: the children; w: their tokens' weights, 0 for a token tried before.
+__device__ __forceinline__ uint32_t next_node(const TreeArgs& tree, const Nodes& n, uint32_t cur, uint32_t depth, const DrawRow& d,
+                                              uint64_t& tried, double& w) {
+  const DraftArgs& a = tree.d;
+  const uint32_t lane = threadIdx.x & 63;
+  const bool child = depth < tree.max_depth && lane > cur && n.parent == int32_t(cur);
+  tried = __ballot(child);
+  w = child && n.token < a.vocab ? row_weight(d, n.token, a.logits[d.row * a.stride + n.token]) : 0.0;
+  double left = 1.0;
+  for (uint64_t rest = tried; rest; rest &= rest - 1) {
+    const int c = __builtin_ctzll(rest);
+    const uint32_t is = from_lane(n.token, c);
+    const uint64_t before = __ballot(child && n.token == is) & ((1ull << c) - 1);
+    if (before && int(lane) == c) w = 0.0;
+    const double p = from_lane(w, c) * d.inv_total;
+    if (double(from_lane(n.accept, c)) * left < p) return uint32_t(c);
+    left -= p;
+  }
+  return kNone;
+}
+// What an accepted child leaves: its token, at depth `depth` of the path before it.
+__device__ __forceinline__ void take_node(const TreeArgs& tree, const Nodes& n, const DrawRow& d, uint32_t depth, uint32_t next) {
+  const DraftArgs& a = tree.d;
+  const uint32_t token = from_lane(n.token, int(next));
+  a.tokens[n.r0 + depth] = token;
+  if (a.logprobs) a.logprobs[n.r0 + depth] = log_weight(d, a.logits[d.row * a.stride + token], n.t);
+}
+
+// Level `level` of the walks, of trees too large for every row's sums: the workgroups of a sequence, one or four chunks
+// each as k_draft_sums has them, all take the step from the level before, and then sum the row it led to. So a level
+// is one launch and reads one row a sequence.
+template <int WAVES>
+__global__ __launch_bounds__(256) void k_tree_level(TreeArgs tree, uint32_t level) {
+  constexpr int N = 32 / WAVES;
+  __shared__ ChunkSum shares[WAVES];
+  const DraftArgs& a = tree.d;
+  const uint32_t s = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t c0;
+  const uint32_t c = chunk_of<WAVES>(c0);
+  const bool first = blockIdx.x == 0;
+  const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
+  if (r1 <= r0) return;
+  uint32_t cur = 0;
+  if (level) {
+    const Walk at = tree.walks[(level - 1 & 1) * a.n_seqs + s];
+    uint32_t next = kNone;
+    if (!at.done) {
+      const Nodes n = nodes_of(tree, s);
+      const DrawRow d = row_of(a, a.sums + (size_t(level - 1 & 1) * a.n_seqs + s) * a.chunks, uint32_t(r0) + at.cur, n.t);
+      uint64_t tried;
+      double w;
+      next = next_node(tree, n, at.cur, at.depth, d, tried, w);
+      if (first && threadIdx.x == 0 && next != kNone) {
+        take_node(tree, n, d, at.depth, next);
+        tree.path[size_t(s) * QE_TREE_NODES + level] = int32_t(next);
+      }
+    }
+    if (first && threadIdx.x == 0)
+      tree.walks[(level & 1) * a.n_seqs + s] = next != kNone ? Walk{next, level, 0, 0} : Walk{at.cur, at.depth, 1, 0};
+    if (next == kNone) return;
+    cur = next;
+  } else if (first && threadIdx.x == 0) {
+    tree.walks[s] = Walk{0, 0, 0, 0};
+  }
+  ChunkSum sum;
+  const uint32_t r = uint32_t(r0) + cur;
+  if (c >= a.chunks) return;  // (a wave that shares nothing, or, of WAVES > 1, none)
+  float x[N];
+  load_values(a.logits + r * a.stride, c0, a.vocab, -INFINITY, x);
+  sum = chunk_sum<WAVES>(x, c0, temperature(a, s), shares);
+  if (lane == 0 && (WAVES == 1 || wave == 0)) a.sums[(size_t(level & 1) * a.n_seqs + s) * a.chunks + c] = sum;
+}
+
+// A workgroup per sequence walks its tree (LEVELS: it is where k_tree_level left it, and only draws): every wave walks
+// for itself, and all of them draw at the end.
+template <bool LEVELS>
+__global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_t levels) {
   constexpr int N = kChunk / kThreads;
   __shared__ Scratch sc;
   const DraftArgs& a = tree.d;
   const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int64_t r0 = max(a.starts[s], 0), r1 = min(int64_t(a.starts[s + 1]), int64_t(a.n_rows));
   int32_t* const path = tree.path + size_t(s) * QE_TREE_NODES;
+  const Nodes nodes = nodes_of(tree, s);
+  const int64_t r0 = nodes.r0, r1 = nodes.r1;
   if (r1 <= r0) {
     if (tid == 0) a.count[s] = 0;
     if (tid < QE_TREE_NODES) path[tid] = -1;
     return;
   }
-  const float t = temperature(a, s);
-  const bool node = lane < r1 - r0;
-  const int32_t parent = node ? tree.parents[r0 + lane] : -1;
-  const uint32_t token = node ? a.drafts[r0 + lane] : kNone;
-  const float accept = node ? a.accept[r0 + lane] : 0.f;
-  uint32_t cur = 0, depth = 0, mine = lane == 0 ? 0u : kNone;  // mine: the path's row at depth `lane`
+  const float t = nodes.t;
+  const uint32_t token = nodes.token;
+  Walk at{};
+  if constexpr (LEVELS) at = tree.walks[(levels - 1 & 1) * a.n_seqs + s];
+  uint32_t cur = at.cur, depth = at.depth, mine = lane == 0 ? 0u : kNone;  // mine: the path's row at depth `lane`
   DrawRow d;
-  uint64_t tried;  // children of the last node
-  double w = 0.0;  // their tokens' weights, 0 for a token tried before
+  const ChunkSum* sums;
+  uint64_t tried;
+  double w;
   while (true) {
-    d = row_of(a, uint32_t(r0) + cur, t);
-    const bool child = depth < tree.max_depth && lane > cur && parent == int32_t(cur);
-    tried = __ballot(child);
-    if (!tried) break;
-    w = child && token < a.vocab ? row_weight(d, token, a.logits[d.row * a.stride + token]) : 0.0;
-    double left = 1.0;
-    uint32_t next = kNone;
-    for (uint64_t rest = tried; rest; rest &= rest - 1) {
-      const int c = __builtin_ctzll(rest);
-      const uint32_t is = from_lane(token, c);
-      const uint64_t before = __ballot(child && token == is) & ((1ull << c) - 1);
-      if (before && int(lane) == c) w = 0.0;
-      const double p = from_lane(w, c) * d.inv_total;
-      if (double(from_lane(accept, c)) * left < p) {
-        next = uint32_t(c);
-        break;
-      }
-      left -= p;
-    }
-    if (next == kNone) break;
-    const float x = a.logits[d.row * a.stride + from_lane(token, int(next))];
-    if (tid == 0) {
-      a.tokens[r0 + depth] = from_lane(token, int(next));
-      if (a.logprobs) a.logprobs[r0 + depth] = log_weight(d, x, t);
-    }
+    sums = a.sums + (LEVELS ? size_t(depth & 1) * a.n_seqs + s : size_t(r0) + cur) * a.chunks;
+    d = row_of(a, sums, uint32_t(r0) + cur, t);
+    const uint32_t next = next_node(tree, nodes, cur, depth, d, tried, w);
+    if (LEVELS || next == kNone) break;
+    if (tid == 0) take_node(tree, nodes, d, depth, next);
     depth++;
     if (lane == depth) mine = next;
     cur = next;
   }
+  if (LEVELS && lane > 0 && lane <= depth) mine = uint32_t(path[lane]);
   if (tid < QE_TREE_NODES) path[tid] = int32_t(mine);
   if (tid == 0) a.count[s] = depth + 1;
   for (int64_t e = r0 + depth + 1 + tid; e < r1; e += kThreads) {
@@ -706,7 +795,7 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree) {
     for (int i = 0; i < kLaneChunks; i++) {
       chunk[i] = 0.0;
       if (uint32_t(i) < n && c0 + i < a.chunks) {
-        const ChunkSum z = a.sums[size_t(d.row) * a.chunks + c0 + i];
+        const ChunkSum z = sums[c0 + i];
         if (d.greedy) chunk[i] = d.best / kChunk == c0 + i ? 1.0 : 0.0;
         else chunk[i] = z.sum * chunk_scale(z.top, d.top, d.k);
       }
@@ -729,7 +818,7 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree) {
     c = find_chunk(chunk, n, share, before);
   }
   double z[N];
-  float y[N];
+  f32x4 y;
   const uint32_t i0 = c * kChunk + tid * N;
 #pragma unroll
   for (int e = 0; e < N; e++) {
@@ -759,6 +848,13 @@ DraftWork draft_work(uint64_t n_rows, uint64_t n_seqs, uint64_t vocab) {
   w.draws = w.rests + n_seqs * w.chunks * sizeof(double);
   w.bytes = w.draws + n_seqs * sizeof(DrawRow);
   return w;
+}
+
+static_assert(2 * sizeof(Walk) <= sizeof(DrawRow), "a check by levels keeps its walks where draws lie");
+// Whether a check goes level by level, a launch each (7 us a level that some sequence reaches, 3 below), and reads one row
+// a level and sequence, or sums all rows first (8 KB a chunk at 4.8 TB/s).
+bool by_levels(uint64_t n_rows, uint64_t n_seqs, uint64_t chunks, uint64_t levels) {
+  return n_rows >= 2 * n_seqs && double(n_rows * chunks) * 8192 / 4.8e6 > 7.0 * double(levels);
 }
 
 }  // namespace
@@ -871,13 +967,22 @@ int qe_op_verify_tree(const float* logits, uint64_t n_rows, uint64_t vocab, uint
   a.path = path_out;
   a.max_depth = max_depth && max_depth < QE_TREE_NODES ? uint32_t(max_depth) : QE_TREE_NODES - 1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n_rows) {
-    const bool few = n_rows * w.chunks <= qe::kFewChunks;
-    const uint32_t y = a.d.n_rows < qe::kRowsAcross ? a.d.n_rows : qe::kRowsAcross;
-    const dim3 grid(few ? a.d.chunks : qe::ceil_div(a.d.chunks, 4u), y, qe::ceil_div(a.d.n_rows, qe::kRowsAcross));
-    (few ? qe::k_draft_sums<4> : qe::k_draft_sums<1>)<<<grid, 256, 0, st>>>(a.d);
+  const uint64_t levels = a.max_depth + 1;
+  if (qe::by_levels(n_rows, n_seqs, w.chunks, levels)) {
+    a.walks = reinterpret_cast<qe::Walk*>(base + w.draws);
+    const bool few = n_seqs * w.chunks <= qe::kFewChunks;
+    const dim3 grid(few ? a.d.chunks : qe::ceil_div(a.d.chunks, 4u), a.d.n_seqs);
+    for (uint32_t l = 0; l < levels; l++) (few ? qe::k_tree_level<4> : qe::k_tree_level<1>)<<<grid, 256, 0, st>>>(a, l);
+    qe::k_tree_decide<true><<<a.d.n_seqs, qe::kThreads, 0, st>>>(a, uint32_t(levels));
+  } else {
+    if (n_rows) {
+      const bool few = n_rows * w.chunks <= qe::kFewChunks;
+      const uint32_t y = a.d.n_rows < qe::kRowsAcross ? a.d.n_rows : qe::kRowsAcross;
+      const dim3 grid(few ? a.d.chunks : qe::ceil_div(a.d.chunks, 4u), y, qe::ceil_div(a.d.n_rows, qe::kRowsAcross));
+      (few ? qe::k_draft_sums<4> : qe::k_draft_sums<1>)<<<grid, 256, 0, st>>>(a.d);
+    }
+    qe::k_tree_decide<false><<<a.d.n_seqs, qe::kThreads, 0, st>>>(a, 0);
   }
-  qe::k_tree_decide<<<a.d.n_seqs, qe::kThreads, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "verify tree launch failed: %s", hipGetErrorString(e));
   return QE_OK;

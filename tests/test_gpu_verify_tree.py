@@ -214,3 +214,33 @@ def test_many_trees(gpu):
     np.testing.assert_array_equal(got[1][:, 1], np.where(one, 1, np.where(two, 2, -1)))
     np.testing.assert_array_equal(got[0][::3], best[::3])
     np.testing.assert_array_equal(got[0][1::3], np.where(one, best[1::3], np.where(two, best[2::3], NONE)))
+
+
+@pytest.mark.parametrize("max_depth,n", [(1, 8), (3, 12), (7, 18)])
+def test_large_trees_level_by_level(gpu, max_depth, n):
+    """so many rows that the check goes from level to level instead of summing all of them; trees that end at
+    every depth, single roots, no rows, more rows than a tree has, greedy ones, rows that are not finite"""
+    rng = np.random.default_rng([n, 5])
+    vocab = 70001
+    sizes = [64, 1, 0, 80, 64, 2] + [64] * (n - 6)
+    starts = np.concatenate([[1], 1 + np.cumsum(sizes)])
+    rows = starts[-1] + 2
+    parents = np.full(rows, -1)
+    for s, m in enumerate(sizes):
+        parents[starts[s]:starts[s] + m] = random_tree(m, s, width=4)
+    x = rng.standard_normal((rows, vocab), dtype=np.float32) * 2
+    nodes = rng.integers(0, vocab, rows).astype(np.uint32)
+    for a, b in zip(starts[:-1], starts[1:]):
+        seen = {}
+        for i in range(a, b):
+            p = parents[i]
+            if 0 <= p < i - a:
+                rank = seen[p] = seen.get(p, -1) + 1
+                if rank < 3 and rng.random() < 0.9:
+                    x[a + p, nodes[i]] = 14.0 - rank
+    x[starts[0], 5::7] = np.nan
+    x[starts[4], 100:200] = np.inf
+    nodes[starts[4] + 1] = 150
+    temps = np.array([(0.7, 1.0, 0.0, 1.3, 0.9)[i % 5] for i in range(n)], np.float32)
+    count = check(x, starts, parents, nodes, rng.random(rows, np.float32), rng.random(n, np.float32), temps, max_depth)
+    assert count.max() > 1
