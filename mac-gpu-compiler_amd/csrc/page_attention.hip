@@ -145,15 +145,20 @@ __device__ __forceinline__ int32_t tile_row_position(const A& a, const Seq& q, u
 }
 
 // ---- trees ----
-// Of each node of sequence q, bit i: node i is the node itself or one of its ancestors; into kin[kNodes] of the calling
-// wave. Lane i has node i: after n rounds its word holds its 2^n nearest, and `at` is the next one above.
-__device__ __forceinline__ void find_families(const TreeAttnArgs& a, const Seq& q, uint64_t* kin) {
-  const uint32_t lane = threadIdx.x & 63, n = token_of(a, q.rows);
-  uint32_t at = lane;
-  if (lane < n) {
-    const int32_t parent = a.parents[uint32_t(q.row0) + lane];
-    if (uint32_t(parent) < lane) at = uint32_t(parent);
+// The parent of the lane's node of sequence q.
+template <class A>
+__device__ __forceinline__ int32_t load_parent(const A& a, const Seq& q) {
+  if constexpr (A::kTree) {
+    const uint32_t lane = threadIdx.x & 63;
+    if (lane < token_of(a, q.rows)) return a.parents[uint32_t(q.row0) + lane];
   }
+  return -1;
+}
+// Of each node of a sequence, bit i: node i is the node itself or one of its ancestors; into kin[kNodes] of the calling
+// wave. Lane i has node i: after n rounds its word holds its 2^n nearest, and `at` is the next one above.
+__device__ __forceinline__ void find_families(int32_t parent, uint64_t* kin) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t at = uint32_t(parent) < lane ? uint32_t(parent) : lane;
   uint32_t lo = lane < 32 ? 1u << lane : 0, hi = lane < 32 ? 0 : 1u << (lane - 32);
 #pragma unroll
   for (int i = 0; i < 6; i++) {
@@ -433,7 +438,7 @@ __device__ __forceinline__ uint32_t find_part(A& a, uint32_t w, uint32_t W, uint
 // How many of the workgroups of an item's n parts join it: more than one where a row's 16 threads would have more
 // than two rounds of parts. Small tiles: they share the rows; large ones (R >= 128): the dims, a power of two of them.
 __device__ __forceinline__ uint32_t joiners(uint32_t n, uint32_t rows, uint32_t R) {
-  if (R < 128) return n * min(rows, 16u) > 128 ? min(n, 16u) : 1;
+  if (R <= 32) return n * min(rows, 16u) > 128 ? min(n, 16u) : 1;
   return n > 64 ? 16 : n > 32 ? 8 : n > 16 ? 4 : 1;
 }
 
@@ -668,7 +673,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
     // the least position any row attends up to: below it no score is masked
     const int32_t free_to = free_position(a, cu.q, cu.tile * R, cu.tile * R + rows);
     const bool one_token = token_of(a, cu.tile * R) == token_of(a, cu.tile * R + rows - 1);
-    if constexpr (TREE) find_families(a, cu.q, kin[wave]);
+    const int32_t parent = load_parent(a, cu.q);  // (worked on when the first K and V are under way)
     auto family_of = [&](int n) __attribute__((always_inline)) {  // of the lane's row of group n (those that attend nothing: any)
       return kin[TREE ? wave : 0][TREE ? min(token_of(a, cu.tile * R + 16 * n + col), kNodes - 1) : 0];
     };
@@ -840,6 +845,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
       look_up(x, kp, vp);
       load(d0, x, kp, vp);
       look_up(x + 4 * KEYS, kp, vp);
+      if constexpr (TREE) find_families(parent, kin[wave]);
       while (true) {
         // (past the end the loads of a step are of pages that are there, and unused)
         load(d1, x + 4 * KEYS, kp, vp);
@@ -954,7 +960,7 @@ __global__ __launch_bounds__(256, BF16_ROWS && NQ == 1 ? 2 : 1) void k_page_attn
 template <bool FP8, bool BF16_ROWS, int WAVES, class A>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(A a) {
   constexpr bool TREE = A::kTree;
-  static_assert(BF16_ROWS || WAVES == 8, "f32 rows: 8 waves of 16");
+  static_assert(BF16_ROWS || WAVES == 8 || TREE, "causal f32 rows: 8 waves of 16");
   constexpr int NS = BF16_ROWS ? 1 : 3, WR = BF16_ROWS ? 32 : 16, R = WR * WAVES;
   constexpr int NJ = BF16_ROWS ? 8 : 4, NSUM = BF16_ROWS ? 16 : 8;  // fragments of a row of q; 4 dims of the sums each
   typedef typename std::conditional<BF16_ROWS, f32x16, f32x4>::type Acc;
@@ -996,7 +1002,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(A a) {
     const uint32_t fresh = afresh(tid & 63), r = wr0 + (fresh & (WR - 1));
     const bool real = (fresh & (WR - 1)) < wrows;
     const int32_t row_pos = real ? tile_row_position(a, cu.q, r) : -1;
-    if constexpr (TREE) find_families(a, cu.q, kin[wave]);
+    const int32_t parent = load_parent(a, cu.q);  // (worked on when the first blocks are under way)
     auto family = [&] __attribute__((always_inline)) {  // of the lane's row (one that attends nothing: any)
       return kin[TREE ? wave : 0][TREE ? min(token_of(a, wr0 + (afresh(tid) & (WR - 1))), kNodes - 1) : 0];
     };
@@ -1267,6 +1273,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_page_attn_tiles(A a) {
     if (first < last) {
       fetch(first, 0, page0);
       if (!FP8 && STAGES == 3 && first + kBlock < last) fetch(first + kBlock, 1, page1);
+      if constexpr (TREE) find_families(parent, kin[wave]);
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -1548,6 +1555,8 @@ uint64_t attention_work_bytes(uint64_t n_heads, uint64_t n_kv_heads, uint64_t ma
 template <class A>
 void launch(const A& a, uint32_t R, uint32_t grid, bool fp8, bool bf16, hipStream_t st) {
   auto go = [&](auto* kern) { kern<<<grid, R == 256 || (R == 128 && !bf16) ? 512 : 256, 0, st>>>(a); };
+  if constexpr (A::kTree)
+    if (R == 64) return go(fp8 ? k_page_attn_tiles<true, false, 4, A> : k_page_attn_tiles<false, false, 4, A>);
   if (R == 256) {
     go(fp8 ? k_page_attn_tiles<true, true, 8, A> : k_page_attn_tiles<false, true, 8, A>);
   } else if (R == 128) {
@@ -1596,7 +1605,7 @@ int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* o
   if (parents && overlap(rows, span(parents, 4 * n_rows, 4 * n_rows, 1)))
     return set_error(QE_ERR_ARG, "out must not overlap parents");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool bf16 = dtype == QE_KV_BF16;
+  const bool bf16 = dtype == QE_KV_BF16, tree = parents;
   a.q = static_cast<const uint8_t*>(q);
   a.out = static_cast<uint8_t*>(out);
   a.q_stride = q_stride;
@@ -1611,21 +1620,23 @@ int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* o
   a.parts = reinterpret_cast<float*>(a.joints + kWorkgroups);
   // (fewer rows than max_new says need no more than the work that was asked for)
   const uint64_t bound = max_new && max_new < n_rows ? max_new : n_rows;
-  const Cut c = cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
+  Cut c = cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
+  // f32 rows of trees that fill half a tile: four waves of 16 rows and two workgroups on a CU
+  if (tree && c.rows == 128 && !bf16 && bound * a.group <= 64) c = {64, kWorkgroups};
   const uint32_t R = c.rows, grid = c.workgroups;
   a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= kWholeItems;
   a.join = !a.whole_items;
-  if (parents) {
-    TreeAttnArgs tree{a};
-    tree.parents = parents;
-    launch(tree, R, grid, fp8, bf16, st);
+  if (tree) {
+    TreeAttnArgs trees{a};
+    trees.parents = parents;
+    launch(trees, R, grid, fp8, bf16, st);
   } else {
     launch(a, R, grid, fp8, bf16, st);
   }
   if (a.join) {
     const dim3 join(grid, R / 16);
     auto join_by = [&](auto* kern) { kern<<<join, 256, 0, st>>>(a, R); };
-    if (R >= 128) join_by(bf16 ? k_page_join<true, true> : k_page_join<false, true>);
+    if (R > 32) join_by(bf16 ? k_page_join<true, true> : k_page_join<false, true>);
     else join_by(bf16 ? k_page_join<true, false> : k_page_join<false, false>);
   }
   const hipError_t e = hipGetLastError();
