@@ -1621,8 +1621,16 @@ int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* o
   // (fewer rows than max_new says need no more than the work that was asked for)
   const uint64_t bound = max_new && max_new < n_rows ? max_new : n_rows;
   Cut c = cut_of(bound, a.group, bf16, uint64_t(a.p.n_seqs) * a.p.n_kv);
-  // f32 rows of trees that fill half a tile: four waves of 16 rows and two workgroups on a CU
-  if (tree && c.rows == 128 && !bf16 && bound * a.group <= 64) c = {64, kWorkgroups};
+  if (tree) {
+    const uint64_t most = bound * a.group;
+    // short tables, few items: tiles of 16 rows, which read K and V again but share the work among more workgroups
+    if (pages->table_stride * pages->page_size <= kWholeItems &&
+        uint64_t(a.p.n_seqs) * a.p.n_kv * ((most + 15) / 16) <= kWorkgroups)
+      c = {16, kWorkgroups};
+    // f32 rows that fill half a tile: four waves of 16 rows and two workgroups on a CU
+    else if (c.rows == 128 && !bf16 && most <= 64)
+      c = {64, kWorkgroups};
+  }
   const uint32_t R = c.rows, grid = c.workgroups;
   a.whole_items = R <= 32 && pages->table_stride * pages->page_size <= kWholeItems;
   a.join = !a.whole_items;
