@@ -619,27 +619,40 @@ struct TreeArgs {
 // The sum of a row's weights from its chunks' sums, and what a draw needs of it, by each wave for itself.
 __device__ __forceinline__ DrawRow row_of(const DraftArgs& a, const ChunkSum* sums, uint32_t r, float t) {
   const uint32_t lane = threadIdx.x & 63;
+  ChunkSum z[2];  // (the first 128 chunks: most vocabularies' all)
+#pragma unroll
+  for (uint32_t e = 0; e < 2; e++) z[e] = sums[min(lane + 64 * e, a.chunks - 1)];
   DrawRow d;
   d.k = rate(t);
   d.row = r;
   d.draft = kNone;
   float top = -INFINITY;
-  for (uint32_t c = lane; c < a.chunks; c += 64) top = fmaxf(top, sums[c].top);
+#pragma unroll
+  for (uint32_t e = 0; e < 2; e++) {
+    if (lane + 64 * e >= a.chunks) z[e] = ChunkSum{0.0, -INFINITY, kNone};
+    top = fmaxf(top, z[e].top);
+  }
+  for (uint32_t c = lane + 128; c < a.chunks; c += 64) top = fmaxf(top, sums[c].top);
   d.top = wave_max(top);
   d.greedy = !(t > 0.f) || !(d.top > -INFINITY);
   uint32_t best = kNone;
   double sum = 0.0;
-  for (uint32_t c = lane; c < a.chunks; c += 64) {
-    const ChunkSum z = sums[c];
+  auto add = [&](const ChunkSum& z) __attribute__((always_inline)) {
     if (d.greedy) {
       if (z.top == d.top) best = min(best, z.best);
     } else if (z.top > -INFINITY) {
       sum += z.sum * chunk_scale(z.top, d.top, d.k);
     }
-  }
+  };
 #pragma unroll
-  for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
-  d.best = best < a.vocab && d.top > -INFINITY && d.greedy ? best : 0;
+  for (uint32_t e = 0; e < 2; e++) add(z[e]);
+  for (uint32_t c = lane + 128; c < a.chunks; c += 64) add(sums[c]);
+  d.best = 0;
+  if (d.greedy) {
+#pragma unroll
+    for (int e = 1; e < 64; e *= 2) best = min(best, uint32_t(__shfl_xor(int(best), e)));
+    if (best < a.vocab && d.top > -INFINITY) d.best = best;
+  }
   d.total = d.greedy ? 1.0 : wave_sum64(sum);
   d.inv_total = 1.0 / d.total;
   return d;
@@ -671,15 +684,23 @@ __device__ __forceinline__ Nodes nodes_of(const TreeArgs& tree, uint32_t s) {
   return n;
 }
 
-// One step of a walk by each wave for itself: the first child of node `cur` that is accepted, or kNone. d: cur's row;
-// tried: the children; w: their tokens' weights, 0 for a token tried before.
-__device__ __forceinline__ uint32_t next_node(const TreeArgs& tree, const Nodes& n, uint32_t cur, uint32_t depth, const DrawRow& d,
-                                              uint64_t& tried, double& w) {
+// Whether the lane's node is tried after node `cur` of depth `depth`, and its token's logit there (loaded before the
+// row's sums are waited for).
+__device__ __forceinline__ bool is_child(const TreeArgs& tree, const Nodes& n, uint32_t cur, uint32_t depth, float& x) {
   const DraftArgs& a = tree.d;
   const uint32_t lane = threadIdx.x & 63;
   const bool child = depth < tree.max_depth && lane > cur && n.parent == int32_t(cur);
+  x = child && n.token < a.vocab ? a.logits[uint64_t(n.r0 + cur) * a.stride + n.token] : 0.f;
+  return child;
+}
+// One step of a walk by each wave for itself: the first child that is accepted, or kNone. d: the node's row; child, x:
+// is_child's; tried: the children; w: their tokens' weights, 0 for a token tried before.
+__device__ __forceinline__ uint32_t next_node(const TreeArgs& tree, const Nodes& n, const DrawRow& d, bool child, float x,
+                                              uint64_t& tried, double& w) {
+  const DraftArgs& a = tree.d;
+  const uint32_t lane = threadIdx.x & 63;
   tried = __ballot(child);
-  w = child && n.token < a.vocab ? row_weight(d, n.token, a.logits[d.row * a.stride + n.token]) : 0.0;
+  w = child && n.token < a.vocab ? row_weight(d, n.token, x) : 0.0;
   double left = 1.0;
   for (uint64_t rest = tried; rest; rest &= rest - 1) {
     const int c = __builtin_ctzll(rest);
@@ -692,12 +713,11 @@ __device__ __forceinline__ uint32_t next_node(const TreeArgs& tree, const Nodes&
   }
   return kNone;
 }
-// What an accepted child leaves: its token, at depth `depth` of the path before it.
-__device__ __forceinline__ void take_node(const TreeArgs& tree, const Nodes& n, const DrawRow& d, uint32_t depth, uint32_t next) {
+// What an accepted child leaves: its token, at depth `depth` of the path before it; by the lane that has it.
+__device__ __forceinline__ void take_node(const TreeArgs& tree, const Nodes& n, const DrawRow& d, uint32_t depth, float x) {
   const DraftArgs& a = tree.d;
-  const uint32_t token = from_lane(n.token, int(next));
-  a.tokens[n.r0 + depth] = token;
-  if (a.logprobs) a.logprobs[n.r0 + depth] = log_weight(d, a.logits[d.row * a.stride + token], n.t);
+  a.tokens[n.r0 + depth] = n.token;
+  if (a.logprobs) a.logprobs[n.r0 + depth] = log_weight(d, x, n.t);
 }
 
 // Level `level` of the walks, of trees too large for every row's sums: the workgroups of a sequence, one or four chunks
@@ -720,12 +740,14 @@ __global__ __launch_bounds__(256) void k_tree_level(TreeArgs tree, uint32_t leve
     uint32_t next = kNone;
     if (!at.done) {
       const Nodes n = nodes_of(tree, s);
+      float x;
+      const bool child = is_child(tree, n, at.cur, at.depth, x);
       const DrawRow d = row_of(a, a.sums + (size_t(level - 1 & 1) * a.n_seqs + s) * a.chunks, uint32_t(r0) + at.cur, n.t);
       uint64_t tried;
       double w;
-      next = next_node(tree, n, at.cur, at.depth, d, tried, w);
-      if (first && threadIdx.x == 0 && next != kNone) {
-        take_node(tree, n, d, at.depth, next);
+      next = next_node(tree, n, d, child, x, tried, w);
+      if (first && threadIdx.x == next) {
+        take_node(tree, n, d, at.depth, x);
         tree.path[size_t(s) * QE_TREE_NODES + level] = int32_t(next);
       }
     }
@@ -772,10 +794,13 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_
   double w;
   while (true) {
     sums = a.sums + (LEVELS ? size_t(depth & 1) * a.n_seqs + s : size_t(r0) + cur) * a.chunks;
+    float x;
+    const bool child = is_child(tree, nodes, cur, depth, x);
     d = row_of(a, sums, uint32_t(r0) + cur, t);
-    const uint32_t next = next_node(tree, nodes, cur, depth, d, tried, w);
+    const uint32_t next = next_node(tree, nodes, d, child, x, tried, w);
     if (LEVELS || next == kNone) break;
-    if (tid == 0) take_node(tree, nodes, d, depth, next);
+    // (a wave for each, so that none waits for more than one logarithm)
+    if (tid / 64 == depth % (kThreads / 64) && lane == next) take_node(tree, nodes, d, depth, x);
     depth++;
     if (lane == depth) mine = next;
     cur = next;
