@@ -349,7 +349,9 @@ int qe_op_page_tree_attention(const qe_pages* pages, const int32_t* parents, con
  * at least table_stride * page_size. Weights and sums are f32, of rows of either type; the sums are the
  * same every time. A row with a score that is not finite may make any position it attends NaN. mass
  * must not overlap q, the pages or work. n_rows * n_heads is below 2^28, and n_seqs * n_kv_heads times the
- * positions of a table's row / 256 below 2^24. */
+ * positions of a table's row / 256 below 2^24. max_new as there; with more new tokens than it says a call may take
+ * much longer, never give another result than its sums' rounding. work is scratch of the call, of the size for the same
+ * values (positions: table_stride * page_size); calls that may overlap need one each. */
 uint64_t qe_op_page_weigh_work_bytes(uint64_t n_rows, uint64_t n_heads, uint64_t n_kv_heads, uint64_t n_seqs,
                                      uint64_t positions, uint64_t max_new);
 int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint64_t n_heads, uint64_t q_stride,
@@ -412,8 +414,8 @@ int qe_op_verify_drafts(const float* logits, uint64_t n_rows, uint64_t vocab, ui
  * of the node / temperature[s]), the node's children are tried in the order of their rows; child c is accepted
  * while accept[c] * (1 - sum of the p of those tried before) < p[nodes[c]], a token that was tried before
  * having no p left. The walk goes on from the first accepted child. Where none is, or max_depth drafts
- * (0: no bound) have been accepted, the last token is drawn from p without the tokens tried (of a node at
- * max_depth none are) by sample[s]. What is emitted follows the target's distribution whatever the tree is.
+ * (0: no bound; large trees are checked faster with one) have been accepted, the last token is drawn from p
+ * without the tokens tried (of a node at max_depth none are) by sample[s]. What is emitted follows the target's distribution whatever the tree is.
  * accept [n_rows] and sample [n_seqs] are numbers in [0, 1). Logits, temperature, draws, logprobs_out and work
  * as in qe_op_verify_drafts; tokens_out [n_rows]: the accepted nodes' tokens, then the drawn one, then
  * 0xFFFFFFFF; path_out [n_seqs][QE_TREE_NODES] (int32): 0 for the root, the accepted nodes' rows counted from

@@ -31,8 +31,7 @@ struct KeepArgs {
 };
 
 // A wave has a contiguous part of the row, in groups of 256 positions, a lane 4 consecutive ones of each.
-constexpr uint32_t kGroup = 256, kGroupsInRegs = 8, kWaves = kKeepThreads / 64;
-constexpr uint32_t kInRegs = kWaves * kGroupsInRegs * kGroup;  // positions of a row that fit in registers
+constexpr uint32_t kGroup = 256, kWaves = kKeepThreads / 64;
 constexpr uint32_t kDigits = 2048, kCopies = 4;
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -47,9 +46,13 @@ __device__ __forceinline__ uint32_t sum_below(const uint32_t* waves, uint32_t wa
 // digits from the top, 11, 11 and 10 bits: the values that agree so far are counted by their next digit in LDS (the
 // first time in four copies, since masses share few exponents), and the digit is where the count from above
 // reaches `need`. Then everything above that value is kept, and of what equals it the first.
-// Bound by latency, not by the 4 bytes a position: some ten barriers, and LDS counts that meet in one place.
-template <bool REGS>
+// Bound by latency, not by the 4 bytes a position: a chain of some ten barriers, and a few operations a value on each CU.
+// 8 rows of 4500 values to 1024 7.8 us; 256 rows of up to 32,000 to 4096 19.5 (the row 6, the digits 8, the places 5); 8
+// of up to 43,632 23. A row that is read again for each pass: 8 of up to 70,000 51.
+// GROUPS: of a wave, that are held in registers (0: the row is read again for each pass).
+template <int GROUPS>
 __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
+  constexpr bool REGS = GROUPS > 0;
   __shared__ uint32_t digits[(kCopies + 2) * kDigits];
   __shared__ uint32_t waves[3][kWaves], found[3][2], above[kWaves], equal[kWaves];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -81,17 +84,17 @@ __global__ __launch_bounds__(kKeepThreads) void k_page_keep(KeepArgs a) {
       for (int e = 0; e < 4; e++)
         if (j + e < len && (j + e < from || j + e >= to)) key[e] = kAlways;
   };
-  uint32_t keys[REGS ? kGroupsInRegs : 1][4];
+  uint32_t keys[REGS ? GROUPS : 1][4];
   if constexpr (REGS) {
 #pragma unroll
-    for (uint32_t g = 0; g < kGroupsInRegs; g++)
+    for (uint32_t g = 0; g < GROUPS; g++)
       if (g < groups) load(g, keys[g]);
   }
   // f(first position, keys) of each group
   auto each = [&](auto f) __attribute__((always_inline)) {
     if constexpr (REGS) {
 #pragma unroll
-      for (uint32_t g = 0; g < kGroupsInRegs; g++)
+      for (uint32_t g = 0; g < GROUPS; g++)
         if (g < groups) f(j0 + g * kGroup, keys[g]);
     } else {
       for (uint32_t g = 0; g < groups; g++) {
@@ -309,7 +312,7 @@ __device__ __forceinline__ void move_rest(const MoveArgs& a, const Moves& m, uin
 }
 
 // Up to 64 rows of a sequence and KV head, as a path has them: a workgroup reads all of them and writes them.
-// Bound by its chain: count, src, table, rows.
+// Bound by its chain: count, src, table, rows. 48 sequences of 8 KV heads, paths of a few rows, e4m3: 5.1 us.
 constexpr uint32_t kFewMoves = 64;
 template <bool FP8>
 __global__ __launch_bounds__(kMoveThreads) void k_page_move_few(MoveArgs a) {
@@ -355,7 +358,9 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move_few(MoveArgs a) {
 // 8 dims of V; one has what there is one of for a row. Rows ascend and only ever move to the front, so what a chunk
 // of rows writes no later chunk reads: within one everything is read before anything is written, and the next one's
 // reads are under way while it is written. Where the rows lie is found for 2048 of them at a time (src, then the
-// table: two load latencies, which a chunk would otherwise wait for). Workgroup (part, item): the parts of an item share
+// table: two load latencies, which a chunk would otherwise wait for). V is gathered 2 bytes (1 of e4m3) at a time and
+// stored in whole runs of 16 positions. Bound by those gathers: 6 sequences of up to 8192 positions, 8 KV heads, bf16, to
+// 2048 with their mass, 40 us (K alone 18, V alone 36; 16 dims of V a workgroup 54 in all, 4 dims 51). Runs staged whole in LDS took 90. Workgroup (part, item): the parts of an item share
 // an XCD where the items are a multiple of 8.
 constexpr uint32_t kPlan = 2048, kSliceV = 8;
 template <bool FP8>
@@ -489,8 +494,9 @@ int qe_op_page_keep(const float* mass, uint64_t mass_stride, const int32_t* lens
   if (k.meets(m) || k.meets(l) || k.meets(c) || c.meets(m) || c.meets(l))
     return qe::set_error(QE_ERR_ARG, "kept and count must not overlap each other, mass or lens");
   qe::KeepArgs a{mass, lens, kept, count, mass_stride, kept_stride, uint32_t(n_kv_heads), uint32_t(keep), uint32_t(sinks), uint32_t(recent)};
-  (mass_stride <= qe::kInRegs ? qe::k_page_keep<true> : qe::k_page_keep<false>)<<<uint32_t(rows), qe::kKeepThreads, 0,
-                                                                                  static_cast<hipStream_t>(stream)>>>(a);
+  // positions of a row that registers hold: groups x 256 x 16 waves
+  auto* const kern = mass_stride <= 8 * 4096 ? qe::k_page_keep<8> : mass_stride <= 16 * 4096 ? qe::k_page_keep<16> : qe::k_page_keep<0>;
+  kern<<<uint32_t(rows), qe::kKeepThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return qe::set_error(QE_ERR_HIP, "page keep launch failed: %s", hipGetErrorString(e));
   return QE_OK;

@@ -246,3 +246,59 @@ def test_a_bounded_cache_as_a_graph(gpu):
             assert torch.equal(a["case"].dev[n].view(torch.int16), b["case"].dev[n].view(torch.int16)), (i, n)
         torch.randn(1000, device="cuda").sum()
     assert a["count"].tolist() == [100, 86]
+
+
+def test_two_loops_on_two_streams(gpu):
+    """two serving loops with trees on two streams at once, as graphs, each with work of its own: equal to each alone"""
+    kinds = [("fp8", torch.float32), ("bf16", torch.bfloat16)]
+    alone, both = [Trees(*k) for k in kinds], [Trees(*k) for k in kinds]
+    streams, graphs = [torch.cuda.Stream() for _ in kinds], []
+    for x in alone + both:
+        x.fill()
+    torch.cuda.synchronize()
+    for x, st in zip(both, streams):
+        with torch.cuda.stream(st):
+            x.step()
+    for x in alone:
+        x.step()
+    torch.cuda.synchronize()
+    for x, st in zip(both, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=st):
+            x.step()
+    torch.cuda.synchronize()
+    for i in range(4):
+        for x in alone + both:
+            x.fill()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(alone, both):
+            x.step()
+            for a, b in zip(x.state(), y.state()):
+                assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 70]])
+def test_weights_of_two_plans_on_two_streams(gpu, new):
+    cases = [Case(new, [700, 30, 300], 32, 2, kv, seed=105 + i) for i, kv in enumerate(("fp8", "bf16"))]
+    q = torch.randn(sum(new), 8, D, generator=torch.Generator().manual_seed(3)).cuda()
+    pages = [c.pages() for c in cases]
+    positions = [c.host["table"].shape[1] * 32 for c in cases]
+    size = [qe.op_page_weigh_work_bytes(sum(new), 8, 2, 3, p, max(new)) for p in positions]
+    work = [torch.empty(s, dtype=torch.uint8, device="cuda") for s in size]
+    mass = [torch.zeros(3, 2, p, device="cuda") for p in positions]
+    alone = [torch.zeros_like(m) for m in mass]
+    for i in range(2):
+        for _ in range(6):
+            qe.op_page_weigh(pages[i], q, alone[i], work[i], max(new))
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            qe.op_page_weigh(pages[i], q, mass[i], work[i], max(new), stream=st)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, mass):
+        assert torch.equal(a, b)

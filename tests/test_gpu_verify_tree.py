@@ -244,3 +244,17 @@ def test_large_trees_level_by_level(gpu, max_depth, n):
     temps = np.array([(0.7, 1.0, 0.0, 1.3, 0.9)[i % 5] for i in range(n)], np.float32)
     count = check(x, starts, parents, nodes, rng.random(rows, np.float32), rng.random(n, np.float32), temps, max_depth)
     assert count.max() > 1
+
+
+@pytest.mark.parametrize("vocab", [262144, 262145, 400003, 1 << 20])
+def test_large_vocabularies(gpu, vocab):
+    """more chunks than a wave holds in registers, up to the largest"""
+    rng = np.random.default_rng([vocab, 9])
+    starts, parents = np.array([0, 5, 9]), np.array([-1, 0, 0, 1, 1, -1, 0, 1, 2])
+    x = rng.standard_normal((9, vocab), dtype=np.float32)
+    nodes = rng.integers(0, vocab, 9).astype(np.uint32)
+    nodes[[1, 6]] = [vocab - 1, vocab // 2]
+    x[0, vocab - 1] = x[5, vocab // 2] = 16.0
+    for depth in (0, 1):
+        check(x, starts, parents, nodes, np.full(9, 0.2, np.float32), np.array([0.3, 0.999], np.float32),
+              np.array([1.0, 0.8], np.float32), depth)
