@@ -1,4 +1,4 @@
-// qe_op_verify_drafts: drafted tokens checked against the target's probabilities, from given random
+// qe_op_verify_drafts and qe_op_verify_tree: drafted tokens checked against the target's probabilities, from given random
 // numbers. It is qe_verify_greedy's rule for sampled decoding: what the accepted drafts and the
 // token drawn after them follow is exactly the target's distribution. No reference counterpart.
 //
