@@ -332,7 +332,7 @@ int qe_op_page_attention(const qe_pages* pages, const void* q, void* out, uint64
  * earlier one (0 .. i - 1); any other value: it has none. A node attends the positions before the new
  * tokens, its ancestors and itself; what the others hold has no part in it. A row behind its sequence's
  * first QE_TREE_NODES is zeros. max_new: at most QE_TREE_NODES; work_bytes and all else as
- * qe_op_page_attention, and out must not overlap parents either. */
+ * qe_op_page_attention, and out and work must not overlap parents. */
 #define QE_TREE_NODES 64
 int qe_op_page_tree_attention(const qe_pages* pages, const int32_t* parents, const void* q, void* out, uint64_t n_rows,
                               uint64_t n_heads, uint64_t q_stride, uint64_t out_stride, uint64_t max_new, int dtype,

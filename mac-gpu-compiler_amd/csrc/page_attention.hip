@@ -1605,8 +1605,11 @@ int attend(const qe_pages* pages, const int32_t* parents, const void* q, void* o
   if (overlap(rows, span(q, q_stride * el, n_heads * kPageDim * el, n_rows)) || over(pages->k, kv_bytes) ||
       over(pages->v, kv_bytes) || (fp8 && (over(pages->k_exp, pages->page_size) || over(pages->v_exp, pages->page_size))))
     return set_error(QE_ERR_ARG, "out must not overlap q or the pages");
-  if (parents && overlap(rows, span(parents, 4 * n_rows, 4 * n_rows, 1)))
-    return set_error(QE_ERR_ARG, "out must not overlap parents");
+  if (parents) {
+    const Bytes tree{parents, 4 * n_rows};
+    if (overlap(rows, span(parents, 4 * n_rows, 4 * n_rows, 1)) || tree.meets({work, work_bytes}))
+      return set_error(QE_ERR_ARG, "out and work must not overlap parents");
+  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf16 = dtype == QE_KV_BF16, tree = parents;
   a.q = static_cast<const uint8_t*>(q);

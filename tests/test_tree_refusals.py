@@ -12,7 +12,7 @@ MB = 1 << 20
 
 
 def tree(pages, parents=ADDR, rows=4, heads=4, q=ADDR + MB, out=ADDR + 2 * MB, qs=512, os=512, new=1, dtype=qe.QE_KV_F32,
-         work=ADDR, size=None):
+         work=ADDR + 64 * MB, size=None):
     L = qe.lib()
     size = L.qe_op_page_attention_work_bytes(heads, 2, new) if size is None else size
     return L.qe_op_page_tree_attention(None if pages is None else ctypes.byref(pages), parents, q, out, rows, heads, qs, os,
@@ -58,7 +58,8 @@ def test_tree_arguments():
     for kw in (dict(q=None), dict(out=None), dict(work=None), dict(parents=None), dict(parents=ADDR + 2), dict(heads=0),
                dict(heads=3), dict(heads=1 << 17), dict(q=ADDR + 8), dict(out=ADDR + 4), dict(work=ADDR + 8), dict(qs=511),
                dict(os=514), dict(qs=1 << 33), dict(dtype=2), dict(rows=1 << 31), dict(size=0), dict(new=65),
-               dict(out=ADDR + MB), dict(out=ADDR + MB + 4096), dict(out=ADDR), dict(parents=ADDR + 2 * MB + 8188)):
+               dict(out=ADDR + MB), dict(out=ADDR + MB + 4096), dict(out=ADDR), dict(parents=ADDR + 2 * MB + 8188),
+               dict(parents=ADDR + 64 * MB + 4), dict(work=ADDR - 16)):
         assert tree(p, **kw) == qe.QE_ERR_ARG, kw
     assert tree(None) == qe.QE_ERR_ARG
     assert tree(p, rows=0, q=None, out=None, work=None, parents=None) == qe.QE_OK
