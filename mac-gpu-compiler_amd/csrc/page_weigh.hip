@@ -6,8 +6,9 @@
 //
 // A weight needs its row's sum over all positions. Up to 16 rows (tokens x q heads) of a sequence and KV head:
 // k_weigh_few leaves the scores, 4 bytes a row and position where K has 128 or 256 for all rows, and k_weigh_kept makes
-// weights of them. More rows: the scores are computed twice. k_weigh<false> leaves each row's maximum and sum over
-// each block of positions, k_weigh_rows joins them, and k_weigh<true> adds up the weights.
+// weights of them. More rows: the scores are computed twice. k_weigh<kStats> leaves each row's maximum and sum over
+// each block of positions, k_weigh_rows joins them, and k_weigh<kSums> adds up the weights; where tables hold no more than
+// a block, k_weigh<kBoth> does all of it.
 //
 // Those two passes hold K still: a workgroup has 256 positions of a sequence and KV head, 64 a wave, as operand
 // A of v_mfma_f32_32x32x16_bf16 in registers, and passes the rows by, 32 at a time through LDS. So K is read
@@ -18,7 +19,8 @@
 // Measured: the last 32 rows of each of 4 sequences of up to 16,000 positions, 16 over 8 heads, bf16 (82 MB of K), 48
 // us: two passes of 21 and 24, bound by K (4 and 3.4 TB/s), and 5 the join. Up to 1024 f32 rows of 3 sequences over up to
 // 4096 positions, 226: two passes of 115, 890 of the 1239 TFLOP/s that a large library product reaches, with
-// exponentials, sums and the parts of f32 rows on the vector unit as long as the products.
+// exponentials, sums and the parts of f32 rows on the vector unit as long as the products. Up to 88 f32 rows of each of 19
+// sequences over up to 112 positions, 24 over 8 heads, by k_weigh<kBoth> 25 us, by the passes 41.
 #include "pages.h"
 
 #include "device_common.h"
@@ -166,11 +168,16 @@ struct RowTile {
   }
 };
 
-template <bool FP8, bool BF16_ROWS, bool SUMS>
+// What a pass does: the rows' maxima and sums over the block (kStats), the weights by them (kSums), or both, where one
+// block holds all positions (kBoth: the scores are still there when the four waves know a row's sum).
+enum Pass { kStats, kSums, kBoth };
+
+template <bool FP8, bool BF16_ROWS, Pass PASS>
 __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
   constexpr int NS = BF16_ROWS ? 1 : 3, EL = FP8 ? 1 : 2;
+  constexpr bool STATS = PASS != kSums, SUMS = PASS != kStats;
   __shared__ __align__(16) uint8_t buf[2][NS][kTile * 256];
-  __shared__ float2 stat[SUMS ? 1 : 2][SUMS ? 1 : 4][SUMS ? 1 : kTile];
+  __shared__ float2 stat[STATS ? 2 : 1][STATS ? 4 : 1][STATS ? kTile : 1];
   const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t at = blockIdx.x;
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
     const int32_t last = real ? int32_t(max(min(q.first + token, capacity_of(a.p) - 1), int64_t(-1))) : -1;  // the last position it attends
     const uint64_t stat_at = (uint64_t(q.row0) + token) * a.group * a.p.n_kv + head * a.group + (r - token * a.group);
     float2 rs = make_float2(0.f, 0.f);
-    if constexpr (SUMS)
+    if constexpr (PASS == kSums)
       if (real) rs = a.rows[stat_at];
     f32x16 v[2];
     v[0] = 0.f;
@@ -258,23 +265,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
       const uint32_t in = 32 * u + 8 * (e / 4) + (e & 3);
       return int32_t(x + in + 4 * half) > last || !(there >> (2 * u + e / 8) & 1);
     };
-    if constexpr (SUMS) {
-      const float ref = rs.x == -INFINITY ? 0.f : rs.x;
-      if (masked) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const float w = exp2_fast(fmaf(v[u][e], a.c, -ref)) * rs.y;
-            sum[u][e] += hidden(u, e) ? 0.f : w;
-          }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) sum[u][e] = fmaf(exp2_fast(fmaf(v[u][e], a.c, -ref)), rs.y, sum[u][e]);
-      }
-    } else {
+    if constexpr (STATS) {
       if (masked) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -296,21 +287,44 @@ __global__ __launch_bounds__(256, 2) void k_weigh(WeighArgs a) {
       l = add_halves(l);
       if (half == 0) stat[i & 1][wave][col] = make_float2(m, l);
     }
+    // a row's maximum and sum over the block, of the four waves'
+    auto of_block = [&] __attribute__((always_inline)) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) m = fmaxf(m, stat[i & 1][w][col].x);
+#pragma unroll
+      for (int w = 0; w < 4; w++) l = fmaf(stat[i & 1][w][col].y, rebase(stat[i & 1][w][col].x, m), l);
+      return make_float2(m, l);
+    };
+    if constexpr (PASS == kBoth) {
+      __syncthreads();
+      rs = of_block();
+      rs.y = rs.y == 0.f ? 0.f : 1.f / rs.y;
+    }
+    if constexpr (SUMS) {
+      const float ref = rs.x == -INFINITY ? 0.f : rs.x;
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float w = exp2_fast(fmaf(v[u][e], a.c, -ref)) * rs.y;
+            sum[u][e] += hidden(u, e) ? 0.f : w;
+          }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) sum[u][e] = fmaf(exp2_fast(fmaf(v[u][e], a.c, -ref)), rs.y, sum[u][e]);
+      }
+    }
     if (i + 1 < to) {
       rows.store(buf[(i + 1) & 1]);
       if (i + 2 < to) rows.load(a, q, head, (i + 2) * kTile);
     }
     __syncthreads();
-    if constexpr (!SUMS) {
-      if (tid < kTile && real) {  // (wave 0, whose lane has this row)
-        float m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) m = fmaxf(m, stat[i & 1][w][col].x);
-#pragma unroll
-        for (int w = 0; w < 4; w++) l = fmaf(stat[i & 1][w][col].y, rebase(stat[i & 1][w][col].x, m), l);
-        a.parts[stat_at * a.blocks + block] = make_float2(m, l);
-      }
-    }
+    if constexpr (PASS == kStats)
+      if (tid < kTile && real) a.parts[stat_at * a.blocks + block] = of_block();  // (wave 0, whose lane has this row)
   }
   if constexpr (SUMS) {
     float all[32];
@@ -723,19 +737,25 @@ int qe_op_page_weigh(const qe_pages* pages, const void* q, uint64_t n_rows, uint
   a.c = 1.44269504f / sqrtf(float(qe::kPageDim));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t grid = uint32_t(items * cut.splits);
-  auto go = [&](auto* few, auto* kept, auto* first, auto* second) {
+  auto go = [&](auto* few, auto* kept, auto* first, auto* second, auto* both) {
     if (a.few) {
       const uint32_t blocks = uint32_t((capacity + 1023) / 1024);
       few<<<grid, 256, 0, st>>>(a);
       kept<<<blocks * a.p.n_seqs * a.p.n_kv, 256, 0, st>>>(a, blocks);
       return;
     }
-    first<<<grid, 256, 0, st>>>(a);
-    qe::k_weigh_rows<<<uint32_t((n_rows * n_heads + 15) / 16), 256, 0, st>>>(a);
-    second<<<grid, 256, 0, st>>>(a);
+    if (a.blocks == 1) {
+      both<<<grid, 256, 0, st>>>(a);
+    } else {
+      first<<<grid, 256, 0, st>>>(a);
+      qe::k_weigh_rows<<<uint32_t((n_rows * n_heads + 15) / 16), 256, 0, st>>>(a);
+      second<<<grid, 256, 0, st>>>(a);
+    }
     if (a.splits > 1) qe::k_weigh_add<<<uint32_t(items), 256, 0, st>>>(a);
   };
-#define QE_WEIGH(F, B) go(qe::k_weigh_few<F, B>, qe::k_weigh_kept<F, B>, qe::k_weigh<F, B, false>, qe::k_weigh<F, B, true>)
+#define QE_WEIGH(F, B)                                                                                              \
+  go(qe::k_weigh_few<F, B>, qe::k_weigh_kept<F, B>, qe::k_weigh<F, B, qe::kStats>, qe::k_weigh<F, B, qe::kSums>, \
+     qe::k_weigh<F, B, qe::kBoth>)
   const bool bf16 = dtype == QE_KV_BF16;
   if (fp8 && bf16) QE_WEIGH(true, true);
   else if (fp8) QE_WEIGH(true, false);

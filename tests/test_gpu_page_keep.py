@@ -117,6 +117,15 @@ def test_weigh_many_sequences(gpu, n_seqs, most):
     check_weigh(Case(new, [(i * 37) % 90 for i in range(n_seqs)], 16, 1, "bf16", seed=85), 2, F32)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("rows", [F32, BF16])
+@pytest.mark.parametrize("new,ctx,page,heads", [([100, 31], [156, 0], 16, 2), ([100, 31], [157, 0], 16, 2), ([200, 3], [56, 250], 64, 4),
+                                                ([17, 64], [238, 5], 256, 1), ([256], [0], 32, 6)])
+def test_weigh_a_block_of_positions(gpu, new, ctx, page, heads, rows, kv):
+    """tables that hold just what one workgroup has, and a little more"""
+    check_weigh(Case(new, ctx, page, 1, kv, seed=94, lead=2, tail=1), heads, rows, gap=8)
+
+
 @pytest.mark.parametrize("entry", [-1, 1 << 30, -(1 << 31)])
 @pytest.mark.parametrize("new", [[20, 5, 3], [1, 1, 1], [100, 5, 80]])
 def test_weigh_pages_that_are_not_there(gpu, entry, new):
