@@ -1,4 +1,5 @@
-// qe_op_page_attention: causal GQA attention of packed new tokens over the paged K/V cache. No
+// qe_op_page_attention: causal GQA attention of packed new tokens over the paged K/V cache; and
+// qe_op_page_tree_attention: the same for trees of drafted tokens (see TreeAttnArgs). No
 // reference counterpart (its attention reads one sequence's contiguous cache, one token at a time:
 // cpu_inference.rs:144-162).
 //
