@@ -608,8 +608,8 @@ __global__ __launch_bounds__(kThreads) void k_draft_draw(DraftArgs a) {
 // accepted if u_c R < p(d), else R -= p(d) and d has no p left; if none is, the token is drawn from what is left of p. Given
 // the ones tried before, child c is accepted with p(d) / R, which is d's share of what is left; so the token that
 // comes out has p, whatever the children are.
-// The sums of p are k_draft_sums', or a level's. A draw takes the tokens tried out of their chunks' sums: a refused child
-// leaves at least 2^-24 of R, a sum is off by some 2^-50 of the row's.
+// The sums of p are k_draft_sums', or a level's. A draw takes the tokens tried out of their chunks' sums, and sums a chunk
+// anew of which that leaves next to nothing.
 // Measured (151,936 tokens): a tree of 13 nodes 14 us, two launches (sums 5; the walk 2 a step, the draw 4, links of dependent
 // loads); 24 trees of up to 48 nodes by levels 50, 8 launches of 2 to 7 and the draw 9.
 //
@@ -823,7 +823,7 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_
   }
   // the draw: the chunks' sums without the tokens tried, then a chunk's tokens
   const uint32_t n = (a.chunks + 63) / 64, c0 = lane * n;
-  double chunk[kLaneChunks], before, aim = 0.0;
+  double chunk[kLaneChunks], gone[kLaneChunks] = {}, before, aim = 0.0;
   auto plain_chunks = [&] {
 #pragma unroll
     for (int i = 0; i < kLaneChunks; i++) {
@@ -835,6 +835,27 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_
       }
     }
   };
+  // weights z and logits y of this thread's tokens of chunk c, those tried weigh nothing
+  double z[N];
+  f32x4 y;
+  auto load_chunk = [&](uint32_t c) __attribute__((always_inline)) {
+    const uint32_t i0 = c * kChunk + tid * N;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      z[e] = 0.0;
+      y[e] = 0.f;
+      if (c != kNone && i0 + e < a.vocab) {
+        y[e] = a.logits[d.row * a.stride + i0 + e];
+        z[e] = row_weight(d, i0 + e, y[e]);
+      }
+    }
+    for (uint64_t rest = tried; rest; rest &= rest - 1) {
+      const uint32_t is = from_lane(token, __builtin_ctzll(rest));
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        if (is == i0 + e) z[e] = 0.0;
+    }
+  };
   auto share = [&](double all) { return aim = double(a.sample[s]) * all; };
   plain_chunks();
   for (uint64_t rest = tried; rest; rest &= rest - 1) {
@@ -843,7 +864,34 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_
     const double less = from_lane(w, c);
 #pragma unroll
     for (int i = 0; i < kLaneChunks; i++)
-      if (uint32_t(i) < n && is < a.vocab && is / kChunk == c0 + i) chunk[i] = fmax(chunk[i] - less, 0.0);
+      if (uint32_t(i) < n && is < a.vocab && is / kChunk == c0 + i) gone[i] += less;
+  }
+  // A difference is off by some 2^-50 of the chunk's sum, so where 2^-26 of it or less is left (or the chunk weighs so
+  // little that its other tokens may weigh 0) what is left is summed anew: no chunk has weight that its tokens have not.
+  uint32_t thin = 0;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; i++) {
+    const double whole = chunk[i];
+    if (gone[i] > 0.0) chunk[i] = whole - gone[i];
+    if (gone[i] > 0.0 && !(chunk[i] > 0x1p-26 * whole && whole > 0x1p-900)) thin |= 1u << i;
+  }
+  while (const uint64_t lanes = __ballot(thin)) {  // (every wave has the same)
+    const int at = __builtin_ctzll(lanes);
+    const uint32_t i = uint32_t(from_lane(uint32_t(__builtin_ctz(thin | 1u << 31)), at));
+    load_chunk(uint32_t(at) * n + i);
+    const double mine = wave_sum64((z[0] + z[1]) + (z[2] + z[3]));
+    if (lane == 0) sc.wave[tid / 64] = mine;
+    __syncthreads();
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kThreads / 64; k++) sum += sc.wave[k];
+    __syncthreads();
+    if (int(lane) == at) {
+      thin &= thin - 1;
+#pragma unroll
+      for (int k = 0; k < kLaneChunks; k++)
+        if (uint32_t(k) == i) chunk[k] = sum;
+    }
   }
   uint32_t c = find_chunk(chunk, n, share, before);
   if (c == kNone) {  // nothing is left: from p
@@ -851,24 +899,8 @@ __global__ __launch_bounds__(kThreads) void k_tree_decide(TreeArgs tree, uint32_
     plain_chunks();
     c = find_chunk(chunk, n, share, before);
   }
-  double z[N];
-  f32x4 y;
+  load_chunk(c);
   const uint32_t i0 = c * kChunk + tid * N;
-#pragma unroll
-  for (int e = 0; e < N; e++) {
-    z[e] = 0.0;
-    y[e] = 0.f;
-    if (c != kNone && i0 + e < a.vocab) {
-      y[e] = a.logits[d.row * a.stride + i0 + e];
-      z[e] = row_weight(d, i0 + e, y[e]);
-    }
-  }
-  for (uint64_t rest = tried; rest; rest &= rest - 1) {
-    const uint32_t is = from_lane(token, __builtin_ctzll(rest));
-#pragma unroll
-    for (int e = 0; e < N; e++)
-      if (is == i0 + e) z[e] = 0.0;
-  }
   place_token(a, d, uint32_t(r0) + depth, i0, z, y, aim - before, t, sc);
 }
 

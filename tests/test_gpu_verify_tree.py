@@ -258,3 +258,53 @@ def test_large_vocabularies(gpu, vocab):
     for depth in (0, 1):
         check(x, starts, parents, nodes, np.full(9, 0.2, np.float32), np.array([0.3, 0.999], np.float32),
               np.array([1.0, 0.8], np.float32), depth)
+
+
+def few_tokens(n, vocab, at, values):
+    """rows [n, vocab] that are -inf but for the tokens `at` (each row's own, or the same for all), with `values`"""
+    x = np.full((n, vocab), -np.inf, np.float32)
+    x[np.arange(n)[:, None], np.broadcast_to(at, values.shape)] = values
+    return x
+
+
+# trees: few, whose rows are all summed first; many, which go level by level
+@pytest.mark.parametrize("n", [200, 700])
+@pytest.mark.parametrize("children", [(3, 900), (900, 3, 2047), (5, 4, 3, 2, 1)])
+def test_chunks_of_which_all_is_refused(gpu, n, children):
+    """logits masked to a few tokens (a row of 2048 that holds only refused children has nothing left, whatever
+    its sums leave by rounding): the draw is one of the others, from the first number on"""
+    rng = np.random.default_rng([n, len(children)])
+    vocab, m = 6000, len(children)
+    others = (2500, 5999)
+    x = few_tokens(n, vocab, np.array(children + others), (rng.standard_normal((n, m + 2)) * 1.5).astype(np.float32))
+    logits = np.repeat(x, 1 + m, 0)
+    starts = np.arange(n + 1) * (1 + m)
+    u_last = np.nextafter(np.float32(1), np.float32(0))
+    for v in (0.0, 1e-30, 0.5, u_last):
+        args = (logits, starts, np.tile([-1] + [0] * m, n), np.tile([0, *children], n), np.full(len(logits), u_last, np.float32),
+                np.full(n, v, np.float32))
+        count = check(*args, max_depth=1)
+        assert (count == 1).all()
+        if v in (0.0, u_last):
+            np.testing.assert_array_equal(call(*args, None, 1)[0][::1 + m], others[0] if v == 0.0 else others[1])
+
+
+@pytest.mark.parametrize("n", [200, 900])
+def test_little_is_left_of_a_chunk(gpu, n):
+    """two refused children that are all but 1e-14 of a chunk: what is left of it is drawn by its own sum, which the
+    difference from the chunk's would give to a few percent"""
+    rng = np.random.default_rng([n, 4])
+    vocab = 5000
+    # (each refused child leaves about 1e-7 of what there was, which a number just below 1 refuses)
+    values = np.stack([np.zeros(n), np.full(n, -16.0), np.full(n, -32.0), np.full(n, -32.0)], 1) + rng.random((n, 4)) * 0.2
+    values[:, 3] += rng.standard_normal(n)
+    values = values.astype(np.float32)
+    logits = np.repeat(few_tokens(n, vocab, np.array([70, 1500, 1999, 2048]), values), 3, 0)
+    w = np.exp(values[:, 2:].astype(np.float64) - values[:, 3:])
+    border = w[:, 0] / w.sum(1)
+    u_last = np.nextafter(np.float32(1), np.float32(0))
+    for side, token in ((1 - 2.0 ** -12, 1999), (1 + 2.0 ** -12, 2048)):
+        args = (logits, np.arange(n + 1) * 3, np.tile([-1, 0, 0], n), np.tile([0, 70, 1500], n), np.full(3 * n, u_last, np.float32),
+                (border * side).astype(np.float32))
+        np.testing.assert_array_equal(call(*args, None, 1)[0][::3], token)
+        check(*args, max_depth=1)
