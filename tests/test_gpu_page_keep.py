@@ -385,3 +385,82 @@ def test_move_past_32_bits(gpu):
     qe.op_page_read(pages, *out)
     assert torch.equal(out[0][:300], k[at.cuda()]) and torch.equal(out[1][:300], v[at.cuda()])
     assert torch.equal(out[0][300:], k[300:]) and torch.equal(out[1][300:], v[300:])
+
+
+def widened(src, wide):
+    """src with -1 behind each row, up to `wide` of them"""
+    return torch.nn.functional.pad(src, (0, wide - src.shape[-1]), value=-1)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_move_paths_of_wide_rows(gpu, page, kv):
+    """what test_move_paths moves, of a src that has room for more"""
+    g = torch.Generator().manual_seed(16)
+    new = [1 + i % 64 for i in range(0, 23 * 5, 5)]
+    ctx = list(range(0, 3 * len(new), 3))
+    case = Case(new, ctx, page, 2, kv, seed=95)
+    src, count = torch.full((len(new), 90), -1), []
+    for s, n in enumerate(new):
+        m = int(torch.randint(0, n + 1, (1,), generator=g))
+        src[s, :m] = chosen(g, 1, m, n)[0]
+        count.append(m)
+    mass = torch.rand(len(new), 2, case.host["table"].shape[1] * page, generator=g)
+    check_move(case, src, count, ctx)
+    check_move(case, src, count, ctx, mass)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("page,share", [(16, 0.4), (64, 0.95), (256, 0.7)])
+def test_move_of_many_rows_from_any_start(gpu, page, share, kv):
+    """counts of 65 to some 600 behind a first of every alignment to the runs of 16, and before the start"""
+    g = torch.Generator().manual_seed(17)
+    first = [*range(16), 64 + 9, -1, -16, -21, -100]
+    lens = [200 + 29 * (i * 7 % len(first)) for i in range(len(first))]
+    case = Case([0] * len(first), lens, page, 1, kv, seed=96, spare=1)
+    count = [max(65, int((ln - f) * share)) for ln, f in zip(lens, first)]
+    src = torch.stack([widened(chosen(g, 1, n, ln - f), max(count) + 1) for n, ln, f in zip(count, lens, first)])
+    mass = torch.rand(len(first), 1, case.host["table"].shape[1] * page, generator=g)
+    check_move(case, src, count, first)
+    check_move(case, src, count, first, mass)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_move_of_many_rows_at_the_edges(gpu, kv):
+    """pages that are not there as source and destination, positions past the table and past mass, counts of
+    nothing, below 0 and above what src holds; all rows where they are"""
+    holes = [(0, 2, -1), (0, 9, 1 << 30), (1, 1, -(1 << 31)), (1, 2, -1), (2, 0, -5), (3, 5, -1)]
+    case = Case([0] * 4, [300, 260, 140, 290], 16, 2, kv, seed=97, holes=holes)
+    g = torch.Generator().manual_seed(18)
+    src = torch.stack([widened(chosen(g, 2, n, ln), 150) for n, ln in ((150, 300), (150, 260), (120, 140), (150, 390))])
+    mass = torch.rand(4, 2, case.host["table"].shape[1] * 16, generator=g)
+    for count in ([150, 149, 120, 150], [0, -3, 1, 1 << 30], [-(1 << 31), 70, 65, 16]):
+        check_move(case, src, count, mass=mass)
+        check_move(case, src, count, [0, 20, -7, 60], mass)
+        check_move(case, src, count, [290, 1 << 30, -(1 << 31), (1 << 31) - 1], mass)
+    same = torch.arange(100).expand(4, 2, 100).contiguous()
+    check_move(case, same, [100, 70, 10, 0], mass=mass)
+    case.host["lens"] = torch.tensor([1 << 30, -5, 0, 304], dtype=torch.int32)
+    check_move(case, src, [130, 2, 3, 80], mass=mass)
+    check_move(case, src, [130, 66, 70, 80], mass=mass[..., :90].contiguous())
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("first", [0, 5])
+def test_move_of_thousands_of_rows(gpu, first, kv):
+    """counts around 2048 rows, of which the kernel finds the places at a time, and of more than twice that"""
+    g = torch.Generator().manual_seed(19)
+    count, lens = [2047, 2048, 2049, 4999, 2043], [2100, 4100, 2070, 5600, 3000]
+    case = Case([0] * 5, lens, 64, 1, kv, seed=98)
+    src = torch.stack([widened(chosen(g, 1, n, ln - first), 5000) for n, ln in zip(count, lens)])
+    mass = torch.rand(5, 1, case.host["table"].shape[1] * 64, generator=g)
+    check_move(case, src, count, [first] * 5, mass)
+
+
+def test_move_by_one(gpu):
+    """a cache at its bound that drops one position of each head: all rows behind it move by one"""
+    case = Case([0] * 2, [600, 577], 64, 2, "fp8", seed=99)
+    src = torch.stack([torch.stack([torch.cat([torch.arange(d), torch.arange(d + 1, 600)]) for d in drop])
+                       for drop in ((0, 300), (17, 575))])
+    mass = torch.rand(2, 2, case.host["table"].shape[1] * 64, generator=torch.Generator().manual_seed(20))
+    check_move(case, src, [599, 576], mass=mass)
