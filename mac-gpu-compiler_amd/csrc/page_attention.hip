@@ -440,7 +440,7 @@ __device__ __forceinline__ uint32_t find_part(A& a, uint32_t w, uint32_t W, uint
 }
 
 // How many of the workgroups of an item's n parts join it: more than one where a row's 16 threads would have more
-// than two rounds of parts. Small tiles: they share the rows; large ones (R >= 128): the dims, a power of two of them.
+// than two rounds of parts. Small tiles: they share the rows; large ones (R > 32): the dims, a power of two of them.
 __device__ __forceinline__ uint32_t joiners(uint32_t n, uint32_t rows, uint32_t R) {
   if (R <= 32) return n * min(rows, 16u) > 128 ? min(n, 16u) : 1;
   return n > 64 ? 16 : n > 32 ? 8 : n > 16 ? 4 : 1;

@@ -253,3 +253,21 @@ def test_calls_on_two_streams(gpu):
             with torch.cuda.stream(st):
                 graphs[i].replay()
         same()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("new,ctx,n_kv,heads", [([20], [1500], 1, 2), ([11], [3000], 1, 3), ([13], [9000], 1, 4), ([64], [5000], 1, 1),
+                                                ([21, 3, 17], [7000, 40, 2500], 1, 3), ([17, 32], [2600, 4000], 2, 4),
+                                                ([33, 1], [16000, 16000], 1, 1)])
+def test_half_filled_tiles_over_a_long_axis(gpu, new, ctx, n_kv, heads, kv):
+    """33 to 64 f32 rows a KV head, whose items are cut into 17 to 32, 33 to 64 and more parts"""
+    check(Case(new, ctx, 64, n_kv, kv, seed=76, lead=1, tail=1), [random_tree(n, n) for n in new], heads, F32, gap=16)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_half_filled_tiles_of_many_sequences(gpu, kv):
+    """33 to 64 f32 rows a KV head of more sequences than a wave has lanes, one of them long, and rows behind the 64th node"""
+    new = [(i * 7) % 31 for i in range(70)]
+    ctx = [(i * 37) % 200 for i in range(70)]
+    new[33], ctx[33], new[50] = 30, 6000, 70
+    check(Case(new, ctx, 32, 1, kv, seed=77), [random_tree(n, i) for i, n in enumerate(new)], 2, F32, max_new=30)
