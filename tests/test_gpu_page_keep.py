@@ -464,3 +464,32 @@ def test_move_by_one(gpu):
                        for drop in ((0, 300), (17, 575))])
     mass = torch.rand(2, 2, case.host["table"].shape[1] * 64, generator=torch.Generator().manual_seed(20))
     check_move(case, src, [599, 576], mass=mass)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("new,ctx,heads,max_new", [([1, 1], [700, 90], 4, 1), ([8, 3], [300, 20], 2, 8), ([70, 9], [500, 100], 2, 70),
+                                                   ([90, 40], [20, 0], 1, 90), ([30], [200], 2, 3)])
+def test_weigh_the_last_bits_of_f32_rows(gpu, new, ctx, heads, max_new, kv):
+    """scores that only the lowest 8 bits of q decide: q has whole numbers from 2^23 on, in pairs that differ by at most
+    60, and each position's K takes the difference of one pair. Few rows, many, one block of positions, and more rows than
+    max_new says."""
+    case = Case(new, ctx, 16, 1, kv, seed=100)
+    g = torch.Generator().manual_seed(21)
+    for s, ln in enumerate(case.lens):
+        for j in range(ln):
+            row = torch.zeros(D)
+            i, sign = int(torch.randint(0, 64, (1,), generator=g)), 1 - 2 * (j % 2)
+            row[2 * i], row[2 * i + 1] = sign, -sign
+            page, off = int(case.host["table"][s, j // 16]), j % 16
+            case.host["k"][page, 0, off] = row.to(case.host["k"].dtype)
+            if kv == "fp8":
+                case.host["ke"][page, 0, off] = 127
+            case.rows[s][0][0, j] = row.double()
+    q = (2 ** 23 + 256 * torch.randint(0, 2 ** 14, (case.total, heads, 64, 1), generator=g)
+         + torch.randint(0, 61, (case.total, heads, 64, 2), generator=g)).flatten(2).float()
+    added, _ = weights(case, q)
+    got = weigh(case, q, torch.zeros(added.shape), max_new).double()
+    # Sums of whole numbers below 2^24 are exact. The exponent's argument is at most 60 log2(e) / sqrt(128) = 7.7, a
+    # difference 15.4, each rounded, and c too: 2^-19, in numerator and denominator; the exponential 2^-23; at most 2^10
+    # values are summed one after another for a row (2^-14) and the rows' weights for an entry (2^-16)
+    assert ((got - added).abs() <= added * (2.0 ** -17 + 2.0 ** -13)).all()
