@@ -308,3 +308,42 @@ def test_little_is_left_of_a_chunk(gpu, n):
                 (border * side).astype(np.float32))
         np.testing.assert_array_equal(call(*args, None, 1)[0][::3], token)
         check(*args, max_depth=1)
+
+
+@pytest.mark.parametrize("n,vocab", [(1500, 5000), (560, 20001)])
+def test_many_trees_level_by_level(gpu, n, vocab):
+    """so many trees that a wave has a chunk of the level's row: trees of 1 to 5 nodes, none, and rows without weight"""
+    rng = np.random.default_rng([n, 6])
+    sizes = rng.integers(0, 6, n)
+    starts = np.concatenate([[0], np.cumsum(sizes)])
+    rows = int(starts[-1])
+    parents = np.concatenate([np.asarray(random_tree(int(m), s, width=3), np.int64) for s, m in enumerate(sizes)])
+    x = rng.standard_normal((rows, vocab), dtype=np.float32)
+    nodes = rng.integers(0, vocab, rows).astype(np.uint32)
+    for a, b in zip(starts[:-1], starts[1:]):
+        for i in range(a + 1, b):
+            x[a + parents[i], nodes[i]] = 10.0
+    x[rng.integers(0, rows, 20)] = -np.inf
+    x[rng.integers(0, rows, 20), ::3] = np.nan
+    temps = np.array([(0.7, 1.0, 0.0, 1.3)[i % 4] for i in range(n)], np.float32)
+    count = check(x, starts, parents, nodes, rng.random(rows, np.float32), rng.random(n, np.float32), temps, 2)
+    assert set(count) == {0, 1, 2, 3}
+
+
+@pytest.mark.parametrize("n", [4, 40])
+@pytest.mark.parametrize("vocab", [262145, 1 << 20])
+def test_few_tokens_of_a_large_vocabulary(gpu, vocab, n):
+    """logits masked to a few tokens, some in one chunk with refused children only; trees whose rows are summed first (4 of
+    the smaller vocabulary), and level by level, with four waves and with one for a chunk"""
+    rng = np.random.default_rng([vocab, n])
+    at = np.array([5, 2047, 4096, 4097, 130000, 131071, 200000, vocab - 2, vocab - 1])
+    x = few_tokens(n, vocab, at, (rng.standard_normal((n, len(at))) * 1.5).astype(np.float32))
+    children = np.stack([rng.permutation(at)[:4] for _ in range(n)])
+    children[0], children[1], children[2] = at[:4], at[[0, 1, 7, 8]], at[2:6]
+    logits = np.repeat(x, 5, 0)
+    u_last = np.nextafter(np.float32(1), np.float32(0))
+    nodes = np.concatenate([np.zeros((n, 1), np.int64), children], 1).ravel()
+    for v in (0.0, 0.4, u_last):
+        count = check(logits, np.arange(n + 1) * 5, np.tile([-1, 0, 0, 0, 0], n), nodes, np.full(5 * n, u_last, np.float32),
+                      np.full(n, v, np.float32), max_depth=1)
+        assert (count == 1).all()
