@@ -64,7 +64,7 @@ struct AttnArgs {
 // before `first`, its ancestors and itself, all of them positions that it attends as a causal row too: blocks
 // that begin behind `first` are masked by `family`, all else is as for causal rows. Rows from kNodes on attend nothing.
 // Measured: up to 61 nodes of each of 32 sequences of up to 8253 positions, 32 over 8 heads, bf16 rows and pages (660 MB,
-// 119 GFLOP), 210 us; others below, where a call is cut.
+// 119 GFLOP), 212 us; others below, where a call is cut.
 struct TreeAttnArgs : AttnArgs {
   static constexpr bool kTree = true;
   const int32_t* parents;  // [n_rows]

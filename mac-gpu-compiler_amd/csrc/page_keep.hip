@@ -360,7 +360,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_page_move_few(MoveArgs a) {
 // reads are under way while it is written. Where the rows lie is found for 2048 of them at a time (src, then the
 // table: two load latencies, which a chunk would otherwise wait for). V is gathered 2 bytes (1 of e4m3) at a time and
 // stored in whole runs of 16 positions. Bound by those gathers: 6 sequences of up to 8192 positions, 8 KV heads, bf16, to
-// 2048 with their mass, 40 us (K alone 18, V alone 36; 16 dims of V a workgroup 54 in all, 4 dims 51). Runs staged whole in LDS took 90. Workgroup (part, item): the parts of an item share
+// 2048 with their mass, 40 us, e4m3 25 (K alone 18, V alone 36; 16 dims of V a workgroup 54 in all, 4 dims 51). Runs staged whole in LDS took 90. Workgroup (part, item): the parts of an item share
 // an XCD where the items are a multiple of 8.
 constexpr uint32_t kPlan = 2048, kSliceV = 8;
 template <bool FP8>

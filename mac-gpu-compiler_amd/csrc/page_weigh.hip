@@ -18,9 +18,9 @@
 //
 // Measured: the last 32 rows of each of 4 sequences of up to 16,000 positions, 16 over 8 heads, bf16 (82 MB of K), 48
 // us: two passes of 21 and 24, bound by K (4 and 3.4 TB/s), and 5 the join. Up to 1024 f32 rows of 3 sequences over up to
-// 4096 positions, 226: two passes of 115, 890 of the 1239 TFLOP/s that a large library product reaches, with
+// 4096 positions, 223: two passes of 114, 900 of the 1239 TFLOP/s that a large library product reaches, with
 // exponentials, sums and the parts of f32 rows on the vector unit as long as the products. Up to 88 f32 rows of each of 19
-// sequences over up to 112 positions, 24 over 8 heads, by k_weigh<kBoth> 25 us, by the passes 41.
+// sequences over up to 112 positions, 24 over 8 heads, by k_weigh<kBoth> 24 us, by the passes 41.
 #include "pages.h"
 
 #include "device_common.h"
